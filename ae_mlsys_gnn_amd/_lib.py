@@ -71,6 +71,12 @@ _SIGNATURES = {
     "fgnn_tall_product_workgroups": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int]),
     "fgnn_tall_reduce_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "fgnn_tall_reduce": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fgnn_rms_norm": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float] + [c_void_p] * 4),
+    "fgnn_rms_norm_q8": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float, c_int] + [c_void_p] * 4),
+    "fgnn_quantize_rows": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "fgnn_rms_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "fgnn_rms_norm_backward": (c_int, [c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_size_t, c_void_p]),
     "fgnn_knn_graph": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "fgnn_gmm_forward_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int]),
     "fgnn_gmm_forward": (c_int, [c_int, c_int64, c_int, c_int, c_int] + [c_void_p] * 9 + [c_int]
@@ -170,6 +176,25 @@ def stream_ptr():
     """The current stream of the current device.  Asked for as a raw handle: building a torch Stream object around it took 10 us a
     call, five times a layer step."""
     return c_void_p(torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(_current_device()))
+
+
+# Element types of the dense operators (FGNN_F32 and following in include/fgnn.h).
+FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+EIGHT_TYPES = {torch.int8: 3, torch.float8_e4m3fn: 4}
+
+
+def rows_of(t, what):
+    """(t as [rows, columns] with unit column stride, its row stride); copied only where no view of that kind exists."""
+    if t.dim() == 0:
+        raise FgnnError("%s: no dimension of features" % what)
+    cols = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, cols) if cols else t.reshape(t.shape[:-1].numel(), 0)
+    rows, step = t.shape[0], t.stride(0)
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and step < cols:
+        t = t.contiguous()
+        step = cols
+    return t, step if rows > 1 else cols
 
 
 def require_cuda(*tensors):

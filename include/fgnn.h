@@ -307,6 +307,32 @@ size_t fgnn_column_sum_workspace_bytes(int64_t n, int c);
 int fgnn_column_sum(int64_t n, int c, const float *x, int64_t ldx, float *out, void *workspace, size_t workspace_bytes,
                     void *stream);
 
+/* ---------------------------------------------------------------- dense operators of residual blocks
+ * Element types of the rows that these take.  Matrices are row-major with unit column stride; ld* are row strides in elements. */
+#define FGNN_F32  0
+#define FGNN_BF16 1
+#define FGNN_F16  2
+#define FGNN_I8   3
+#define FGNN_E4M3 4    /* 8-bit floats, 1-4-3, largest value 448 */
+
+/* Root-mean-square norm of rows with the residual's addition: h = x + residual, y = h (mean h^2 + eps)^-1/2 weight.  residual NULL: h = x and is
+ * not written; weight NULL: ones, else of type wtype (that of the rows, or FGNN_F32).  h, y contiguous; rstd [rows] (NULL: not wanted) receives
+ * (mean h^2 + eps)^-1/2 for the backward pass.  Rows of up to 64 KB.
+ * _q8 writes y in 8 bits (eight: FGNN_I8 or FGNN_E4M3) and scale [rows] with y = q * scale, scale = max |y| / (127 or 448); a row with an infinity
+ * or a NaN gets the scale NaN.  fgnn_quantize_rows does so to rows as they are.
+ * _backward: gy, gh (either may be NULL: zeros) contiguous, h as written (x without a residual), dx [rows, cols] is the gradient of x and of the
+ * residual, dweight [cols] of type wtype (that of the rows without weights); either may be NULL.  Deterministic. */
+int fgnn_rms_norm(int64_t rows, int cols, int type, const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                  const void *weight, int wtype, float eps, void *h, void *y, float *rstd, void *stream);
+int fgnn_rms_norm_q8(int64_t rows, int cols, int type, const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                     const void *weight, int wtype, float eps, int eight, void *h, void *q, float *scale, void *stream);
+int fgnn_quantize_rows(int64_t rows, int cols, int type, const void *x, int64_t ldx, int eight, void *q, float *scale,
+                       void *stream);
+size_t fgnn_rms_norm_backward_workspace_bytes(int64_t rows, int cols, int type);
+int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const void *gy, const void *gh, const void *h, int64_t ldh,
+                           const void *weight, int wtype, const float *rstd, void *dx, void *dweight, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
 /* k-nearest-neighbour graph of batched point clouds, the input of fgnn_edgeconv_forward: points
  * [n_clouds*P, D]; src_ind [n_clouds*P*k] gets, for every point, the global ids of the k nearest
  * points of its own cloud (itself included), nearest first, ties to the smaller id; 1 <= k <= min(P,

@@ -1,0 +1,220 @@
+"""The norm of rows with the residual's addition, its gradient, and its output in 8 bits, against float64."""
+import pytest
+import torch
+
+from ae_mlsys_gnn_amd import _lib
+from ae_mlsys_gnn_amd.operators import quantize_rows, rms_norm, rms_norm_q8
+
+# unit roundoff of each type; statistics and sums are 32 bits
+UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TYPES = list(UNIT)
+# either side of every change of threads and vectors a row, odd widths, one column, the widest rows
+COLS = [1, 3, 8, 64, 65, 128, 129, 255, 602, 1000, 1433, 4096, 8191, 16384]
+TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def normed(h, w, eps):
+    s = (h.square().mean(-1, keepdim=True) + eps).rsqrt()
+    return h * s * w, s
+
+
+def within(got, ref, unit, scale, what):
+    """|got - ref| <= one rounding of the result (unit |ref|) and c roundings in 32 bits of `scale`, what the sums behind it are made of."""
+    got, ref = got.detach().double().cpu(), ref.cpu()
+    tol = unit * ref.abs() * 1.01 + 2.0 ** -24 * scale.cpu() + (2.0 ** -25 if unit == 2.0 ** -11 else 0)     # (fp16's smallest step)
+    bad = (got - ref).abs() > tol
+    assert not bool(bad.any()), "%s: %d of %d, worst %.3g" % (what, int(bad.sum()), bad.numel(), float(((got - ref).abs() / tol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", COLS)
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_and_gradient(dtype, cols, residual):
+    g = torch.Generator().manual_seed(cols)
+    rows = 70 if cols > 2000 else 533
+    x, r, gy, gh = (torch.randn(rows, cols, generator=g).to(dtype) for _ in range(4))
+    w = (1 + 0.3 * torch.randn(cols, generator=g)).to(dtype)
+    leaves = [t.cuda().requires_grad_(True) for t in ((x, w, r) if residual else (x, w))]
+    got = rms_norm(leaves[0], leaves[1], residual=leaves[2] if residual else None, eps=1e-5)
+    y, h = got if residual else (got, None)
+    torch.autograd.backward((y, h) if residual else (y,), (gy.cuda(), gh.cuda()) if residual else (gy.cuda(),))
+
+    unit = UNIT[dtype]
+    xd, rd, wd, gyd, ghd = (t.double() for t in (x, r, w, gy, gh))
+    hd = xd + rd if residual else xd
+    yd, s = normed(hd, wd, 1e-5)
+    # a sum of `cols` squares in 32 bits: its relative error counts for a handful of roundings of every element
+    within(y, yd, unit, 16 * yd.abs(), "y")
+    if residual:
+        within(h, hd, unit, hd.abs(), "h")
+        # the backward pass reads h as it was handed out
+        hd = h.detach().double().cpu()
+    gw = gyd * wd
+    dot = (gw * hd).mean(-1, keepdim=True)
+    dx = s * gw - hd * s ** 3 * dot + (ghd if residual else 0)
+    parts = (s * gw).abs() + hd.abs() * s ** 3 * (gw * hd).abs().mean(-1, keepdim=True) + (ghd.abs() if residual else 0)
+    within(leaves[0].grad, dx, unit, 16 * parts, "dx")
+    dw = (gyd * hd * s).sum(0)
+    within(leaves[1].grad, dw, unit, 16 * (gyd * hd * s).abs().sum(0), "dw")
+    if residual:
+        assert torch.equal(leaves[2].grad, leaves[0].grad)
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    g = torch.Generator().manual_seed(5)
+    x, r, gy, gh = (torch.randn(7, 40, generator=g) for _ in range(4))
+    w = 1 + 0.3 * torch.randn(40, generator=g)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, r)]
+    out = rms_norm(leaves[0], leaves[1], residual=leaves[2], eps=1e-5)
+    torch.autograd.backward(out, (gy.cuda(), gh.cuda()))
+    base = [t.double() for t in (x, w, r)]
+
+    def value(a, b, c):
+        y, _ = normed(a + c, b, 1e-5)
+        return float((y * gy.double()).sum() + ((a + c) * gh.double()).sum())
+    step = 1e-5
+    for which, leaf in enumerate(leaves):
+        for at in range(0, leaf.numel(), 13):
+            ends = []
+            for sign in (1, -1):
+                moved = [t.clone() for t in base]
+                moved[which].view(-1)[at] += sign * step
+                ends.append(value(*moved))
+            # second order in the step, and float64 rounding of a value of order 10 over the step
+            assert abs(float(leaf.grad.view(-1)[at]) - (ends[0] - ends[1]) / (2 * step)) < 2e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_types_of_weights_and_missing_gradients(dtype):
+    g = torch.Generator().manual_seed(2)
+    wide = torch.randn(50, 3 * 96 + 5, generator=g).to(dtype).cuda()
+    x = wide[:, 3:99]                                  # rows that start anywhere
+    w = torch.randn(96, generator=g).cuda()            # fp32 beside any rows
+    y, _ = normed(x.double(), w.double(), 1e-6)
+    within(rms_norm(x, w), y, UNIT[dtype], 16 * y.abs(), "strided rows")
+    within(rms_norm(x.t().contiguous().t(), w), y, UNIT[dtype], 16 * y.abs(), "strided columns")
+    within(rms_norm(x.reshape(2, 25, 96), w).reshape(50, 96), y, UNIT[dtype], 16 * y.abs(), "three dimensions")
+    one = x[:1].expand(50, 96)
+    assert torch.equal(rms_norm(one, w), rms_norm(one.contiguous(), w))
+    plain, _ = normed(x.double(), 1.0, 1e-6)
+    within(rms_norm(x), plain, UNIT[dtype], 16 * plain.abs(), "no weights")
+    # either output alone, and weights alone
+    a, r = (torch.randn(50, 96, generator=g).to(dtype).cuda().requires_grad_(True) for _ in range(2))
+    wl = w.clone().requires_grad_(True)
+    y, h = rms_norm(a, wl, residual=r)
+    up = torch.randn(50, 96, generator=g).to(dtype).cuda()
+    da, dr = torch.autograd.grad(h, (a, r), up, retain_graph=True)
+    assert torch.equal(da, up) and torch.equal(dr, up)
+    full = torch.autograd.grad((y, h), (a, wl), (up, torch.zeros_like(up)), retain_graph=True)
+    alone = torch.autograd.grad(y, (a, wl), up)
+    assert torch.equal(full[0], alone[0]) and torch.equal(full[1], alone[1])
+    frozen, _ = rms_norm(a.detach(), wl, residual=r.detach())
+    assert torch.equal(torch.autograd.grad(frozen, wl, up)[0], alone[1])
+
+
+@pytest.mark.gpu
+def test_rows_of_zeros_infinities_and_no_rows():
+    x = torch.randn(6, 200).cuda()
+    x[1] = 0
+    x[2, 7] = float("inf")
+    x[3, 9] = float("nan")
+    x[4] *= 1e-30
+    w = torch.ones(200).cuda()
+    y = rms_norm(x, w, eps=0.0)
+    assert y[1].isnan().all() and y[2, 7].isnan() and (y[2, 8:] == 0).all() and y[3].isnan().all()
+    y = rms_norm(x, w, eps=1e-6)
+    assert (y[1] == 0).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[5]).all()
+    q, scale = rms_norm_q8(x, w)
+    assert scale[1] == 0 and (q[1] == 0).all() and scale[2].isnan() and scale[3].isnan() and torch.isfinite(scale[[0, 4, 5]]).all()
+    for dtype in TOP:
+        q, scale = quantize_rows(x, dtype)
+        back = q.float() * scale[:, None]
+        assert back[2].isnan().all() and back[3].isnan().all() and (back[1] == 0).all() and (back[0] - x[0]).abs().max() < 0.3
+        q, scale = quantize_rows(torch.full((1, 40), 1e-39).cuda(), dtype)
+        assert scale[0] == 0 and (q.float() == 0).all()
+    empty = torch.empty(0, 200).cuda().requires_grad_(True)
+    wl = w.clone().requires_grad_(True)
+    y = rms_norm(empty, wl)
+    de, dw = torch.autograd.grad(y, (empty, wl), torch.empty(0, 200).cuda())
+    assert y.shape == de.shape == (0, 200) and (dw == 0).all()
+    assert rms_norm_q8(empty.detach(), w)[0].shape == (0, 200)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("eight", list(TOP))
+@pytest.mark.parametrize("cols", COLS)
+def test_eight_bits(dtype, eight, cols):
+    g = torch.Generator().manual_seed(cols)
+    rows = 70 if cols > 2000 else 333
+    x, r = (torch.randn(rows, cols, generator=g).to(dtype) for _ in range(2))
+    w = 1 + 0.3 * torch.randn(cols, generator=g)
+    for residual in (False, True):
+        q, scale, *h = rms_norm_q8(x.cuda(), w.cuda(), residual=r.cuda() if residual else None, eps=1e-5, dtype=eight)
+        hd = x.double() + r.double() if residual else x.double()
+        y, _ = normed(hd, w.double(), 1e-5)
+        top = y.abs().amax(-1)
+        # a scale is a row's maximum: as exact as y in 32 bits, and one division
+        assert ((scale.cpu().double() - top / TOP[eight]).abs() <= 20 * 2.0 ** -24 * top / TOP[eight]).all()
+        if residual:
+            within(h[0], hd, UNIT[dtype], hd.abs(), "h")
+        got = q.cpu().double()
+        units = y / (top / TOP[eight])[:, None]
+        if eight is torch.int8:
+            # half a step, and what 32 bits may move a value near the middle between two
+            assert ((got - units).abs() <= 0.5 + 127 * 40 * 2.0 ** -24).all()
+        else:
+            step = torch.exp2(torch.floor(torch.log2(units.abs().clamp_min(2.0 ** -6))) - 3)
+            assert ((got - units).abs() <= 0.5 * step * (1 + 1e-4) + 448 * 40 * 2.0 ** -24).all()
+        assert got.abs().max() == TOP[eight]
+    q, scale = quantize_rows(x.cuda(), eight)
+    assert torch.equal(scale.cpu(), x.float().abs().amax(-1) / TOP[eight])
+
+
+@pytest.mark.gpu
+def test_many_rows_and_other_streams():
+    x = torch.randn(70001, 33).cuda()
+    w = torch.randn(33).cuda()
+    y, _ = normed(x.double(), w.double(), 1e-6)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = rms_norm(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    within(got, y, 2.0 ** -24, 16 * y.abs(), "side stream")
+    # one order of summation whatever else runs
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    grads = [torch.autograd.grad(rms_norm(xl, wl), wl, torch.ones_like(x))[0] for _ in range(3)]
+    assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+def test_refusals():
+    x, w = torch.randn(4, 8), torch.randn(8)
+    for call in (lambda: rms_norm(x, w), lambda: rms_norm_q8(x, w), lambda: quantize_rows(x)):
+        with pytest.raises(_lib.FgnnError):
+            call()
+    with pytest.raises(_lib.FgnnError):
+        quantize_rows(x, torch.uint8)
+    l = _lib.lib()
+    p = 256
+    assert l.fgnn_rms_norm(2, 8, 0, p, 7, None, 0, p, 0, 1e-6, None, p, None, None) == -2             # row stride below the columns
+    assert l.fgnn_rms_norm(2, 8, 3, p, 8, None, 0, p, 0, 1e-6, None, p, None, None) == -2             # 8-bit input
+    assert l.fgnn_rms_norm(2, 8, 1, p, 8, None, 0, p, 2, 1e-6, None, p, None, None) == -2             # weights of the other 16-bit type
+    assert l.fgnn_rms_norm(2, 16385, 0, p, 16385, None, 0, p, 0, 1e-6, None, p, None, None) == -4     # rows of more than 64 KB
+    assert l.fgnn_rms_norm(2, 8, 0, p, 8, p, 8, p, 0, 1e-6, None, p, None, None) == -1                # residual without h
+    assert l.fgnn_rms_norm_q8(2, 8, 0, p, 8, None, 0, p, 0, 1e-6, 0, None, p, p, None) == -2          # not an 8-bit type
+    assert l.fgnn_rms_norm_q8(2, 8, 0, p, 8, None, 0, p, 0, 1e-6, 3, None, p, None, None) == -1
+    assert l.fgnn_rms_norm_backward(2, 8, 0, p, None, p, 8, p, 0, p, p, p, None, 0, None) == -5       # no workspace
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    x, w = torch.randn(4, 8).cuda(), torch.randn(8).cuda()
+    for bad in (lambda: rms_norm(x.double(), w), lambda: rms_norm(x, w[:7]), lambda: rms_norm(x, w.half()), lambda: rms_norm(x, w, residual=x[:3]),
+                lambda: rms_norm(x, w, residual=x.half()), lambda: rms_norm(x, w.cpu()), lambda: rms_norm(x[:, :0]), lambda: rms_norm(torch.randn(2, 16385).cuda()),
+                lambda: rms_norm_q8(x, w, dtype=torch.float16), lambda: rms_norm(x[0, 0])):
+        with pytest.raises(_lib.FgnnError):
+            bad()
