@@ -10,6 +10,7 @@ template <typename T> struct fe_vec { typedef T type __attribute__((ext_vector_t
 template <typename T> constexpr int fe_width = 16 / sizeof(T);
 
 static inline int fe_size(int type) { return type == FGNN_F32 ? 4 : type == FGNN_BF16 || type == FGNN_F16 ? 2 : 1; }
+template <int TYPE> constexpr int fe_size_of = TYPE == FGNN_F32 ? 4 : TYPE == FGNN_BF16 || TYPE == FGNN_F16 ? 2 : 1;
 static inline bool fe_is_float(int type) { return type == FGNN_F32 || type == FGNN_BF16 || type == FGNN_F16; }
 static inline bool fe_is_eight(int type) { return type == FGNN_I8 || type == FGNN_E4M3; }
 // The largest value that rows are scaled to in 8 bits.
@@ -35,3 +36,6 @@ static inline void fe_dispatch(int type, Fn &&f)
     else if (type == FGNN_BF16) f.template operator()<__bf16>();
     else f.template operator()<_Float16>();
 }
+
+// out [cols], of a floating type = the column sums of part [rows, cols], added in a fixed order (fgnn_norm.hip).
+int fgnn_sum_parts(const float *part, int rows, int cols, void *out, int type, hipStream_t st);

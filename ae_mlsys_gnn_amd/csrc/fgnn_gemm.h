@@ -1,0 +1,482 @@
+// Products of dense matrices on the matrix instructions, the core of the dense operators:
+//     D[m][n] = sum_k Q(m, k) P(n, k)          rows m, columns n (contiguous in D), reduction k
+// Either operand comes with its reduction contiguous ("C": element (i, k) at p[i ld + k]) or strided ("S": at p[k ld + i]), so that a forward
+// product (C, C), the gradient of its input (P strided) and of its weights (both strided) read the matrices as they lie in memory.
+//
+// P is the first operand of the instructions: a lane ends up with four consecutive n of one m.  The four 16-row tiles of a 64-row block of P are
+// interleaved (instruction row r of tile t is n = 16 (r / 4) + 4 t + r % 4), so that a lane holds 16 consecutive n of a row: a row's 64 columns are
+// one run in memory for four lanes, as are bias and residual.
+//
+// Element kinds: 16-bit values (products of 8 significant bits and sums in 32 bits), 8-bit integers (sums in integers: exact), 8-bit floats, and
+// fp32.  fp32 operands are cut into three parts of 8 significant bits (truncated, so that the three are exact), and the six products that reach above
+// 2^-24 of the result are summed in 32 bits: the matrix unit does 16 of them in the time of one fp32 product.
+#pragma once
+#include <algorithm>
+#include "fgnn_elem.h"
+
+typedef float gm_f4 __attribute__((ext_vector_type(4)));
+typedef int gm_i4 __attribute__((ext_vector_type(4)));
+typedef short gm_s4 __attribute__((ext_vector_type(4)));
+typedef __bf16 gm_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 gm_h8 __attribute__((ext_vector_type(8)));
+
+enum { GM_NONE = 0, GM_RELU = 1, GM_GELU = 2, GM_SILU = 3, GM_LEAKY = 4 };
+
+__device__ __forceinline__ float gm_act(float z, int act, float slope)
+{
+    switch (act) {
+    case GM_RELU: return z > 0.f ? z : z == z ? 0.f : z;
+    case GM_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case GM_SILU: return z / (1.f + expf(-z));
+    case GM_LEAKY: return z > 0.f ? z : slope * z;
+    default: return z;
+    }
+}
+__device__ __forceinline__ float gm_act_slope(float z, int act, float slope)
+{
+    switch (act) {
+    case GM_RELU: return z > 0.f ? 1.f : 0.f;
+    case GM_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case GM_SILU: { const float p = 1.f / (1.f + expf(-z)); return p * (1.f + z * (1.f - p)); }
+    case GM_LEAKY: return z > 0.f ? 1.f : slope;
+    default: return 1.f;
+    }
+}
+
+// What becomes of the sums: y = act(z) + residual, z = acc sx[m] sw[n] + bias[n], in type E.
+struct GemmEpi {
+    int64_t m; int n;
+    const float *sx, *sw;                   // NULL: 1
+    const void *bias; int btype;
+    const void *res; int64_t ldr;
+    int act; float slope;
+    void *z, *y;                            // contiguous [m, n]; z NULL: not wanted
+};
+
+// W consecutive elements of a row, the first `count` of them where fewer are left.
+template <typename E, int W>
+__device__ __forceinline__ void gm_load(float (&v)[W], const E *p, int count)
+{
+    constexpr int V = fe_width<E> < W ? fe_width<E> : W;
+    typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
+    if (count >= W) {
+#pragma unroll
+        for (int j = 0; j < W / V; ++j) {
+            const vec u = *reinterpret_cast<const vec *>(p + j * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[j * V + i] = (float)u[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = i < count ? (float)p[i] : 0.f;
+    }
+}
+template <typename E, int W>
+__device__ __forceinline__ void gm_store(const float (&v)[W], E *p, int count)
+{
+    constexpr int V = fe_width<E> < W ? fe_width<E> : W;
+    typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
+    if (count >= W) {
+#pragma unroll
+        for (int j = 0; j < W / V; ++j) {
+            vec u;
+#pragma unroll
+            for (int i = 0; i < V; ++i) u[i] = (E)v[j * V + i];
+            *reinterpret_cast<vec *>(p + j * V) = u;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) if (i < count) p[i] = (E)v[i];
+    }
+}
+
+// The W columns n .. n + W - 1 that a lane works on: what does not depend on the row is read once.
+template <int W> struct GemmCols { float bias[W], sw[W]; };
+template <int W>
+__device__ __forceinline__ void gm_columns(const GemmEpi &e, int n, GemmCols<W> &c)
+{
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const int j = n + i < e.n ? n + i : e.n - 1;
+        c.bias[i] = e.bias ? fe_load(e.bias, j, e.btype) : 0.f;
+        c.sw[i] = e.sw ? e.sw[j] : 1.f;
+    }
+}
+template <typename E, int W>
+__device__ __forceinline__ void gm_finish(const GemmEpi &e, const GemmCols<W> &c, int64_t m, int n, float (&v)[W])
+{
+    const int count = e.n - n;
+    if (m >= e.m || count <= 0) return;
+    const int64_t at = m * e.n + n;
+    if (e.sx) {
+        const float s = e.sx[m];
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] *= s * c.sw[i];
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] += c.bias[i];
+    if (e.z) gm_store<E, W>(v, (E *)e.z + at, count);
+    if (e.act) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = gm_act(v[i], e.act, e.slope);
+    }
+    if (e.res) {
+        float r[W];
+        gm_load<E, W>(r, (const E *)e.res + m * e.ldr + n, count);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] += r[i];
+    }
+    gm_store<E, W>(v, (E *)e.y + at, count);
+}
+
+struct GemmP {
+    int64_t m, k;
+    int n;
+    const void *q, *p; int64_t ldq, ldp;
+    int tiles_m, tiles_n, splits;
+    int64_t slabs;                          // slabs of the reduction a split takes
+    float *part;                            // [splits][m][n] where splits > 1
+    GemmEpi epi;
+};
+
+// Workgroup w runs on XCD w % 8: every XCD gets a run of neighbouring tiles, eight rows of tiles high, so that its L2 holds what they share.
+__device__ __forceinline__ void gm_tile(const GemmP &p, int &tm, int &tn, int &split)
+{
+    const int total = (int)gridDim.x, b = (int)blockIdx.x, xcd = b % FGNN_NUM_XCD, q = total / FGNN_NUM_XCD, r = total % FGNN_NUM_XCD;
+    int t = xcd * q + min(xcd, r) + b / FGNN_NUM_XCD;
+    const int tiles = p.tiles_m * p.tiles_n;
+    split = t / tiles;
+    t -= split * tiles;
+    constexpr int HIGH = 8;
+    const int band = t / (HIGH * p.tiles_n), first = band * HIGH, high = min(HIGH, p.tiles_m - first);
+    t -= band * HIGH * p.tiles_n;
+    tm = first + t % high;
+    tn = t / high;
+}
+
+// ------------------------------------------------------------------------------------------------ element kinds
+template <int KIND> struct GemmKind {       // 16-bit values
+    static constexpr int planes = 1, slab = 64, size = 2, chunk = 8, words = 4;
+    typedef gm_f4 acc;
+};
+template <> struct GemmKind<FGNN_F32> {     // slab: reduction elements a tile; chunk: elements a thread loads at a time, as `words` registers
+    static constexpr int planes = 3, slab = 32, size = 4, chunk = 8, words = 8;
+    typedef gm_f4 acc;
+};
+template <> struct GemmKind<FGNN_I8> {
+    static constexpr int planes = 1, slab = 128, size = 1, chunk = 16, words = 4;
+    typedef gm_i4 acc;
+};
+template <> struct GemmKind<FGNN_E4M3> {    // wait in LDS as fp16, which holds them exactly: see gm_widen
+    static constexpr int planes = 1, slab = 64, size = 1, chunk = 16, words = 4;
+    typedef gm_f4 acc;
+};
+
+// LDS tile of an operand with `rows` rows (of D's rows or columns), one plane of a slab.  C: [rows][row bytes], 64 bytes a row for fp32's parts and 128
+// else; S: [slab][rows] 16-bit values.  16-byte chunks of a row are exchanged so that the lanes of one LDS pass meet different banks.
+template <int KIND> constexpr int gm_row_bytes = GemmKind<KIND>::slab *(KIND == FGNN_I8 ? 1 : 2);
+template <int KIND, bool INTERLEAVED>
+__device__ __forceinline__ int gm_at_c(int row, int chunk)
+{
+    constexpr int RB = gm_row_bytes<KIND>;
+    int f;
+    if constexpr (RB == 128) f = INTERLEAVED ? (row & 3) | ((row >> 4) & 1) << 2 : row & 7;
+    else f = INTERLEAVED ? ((row >> 1) & 1) | ((row >> 4) & 1) << 1 : (row >> 1) & 3;
+    return row * RB + ((chunk ^ f) << 4);
+}
+template <int ROWS, bool INTERLEAVED>
+__device__ __forceinline__ int gm_at_s(int k, int chunk)
+{
+    const int f = INTERLEAVED ? (k & 1) | ((k >> 1) & 1) << (ROWS >= 128 ? 3 : 2) : (k & 3) << 1;
+    return k * (ROWS * 2) + ((chunk ^ f) << 4);
+}
+
+// Operand registers of 16 rows and one instruction's reduction.
+template <int KIND, int ROWS, bool S, bool INTERLEAVED>
+__device__ __forceinline__ gm_i4 gm_operand(const char *tile, int block, int t, int step, int lane)
+{
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (!S) {
+        const int row = INTERLEAVED ? 64 * block + 16 * (r >> 2) + 4 * t + (r & 3) : 16 * t + r;
+        return *reinterpret_cast<const gm_i4 *>(tile + gm_at_c<KIND, INTERLEAVED>(row, 4 * step + g));
+    } else {
+        // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
+        const int i = INTERLEAVED ? 64 * block + 16 * (r & 3) + 4 * t : 16 * t + 4 * (r & 3);
+        const int k = 32 * step + 8 * g + (r >> 2);
+        typedef __attribute__((address_space(3))) gm_s4 *lds_p;
+        const char *a = tile + gm_at_s<ROWS, INTERLEAVED>(k, i >> 3) + ((i >> 2) & 1) * 8;
+        const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 4 * ROWS * 2));
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        const s8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return *reinterpret_cast<const gm_i4 *>(&v);
+    }
+}
+
+template <int KIND>
+__device__ __forceinline__ typename GemmKind<KIND>::acc gm_mfma(gm_i4 a, gm_i4 b, typename GemmKind<KIND>::acc c)
+{
+    if constexpr (KIND == FGNN_I8) return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+    else if constexpr (KIND == FGNN_F16 || KIND == FGNN_E4M3) return __builtin_amdgcn_mfma_f32_16x16x32_f16(*(gm_h8 *)&a, *(gm_h8 *)&b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(gm_b8 *)&a, *(gm_b8 *)&b, c, 0, 0, 0);
+}
+// One slab: a wave's 64 columns (block wp of P's tile) by 16 TQ rows (16-row tiles from tq0 on of Q's).
+template <int KIND, int BM, int BN, bool QS, bool PS, int TQ>
+__device__ __forceinline__ void gm_slab(const char *lq, const char *lp, int wp, int tq0, int lane, typename GemmKind<KIND>::acc (&acc)[TQ][4])
+{
+    constexpr int PLQ = BM * GemmKind<KIND>::slab * 2, PLP = BN * GemmKind<KIND>::slab * 2;      // bytes a plane (where there are several)
+    if constexpr (KIND == FGNN_F32) {
+        gm_i4 a[4][3];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int h = 0; h < 3; ++h) a[t][h] = gm_operand<KIND, BN, PS, true>(lp + h * PLP, wp, t, 0, lane);
+#pragma unroll
+        for (int q = 0; q < TQ; ++q) {
+            gm_i4 b[3];
+#pragma unroll
+            for (int h = 0; h < 3; ++h) b[h] = gm_operand<KIND, BM, QS, false>(lq + h * PLQ, 0, tq0 + q, 0, lane);
+            // the small products first
+#pragma unroll
+            for (int s = 2; s >= 0; --s)
+#pragma unroll
+                for (int h = 0; h <= s; ++h)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[q][t] = gm_mfma<FGNN_BF16>(a[t][s - h], b[h], acc[q][t]);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            gm_i4 a[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) a[t] = gm_operand<KIND, BN, PS, true>(lp, wp, t, s, lane);
+#pragma unroll
+            for (int q = 0; q < TQ; ++q) {
+                const gm_i4 b = gm_operand<KIND, BM, QS, false>(lq, 0, tq0 + q, s, lane);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[q][t] = gm_mfma<KIND>(a[t], b, acc[q][t]);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ operands of any alignment, through registers
+// `words` registers of CH elements, the first `valid` of them from memory and zeros after them.
+template <int KIND>
+__device__ __forceinline__ void gm_fetch(uint32_t (&w)[GemmKind<KIND>::words], const char *p, int valid)
+{
+    constexpr int CH = GemmKind<KIND>::chunk, SIZE = GemmKind<KIND>::size, W = GemmKind<KIND>::words;
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(1)));
+    if (valid >= CH) {
+#pragma unroll
+        for (int j = 0; j < W / 4; ++j) {
+            const u4 u = reinterpret_cast<const u4 *>(p)[j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[4 * j + i] = u[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (i < valid) {
+                if constexpr (SIZE == 4) w[i] = ((const uint32_t *)p)[i];
+                else if constexpr (SIZE == 2) w[i / 2] |= (uint32_t)((const uint16_t *)p)[i] << (16 * (i & 1));
+                else w[i / 4] |= (uint32_t)((const uint8_t *)p)[i] << (8 * (i & 3));
+            }
+    }
+}
+
+// Eight fp32 values as three parts of eight significant bits that add up to them exactly.
+__device__ __forceinline__ void gm_split(const uint32_t (&w)[8], gm_i4 (&part)[3])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t p[2][3];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float x = __uint_as_float(w[2 * j + i]);
+            const uint32_t hi = w[2 * j + i] & 0xffff0000u;
+            const float r1 = x - __uint_as_float(hi);           // (of an infinity or a NaN: NaN, which gm_repair sees to)
+            const uint32_t mid = __float_as_uint(r1) & 0xffff0000u;
+            const float r2 = r1 - __uint_as_float(mid);
+            p[i][0] = hi; p[i][1] = mid; p[i][2] = __float_as_uint(r2);
+        }
+#pragma unroll
+        for (int h = 0; h < 3; ++h) part[h][j] = (int)__builtin_amdgcn_perm(p[1][h], p[0][h], 0x07060302u);
+    }
+}
+
+// Sixteen 8-bit floats as fp16, exactly.  The instructions that take 8-bit floats as they are would be twice as fast, but align the products of a sum to
+// its largest with few bits below: 2^-18 of the sum of magnitudes was off for values within a factor of 32, 2^-13 over the type's whole range (2^-23 here).
+__device__ __forceinline__ void gm_widen(const uint32_t (&w)[4], gm_i4 (&half)[2])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.f, true);
+        half[i / 2][2 * (i % 2)] = *(const int *)&lo;
+        half[i / 2][2 * (i % 2) + 1] = *(const int *)&hi;
+    }
+}
+
+template <int KIND, int ROWS, bool S, int THREADS>
+struct GemmLoader {
+    static constexpr int CH = GemmKind<KIND>::chunk, SLAB = GemmKind<KIND>::slab, SIZE = GemmKind<KIND>::size, W = GemmKind<KIND>::words;
+    static constexpr int INNER = (S ? ROWS : SLAB) / CH, COUNT = ROWS * SLAB / CH / THREADS, STEP = THREADS / INNER;     // chunks a row, chunks and row step a thread
+    static_assert(THREADS % INNER == 0 && (ROWS * SLAB / CH) % THREADS == 0, "threads share a tile evenly");
+    const char *base; int64_t ld;           // ld in bytes
+    int outer, inner, rows;                 // place in the tile; rows left of the operand from the tile's first on
+    uint32_t w[COUNT][W];
+
+    __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t rows_, int64_t k0)
+    {
+        outer = (int)threadIdx.x / INNER;
+        inner = (int)threadIdx.x % INNER;
+        ld = ld_ * SIZE;
+        rows = (int)min((int64_t)ROWS, rows_ - row0);
+        base = (const char *)p + (S ? (k0 + outer) * ld + (row0 + inner * CH) * SIZE : (row0 + outer) * ld + (k0 + inner * CH) * SIZE);
+    }
+    // the slab that `base` stands at, of which `left` reduction elements exist; moves on
+    __device__ __forceinline__ void fetch(int64_t left)
+    {
+        const bool whole = rows == ROWS && left >= SLAB;
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) {
+            const int o = outer + c * STEP;
+            const char *p = base + (int64_t)c * STEP * ld;
+            int valid = CH;
+            if (!whole) {
+                if (S) valid = o < left ? rows - inner * CH : 0;
+                else valid = o < rows ? (int)min((int64_t)CH, left - inner * CH) : 0;
+            }
+            gm_fetch<KIND>(w[c], p, valid);
+        }
+        base += S ? (int64_t)SLAB * ld : (int64_t)SLAB * SIZE;
+    }
+    template <bool INTERLEAVED>
+    __device__ __forceinline__ void store(char *tile)
+    {
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) {
+            const int o = outer + c * STEP, at = S ? gm_at_s<ROWS, INTERLEAVED>(o, inner) : gm_at_c<KIND, INTERLEAVED>(o, inner);
+            if constexpr (KIND == FGNN_E4M3) {
+                gm_i4 half[2];
+                gm_widen(w[c], half);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) *reinterpret_cast<gm_i4 *>(tile + gm_at_c<KIND, INTERLEAVED>(o, 2 * inner + h)) = half[h];
+            } else if constexpr (KIND == FGNN_F32) {
+                gm_i4 part[3];
+                gm_split(w[c], part);
+#pragma unroll
+                for (int h = 0; h < 3; ++h) *reinterpret_cast<gm_i4 *>(tile + h * (ROWS * SLAB * 2) + at) = part[h];
+            } else *reinterpret_cast<gm_i4 *>(tile + at) = gm_i4{(int)w[c][0], (int)w[c][1], (int)w[c][2], (int)w[c][3]};
+        }
+    }
+};
+
+// Sums of fp32 parts that are no finite numbers, formed again by the fp32 instruction: an infinity times another operand's empty part is NaN, where the
+// product of the whole values is an infinity.  Elements of D whose sums are finite keep them.  Straight from memory: for rows that hold infinities or NaN.
+template <bool QS, bool PS, int TQ>
+__device__ __forceinline__ void gm_repair(const GemmP &p, int64_t m0, int n0, int64_t k0, int64_t k1, int lane, gm_f4 (&acc)[TQ][4])
+{
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int q = 0; q < TQ; ++q) {
+        bool bad = false;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bad |= !__builtin_isfinite(acc[q][t][j]);
+        if (__ballot(bad) == 0) continue;
+        const int64_t m = min(m0 + 16 * q + r, p.m - 1);
+        gm_f4 sum[4] = {};
+#pragma unroll 1
+        for (int64_t k = k0; k < k1; k += 4) {
+            const int64_t kk = min(k + g, k1 - 1);
+            const bool in = k + g < k1;
+            const float b = in ? ((const float *)p.q)[QS ? kk * p.ldq + m : m * p.ldq + kk] : 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int64_t n = min(n0 + 16 * (r >> 2) + 4 * t + (r & 3), p.n - 1);
+                const float a = in ? ((const float *)p.p)[PS ? kk * p.ldp + n : n * p.ldp + kk] : 0.f;
+                sum[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, sum[t], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (!__builtin_isfinite(acc[q][t][j])) acc[q][t][j] = sum[t][j];
+    }
+}
+
+// 128 x 128 tiles, four waves of 64 x 64 each.  A slab waits in registers while the one before it is multiplied out of LDS; two workgroups share a compute
+// unit, so that one multiplies while the other converts and stores.
+template <int KIND, typename E, bool QS, bool PS>
+__global__ __launch_bounds__(256, 2) void gemm_any_kernel(GemmP p)
+{
+    constexpr int BM = 128, BN = 128, SLAB = GemmKind<KIND>::slab, TQ = 4;
+    constexpr int BYTES = 128 * gm_row_bytes<KIND> * GemmKind<KIND>::planes;
+    __shared__ __attribute__((aligned(16))) char lds[2 * BYTES];
+    char *lq = lds, *lp = lds + BYTES;
+    int tm, tn, split;
+    gm_tile(p, tm, tn, split);
+    const int lane = fg_lane(), wave = fg_wave(), wp = wave & 1, tq0 = (wave >> 1) * TQ;
+    const int64_t k0 = split * p.slabs * SLAB, k1 = min(p.k, k0 + p.slabs * SLAB);
+    typename GemmKind<KIND>::acc acc[TQ][4] = {};
+    GemmLoader<KIND, BM, QS, 256> q;
+    GemmLoader<KIND, BN, PS, 256> b;
+    q.init(p.q, p.ldq, (int64_t)tm * BM, p.m, k0);
+    b.init(p.p, p.ldp, (int64_t)tn * BN, p.n, k0);
+    if (k0 < k1) {
+        q.fetch(k1 - k0);
+        b.fetch(k1 - k0);
+    }
+#pragma unroll 1
+    for (int64_t k = k0; k < k1; k += SLAB) {
+        __syncthreads();                    // the slab before has been read
+        q.template store<false>(lq);
+        b.template store<true>(lp);
+        __syncthreads();
+        if (k + SLAB < k1) {
+            q.fetch(k1 - k - SLAB);
+            b.fetch(k1 - k - SLAB);
+        }
+        gm_slab<KIND, BM, BN, QS, PS, TQ>(lq, lp, wp, tq0, lane, acc);
+    }
+    if constexpr (KIND == FGNN_F32) gm_repair<QS, PS, TQ>(p, (int64_t)tm * BM + 16 * tq0, tn * BN + 64 * wp, k0, k1, lane, acc);
+    const int n = tn * BN + 64 * wp + 16 * (lane >> 4);
+    GemmCols<16> cols;
+    if (p.splits == 1) gm_columns(p.epi, n, cols);
+#pragma unroll
+    for (int i = 0; i < TQ; ++i) {
+        const int64_t m = (int64_t)tm * BM + 16 * (tq0 + i) + (lane & 15);
+        float v[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * t + j] = (float)acc[i][t][j];
+        if (p.splits == 1) gm_finish<E, 16>(p.epi, cols, m, n, v);
+        else if (m < p.m && n < p.n) gm_store<float, 16>(v, p.part + ((int64_t)split * p.m + m) * p.n + n, p.n - n);
+    }
+}
+
+// The partial sums of a reduction cut into `splits`, added up in their order; four columns a thread.
+template <typename E>
+__global__ __launch_bounds__(256) void gemm_join_kernel(GemmP p)
+{
+    const int quads = (p.n + 3) / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / quads;
+    if (m >= p.m) return;
+    const int n = (int)(i - m * quads) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        float u[4];
+        gm_load<float, 4>(u, p.part + ((int64_t)s * p.m + m) * p.n + n, p.n - n);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += u[j];
+    }
+    GemmCols<4> cols;
+    gm_columns(p.epi, n, cols);
+    gm_finish<E, 4>(p.epi, cols, m, n, v);
+}

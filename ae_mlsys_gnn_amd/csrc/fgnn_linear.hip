@@ -1,0 +1,228 @@
+// Linear maps with bias, activation and residual in the product's epilogue, and what their gradient needs:
+//     z = x W^T + b,  y = act(z) + r;      dz = gy act'(z),  db = sum_i dz_i,  dx = dz W,  dW = dz^T x .
+// The products are those of fgnn_gemm.h.  z is kept for the backward pass in the rows' type: the slope of an activation changes by less than z itself does
+// by that rounding.
+#include "fgnn_gemm.h"
+
+// How a reduction is cut so that a small result still fills the device: two workgroups a compute unit, four slabs each at the least.
+static void gm_plan(GemmP *p, int bm, int bn, int slab, int cus)
+{
+    p->tiles_m = (int)((p->m + bm - 1) / bm);
+    p->tiles_n = (p->n + bn - 1) / bn;
+    const int64_t tiles = (int64_t)p->tiles_m * p->tiles_n, slabs = (p->k + slab - 1) / slab;
+    int64_t splits = 1;
+    if (tiles > 0 && tiles < 2 * cus) splits = std::max<int64_t>(1, std::min<int64_t>({2 * cus / tiles, slabs / 4, 256}));
+    p->slabs = std::max<int64_t>(1, (slabs + splits - 1) / splits);
+    p->splits = (int)std::max<int64_t>(1, (slabs + p->slabs - 1) / p->slabs);
+}
+static int gm_slab_of(int kind) { return kind == FGNN_F32 ? 32 : kind == FGNN_I8 ? 128 : 64; }
+static int gm_units() { const int cus = fgnn_current_device_compute_units(); return cus > 0 ? cus : 256; }
+
+template <int KIND, typename E>
+static void gm_launch_any(const GemmP &p, bool qs, bool ps, hipStream_t st)
+{
+    const dim3 g((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), b(256);
+    if constexpr (fe_size_of<KIND> == 1) hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, false>), g, b, 0, st, p);
+    else if (qs) hipLaunchKernelGGL((gemm_any_kernel<KIND, E, true, true>), g, b, 0, st, p);
+    else if (ps) hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, true>), g, b, 0, st, p);
+    else hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, false>), g, b, 0, st, p);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((gemm_join_kernel<E>), dim3((unsigned)((p.m * ((p.n + 3) / 4) + 255) / 256)), b, 0, st, p);
+}
+
+static size_t gm_workspace(int64_t m, int n, int64_t k, int kind)
+{
+    GemmP p{};
+    p.m = m; p.n = n; p.k = k;
+    gm_plan(&p, 128, 128, gm_slab_of(kind), gm_units());
+    return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
+}
+
+// D [m, n] of type `type` from operands of kind `kind`; qs: Q is strided along the reduction (and P then too).
+static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, bool ps, void *workspace, size_t workspace_bytes, hipStream_t st)
+{
+    if (p.m == 0 || p.n == 0) return 0;
+    gm_plan(&p, 128, 128, gm_slab_of(kind), gm_units());
+    FGNN_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1ll << 31) && (p.m * ((p.n + 3) / 4) + 255) / 256 < (1ll << 31), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
+    FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * p.m * p.n * sizeof(float)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
+                 workspace_bytes);
+    p.part = (float *)workspace;
+    p.epi.m = p.m; p.epi.n = p.n;
+    if (kind == FGNN_F32) gm_launch_any<FGNN_F32, float>(p, qs, ps, st);
+    else if (kind == FGNN_BF16) gm_launch_any<FGNN_BF16, __bf16>(p, qs, ps, st);
+    else if (kind == FGNN_F16) gm_launch_any<FGNN_F16, _Float16>(p, qs, ps, st);
+    else fe_dispatch(type, [&]<typename E>() {
+        if (kind == FGNN_I8) gm_launch_any<FGNN_I8, E>(p, qs, ps, st);
+        else gm_launch_any<FGNN_E4M3, E>(p, qs, ps, st);
+    });
+    return fgnn_launch_status(who);
+}
+
+static int gm_check_epilogue(const char *who, int type, const void *bias, int btype, const void *res, int64_t ldr, int n, int act)
+{
+    FGNN_REQUIRE(fe_is_float(type) && (!bias || btype == type || btype == FGNN_F32), FGNN_ERR_SHAPE, "%s: element type %d with bias of type %d", who, type, btype);
+    FGNN_REQUIRE(act >= GM_NONE && act <= GM_LEAKY, FGNN_ERR_SHAPE, "%s: activation %d", who, act);
+    FGNN_REQUIRE(!res || ldr >= n, FGNN_ERR_SHAPE, "%s: residual rows of %lld", who, (long long)ldr);
+    return 0;
+}
+
+extern "C" size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind)
+{
+    if (rows < 1 || n < 1 || k < 0 || kind < FGNN_F32 || kind > FGNN_E4M3) return 0;
+    return gm_workspace(rows, n, k, kind);
+}
+
+extern "C" int fgnn_linear(int64_t rows, int n, int k, int type, const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int btype,
+                           const void *residual, int64_t ldr, int act, float slope, void *z, void *y, void *workspace, size_t workspace_bytes, void *stream)
+{
+    FGNN_REQUIRE(rows >= 0 && n >= 0 && k >= 0 && ldx >= k && ldw >= k, FGNN_ERR_SHAPE, "fgnn_linear: bad sizes rows=%lld n=%d k=%d ldx=%lld ldw=%lld",
+                 (long long)rows, n, k, (long long)ldx, (long long)ldw);
+    const int rc = gm_check_epilogue("fgnn_linear", type, bias, btype, residual, ldr, n, act);
+    if (rc) return rc;
+    FGNN_REQUIRE(rows == 0 || n == 0 || (y && (k == 0 || (x && weight))), FGNN_ERR_NULL, "fgnn_linear: NULL argument");
+    GemmP p{};
+    p.m = rows; p.n = n; p.k = k; p.q = x; p.ldq = ldx; p.p = weight; p.ldp = ldw;
+    p.epi.bias = bias; p.epi.btype = btype; p.epi.res = residual; p.epi.ldr = ldr; p.epi.act = act; p.epi.slope = slope; p.epi.z = z; p.epi.y = y;
+    return gm_product("fgnn_linear", p, type, type, false, false, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int fgnn_linear_q8(int64_t rows, int n, int k, int eight, int type, const void *q, int64_t ldq, const float *scale, const void *weight, int64_t ldw,
+                              const float *weight_scale, const void *bias, int btype, const void *residual, int64_t ldr, int act, float slope, void *y,
+                              void *workspace, size_t workspace_bytes, void *stream)
+{
+    FGNN_REQUIRE(rows >= 0 && n >= 0 && k >= 0 && ldq >= k && ldw >= k, FGNN_ERR_SHAPE, "fgnn_linear_q8: bad sizes rows=%lld n=%d k=%d ldq=%lld ldw=%lld",
+                 (long long)rows, n, k, (long long)ldq, (long long)ldw);
+    FGNN_REQUIRE(fe_is_eight(eight), FGNN_ERR_SHAPE, "fgnn_linear_q8: operand type %d", eight);
+    FGNN_REQUIRE(eight != FGNN_I8 || k <= 131072, FGNN_ERR_LIMIT, "fgnn_linear_q8: sums of %d products of 8-bit integers do not fit 32 bits", k);
+    const int rc = gm_check_epilogue("fgnn_linear_q8", type, bias, btype, residual, ldr, n, act);
+    if (rc) return rc;
+    FGNN_REQUIRE(rows == 0 || n == 0 || (y && scale && weight_scale && (k == 0 || (q && weight))), FGNN_ERR_NULL, "fgnn_linear_q8: NULL argument");
+    GemmP p{};
+    p.m = rows; p.n = n; p.k = k; p.q = q; p.ldq = ldq; p.p = weight; p.ldp = ldw;
+    p.epi.sx = scale; p.epi.sw = weight_scale;
+    p.epi.bias = bias; p.epi.btype = btype; p.epi.res = residual; p.epi.ldr = ldr; p.epi.act = act; p.epi.slope = slope; p.epi.y = y;
+    return gm_product("fgnn_linear_q8", p, eight, type, false, false, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *weight, int64_t ldw, void *dx, void *workspace,
+                              size_t workspace_bytes, void *stream)
+{
+    FGNN_REQUIRE(rows >= 0 && n >= 0 && k >= 0 && ldz >= n && ldw >= k && fe_is_float(type), FGNN_ERR_SHAPE, "fgnn_linear_dx: bad sizes rows=%lld n=%d k=%d ldz=%lld ldw=%lld type=%d",
+                 (long long)rows, n, k, (long long)ldz, (long long)ldw, type);
+    FGNN_REQUIRE(rows == 0 || k == 0 || (dx && (n == 0 || (dz && weight))), FGNN_ERR_NULL, "fgnn_linear_dx: NULL argument");
+    GemmP p{};
+    p.m = rows; p.n = k; p.k = n; p.q = dz; p.ldq = ldz; p.p = weight; p.ldp = ldw;
+    p.epi.y = dx;
+    return gm_product("fgnn_linear_dx", p, type, type, false, true, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *x, int64_t ldx, void *dw, void *workspace,
+                              size_t workspace_bytes, void *stream)
+{
+    FGNN_REQUIRE(rows >= 0 && n >= 0 && k >= 0 && ldz >= n && ldx >= k && fe_is_float(type), FGNN_ERR_SHAPE, "fgnn_linear_dw: bad sizes rows=%lld n=%d k=%d ldz=%lld ldx=%lld type=%d",
+                 (long long)rows, n, k, (long long)ldz, (long long)ldx, type);
+    FGNN_REQUIRE(n == 0 || k == 0 || (dw && (rows == 0 || (dz && x))), FGNN_ERR_NULL, "fgnn_linear_dw: NULL argument");
+    GemmP p{};
+    p.m = n; p.n = k; p.k = rows; p.q = dz; p.ldq = ldz; p.p = x; p.ldp = ldx;
+    p.epi.y = dw;
+    return gm_product("fgnn_linear_dw", p, type, type, true, true, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type)
+{
+    if (rows < 1 || n < 1 || k < 1 || !fe_is_float(type)) return 0;
+    return std::max(gm_workspace(rows, k, n, type), gm_workspace(n, k, rows, type));
+}
+
+// ------------------------------------------------------------------------------------------------ slope and column sums
+// dz = gy act'(z) and its column sums in one pass: bound by memory.  A workgroup takes a strip of columns (TX 16-byte vectors) and every grid.y-th batch of
+// 256 / TX rows; the sums of its rows go to memory as one row of partial sums, added up in a fixed order afterwards.
+struct SlopeP {
+    int64_t rows; int n;
+    const void *gy; int64_t ldg; const void *z;
+    int act; float slope;
+    void *dz;                               // contiguous; NULL: not wanted
+    float *part;                            // [grid.y][n]; NULL: not wanted
+};
+template <typename E, int TX>
+__global__ __launch_bounds__(256) void linear_slope_kernel(SlopeP p)
+{
+    constexpr int V = fe_width<E>, TY = 256 / TX;
+    __shared__ float sums[TY > 1 ? TY : 1][TX * V];
+    const int tx = (int)threadIdx.x % TX, ty = (int)threadIdx.x / TX, c = ((int)blockIdx.x * TX + tx) * V, count = p.n - c;
+    float sum[V] = {};
+    if (count > 0) {
+        for (int64_t row = (int64_t)blockIdx.y * TY + ty; row < p.rows; row += (int64_t)gridDim.y * TY) {
+            float g[V];
+            gm_load<E, V>(g, (const E *)p.gy + row * p.ldg + c, count);
+            if (p.act) {
+                float z[V];
+                gm_load<E, V>(z, (const E *)p.z + row * p.n + c, count);
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] *= gm_act_slope(z[i], p.act, p.slope);
+            }
+            if (p.dz) gm_store<E, V>(g, (E *)p.dz + row * p.n + c, count);
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += g[i];
+        }
+    }
+    if (!p.part) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[ty][tx * V + i] = sum[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < TX * V; i += 256) {
+        const int col = (int)blockIdx.x * TX * V + i;
+        if (col >= p.n) break;
+        float v = 0.f;
+#pragma unroll
+        for (int t = 0; t < TY; ++t) v += sums[t][i];
+        p.part[(int64_t)blockIdx.y * p.n + col] = v;
+    }
+}
+
+static int sl_width(int n, int type)
+{
+    const int vectors = (n + 16 / fe_size(type) - 1) / (16 / fe_size(type));
+    return vectors <= 8 ? 8 : vectors <= 32 ? 32 : vectors <= 64 ? 64 : 256;
+}
+static dim3 sl_grid(int64_t rows, int n, int type)
+{
+    const int tx = sl_width(n, type), v = 16 / fe_size(type), strips = (n + tx * v - 1) / (tx * v), high = 256 / tx;
+    const int64_t most = std::max(1, 4 * gm_units() / strips);
+    return dim3((unsigned)strips, (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + high - 1) / high, most)));
+}
+
+extern "C" size_t fgnn_linear_slope_workspace_bytes(int64_t rows, int n, int type)
+{
+    if (rows < 1 || n < 1 || !fe_is_float(type)) return 0;
+    return (size_t)sl_grid(rows, n, type).y * n * sizeof(float);
+}
+
+extern "C" int fgnn_linear_slope(int64_t rows, int n, int type, const void *gy, int64_t ldg, const void *z, int act, float slope, void *dz, void *dbias, int btype,
+                                 void *workspace, size_t workspace_bytes, void *stream)
+{
+    FGNN_REQUIRE(rows >= 0 && n >= 1 && ldg >= n && fe_is_float(type) && act >= GM_NONE && act <= GM_LEAKY, FGNN_ERR_SHAPE,
+                 "fgnn_linear_slope: bad sizes rows=%lld n=%d ldg=%lld type=%d act=%d", (long long)rows, n, (long long)ldg, type, act);
+    FGNN_REQUIRE(!dbias || btype == type || btype == FGNN_F32, FGNN_ERR_SHAPE, "fgnn_linear_slope: bias of type %d", btype);
+    FGNN_REQUIRE(rows == 0 || (gy && (act == GM_NONE || z)), FGNN_ERR_NULL, "fgnn_linear_slope: NULL argument");
+    FGNN_REQUIRE(!dbias || rows == 0 || (workspace && workspace_bytes >= fgnn_linear_slope_workspace_bytes(rows, n, type)), FGNN_ERR_WORKSPACE,
+                 "fgnn_linear_slope: workspace of %zu bytes", workspace_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    int parts = 0;
+    if (rows > 0 && (dz || dbias)) {
+        const dim3 g = sl_grid(rows, n, type);
+        parts = (int)g.y;
+        SlopeP p{rows, n, gy, ldg, z, act, slope, dz, dbias ? (float *)workspace : nullptr};
+        fe_dispatch(type, [&]<typename E>() {
+            switch (sl_width(n, type)) {
+            case 8: hipLaunchKernelGGL((linear_slope_kernel<E, 8>), g, dim3(256), 0, st, p); break;
+            case 32: hipLaunchKernelGGL((linear_slope_kernel<E, 32>), g, dim3(256), 0, st, p); break;
+            case 64: hipLaunchKernelGGL((linear_slope_kernel<E, 64>), g, dim3(256), 0, st, p); break;
+            default: hipLaunchKernelGGL((linear_slope_kernel<E, 256>), g, dim3(256), 0, st, p);
+            }
+        });
+        const int rc = fgnn_launch_status("linear_slope_kernel");
+        if (rc) return rc;
+    }
+    return dbias ? fgnn_sum_parts((const float *)workspace, parts, n, dbias, btype, st) : 0;
+}

@@ -267,6 +267,12 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(const float *__restrict_
     }
 }
 
+int fgnn_sum_parts(const float *part, int rows, int cols, void *out, int type, hipStream_t st)
+{
+    hipLaunchKernelGGL(norm_sum_kernel, dim3((cols + 15) / 16), dim3(1024), 0, st, part, rows, cols, out, type);
+    return fgnn_launch_status("norm_sum_kernel");
+}
+
 // Threads a row and vectors a thread; columns that are no multiple of the vector take part of one.
 template <typename Fn>
 static bool nm_shape(int64_t vectors, Fn &&f)
@@ -378,9 +384,5 @@ extern "C" int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const vo
         const int launched = fgnn_launch_status("norm_backward_kernel");
         if (launched) return launched;
     }
-    if (dweight) {
-        hipLaunchKernelGGL(norm_sum_kernel, dim3((cols + 15) / 16), dim3(1024), 0, st, (const float *)workspace, parts, cols, dweight, weight ? wtype : type);
-        return fgnn_launch_status("norm_sum_kernel");
-    }
-    return 0;
+    return dweight ? fgnn_sum_parts((const float *)workspace, parts, cols, dweight, weight ? wtype : type, st) : 0;
 }

@@ -333,6 +333,31 @@ int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const void *gy, con
                            const void *weight, int wtype, const float *rstd, void *dx, void *dweight, void *workspace,
                            size_t workspace_bytes, void *stream);
 
+/* Linear maps with the epilogue in the product: y [rows, n] = act(x [rows, k] weight [n, k]^T + bias) + residual, all of one floating type (bias of
+ * that type or FGNN_F32).  act: 0 none, 1 relu, 2 gelu (by the error function), 3 silu, 4 leaky relu with `slope`.  bias, residual, z NULL: none; z
+ * receives the activation's argument for the backward pass.  y, z contiguous.  fp32 products are summed from parts of 8 significant bits, to about
+ * 2^-23 of the sum of magnitudes.
+ * _q8: operands in 8 bits (eight: FGNN_I8, k <= 131072, or FGNN_E4M3) with scale [rows] and weight_scale [n]; bias, residual and y are of type `type`.
+ * _slope: dz = gy act'(z) (NULL: not wanted) and dbias = its column sums (NULL: not wanted), summed before dz is rounded.
+ * _dx: dx [rows, k] = dz weight;  _dw: dw [n, k] = dz^T x.  All are deterministic.  Workspaces: fgnn_linear and _q8 fgnn_linear_workspace_bytes (kind: type or
+ * eight), _dx and _dw fgnn_linear_backward_workspace_bytes. */
+size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind);
+int fgnn_linear(int64_t rows, int n, int k, int type, const void *x, int64_t ldx, const void *weight, int64_t ldw,
+                const void *bias, int btype, const void *residual, int64_t ldr, int act, float slope, void *z, void *y,
+                void *workspace, size_t workspace_bytes, void *stream);
+int fgnn_linear_q8(int64_t rows, int n, int k, int eight, int type, const void *q, int64_t ldq, const float *scale,
+                   const void *weight, int64_t ldw, const float *weight_scale, const void *bias, int btype,
+                   const void *residual, int64_t ldr, int act, float slope, void *y, void *workspace,
+                   size_t workspace_bytes, void *stream);
+size_t fgnn_linear_slope_workspace_bytes(int64_t rows, int n, int type);
+int fgnn_linear_slope(int64_t rows, int n, int type, const void *gy, int64_t ldg, const void *z, int act, float slope,
+                      void *dz, void *dbias, int btype, void *workspace, size_t workspace_bytes, void *stream);
+size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type);
+int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *weight, int64_t ldw,
+                   void *dx, void *workspace, size_t workspace_bytes, void *stream);
+int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *x, int64_t ldx,
+                   void *dw, void *workspace, size_t workspace_bytes, void *stream);
+
 /* k-nearest-neighbour graph of batched point clouds, the input of fgnn_edgeconv_forward: points
  * [n_clouds*P, D]; src_ind [n_clouds*P*k] gets, for every point, the global ids of the k nearest
  * points of its own cloud (itself included), nearest first, ties to the smaller id; 1 <= k <= min(P,
