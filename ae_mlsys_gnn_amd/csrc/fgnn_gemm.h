@@ -136,6 +136,7 @@ struct GemmP {
     int tiles_m, tiles_n, splits;
     int64_t slabs;                          // slabs of the reduction a split takes
     float *part;                            // [splits][m][n] where splits > 1
+    int64_t batch_q, batch_p, plane_q, plane_p;                                // bytes between the batch's matrices, and between planes
     GemmEpi epi;
 };
 
@@ -480,3 +481,108 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmP p)
     gm_columns(p.epi, n, cols);
     gm_finish<E, 4>(p.epi, cols, m, n, v);
 }
+
+// ------------------------------------------------------------------------------------------------ aligned operands, from memory to LDS
+// Operands whose rows start at 16 bytes and hold whole 16-byte chunks go from memory to LDS without passing registers; a slab is in flight while the one
+// before it is multiplied, in the other half of LDS.
+// SEGS = 3: both operands are sums of two planes (`plane_q`, `plane_p` bytes apart); their product is hi hi + hi lo + lo hi, three slabs a
+// step of the reduction.
+template <int KIND, int ROWS, bool S, int WAVES>
+struct GemmMover {
+    static constexpr int SIZE = GemmKind<KIND>::size, SLAB = GemmKind<KIND>::slab, CH = 16 / SIZE, COUNT = ROWS * 128 / 1024 / WAVES;
+    static_assert(SLAB * SIZE == 128 && ROWS * 128 % (1024 * WAVES) == 0, "a wave moves whole kilobytes");
+    uint32_t at[COUNT];                     // of the lane's chunks, from the slab's first byte on
+    int along[COUNT];                       // their first reduction element in the slab
+    const char *base; int64_t step;
+
+    template <bool INTERLEAVED>
+    __device__ __forceinline__ void init(const void *p, int64_t ld, int64_t row0, int64_t rows, int lane, int wave)
+    {
+        const int left = (int)min((int64_t)ROWS, rows - row0);
+        base = (const char *)p + (S ? row0 : row0 * ld) * SIZE;
+        step = S ? SLAB * ld * SIZE : 128;
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) {
+            const int pos = (c * WAVES + wave) * 64 + lane;                 // 16-byte place in the LDS tile
+            if constexpr (S) {
+                constexpr int PER = ROWS / 8;
+                const int k = pos / PER, chunk = (gm_at_s<ROWS, INTERLEAVED>(k, pos % PER) - k * (ROWS * 2)) >> 4;
+                // columns past the operand's last are never stored: any of its values will do
+                at[c] = (uint32_t)(k * ld * SIZE) + 16 * min(chunk, left / CH - 1);
+                along[c] = k;
+            } else {
+                const int row = pos / 8, chunk = (gm_at_c<KIND, INTERLEAVED>(row, pos % 8) - row * 128) >> 4;
+                at[c] = (uint32_t)(min(row, left - 1) * ld * SIZE) + 16 * chunk;
+                along[c] = chunk * CH;
+            }
+        }
+    }
+    // slab `index` of a plane that starts `plane` bytes after the first; `left` reduction elements exist from its first on.  What lies past them is read
+    // as zeros: out of the buffer's range.
+    __device__ __forceinline__ void move(int64_t index, int64_t plane, int64_t left, char *tile, int wave) const
+    {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base + index * step + plane), 0, 0x80000000u, 0x00027000);
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) {
+            const uint32_t v = along[c] < left ? at[c] : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(tile + (c * WAVES + wave) * 1024), 16, v, 0, 0, 0);
+        }
+    }
+};
+
+// Waves of 64 columns by 128 rows in tiles of 256 x 256, by 64 rows in smaller ones.
+constexpr int gm_waves(int bm, int bn) { return bm * bn / 64 / (bm >= 256 ? 128 : 64); }
+template <int KIND, typename F, bool QS, bool PS, int BM, int BN, int SEGS>
+__global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(GemmP p, F f)
+{
+    constexpr int WAVES = gm_waves(BM, BN), WP = BN / 64, TQ = BM / 16 / (WAVES / WP), SLAB = GemmKind<KIND>::slab;
+    extern __shared__ __attribute__((aligned(16))) char lds[];                  // [2][BM + BN][128]
+    constexpr int HALF = (BM + BN) * 128;
+    int tm, tn, split;
+    gm_tile(p, tm, tn, split);
+    const int64_t batch = blockIdx.y;
+    const int lane = fg_lane(), wave = fg_wave(), wp = wave % WP, tq0 = wave / WP * TQ;
+    const int64_t slabs = (p.k + SLAB - 1) / SLAB * SEGS, s0 = split * p.slabs, s1 = min(slabs, s0 + p.slabs);
+    typename GemmKind<KIND>::acc acc[TQ][4] = {};
+    GemmMover<KIND, BM, QS, WAVES> q;
+    GemmMover<KIND, BN, PS, WAVES> b;
+    q.template init<false>((const char *)p.q + batch * p.batch_q, p.ldq, (int64_t)tm * BM, p.m, lane, wave);
+    b.template init<true>((const char *)p.p + batch * p.batch_p, p.ldp, (int64_t)tn * BN, p.n, lane, wave);
+    auto move = [&](int64_t s, char *to) {
+        const int64_t i = SEGS == 1 ? s : s / SEGS;
+        const int seg = SEGS == 1 ? 0 : (int)(s - i * SEGS);
+        const int64_t left = p.k - i * SLAB;
+        q.move(i, seg == 2 ? p.plane_q : 0, left, to, wave);
+        b.move(i, seg == 1 ? p.plane_p : 0, left, to + BM * 128, wave);
+    };
+    if (s0 < s1) move(s0, lds);
+#pragma unroll 1
+    for (int64_t s = s0; s < s1; ++s) {
+        char *now = lds + ((s - s0) & 1) * HALF, *next = lds + ((s - s0 + 1) & 1) * HALF;
+        __syncthreads();                    // this slab has arrived, and the one before it has been read
+        if (s + 1 < s1) move(s + 1, next);
+        gm_slab<KIND, BM, BN, QS, PS, TQ>(now, now + BM * 128, wp, tq0, lane, acc);
+    }
+    const int n = tn * BN + 64 * wp + 16 * (lane >> 4);
+    typename F::Cols cols;
+    if (p.splits == 1) f.columns(n, cols);
+#pragma unroll
+    for (int i = 0; i < TQ; ++i) {
+        const int64_t m = (int64_t)tm * BM + 16 * (tq0 + i) + (lane & 15);
+        float v[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * t + j] = (float)acc[i][t][j];
+        if (p.splits == 1) f.finish(cols, batch, m, n, v);
+        else if (m < p.m && n < p.n) gm_store<float, 16>(v, p.part + ((int64_t)split * p.m + m) * p.n + n, p.n - n);
+    }
+}
+
+template <typename E>
+struct LinearEpi {
+    GemmEpi e;
+    typedef GemmCols<16> Cols;
+    __device__ __forceinline__ void columns(int n, Cols &c) const { gm_columns(e, n, c); }
+    __device__ __forceinline__ void finish(const Cols &c, int64_t, int64_t m, int n, float (&v)[16]) const { gm_finish<E, 16>(e, c, m, n, v); }
+};

@@ -4,19 +4,28 @@
 // by that rounding.
 #include "fgnn_gemm.h"
 
-// How a reduction is cut so that a small result still fills the device: two workgroups a compute unit, four slabs each at the least.
-static void gm_plan(GemmP *p, int bm, int bn, int slab, int cus)
+static int gm_units() { const int cus = fgnn_current_device_compute_units(); return cus > 0 ? cus : 256; }
+static int gm_slab_of(int kind) { return kind == FGNN_F32 ? 32 : kind == FGNN_I8 ? 128 : 64; }
+
+// How a reduction is cut so that a small result still fills the device: two workgroups a compute unit (one of 256 x 256), four slabs each at the least.
+static void gm_cut(GemmP *p, int tile, int kind)
 {
-    p->tiles_m = (int)((p->m + bm - 1) / bm);
-    p->tiles_n = (p->n + bn - 1) / bn;
+    p->tiles_m = (int)((p->m + tile - 1) / tile);
+    p->tiles_n = (p->n + tile - 1) / tile;
+    const int slab = gm_slab_of(kind), fill = (tile == 256 ? 1 : 2) * gm_units();
     const int64_t tiles = (int64_t)p->tiles_m * p->tiles_n, slabs = (p->k + slab - 1) / slab;
     int64_t splits = 1;
-    if (tiles > 0 && tiles < 2 * cus) splits = std::max<int64_t>(1, std::min<int64_t>({2 * cus / tiles, slabs / 4, 256}));
+    if (tiles > 0 && tiles < fill) splits = std::max<int64_t>(1, std::min<int64_t>({fill / tiles, slabs / 4, 256}));
     p->slabs = std::max<int64_t>(1, (slabs + splits - 1) / splits);
     p->splits = (int)std::max<int64_t>(1, (slabs + p->slabs - 1) / p->slabs);
 }
-static int gm_slab_of(int kind) { return kind == FGNN_F32 ? 32 : kind == FGNN_I8 ? 128 : 64; }
-static int gm_units() { const int cus = fgnn_current_device_compute_units(); return cus > 0 ? cus : 256; }
+
+// Whether rows of an operand are whole 16-byte chunks at 16-byte addresses, and near enough for 32-bit offsets in a tile.
+static bool gm_movable(const void *p, int64_t ld, int64_t inner, int kind)
+{
+    const int ch = 16 / fe_size(kind);
+    return kind != FGNN_F32 && kind != FGNN_E4M3 && fgnn_aligned16(p) && ld % ch == 0 && inner % ch == 0 && inner > 0 && ld * fe_size(kind) * 256 < (1ll << 31);
+}
 
 template <int KIND, typename E>
 static void gm_launch_any(const GemmP &p, bool qs, bool ps, hipStream_t st)
@@ -26,15 +35,30 @@ static void gm_launch_any(const GemmP &p, bool qs, bool ps, hipStream_t st)
     else if (qs) hipLaunchKernelGGL((gemm_any_kernel<KIND, E, true, true>), g, b, 0, st, p);
     else if (ps) hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, true>), g, b, 0, st, p);
     else hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, false>), g, b, 0, st, p);
-    if (p.splits > 1)
-        hipLaunchKernelGGL((gemm_join_kernel<E>), dim3((unsigned)((p.m * ((p.n + 3) / 4) + 255) / 256)), b, 0, st, p);
+}
+template <int KIND, typename E, int TILE>
+static void gm_launch_moved(const GemmP &p, bool qs, bool ps, hipStream_t st)
+{
+    const dim3 g((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), b(64 * gm_waves(TILE, TILE));
+    const size_t lds = 4 * TILE * 128;
+    const LinearEpi<E> f{p.epi};
+    if constexpr (fe_size_of<KIND> == 1) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, false, TILE, TILE, 1>), g, b, lds, st, p, f);
+    else if (qs) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, true, true, TILE, TILE, 1>), g, b, lds, st, p, f);
+    else if (ps) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, true, TILE, TILE, 1>), g, b, lds, st, p, f);
+    else hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, false, TILE, TILE, 1>), g, b, lds, st, p, f);
+}
+
+// Tiles of 256 x 256 where there are enough of them for every compute unit, of 128 x 128 else.
+static int gm_tile_for(int64_t m, int n)
+{
+    return ((m + 255) / 256) * ((n + 255) / 256) >= gm_units() ? 256 : 128;
 }
 
 static size_t gm_workspace(int64_t m, int n, int64_t k, int kind)
 {
     GemmP p{};
     p.m = m; p.n = n; p.k = k;
-    gm_plan(&p, 128, 128, gm_slab_of(kind), gm_units());
+    gm_cut(&p, 128, kind);
     return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
 }
 
@@ -42,18 +66,28 @@ static size_t gm_workspace(int64_t m, int n, int64_t k, int kind)
 static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, bool ps, void *workspace, size_t workspace_bytes, hipStream_t st)
 {
     if (p.m == 0 || p.n == 0) return 0;
-    gm_plan(&p, 128, 128, gm_slab_of(kind), gm_units());
+    const bool moved = p.k > 0 && gm_movable(p.q, p.ldq, qs ? p.m : p.k, kind) && gm_movable(p.p, p.ldp, ps ? p.n : p.k, kind);
+    const int tile = moved ? gm_tile_for(p.m, p.n) : 128;
+    gm_cut(&p, tile, kind);
     FGNN_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1ll << 31) && (p.m * ((p.n + 3) / 4) + 255) / 256 < (1ll << 31), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
     FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * p.m * p.n * sizeof(float)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
                  workspace_bytes);
     p.part = (float *)workspace;
     p.epi.m = p.m; p.epi.n = p.n;
-    if (kind == FGNN_F32) gm_launch_any<FGNN_F32, float>(p, qs, ps, st);
-    else if (kind == FGNN_BF16) gm_launch_any<FGNN_BF16, __bf16>(p, qs, ps, st);
-    else if (kind == FGNN_F16) gm_launch_any<FGNN_F16, _Float16>(p, qs, ps, st);
+    auto launch = [&]<int KIND, typename E>() {
+        if constexpr (KIND != FGNN_F32 && KIND != FGNN_E4M3) {
+            if (moved && tile == 256) gm_launch_moved<KIND, E, 256>(p, qs, ps, st);
+            else if (moved) gm_launch_moved<KIND, E, 128>(p, qs, ps, st);
+            else gm_launch_any<KIND, E>(p, qs, ps, st);
+        } else gm_launch_any<KIND, E>(p, qs, ps, st);
+        if (p.splits > 1) hipLaunchKernelGGL((gemm_join_kernel<E>), dim3((unsigned)((p.m * ((p.n + 3) / 4) + 255) / 256)), dim3(256), 0, st, p);
+    };
+    if (kind == FGNN_F32) launch.template operator()<FGNN_F32, float>();
+    else if (kind == FGNN_BF16) launch.template operator()<FGNN_BF16, __bf16>();
+    else if (kind == FGNN_F16) launch.template operator()<FGNN_F16, _Float16>();
     else fe_dispatch(type, [&]<typename E>() {
-        if (kind == FGNN_I8) gm_launch_any<FGNN_I8, E>(p, qs, ps, st);
-        else gm_launch_any<FGNN_E4M3, E>(p, qs, ps, st);
+        if (kind == FGNN_I8) launch.template operator()<FGNN_I8, E>();
+        else launch.template operator()<FGNN_E4M3, E>();
     });
     return fgnn_launch_status(who);
 }
