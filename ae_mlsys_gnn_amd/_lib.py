@@ -87,6 +87,8 @@ _SIGNATURES = {
     "fgnn_linear_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "fgnn_linear_dx": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_linear_dw": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fgnn_orthogonalize_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "fgnn_orthogonalize": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_knn_graph": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "fgnn_gmm_forward_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int]),
     "fgnn_gmm_forward": (c_int, [c_int, c_int64, c_int, c_int, c_int] + [c_void_p] * 9 + [c_int]

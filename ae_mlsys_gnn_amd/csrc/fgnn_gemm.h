@@ -136,6 +136,7 @@ struct GemmP {
     int tiles_m, tiles_n, splits;
     int64_t slabs;                          // slabs of the reduction a split takes
     float *part;                            // [splits][m][n] where splits > 1
+    int64_t rows_q, rows_p;                 // rows that the operands have (more than D has where a strided one is padded to whole chunks)
     int64_t batch_q, batch_p, plane_q, plane_p;                                // bytes between the batch's matrices, and between planes
     GemmEpi epi;
 };
@@ -485,8 +486,8 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmP p)
 // ------------------------------------------------------------------------------------------------ aligned operands, from memory to LDS
 // Operands whose rows start at 16 bytes and hold whole 16-byte chunks go from memory to LDS without passing registers; a slab is in flight while the one
 // before it is multiplied, in the other half of LDS.
-// SEGS = 3: both operands are sums of two planes (`plane_q`, `plane_p` bytes apart); their product is hi hi + hi lo + lo hi, three slabs a
-// step of the reduction.
+// PLANES = 2: both operands are hi + 2^-11 lo (`plane_q`, `plane_p` bytes apart); their product is hi hi + 2^-11 (hi lo + lo hi).  The two small parts are
+// summed first, over the whole reduction, and scaled.
 template <int KIND, int ROWS, bool S, int WAVES>
 struct GemmMover {
     static constexpr int SIZE = GemmKind<KIND>::size, SLAB = GemmKind<KIND>::slab, CH = 16 / SIZE, COUNT = ROWS * 128 / 1024 / WAVES;
@@ -532,7 +533,7 @@ struct GemmMover {
 
 // Waves of 64 columns by 128 rows in tiles of 256 x 256, by 64 rows in smaller ones.
 constexpr int gm_waves(int bm, int bn) { return bm * bn / 64 / (bm >= 256 ? 128 : 64); }
-template <int KIND, typename F, bool QS, bool PS, int BM, int BN, int SEGS>
+template <int KIND, typename F, bool QS, bool PS, int BM, int BN, int PLANES>
 __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(GemmP p, F f)
 {
     constexpr int WAVES = gm_waves(BM, BN), WP = BN / 64, TQ = BM / 16 / (WAVES / WP), SLAB = GemmKind<KIND>::slab;
@@ -542,18 +543,26 @@ __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(Ge
     gm_tile(p, tm, tn, split);
     const int64_t batch = blockIdx.y;
     const int lane = fg_lane(), wave = fg_wave(), wp = wave % WP, tq0 = wave / WP * TQ;
-    const int64_t slabs = (p.k + SLAB - 1) / SLAB * SEGS, s0 = split * p.slabs, s1 = min(slabs, s0 + p.slabs);
+    const int64_t once = (p.k + SLAB - 1) / SLAB, small = PLANES == 2 ? 2 * once : 0;       // slabs of the reduction, and of the small parts
+    const int64_t s0 = split * p.slabs, s1 = min(once + small, s0 + p.slabs);
     typename GemmKind<KIND>::acc acc[TQ][4] = {};
     GemmMover<KIND, BM, QS, WAVES> q;
     GemmMover<KIND, BN, PS, WAVES> b;
-    q.template init<false>((const char *)p.q + batch * p.batch_q, p.ldq, (int64_t)tm * BM, p.m, lane, wave);
-    b.template init<true>((const char *)p.p + batch * p.batch_p, p.ldp, (int64_t)tn * BN, p.n, lane, wave);
+    q.template init<false>((const char *)p.q + batch * p.batch_q, p.ldq, (int64_t)tm * BM, p.rows_q, lane, wave);
+    b.template init<true>((const char *)p.p + batch * p.batch_p, p.ldp, (int64_t)tn * BN, p.rows_p, lane, wave);
     auto move = [&](int64_t s, char *to) {
-        const int64_t i = SEGS == 1 ? s : s / SEGS;
-        const int seg = SEGS == 1 ? 0 : (int)(s - i * SEGS);
-        const int64_t left = p.k - i * SLAB;
-        q.move(i, seg == 2 ? p.plane_q : 0, left, to, wave);
-        b.move(i, seg == 1 ? p.plane_p : 0, left, to + BM * 128, wave);
+        const bool cross = PLANES == 2 && s < small;
+        const int64_t i = cross ? s >> 1 : s - small, left = p.k - i * SLAB;
+        q.move(i, cross && (s & 1) ? p.plane_q : 0, left, to, wave);
+        b.move(i, cross && !(s & 1) ? p.plane_p : 0, left, to + BM * 128, wave);
+    };
+    auto scale = [&]() {
+        if constexpr (PLANES == 2) {
+#pragma unroll
+            for (int i = 0; i < TQ; ++i)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[i][t] *= 0x1p-11f;
+        }
     };
     if (s0 < s1) move(s0, lds);
 #pragma unroll 1
@@ -561,8 +570,10 @@ __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(Ge
         char *now = lds + ((s - s0) & 1) * HALF, *next = lds + ((s - s0 + 1) & 1) * HALF;
         __syncthreads();                    // this slab has arrived, and the one before it has been read
         if (s + 1 < s1) move(s + 1, next);
+        if (PLANES == 2 && s == small) scale();
         gm_slab<KIND, BM, BN, QS, PS, TQ>(now, now + BM * 128, wp, tq0, lane, acc);
     }
+    if (PLANES == 2 && s1 <= small) scale();
     const int n = tn * BN + 64 * wp + 16 * (lane >> 4);
     typename F::Cols cols;
     if (p.splits == 1) f.columns(n, cols);

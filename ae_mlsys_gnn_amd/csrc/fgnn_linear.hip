@@ -73,7 +73,7 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
     FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * p.m * p.n * sizeof(float)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
                  workspace_bytes);
     p.part = (float *)workspace;
-    p.epi.m = p.m; p.epi.n = p.n;
+    p.epi.m = p.rows_q = p.m; p.epi.n = (int)(p.rows_p = p.n);
     auto launch = [&]<int KIND, typename E>() {
         if constexpr (KIND != FGNN_F32 && KIND != FGNN_E4M3) {
             if (moved && tile == 256) gm_launch_moved<KIND, E, 256>(p, qs, ps, st);

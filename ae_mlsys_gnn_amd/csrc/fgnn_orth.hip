@@ -1,0 +1,241 @@
+// Orthogonalised updates of weight matrices by Newton-Schulz products: X_0 = G / (|G|_F + eps), and each step, with the side s the smaller one,
+//     A = X X^T (X^T X for a tall X),   B = b A + c A^2,   X <- a X + B X (X + X B),
+// moves every singular value by a s + b s^3 + c s^5.  4 s^2 w + 2 s^3 operations a step for s x w.
+//
+// A step multiplies rounding errors of small singular values by a (3.4 at the usual coefficients, 490 in five steps), so the products have to carry more than
+// 16-bit values do.  X, A and B are kept as two fp16 planes, 22 significant bits, and a product is hi hi + hi lo + lo hi, summed in 32 bits: three
+// instructions of the fast kind where fp32 takes sixteen.  The low plane is kept 2^11 times as large, since the instructions take subnormal operands for
+// zeros.  fp16 has no exponents to spare, so each matrix is scaled by a power of two that its largest
+// possible element allows: the singular values of X_0 are at most 1, and what a step makes of the bound is known on the host.
+#include <cmath>
+#include "fgnn_gemm.h"
+
+typedef _Float16 or_h8 __attribute__((ext_vector_type(8)));
+
+// v = hi + 2^-11 lo, to 2^-23 of v and 2^-36; nothing is left to a subnormal hi.
+__device__ __forceinline__ void or_split(float v, _Float16 &hi, _Float16 &lo)
+{
+    hi = fabsf(v) < 0x1p-14f ? (_Float16)0.f : (_Float16)v;
+    lo = (_Float16)((v - (float)hi) * 0x1p11f);
+}
+
+// One matrix of the iteration in memory: `rows` rows of `cols` columns, padded with zeros to `ld` (whole 16-byte chunks), two planes, a batch of them.
+struct OrthM { _Float16 *p; int64_t rows, ld; int cols; };
+static int64_t om_plane(const OrthM &m) { return m.rows * m.ld; }
+
+// D = alpha sums + beta C as two planes, or as values of a floating type (`out`, contiguous).
+struct OrthEpi {
+    OrthM c, d;
+    void *out; int type;
+    float alpha, beta;
+    struct Cols {};
+    __device__ __forceinline__ void columns(int, Cols &) const {}
+    __device__ __forceinline__ void finish(const Cols &, int64_t batch, int64_t m, int n, float (&v)[16]) const
+    {
+        const int64_t plane = d.rows * d.ld;
+        const int count = (out ? d.cols : (int)d.ld) - n;
+        if (m >= d.rows || count <= 0) return;
+        const int64_t at = batch * 2 * plane + m * d.ld + n;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= alpha;
+        if (beta != 0.f) {
+            float hi[16], lo[16];
+            gm_load<_Float16, 16>(hi, c.p + at, (int)d.ld - n);
+            gm_load<_Float16, 16>(lo, c.p + plane + at, (int)d.ld - n);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = fmaf(beta, fmaf(lo[i], 0x1p-11f, hi[i]), v[i]);
+        }
+        const int64_t to = (batch * d.rows + m) * d.cols + n;
+        if (out && type == FGNN_F32) gm_store<float, 16>(v, (float *)out + to, count);
+        else if (out && type == FGNN_BF16) gm_store<__bf16, 16>(v, (__bf16 *)out + to, count);
+        else if (out) gm_store<_Float16, 16>(v, (_Float16 *)out + to, count);
+        else {
+            or_h8 hi[2], lo[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                _Float16 a, b;
+                or_split(n + i < d.cols ? v[i] : 0.f, a, b);
+                hi[i / 8][i % 8] = a; lo[i / 8][i % 8] = b;
+            }
+            // (rows are whole chunks of eight)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (8 * j < count) {
+                    *reinterpret_cast<or_h8 *>(d.p + at + 8 * j) = hi[j];
+                    *reinterpret_cast<or_h8 *>(d.p + plane + at + 8 * j) = lo[j];
+                }
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ norm and planes of X_0
+#define OR_PARTS 256                        // most workgroups that share a matrix's norm
+template <typename E>
+__global__ __launch_bounds__(256) void orth_norm_kernel(const E *g, int64_t size, float *part)
+{
+    constexpr int V = fe_width<E>;
+    __shared__ float red[4];
+    g += (int64_t)blockIdx.y * size;
+    float ss = 0.f;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < size; i += (int64_t)gridDim.x * 256 * V) {
+        float v[V];
+        gm_load<E, V>(v, g + i, (int)min((int64_t)V, size - i));
+#pragma unroll
+        for (int k = 0; k < V; ++k) ss = fmaf(v[k], v[k], ss);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if (fg_lane() == 0) red[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+template <typename E>
+__global__ __launch_bounds__(256) void orth_planes_kernel(const E *g, const float *part, int parts, float eps, float scale, OrthM x)
+{
+    __shared__ float red[4];
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < parts; i += 256) ss += part[(int64_t)blockIdx.y * parts + i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if (fg_lane() == 0) red[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    const float k = scale / (sqrtf((red[0] + red[1]) + (red[2] + red[3])) + eps);
+    const int64_t plane = x.rows * x.ld, chunks = plane / 8;
+    const int per = (int)(x.ld / 8);
+    g += (int64_t)blockIdx.y * x.rows * x.cols;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per;
+        const int col = (int)(i - row * per) * 8;
+        float v[8];
+        gm_load<E, 8>(v, g + row * x.cols + col, x.cols - col);
+        or_h8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            _Float16 a, b;
+            or_split(v[j] * k, a, b);
+            hi[j] = a; lo[j] = b;
+        }
+        _Float16 *to = x.p + (int64_t)blockIdx.y * 2 * plane + row * x.ld + col;
+        *reinterpret_cast<or_h8 *>(to) = hi;
+        *reinterpret_cast<or_h8 *>(to + plane) = lo;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// The largest |a s + b s^3 + c s^5| over 0 <= s <= top.
+static double or_reach(double a, double b, double c, double top)
+{
+    auto f = [&](double s) { return std::fabs(s * (a + s * s * (b + s * s * c))); };
+    double most = f(top);
+    // where the derivative a + 3 b t + 5 c t^2 vanishes, t = s^2
+    const double disc = 9 * b * b - 20 * a * c;
+    if (c != 0 && disc >= 0) {
+        for (int sign = -1; sign <= 1; sign += 2) {
+            const double t = (-3 * b + sign * std::sqrt(disc)) / (10 * c);
+            if (t > 0 && t < top * top) most = std::max(most, f(std::sqrt(t)));
+        }
+    } else if (c == 0 && b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < top * top) most = std::max(most, f(std::sqrt(-a / (3 * b))));
+    return most;
+}
+// The largest |b t + c t^2| over 0 <= t <= top.
+static double or_reach_b(double b, double c, double top)
+{
+    double most = std::fabs(top * (b + c * top));
+    const double t = c != 0 ? -b / (2 * c) : -1;
+    if (t > 0 && t < top) most = std::max(most, std::fabs(t * (b + c * t)));
+    return most;
+}
+// The power of two that leaves elements of at most `bound` a factor of two below fp16's largest value.
+static float or_scale(double bound) { return bound > 0 ? (float)std::exp2(std::floor(std::log2(32752.0 / bound))) : 1.f; }
+
+struct OrthShape { int64_t small, wide, ld_x, ld_s; bool tall; int parts; };
+static OrthShape or_shape(int64_t m, int64_t n)
+{
+    OrthShape s{std::min(m, n), std::max(m, n), (n + 7) / 8 * 8, (std::min(m, n) + 7) / 8 * 8, m > n, 0};
+    s.parts = (int)std::min<int64_t>(OR_PARTS, (m * n + 8191) / 8192);
+    return s;
+}
+
+extern "C" size_t fgnn_orthogonalize_workspace_bytes(int batch, int m, int n)
+{
+    if (batch < 1 || m < 1 || n < 1) return 0;
+    const OrthShape s = or_shape(m, n);
+    return (size_t)batch * ((size_t)s.parts * sizeof(float) + 2 * 2 * sizeof(_Float16) * ((size_t)m * s.ld_x + (size_t)s.small * s.ld_s)) + 5 * 256;
+}
+
+template <bool QS, bool PS>
+static void or_product(GemmP p, const OrthEpi &f, int batch, hipStream_t st)
+{
+    p.splits = 1;
+    p.slabs = (p.k + 63) / 64 * 3;
+    auto go = [&]<int TILE>() {
+        p.tiles_m = (int)((p.m + TILE - 1) / TILE);
+        p.tiles_n = (p.n + TILE - 1) / TILE;
+        hipLaunchKernelGGL((gemm_moved_kernel<FGNN_F16, OrthEpi, QS, PS, TILE, TILE, 2>), dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)batch),
+                           dim3(64 * gm_waves(TILE, TILE)), 4 * TILE * 128, st, p, f);
+    };
+    const int cus = fgnn_current_device_compute_units();
+    if (((p.m + 255) / 256) * ((p.n + 255) / 256) * batch >= (cus > 0 ? cus : 256)) go.template operator()<256>();
+    else go.template operator()<128>();
+}
+
+static GemmP or_operands(const OrthM &q, bool qs, const OrthM &p, bool ps, int64_t m, int n, int64_t k)
+{
+    GemmP g{};
+    g.m = m; g.n = n; g.k = k;
+    g.q = q.p; g.ldq = q.ld; g.rows_q = qs ? (m + 7) / 8 * 8 : m; g.plane_q = om_plane(q) * 2; g.batch_q = 2 * g.plane_q;
+    g.p = p.p; g.ldp = p.ld; g.rows_p = ps ? (n + 7) / 8 * 8 : n; g.plane_p = om_plane(p) * 2; g.batch_p = 2 * g.plane_p;
+    return g;
+}
+
+extern "C" int fgnn_orthogonalize(int batch, int m, int n, int type, const void *g, int steps, const float *coefficients, float eps, void *out, void *workspace,
+                                  size_t workspace_bytes, void *stream)
+{
+    FGNN_REQUIRE(batch >= 0 && m >= 0 && n >= 0 && steps >= 1 && fe_is_float(type), FGNN_ERR_SHAPE, "fgnn_orthogonalize: bad sizes batch=%d m=%d n=%d steps=%d type=%d", batch, m, n,
+                 steps, type);
+    FGNN_REQUIRE(batch <= 65535 && std::max(m, n) <= (1 << 21), FGNN_ERR_LIMIT, "fgnn_orthogonalize: more than 65535 matrices, or a side of more than 2 M (%d, %d x %d)", batch, m, n);
+    if (batch == 0 || m == 0 || n == 0) return 0;
+    FGNN_REQUIRE(g && out && coefficients, FGNN_ERR_NULL, "fgnn_orthogonalize: NULL argument");
+    FGNN_REQUIRE(workspace && workspace_bytes >= fgnn_orthogonalize_workspace_bytes(batch, m, n), FGNN_ERR_WORKSPACE, "fgnn_orthogonalize: workspace of %zu bytes", workspace_bytes);
+    double reach = 1.001;
+    for (int i = 0; i < steps; ++i) {
+        const float *c = coefficients + 3 * i;
+        reach = or_reach(c[0], c[1], c[2], reach) * 1.001;
+        FGNN_REQUIRE(reach < 100.0, FGNN_ERR_LIMIT, "fgnn_orthogonalize: the coefficients take a singular value to %g in step %d", reach, i + 1);
+    }
+    const OrthShape s = or_shape(m, n);
+    hipStream_t st = (hipStream_t)stream;
+    char *at = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+    auto take = [&](size_t bytes) { char *p = at; at += fgnn_align256(bytes); return p; };
+    auto matrix = [&](int64_t rows, int cols, int64_t ld) { return OrthM{(_Float16 *)take((size_t)batch * 2 * rows * ld * sizeof(_Float16)), rows, ld, cols}; };
+    OrthM x = matrix(m, n, s.ld_x), y = matrix(m, n, s.ld_x), a = matrix(s.small, (int)s.small, s.ld_s), b = matrix(s.small, (int)s.small, s.ld_s);
+    float *part = (float *)take((size_t)batch * s.parts * sizeof(float));
+
+    double top = 1.001;
+    float sx = or_scale(top);
+    fe_dispatch(type, [&]<typename E>() {
+        hipLaunchKernelGGL((orth_norm_kernel<E>), dim3(s.parts, batch), dim3(256), 0, st, (const E *)g, (int64_t)m * n, part);
+        const unsigned blocks = (unsigned)std::min<int64_t>((om_plane(x) / 8 + 255) / 256, 4096);
+        hipLaunchKernelGGL((orth_planes_kernel<E>), dim3(blocks, batch), dim3(256), 0, st, (const E *)g, (const float *)part, s.parts, eps, sx, x);
+    });
+    for (int i = 0; i < steps; ++i) {
+        const float *c = coefficients + 3 * i;
+        const float sa = or_scale(top * top), sb = or_scale(or_reach_b(c[1], c[2], top * top));
+        top = or_reach(c[0], c[1], c[2], top) * 1.001;
+        const float sy = or_scale(top);
+        const int small = (int)s.small;
+        OrthEpi f{{}, a, nullptr, type, sa / (sx * sx), 0.f};
+        if (s.tall) or_product<true, true>(or_operands(x, true, x, true, small, small, m), f, batch, st);
+        else or_product<false, false>(or_operands(x, false, x, false, small, small, s.ld_x), f, batch, st);
+        f = OrthEpi{a, b, nullptr, type, sb * c[2] / (sa * sa), sb * c[1] / sa};
+        or_product<false, false>(or_operands(a, false, a, false, small, small, s.ld_s), f, batch, st);
+        const bool last = i == steps - 1;
+        f = OrthEpi{x, y, last ? out : nullptr, type, (last ? 1.f : sy) / (sb * sx), (last ? 1.f : sy) * c[0] / sx};
+        if (s.tall) or_product<false, false>(or_operands(x, false, b, false, m, small, s.ld_s), f, batch, st);
+        else or_product<false, true>(or_operands(b, false, x, true, small, n, small), f, batch, st);
+        std::swap(x, y);
+        sx = sy;
+    }
+    return fgnn_launch_status("gemm_moved_kernel");
+}

@@ -11,6 +11,7 @@ from .fused_gmmconv import (GaussianCp, GaussianFunction, GmmConvFuse, GmmConvFu
 from .knn import knn_graph  # noqa: F401
 from .linear import LinearActFunction, linear_act, linear_q8  # noqa: F401
 from .mhspmm import MHSPMMFunction, csrmhspmm, mhsddmm, mhtranspose  # noqa: F401
+from .newton_schulz import orthogonalize  # noqa: F401
 from .norm import RMSNormFunction, quantize_rows, rms_norm, rms_norm_q8  # noqa: F401
 from .sddmm import coo_sddmm, csr_sddmm  # noqa: F401
 from .spmm import SPMMFunction, csrspmm  # noqa: F401

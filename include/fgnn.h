@@ -358,6 +358,13 @@ int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *dz, int64_t
 int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *x, int64_t ldx,
                    void *dw, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Orthogonalised updates of `batch` weight matrices g [m, n] (contiguous, fp32, bf16 or fp16; out of the same type): X = g / (|g| + eps) by the Frobenius
+ * norm, then `steps` times X <- a X + (b A + c A^2) X with A = X X^T (X (b A + c A^2) with A = X^T X where m > n); coefficients [steps][3] = a, b, c on
+ * the HOST.  Products carry 22 significant bits and are summed in 32.  Coefficients that take a singular value of [0, 1] past 100 are refused. */
+size_t fgnn_orthogonalize_workspace_bytes(int batch, int m, int n);
+int fgnn_orthogonalize(int batch, int m, int n, int type, const void *g, int steps, const float *coefficients, float eps,
+                       void *out, void *workspace, size_t workspace_bytes, void *stream);
+
 /* k-nearest-neighbour graph of batched point clouds, the input of fgnn_edgeconv_forward: points
  * [n_clouds*P, D]; src_ind [n_clouds*P*k] gets, for every point, the global ids of the k nearest
  * points of its own cloud (itself included), nearest first, ties to the smaller id; 1 <= k <= min(P,
