@@ -597,3 +597,115 @@ struct LinearEpi {
     __device__ __forceinline__ void columns(int n, Cols &c) const { gm_columns(e, n, c); }
     __device__ __forceinline__ void finish(const Cols &c, int64_t, int64_t m, int n, float (&v)[16]) const { gm_finish<E, 16>(e, c, m, n, v); }
 };
+
+// ------------------------------------------------------------------------------------------------ few rows
+// Products of at most 16 RT rows, bound by reading P once: a workgroup takes 16 CT columns of D, its waves share the reduction (blocks of four instructions' worth,
+// 256 bytes of a row, dealt out in turn) and add up their sums in LDS.  Nothing is staged: a lane's 16 bytes of a row of P are its operand.
+template <int KIND>
+__device__ __forceinline__ void gm_rows_mfma(gm_i4 a, gm_i4 b, typename GemmKind<KIND>::acc &c)
+{
+    if constexpr (KIND == FGNN_F32) {
+        const gm_f4 x = *(const gm_f4 *)&a, y = *(const gm_f4 *)&b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    } else if constexpr (KIND == FGNN_E4M3) {
+        gm_i4 x[2], y[2];
+        gm_widen(*(const uint32_t(*)[4])&a, x);
+        gm_widen(*(const uint32_t(*)[4])&b, y);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) c = gm_mfma<FGNN_F16>(x[j], y[j], c);
+    } else c = gm_mfma<KIND>(a, b, c);
+}
+// 16 bytes at element k of a row of `left` + k elements, zeros past its end
+template <int KIND>
+__device__ __forceinline__ gm_i4 gm_rows_load(const char *p, int64_t left)
+{
+    constexpr int CH = 16 / GemmKind<KIND>::size;
+    typedef int i4 __attribute__((ext_vector_type(4), aligned(1)));
+    if (left >= CH) return *reinterpret_cast<const i4 *>(p);
+    gm_i4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+        if (i < left) {
+            if constexpr (CH == 4) v[i] = ((const int *)p)[i];
+            else if constexpr (CH == 8) v[i / 2] |= (int)((const uint16_t *)p)[i] << (16 * (i & 1));
+            else v[i / 4] |= (int)((const uint8_t *)p)[i] << (8 * (i & 3));
+        }
+    return v;
+}
+
+#define GR_WAVES 8                          // most waves of a workgroup
+template <int KIND, typename E, int RT, int CT>
+__global__ __launch_bounds__(64 * GR_WAVES) void gemm_rows_kernel(GemmP p)
+{
+    constexpr int SIZE = GemmKind<KIND>::size, CH = 16 / SIZE, BLOCK = 256 / SIZE;
+    typedef int i4 __attribute__((ext_vector_type(4), aligned(1)));
+    typedef typename GemmKind<KIND>::acc acc_t;
+    extern __shared__ __attribute__((aligned(16))) char lds[];                  // [waves][RT][CT][64] sums
+    const int lane = fg_lane(), wave = fg_wave(), waves = (int)blockDim.x >> 6, r = lane & 15, g = lane >> 4, n0 = (int)blockIdx.x * 16 * CT;
+    const char *w[CT], *x[RT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) w[c] = (const char *)p.p + (int64_t)min(n0 + 16 * c + r, p.n - 1) * p.ldp * SIZE + 16 * g;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) x[t] = (const char *)p.q + min((int64_t)(16 * t + r), p.m - 1) * p.ldq * SIZE + 16 * g;
+    acc_t acc[RT][CT] = {};
+    const int64_t blocks = (p.k + BLOCK - 1) / BLOCK, whole = p.k / BLOCK;
+    gm_i4 a[CT][4], b[RT][4];
+    auto load = [&](int64_t blk) {
+        const int64_t at = blk * 256;
+        if (blk < whole) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) a[c][s] = *reinterpret_cast<const i4 *>(w[c] + at + 64 * s);
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) b[t][s] = *reinterpret_cast<const i4 *>(x[t] + at + 64 * s);
+        } else {
+            const int64_t left = p.k - blk * BLOCK - CH * g;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int c = 0; c < CT; ++c) a[c][s] = gm_rows_load<KIND>(w[c] + at + 64 * s, left - 4 * CH * s);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) b[t][s] = gm_rows_load<KIND>(x[t] + at + 64 * s, left - 4 * CH * s);
+            }
+        }
+    };
+    int64_t blk = wave;
+    if (blk < blocks) load(blk);
+#pragma unroll 1
+    for (; blk < blocks; blk += waves) {
+        gm_i4 c[CT][4], d[RT][4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int i = 0; i < CT; ++i) c[i][s] = a[i][s];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) d[t][s] = b[t][s];
+        }
+        if (blk + waves < blocks) load(blk + waves);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int i = 0; i < CT; ++i) gm_rows_mfma<KIND>(c[i][s], d[t][s], acc[t][i]);
+    }
+    acc_t *sums = (acc_t *)lds;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < CT; ++i) sums[((wave * RT + t) * CT + i) * 64 + lane] = acc[t][i];
+    __syncthreads();
+    for (int j = wave; j < RT * CT; j += waves) {
+        acc_t s = sums[j * 64 + lane];
+        for (int i = 1; i < waves; ++i) s += sums[(i * RT * CT + j) * 64 + lane];
+        const int n = n0 + 16 * (j % CT) + 4 * g;
+        GemmCols<4> cols;
+        gm_columns(p.epi, min(n, p.n - 1), cols);
+        float v[4] = {(float)s[0], (float)s[1], (float)s[2], (float)s[3]};
+        gm_finish<E, 4>(p.epi, cols, 16 * (j / CT) + r, n, v);
+    }
+}

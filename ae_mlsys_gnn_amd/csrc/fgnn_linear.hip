@@ -48,14 +48,45 @@ static void gm_launch_moved(const GemmP &p, bool qs, bool ps, hipStream_t st)
     else hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, false, TILE, TILE, 1>), g, b, lds, st, p, f);
 }
 
+// Column tiles of a workgroup of the kernel for few rows: two where every compute unit still gets one, and more than 16 rows make it worth reading x half as
+// often (4096 -> 8192 bf16, 32 rows 24 / 18 us, 64 rows 38 / 26; 16 rows 17.0 / 16.8, one row 12.7 / 15.9; 8192 -> 4096 32 rows 24 / 31).
+static int gm_rows_ct(int64_t m, int n) { return m > 16 && n >= 32 * gm_units() ? 2 : 1; }
+// Whether that kernel is taken.  It reads the rows again for every 16 or 32 columns, where the tiles read them once a 128 and join a cut reduction: us,
+// it / tiles, 16 rows 8192 -> 4096 bf16 17.4 / 19.0, 8-bit integers 10.4 / 15.1, 1024 -> 1024 4.1 / 8.0; with 67 MB read again 18.3 / 19.3, with 134 MB 24.2 / 21.3
+// and 26.0 / 23.2.  The tiles that convert their operands are slower: with 134 MB 21.4 / 26.4 (8-bit floats), 268 MB 47 / 54 and 51 / 53, 536 MB 75 / 56 (fp32).
+static bool gm_few(const GemmP &p, int kind, bool moved)
+{
+    const int64_t again = (p.m + 15) / 16 * p.k * p.n * fe_size(kind) / gm_rows_ct(p.m, p.n);
+    return p.m <= 16 || (p.m <= 64 && again <= (moved ? 100000000 : 300000000));
+}
+template <int KIND, typename E>
+static void gm_launch_rows(const GemmP &p, hipStream_t st)
+{
+    const int64_t blocks = (p.k * GemmKind<KIND>::size + 255) / 256;
+    auto go = [&]<int RT, int CT>() {
+        // eight waves a compute unit, and as many a workgroup as that takes (4096 -> 8192, 512 groups, 4 / 8 waves 12.7 / 13.5 us; 8192 -> 4096 in 8 bits, 256
+        // groups, 8.7 / 8.4)
+        const int64_t groups = (p.n + 16 * CT - 1) / (16 * CT);
+        const int waves = (int)std::max<int64_t>(1, std::min<int64_t>(2 * groups > 3 * gm_units() ? 4 : 8, blocks));
+        hipLaunchKernelGGL((gemm_rows_kernel<KIND, E, RT, CT>), dim3((unsigned)groups), dim3(64 * waves), (size_t)waves * RT * CT * 1024, st, p);
+    };
+    const int ct = gm_rows_ct(p.m, p.n);
+    if (p.m <= 16) go.template operator()<1, 1>();
+    else if (p.m <= 32 && ct == 1) go.template operator()<2, 1>();
+    else if (p.m <= 32) go.template operator()<2, 2>();
+    else if (ct == 1) go.template operator()<4, 1>();
+    else go.template operator()<4, 2>();
+}
+
 // Tiles of 256 x 256 where there are enough of them for every compute unit, of 128 x 128 else.
 static int gm_tile_for(int64_t m, int n)
 {
     return ((m + 255) / 256) * ((n + 255) / 256) >= gm_units() ? 256 : 128;
 }
 
-static size_t gm_workspace(int64_t m, int n, int64_t k, int kind)
+static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool strided)
 {
+    if (m <= 16 && !strided) return 0;
     GemmP p{};
     p.m = m; p.n = n; p.k = k;
     gm_cut(&p, 128, kind);
@@ -67,14 +98,17 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
 {
     if (p.m == 0 || p.n == 0) return 0;
     const bool moved = p.k > 0 && gm_movable(p.q, p.ldq, qs ? p.m : p.k, kind) && gm_movable(p.p, p.ldp, ps ? p.n : p.k, kind);
+    const bool few = !qs && !ps && gm_few(p, kind, moved);
     const int tile = moved ? gm_tile_for(p.m, p.n) : 128;
     gm_cut(&p, tile, kind);
+    if (few) p.splits = 1;
     FGNN_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1ll << 31) && (p.m * ((p.n + 3) / 4) + 255) / 256 < (1ll << 31), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
     FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * p.m * p.n * sizeof(float)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
                  workspace_bytes);
     p.part = (float *)workspace;
     p.epi.m = p.rows_q = p.m; p.epi.n = (int)(p.rows_p = p.n);
     auto launch = [&]<int KIND, typename E>() {
+        if (few) return gm_launch_rows<KIND, E>(p, st);
         if constexpr (KIND != FGNN_F32 && KIND != FGNN_E4M3) {
             if (moved && tile == 256) gm_launch_moved<KIND, E, 256>(p, qs, ps, st);
             else if (moved) gm_launch_moved<KIND, E, 128>(p, qs, ps, st);
@@ -103,7 +137,7 @@ static int gm_check_epilogue(const char *who, int type, const void *bias, int bt
 extern "C" size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind)
 {
     if (rows < 1 || n < 1 || k < 0 || kind < FGNN_F32 || kind > FGNN_E4M3) return 0;
-    return gm_workspace(rows, n, k, kind);
+    return gm_workspace(rows, n, k, kind, false);
 }
 
 extern "C" int fgnn_linear(int64_t rows, int n, int k, int type, const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int btype,
@@ -165,7 +199,7 @@ extern "C" int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *
 extern "C" size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type)
 {
     if (rows < 1 || n < 1 || k < 1 || !fe_is_float(type)) return 0;
-    return std::max(gm_workspace(rows, k, n, type), gm_workspace(n, k, rows, type));
+    return std::max(gm_workspace(rows, k, n, type, true), gm_workspace(n, k, rows, type, true));
 }
 
 // ------------------------------------------------------------------------------------------------ slope and column sums

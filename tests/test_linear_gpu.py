@@ -99,6 +99,15 @@ def test_larger_products(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65])
+def test_few_rows(dtype, rows):
+    # either side of every number of row tiles; columns in one tile and two a workgroup; reductions shorter and longer than a block of every wave
+    for k, n in ((20, 40), (700, 100), (2100, 33), (130, 8200)):
+        check_all(rows, k, n, dtype, "relu")
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     x, w, b, r, gy = operands(9, 12, 10, torch.float32)
     for name in (None, "gelu", "silu", "leaky_relu"):
@@ -262,8 +271,8 @@ def test_refusals():
     assert l.fgnn_linear_q8(2, 6, 8, 1, 1, p, 8, p, p, 8, p, None, 1, None, 0, 0, 0.0, p, None, 0, None) == -2
     assert l.fgnn_linear_slope(2, 6, 0, p, 6, None, 1, 0.0, p, None, 0, None, 0, None) == -1                     # an activation without its argument
     assert l.fgnn_linear_slope(2, 6, 0, p, 6, p, 1, 0.0, p, p, 0, None, 0, None) == -5                           # no workspace for the sums
-    big = l.fgnn_linear_workspace_bytes(1, 16, 100000, 1)
-    assert big > 0 and l.fgnn_linear(1, 16, 100000, 1, p, 100000, p, 100000, None, 0, None, 0, 0, 0.0, None, p, p, big - 4, None) == -5
+    big = l.fgnn_linear_workspace_bytes(100, 16, 100000, 1)
+    assert big > 0 and l.fgnn_linear(100, 16, 100000, 1, p, 100000, p, 100000, None, 0, None, 0, 0, 0.0, None, p, p, big - 4, None) == -5
 
 
 @pytest.mark.gpu
