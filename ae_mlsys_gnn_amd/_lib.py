@@ -190,23 +190,20 @@ def stream_ptr():
     return c_void_p(torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(_current_device()))
 
 
-# Element types of the dense operators (FGNN_F32 and following in include/fgnn.h).
-FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-EIGHT_TYPES = {torch.int8: 3, torch.float8_e4m3fn: 4}
+_dense = None
 
 
-def rows_of(t, what):
-    """(t as [rows, columns] with unit column stride, its row stride); copied only where no view of that kind exists."""
-    if t.dim() == 0:
-        raise FgnnError("%s: no dimension of features" % what)
-    cols = t.shape[-1]
-    if t.dim() != 2:
-        t = t.reshape(-1, cols) if cols else t.reshape(t.shape[:-1].numel(), 0)
-    rows, step = t.shape[0], t.stride(0)
-    if cols > 1 and t.stride(1) != 1 or rows > 1 and step < cols:
-        t = t.contiguous()
-        step = cols
-    return t, step if rows > 1 else cols
+def dense():
+    """The dense operators' host side (csrc/fgnn_dense.cpp), which calls the same library; raises when it has not been built."""
+    global _dense
+    if _dense is None:
+        lib()
+        try:
+            from . import _dense as module
+        except ImportError as e:
+            raise FgnnError("_dense.so cannot be loaded from %s; build it with `python -m ae_mlsys_gnn_amd.build`: %s" % (_HERE, e)) from e
+        _dense = module
+    return _dense
 
 
 def require_cuda(*tensors):

@@ -9,10 +9,10 @@ from .fused_gat import (FusedGATFunction, FusedGATFunction_SM, FusedGATFunction_
 from .fused_gmmconv import (GaussianCp, GaussianFunction, GmmConvFuse, GmmConvFuseEb, GmmConvFuseSum, GmmConvStash,  # noqa: F401
                             GmmFuseEbFunction, GmmFuseFunction, GmmStashFunction)
 from .knn import knn_graph  # noqa: F401
-from .linear import LinearActFunction, linear_act, linear_q8  # noqa: F401
+from .linear import linear_act, linear_q8  # noqa: F401
 from .mhspmm import MHSPMMFunction, csrmhspmm, mhsddmm, mhtranspose  # noqa: F401
 from .newton_schulz import orthogonalize  # noqa: F401
-from .norm import RMSNormFunction, quantize_rows, rms_norm, rms_norm_q8  # noqa: F401
+from .norm import quantize_rows, rms_norm, rms_norm_q8  # noqa: F401
 from .sddmm import coo_sddmm, csr_sddmm  # noqa: F401
 from .spmm import SPMMFunction, csrspmm  # noqa: F401
 from .u_add_v import u_add_v_Function, u_add_v_op  # noqa: F401

@@ -287,3 +287,11 @@ def test_refusals_on_the_device():
                 lambda: linear_q8(q, s, wq, ws, dtype=torch.float64), lambda: linear_q8(q, s, wq, ws, b.half()), lambda: linear_q8(q, s, wq[:, :4], ws)):
         with pytest.raises(_lib.FgnnError):
             bad()
+
+
+@pytest.mark.gpu
+def test_second_order_gradients_are_refused():
+    x, w = torch.randn(4, 8).cuda().requires_grad_(True), torch.randn(6, 8).cuda().requires_grad_(True)
+    (dx,) = torch.autograd.grad(linear_act(x, w, activation="gelu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second order"):
+        dx.sum().backward()
