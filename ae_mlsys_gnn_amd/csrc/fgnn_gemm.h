@@ -177,10 +177,9 @@ template <> struct GemmKind<FGNN_E4M3> {    // wait in LDS as fp16, which holds 
 // LDS tile of an operand with `rows` rows (of D's rows or columns), one plane of a slab.  C: [rows][row bytes], 64 bytes a row for fp32's parts and 128
 // else; S: [slab][rows] 16-bit values.  16-byte chunks of a row are exchanged so that the lanes of one LDS pass meet different banks.
 template <int KIND> constexpr int gm_row_bytes = GemmKind<KIND>::slab *(KIND == FGNN_I8 ? 1 : 2);
-template <int KIND, bool INTERLEAVED>
+template <int RB, bool INTERLEAVED>
 __device__ __forceinline__ int gm_at_c(int row, int chunk)
 {
-    constexpr int RB = gm_row_bytes<KIND>;
     int f;
     if constexpr (RB == 128) f = INTERLEAVED ? (row & 3) | ((row >> 4) & 1) << 2 : row & 7;
     else f = INTERLEAVED ? ((row >> 1) & 1) | ((row >> 4) & 1) << 1 : (row >> 1) & 3;
@@ -194,13 +193,13 @@ __device__ __forceinline__ int gm_at_s(int k, int chunk)
 }
 
 // Operand registers of 16 rows and one instruction's reduction.
-template <int KIND, int ROWS, bool S, bool INTERLEAVED>
+template <int RB, int ROWS, bool S, bool INTERLEAVED>
 __device__ __forceinline__ gm_i4 gm_operand(const char *tile, int block, int t, int step, int lane)
 {
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!S) {
         const int row = INTERLEAVED ? 64 * block + 16 * (r >> 2) + 4 * t + (r & 3) : 16 * t + r;
-        return *reinterpret_cast<const gm_i4 *>(tile + gm_at_c<KIND, INTERLEAVED>(row, 4 * step + g));
+        return *reinterpret_cast<const gm_i4 *>(tile + gm_at_c<RB, INTERLEAVED>(row, 4 * step + g));
     } else {
         // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
         const int i = INTERLEAVED ? 64 * block + 16 * (r & 3) + 4 * t : 16 * t + 4 * (r & 3);
@@ -231,12 +230,12 @@ __device__ __forceinline__ void gm_slab(const char *lq, const char *lp, int wp, 
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int h = 0; h < 3; ++h) a[t][h] = gm_operand<KIND, BN, PS, true>(lp + h * PLP, wp, t, 0, lane);
+            for (int h = 0; h < 3; ++h) a[t][h] = gm_operand<gm_row_bytes<KIND>, BN, PS, true>(lp + h * PLP, wp, t, 0, lane);
 #pragma unroll
         for (int q = 0; q < TQ; ++q) {
             gm_i4 b[3];
 #pragma unroll
-            for (int h = 0; h < 3; ++h) b[h] = gm_operand<KIND, BM, QS, false>(lq + h * PLQ, 0, tq0 + q, 0, lane);
+            for (int h = 0; h < 3; ++h) b[h] = gm_operand<gm_row_bytes<KIND>, BM, QS, false>(lq + h * PLQ, 0, tq0 + q, 0, lane);
             // the small products first
 #pragma unroll
             for (int s = 2; s >= 0; --s)
@@ -250,10 +249,10 @@ __device__ __forceinline__ void gm_slab(const char *lq, const char *lp, int wp, 
         for (int s = 0; s < 2; ++s) {
             gm_i4 a[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) a[t] = gm_operand<KIND, BN, PS, true>(lp, wp, t, s, lane);
+            for (int t = 0; t < 4; ++t) a[t] = gm_operand<gm_row_bytes<KIND>, BN, PS, true>(lp, wp, t, s, lane);
 #pragma unroll
             for (int q = 0; q < TQ; ++q) {
-                const gm_i4 b = gm_operand<KIND, BM, QS, false>(lq, 0, tq0 + q, s, lane);
+                const gm_i4 b = gm_operand<gm_row_bytes<KIND>, BM, QS, false>(lq, 0, tq0 + q, s, lane);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) acc[q][t] = gm_mfma<KIND>(a[t], b, acc[q][t]);
             }
@@ -360,12 +359,12 @@ struct GemmLoader {
     {
 #pragma unroll
         for (int c = 0; c < COUNT; ++c) {
-            const int o = outer + c * STEP, at = S ? gm_at_s<ROWS, INTERLEAVED>(o, inner) : gm_at_c<KIND, INTERLEAVED>(o, inner);
+            const int o = outer + c * STEP, at = S ? gm_at_s<ROWS, INTERLEAVED>(o, inner) : gm_at_c<gm_row_bytes<KIND>, INTERLEAVED>(o, inner);
             if constexpr (KIND == FGNN_E4M3) {
                 gm_i4 half[2];
                 gm_widen(w[c], half);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) *reinterpret_cast<gm_i4 *>(tile + gm_at_c<KIND, INTERLEAVED>(o, 2 * inner + h)) = half[h];
+                for (int h = 0; h < 2; ++h) *reinterpret_cast<gm_i4 *>(tile + gm_at_c<gm_row_bytes<KIND>, INTERLEAVED>(o, 2 * inner + h)) = half[h];
             } else if constexpr (KIND == FGNN_F32) {
                 gm_i4 part[3];
                 gm_split(w[c], part);
@@ -484,14 +483,16 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmP p)
 }
 
 // ------------------------------------------------------------------------------------------------ aligned operands, from memory to LDS
-// Operands whose rows start at 16 bytes and hold whole 16-byte chunks go from memory to LDS without passing registers; a slab is in flight while the one
-// before it is multiplied, in the other half of LDS.
+// Operands whose rows start at 16 bytes and hold whole 16-byte chunks go from memory to LDS without passing registers.  A slab is 128 bytes of a row (whole lines
+// of the caches: with 64 the L2 sees twice the requests), two instructions' reduction; LDS holds two slabs.  A wave always has a half slab's operands
+// in registers and reads the next half while it multiplies, so that it meets the others once a slab, in its middle: then the next slab has arrived,
+// and this one is in registers everywhere, so that its place takes the one after next.
 // PLANES = 2: both operands are hi + 2^-11 lo (`plane_q`, `plane_p` bytes apart); their product is hi hi + 2^-11 (hi lo + lo hi).  The two small parts are
 // summed first, over the whole reduction, and scaled.
-template <int KIND, int ROWS, bool S, int WAVES>
+template <int SIZE, int ROWS, bool S, int WAVES>
 struct GemmMover {
-    static constexpr int SIZE = GemmKind<KIND>::size, SLAB = GemmKind<KIND>::slab, CH = 16 / SIZE, COUNT = ROWS * 128 / 1024 / WAVES;
-    static_assert(SLAB * SIZE == 128 && ROWS * 128 % (1024 * WAVES) == 0, "a wave moves whole kilobytes");
+    static constexpr int SLAB = 128 / SIZE, CH = 16 / SIZE, COUNT = ROWS * 128 / 1024 / WAVES;
+    static_assert(ROWS * 128 % (1024 * WAVES) == 0, "a wave moves whole kilobytes");
     uint32_t at[COUNT];                     // of the lane's chunks, from the slab's first byte on
     int along[COUNT];                       // their first reduction element in the slab
     const char *base; int64_t step;
@@ -512,68 +513,130 @@ struct GemmMover {
                 at[c] = (uint32_t)(k * ld * SIZE) + 16 * min(chunk, left / CH - 1);
                 along[c] = k;
             } else {
-                const int row = pos / 8, chunk = (gm_at_c<KIND, INTERLEAVED>(row, pos % 8) - row * 128) >> 4;
+                const int row = pos / 8, chunk = (gm_at_c<128, INTERLEAVED>(row, pos % 8) - row * 128) >> 4;
                 at[c] = (uint32_t)(min(row, left - 1) * ld * SIZE) + 16 * chunk;
                 along[c] = chunk * CH;
             }
         }
     }
-    // slab `index` of a plane that starts `plane` bytes after the first; `left` reduction elements exist from its first on.  What lies past them is read
-    // as zeros: out of the buffer's range.
-    __device__ __forceinline__ void move(int64_t index, int64_t plane, int64_t left, char *tile, int wave) const
+    // Transfer c of slab `index` of a plane that starts `plane` bytes after the first; `left` reduction elements exist from its first on.  What lies past them
+    // is read as zeros: out of the buffer's range.  Written out (it has no output registers), because the compiler would have every transposing read wait
+    // for all transfers before it, whatever their place; gm_arrive waits for the ones that matter, and orders reads against them.
+    __device__ __forceinline__ void move(int c, int64_t index, int64_t plane, int64_t left, uint32_t tile, int wave) const
     {
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base + index * step + plane), 0, 0x80000000u, 0x00027000);
-#pragma unroll
-        for (int c = 0; c < COUNT; ++c) {
-            const uint32_t v = along[c] < left ? at[c] : 0x80000000u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(tile + (c * WAVES + wave) * 1024), 16, v, 0, 0, 0);
-        }
+        const uint64_t from = (uint64_t)(base + index * step + plane);
+        const gm_i4 buffer = {(int)(uint32_t)from, (int)((uint32_t)(from >> 32) & 0xffffu), (int)0x80000000u, 0x00027000};
+        const uint32_t v = along[c] < left ? at[c] : 0x80000000u;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(tile + (c * WAVES + wave) * 1024), "v"(v), "s"(buffer));
     }
 };
 
+// Waits until at most LEFT of the wave's transfers to LDS are on their way and its reads from LDS have ended, and for the other waves to get here.
+template <int LEFT> __device__ __forceinline__ void gm_arrive() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory"); }
+
 // Waves of 64 columns by 128 rows in tiles of 256 x 256, by 64 rows in smaller ones.
 constexpr int gm_waves(int bm, int bn) { return bm * bn / 64 / (bm >= 256 ? 128 : 64); }
+constexpr size_t gm_moved_lds(int bm, int bn) { return (size_t)2 * (bm + bn) * 128; }
 template <int KIND, typename F, bool QS, bool PS, int BM, int BN, int PLANES>
 __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(GemmP p, F f)
 {
-    constexpr int WAVES = gm_waves(BM, BN), WP = BN / 64, TQ = BM / 16 / (WAVES / WP), SLAB = GemmKind<KIND>::slab;
-    extern __shared__ __attribute__((aligned(16))) char lds[];                  // [2][BM + BN][128]
-    constexpr int HALF = (BM + BN) * 128;
+    constexpr int WAVES = gm_waves(BM, BN), WP = BN / 64, TQ = BM / 16 / (WAVES / WP), SIZE = GemmKind<KIND>::size, SLAB = 128 / SIZE;
+    constexpr int MOVES = (BM + BN) * 128 / 1024 / WAVES, HALF = (BM + BN) * 128;          // transfers of a wave, and bytes, a slab
+    extern __shared__ __attribute__((aligned(16))) char lds[];                              // [2][BM + BN][128]
     int tm, tn, split;
     gm_tile(p, tm, tn, split);
     const int64_t batch = blockIdx.y;
     const int lane = fg_lane(), wave = fg_wave(), wp = wave % WP, tq0 = wave / WP * TQ;
     const int64_t once = (p.k + SLAB - 1) / SLAB, small = PLANES == 2 ? 2 * once : 0;       // slabs of the reduction, and of the small parts
-    const int64_t s0 = split * p.slabs, s1 = min(once + small, s0 + p.slabs);
+    const int64_t per = p.slabs * (PLANES == 2 ? 3 : 1), s0 = split * per;
+    const int slabs = (int)max((int64_t)0, min(once + small, s0 + per) - s0);
     typename GemmKind<KIND>::acc acc[TQ][4] = {};
-    GemmMover<KIND, BM, QS, WAVES> q;
-    GemmMover<KIND, BN, PS, WAVES> b;
+    GemmMover<SIZE, BM, QS, WAVES> q;
+    GemmMover<SIZE, BN, PS, WAVES> b;
     q.template init<false>((const char *)p.q + batch * p.batch_q, p.ldq, (int64_t)tm * BM, p.rows_q, lane, wave);
     b.template init<true>((const char *)p.p + batch * p.batch_p, p.ldp, (int64_t)tn * BN, p.rows_p, lane, wave);
-    auto move = [&](int64_t s, char *to) {
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    // transfer c of slab i
+    auto move = [&](int i, int c) {
+        const int64_t s = s0 + i;
         const bool cross = PLANES == 2 && s < small;
-        const int64_t i = cross ? s >> 1 : s - small, left = p.k - i * SLAB;
-        q.move(i, cross && (s & 1) ? p.plane_q : 0, left, to, wave);
-        b.move(i, cross && !(s & 1) ? p.plane_p : 0, left, to + BM * 128, wave);
+        const int64_t at = cross ? s >> 1 : s - small, left = p.k - at * SLAB;
+        const uint32_t to = lds0 + (i & 1) * HALF;
+        if (c < q.COUNT) q.move(c, at, cross && (s & 1) ? p.plane_q : 0, left, to, wave);
+        else b.move(c - q.COUNT, at, cross && !(s & 1) ? p.plane_p : 0, left, to + BM * 128, wave);
     };
+    auto move_all = [&](int i) {
+#pragma unroll
+        for (int c = 0; c < MOVES; ++c) move(i, c);
+    };
+    struct Operands { gm_i4 a[4], b[TQ]; };
+    // operand j of half h of slab i: four of P, then Q's
+    auto read = [&](int i, int h, int j, Operands &o) {
+        const char *from = lds + (i & 1) * HALF;
+        if (j < 4) o.a[j] = gm_operand<128, BN, PS, true>(from + BM * 128, wp, j, h, lane);
+        else o.b[j - 4] = gm_operand<128, BM, QS, false>(from, 0, tq0 + j - 4, h, lane);
+    };
+    auto read_all = [&](int i, int h, Operands &o) {
+#pragma unroll
+        for (int j = 0; j < 4 + TQ; ++j) read(i, h, j, o);
+    };
+    auto multiply = [&](int t, int u, const Operands &o) { acc[t][u] = gm_mfma<KIND>(o.a[u], o.b[t], acc[t][u]); };
     auto scale = [&]() {
         if constexpr (PLANES == 2) {
 #pragma unroll
-            for (int i = 0; i < TQ; ++i)
+            for (int t = 0; t < TQ; ++t)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[i][t] *= 0x1p-11f;
+                for (int u = 0; u < 4; ++u) acc[t][u] *= 0x1p-11f;
         }
     };
-    if (s0 < s1) move(s0, lds);
-#pragma unroll 1
-    for (int64_t s = s0; s < s1; ++s) {
-        char *now = lds + ((s - s0) & 1) * HALF, *next = lds + ((s - s0 + 1) & 1) * HALF;
-        __syncthreads();                    // this slab has arrived, and the one before it has been read
-        if (s + 1 < s1) move(s + 1, next);
-        if (PLANES == 2 && s == small) scale();
-        gm_slab<KIND, BM, BN, QS, PS, TQ>(now, now + BM * 128, wp, tq0, lane, acc);
+    // Multiplies what `now` holds; reads half h of slab i into `next` and, where MOVE, starts the transfers of slab i + 1 on the way, spread over the instructions: a
+    // compute unit takes a transfer every 16 cycles, and waves that begin with all of theirs wait for one another.
+    auto half = [&]<bool MOVE>(int i, int h, const Operands &now, Operands &next) {
+#pragma unroll
+        for (int t = 0; t < TQ; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(t, 0, now);
+            multiply(t, 1, now);
+            if constexpr (MOVE) {
+#pragma unroll
+                for (int c = t * MOVES / TQ; c < (t + 1) * MOVES / TQ; ++c) move(i + 1, c);
+            }
+#pragma unroll
+            for (int j = t * (4 + TQ) / TQ; j < (t + 1) * (4 + TQ) / TQ; ++j) read(i, h, j, next);
+            multiply(t, 2, now);
+            multiply(t, 3, now);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    Operands first, second;
+    if (slabs > 0) {
+        move_all(0);
+        if (slabs > 1) {
+            move_all(1);
+            gm_arrive<MOVES>();
+        } else gm_arrive<0>();
+        read_all(0, 0, first);
     }
-    if (PLANES == 2 && s1 <= small) scale();
+    // nothing that came from scalar loads is on its way into the loop: they end in any order, and would turn every wait for LDS into one for all of it
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    int i = 0;
+#pragma unroll 1
+    for (; i + 2 < slabs; ++i) {
+        if (PLANES == 2 && s0 + i == small) scale();
+        half.template operator()<false>(i, 1, first, second);
+        gm_arrive<0>();
+        half.template operator()<true>(i + 1, 0, second, first);
+    }
+    // the last two, which start nothing any more
+#pragma unroll 1
+    for (; i < slabs; ++i) {
+        if (PLANES == 2 && s0 + i == small) scale();
+        half.template operator()<false>(i, 1, first, second);
+        if (i + 1 < slabs) gm_arrive<0>();
+        // (past the last slab: what is read is not used)
+        half.template operator()<false>(i + 1, 0, second, first);
+    }
+    if (PLANES == 2 && s0 + slabs <= small) scale();
     const int n = tn * BN + 64 * wp + 16 * (lane >> 4);
     typename F::Cols cols;
     if (p.splits == 1) f.columns(n, cols);

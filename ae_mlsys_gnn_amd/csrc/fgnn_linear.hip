@@ -40,7 +40,7 @@ template <int KIND, typename E, int TILE>
 static void gm_launch_moved(const GemmP &p, bool qs, bool ps, hipStream_t st)
 {
     const dim3 g((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), b(64 * gm_waves(TILE, TILE));
-    const size_t lds = 4 * TILE * 128;
+    const size_t lds = gm_moved_lds(TILE, TILE);
     const LinearEpi<E> f{p.epi};
     if constexpr (fe_size_of<KIND> == 1) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, false, TILE, TILE, 1>), g, b, lds, st, p, f);
     else if (qs) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, true, true, TILE, TILE, 1>), g, b, lds, st, p, f);

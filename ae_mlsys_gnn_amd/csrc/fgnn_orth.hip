@@ -168,12 +168,12 @@ template <bool QS, bool PS>
 static void or_product(GemmP p, const OrthEpi &f, int batch, hipStream_t st)
 {
     p.splits = 1;
-    p.slabs = (p.k + 63) / 64 * 3;
+    p.slabs = (p.k + 63) / 64;
     auto go = [&]<int TILE>() {
         p.tiles_m = (int)((p.m + TILE - 1) / TILE);
         p.tiles_n = (p.n + TILE - 1) / TILE;
         hipLaunchKernelGGL((gemm_moved_kernel<FGNN_F16, OrthEpi, QS, PS, TILE, TILE, 2>), dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)batch),
-                           dim3(64 * gm_waves(TILE, TILE)), 4 * TILE * 128, st, p, f);
+                           dim3(64 * gm_waves(TILE, TILE)), gm_moved_lds(TILE, TILE), st, p, f);
     };
     const int cus = fgnn_current_device_compute_units();
     if (((p.m + 255) / 256) * ((p.n + 255) / 256) * batch >= (cus > 0 ? cus : 256)) go.template operator()<256>();
