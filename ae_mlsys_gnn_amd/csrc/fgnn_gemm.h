@@ -3,9 +3,10 @@
 // Either operand comes with its reduction contiguous ("C": element (i, k) at p[i ld + k]) or strided ("S": at p[k ld + i]), so that a forward
 // product (C, C), the gradient of its input (P strided) and of its weights (both strided) read the matrices as they lie in memory.
 //
-// P is the first operand of the instructions: a lane ends up with four consecutive n of one m.  The four 16-row tiles of a 64-row block of P are
-// interleaved (instruction row r of tile t is n = 16 (r / 4) + 4 t + r % 4), so that a lane holds 16 consecutive n of a row: a row's 64 columns are
-// one run in memory for four lanes, as are bias and residual.
+// P is the first operand of the instructions: a lane ends up with four consecutive n of one m, the four lanes of a row with 16.  Results of 16 bits want eight
+// (16 bytes) a lane: then the tiles of P are interleaved in pairs (instruction row r of tile t is n = 32 (t / 2) + 8 (r / 4) + 4 (t % 2) + r % 4).  Either way
+// one store instruction writes 64 bytes of each of 16 rows, as do reads of the residual (with 16 columns a lane, in four stores of 16 bytes each 64
+// apart, the L2 saw four times the requests: 169,343 x 128 -> 256 fp32 with gelu and residual 226 us).
 //
 // Element kinds: 16-bit values (products of 8 significant bits and sums in 32 bits), 8-bit integers (sums in integers: exact), 8-bit floats, and
 // fp32.  fp32 operands are cut into three parts of 8 significant bits (truncated, so that the three are exact), and the six products that reach above
@@ -22,24 +23,70 @@ typedef _Float16 gm_h8 __attribute__((ext_vector_type(8)));
 
 enum { GM_NONE = 0, GM_RELU = 1, GM_GELU = 2, GM_SILU = 3, GM_LEAKY = 4 };
 
-__device__ __forceinline__ float gm_act(float z, int act, float slope)
+// The normal distribution's function P(z) and exp(-z^2 / 2), which its slope needs too.  P(-|z|) = t (c1 + .. + c5 t^4) exp(-z^2 / 2) with t = 1 / (1 + p |z|)
+// (Hastings' approximation, Abramowitz and Stegun 26.2.17: off by 7.5e-8 at the most); one exponential and one reciprocal where the library's erff takes some
+// fifty instructions, which no other workgroup's products hide in the epilogue (169,343 x 128 -> 256 fp32 with gelu and residual 275 / 224 us).
+__device__ __forceinline__ float gm_normal(float z, float &bell)
 {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.2316419f, fabsf(z), 1.f));
+    bell = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+    const float c = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.330274429f, -1.821255978f), 1.781477937f), -0.356563782f), 0.319381530f);
+    const float below = c * (0.39894228f * bell);
+    return z > 0.f ? 1.f - below : z == z ? below : z;
+}
+__device__ __forceinline__ float gm_logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+
+template <int W>
+__device__ __forceinline__ void gm_act(float (&z)[W], int act, float slope)
+{
+    float bell;
     switch (act) {
-    case GM_RELU: return z > 0.f ? z : z == z ? 0.f : z;
-    case GM_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case GM_SILU: return z / (1.f + expf(-z));
-    case GM_LEAKY: return z > 0.f ? z : slope * z;
-    default: return z;
+    case GM_RELU:
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[i] = z[i] > 0.f ? z[i] : z[i] == z[i] ? 0.f : z[i];
+        break;
+    case GM_GELU:
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[i] *= gm_normal(z[i], bell);
+        break;
+    case GM_SILU:
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[i] *= gm_logistic(z[i]);
+        break;
+    case GM_LEAKY:
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[i] = z[i] > 0.f ? z[i] : slope * z[i];
+        break;
     }
 }
-__device__ __forceinline__ float gm_act_slope(float z, int act, float slope)
+// g times the slope at z
+template <int W>
+__device__ __forceinline__ void gm_act_slope(float (&g)[W], const float (&z)[W], int act, float slope)
 {
     switch (act) {
-    case GM_RELU: return z > 0.f ? 1.f : 0.f;
-    case GM_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-    case GM_SILU: { const float p = 1.f / (1.f + expf(-z)); return p * (1.f + z * (1.f - p)); }
-    case GM_LEAKY: return z > 0.f ? 1.f : slope;
-    default: return 1.f;
+    case GM_RELU:
+#pragma unroll
+        for (int i = 0; i < W; ++i) g[i] = z[i] > 0.f ? g[i] : 0.f;
+        break;
+    case GM_GELU:
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            float bell;
+            const float p = gm_normal(z[i], bell);
+            g[i] *= fmaf(z[i], 0.39894228f * bell, p);
+        }
+        break;
+    case GM_SILU:
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float p = gm_logistic(z[i]);
+            g[i] *= fmaf(p * z[i], 1.f - p, p);
+        }
+        break;
+    case GM_LEAKY:
+#pragma unroll
+        for (int i = 0; i < W; ++i) g[i] *= z[i] > 0.f ? 1.f : slope;
+        break;
     }
 }
 
@@ -102,8 +149,20 @@ __device__ __forceinline__ void gm_columns(const GemmEpi &e, int n, GemmCols<W> 
         c.sw[i] = e.sw ? e.sw[j] : 1.f;
     }
 }
+template <typename E, int W> struct GemmVec { typedef E type __attribute__((ext_vector_type(W), aligned(sizeof(E)))); };
+// The residual's W values at (m, n) where all of them exist (anything else: read one by one later), asked for ahead of their use.
 template <typename E, int W>
-__device__ __forceinline__ void gm_finish(const GemmEpi &e, const GemmCols<W> &c, int64_t m, int n, float (&v)[W])
+__device__ __forceinline__ typename GemmVec<E, W>::type gm_ahead(const GemmEpi &e, int64_t m, int n)
+{
+    typename GemmVec<E, W>::type u = {};
+    if (e.res && e.n >= W) {
+        const bool there = m < e.m && n + W <= e.n;
+        u = *reinterpret_cast<const typename GemmVec<E, W>::type *>((const E *)e.res + (there ? m * e.ldr + n : 0));
+    }
+    return u;
+}
+template <typename E, int W>
+__device__ __forceinline__ void gm_finish(const GemmEpi &e, const GemmCols<W> &c, const typename GemmVec<E, W>::type &ahead, int64_t m, int n, float (&v)[W])
 {
     const int count = e.n - n;
     if (m >= e.m || count <= 0) return;
@@ -116,13 +175,12 @@ __device__ __forceinline__ void gm_finish(const GemmEpi &e, const GemmCols<W> &c
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] += c.bias[i];
     if (e.z) gm_store<E, W>(v, (E *)e.z + at, count);
-    if (e.act) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = gm_act(v[i], e.act, e.slope);
-    }
+    if (e.act) gm_act(v, e.act, e.slope);
     if (e.res) {
         float r[W];
-        gm_load<E, W>(r, (const E *)e.res + m * e.ldr + n, count);
+#pragma unroll
+        for (int i = 0; i < W; ++i) r[i] = (float)ahead[i];
+        if (count < W) gm_load<E, W>(r, (const E *)e.res + m * e.ldr + n, count);
 #pragma unroll
         for (int i = 0; i < W; ++i) v[i] += r[i];
     }
@@ -134,6 +192,7 @@ struct GemmP {
     int n;
     const void *q, *p; int64_t ldq, ldp;
     int tiles_m, tiles_n, splits;
+    int lower;                              // only tiles on and below the diagonal: D is symmetric, and the epilogue writes the rest
     int64_t slabs;                          // slabs of the reduction a split takes
     float *part;                            // [splits][m][n] where splits > 1
     int64_t rows_q, rows_p;                 // rows that the operands have (more than D has where a strided one is padded to whole chunks)
@@ -146,9 +205,16 @@ __device__ __forceinline__ void gm_tile(const GemmP &p, int &tm, int &tn, int &s
 {
     const int total = (int)gridDim.x, b = (int)blockIdx.x, xcd = b % FGNN_NUM_XCD, q = total / FGNN_NUM_XCD, r = total % FGNN_NUM_XCD;
     int t = xcd * q + min(xcd, r) + b / FGNN_NUM_XCD;
-    const int tiles = p.tiles_m * p.tiles_n;
+    const int tiles = p.lower ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
     split = t / tiles;
     t -= split * tiles;
+    if (p.lower) {
+        tm = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+        while (tm * (tm + 1) / 2 > t) --tm;
+        while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
+        tn = t - tm * (tm + 1) / 2;
+        return;
+    }
     constexpr int HIGH = 8;
     const int band = t / (HIGH * p.tiles_n), first = band * HIGH, high = min(HIGH, p.tiles_m - first);
     t -= band * HIGH * p.tiles_n;
@@ -177,35 +243,34 @@ template <> struct GemmKind<FGNN_E4M3> {    // wait in LDS as fp16, which holds 
 // LDS tile of an operand with `rows` rows (of D's rows or columns), one plane of a slab.  C: [rows][row bytes], 64 bytes a row for fp32's parts and 128
 // else; S: [slab][rows] 16-bit values.  16-byte chunks of a row are exchanged so that the lanes of one LDS pass meet different banks.
 template <int KIND> constexpr int gm_row_bytes = GemmKind<KIND>::slab *(KIND == FGNN_I8 ? 1 : 2);
-template <int RB, bool INTERLEAVED>
+template <int RB, bool PAIRS>
 __device__ __forceinline__ int gm_at_c(int row, int chunk)
 {
-    int f;
-    if constexpr (RB == 128) f = INTERLEAVED ? (row & 3) | ((row >> 4) & 1) << 2 : row & 7;
-    else f = INTERLEAVED ? ((row >> 1) & 1) | ((row >> 4) & 1) << 1 : (row >> 1) & 3;
+    const int f = RB == 64 ? (row >> 1) & 3 : PAIRS ? (row & 3) | ((row >> 3) & 1) << 2 : row & 7;
     return row * RB + ((chunk ^ f) << 4);
 }
-template <int ROWS, bool INTERLEAVED>
+template <int ROWS, bool PAIRS>
 __device__ __forceinline__ int gm_at_s(int k, int chunk)
 {
-    const int f = INTERLEAVED ? (k & 1) | ((k >> 1) & 1) << (ROWS >= 128 ? 3 : 2) : (k & 3) << 1;
+    const int f = PAIRS ? (k & 3) << 2 : (k & 3) << 1;
     return k * (ROWS * 2) + ((chunk ^ f) << 4);
 }
 
-// Operand registers of 16 rows and one instruction's reduction.
-template <int RB, int ROWS, bool S, bool INTERLEAVED>
-__device__ __forceinline__ gm_i4 gm_operand(const char *tile, int block, int t, int step, int lane)
+// Operand registers of 16 rows (tile t; the tiles of a 64-row block may be interleaved in pairs) and one instruction's reduction.
+template <int RB, int ROWS, bool S, bool PAIRS>
+__device__ __forceinline__ gm_i4 gm_operand(const char *tile, int t, int step, int lane)
 {
+    static_assert(!(PAIRS && RB == 64) && ROWS >= 128, "the exchanges of chunks stay within a row");
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!S) {
-        const int row = INTERLEAVED ? 64 * block + 16 * (r >> 2) + 4 * t + (r & 3) : 16 * t + r;
-        return *reinterpret_cast<const gm_i4 *>(tile + gm_at_c<RB, INTERLEAVED>(row, 4 * step + g));
+        const int row = PAIRS ? 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3) : 16 * t + r;
+        return *reinterpret_cast<const gm_i4 *>(tile + gm_at_c<RB, PAIRS>(row, 4 * step + g));
     } else {
         // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
-        const int i = INTERLEAVED ? 64 * block + 16 * (r & 3) + 4 * t : 16 * t + 4 * (r & 3);
+        const int i = PAIRS ? 32 * (t >> 1) + 8 * (r & 3) + 4 * (t & 1) : 16 * t + 4 * (r & 3);
         const int k = 32 * step + 8 * g + (r >> 2);
         typedef __attribute__((address_space(3))) gm_s4 *lds_p;
-        const char *a = tile + gm_at_s<ROWS, INTERLEAVED>(k, i >> 3) + ((i >> 2) & 1) * 8;
+        const char *a = tile + gm_at_s<ROWS, PAIRS>(k, i >> 3) + ((i >> 2) & 1) * 8;
         const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 4 * ROWS * 2));
         typedef short s8 __attribute__((ext_vector_type(8)));
         const s8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -221,7 +286,7 @@ __device__ __forceinline__ typename GemmKind<KIND>::acc gm_mfma(gm_i4 a, gm_i4 b
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(gm_b8 *)&a, *(gm_b8 *)&b, c, 0, 0, 0);
 }
 // One slab: a wave's 64 columns (block wp of P's tile) by 16 TQ rows (16-row tiles from tq0 on of Q's).
-template <int KIND, int BM, int BN, bool QS, bool PS, int TQ>
+template <int KIND, int BM, int BN, bool QS, bool PS, bool PAIRS, int TQ>
 __device__ __forceinline__ void gm_slab(const char *lq, const char *lp, int wp, int tq0, int lane, typename GemmKind<KIND>::acc (&acc)[TQ][4])
 {
     constexpr int PLQ = BM * GemmKind<KIND>::slab * 2, PLP = BN * GemmKind<KIND>::slab * 2;      // bytes a plane (where there are several)
@@ -230,12 +295,12 @@ __device__ __forceinline__ void gm_slab(const char *lq, const char *lp, int wp, 
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int h = 0; h < 3; ++h) a[t][h] = gm_operand<gm_row_bytes<KIND>, BN, PS, true>(lp + h * PLP, wp, t, 0, lane);
+            for (int h = 0; h < 3; ++h) a[t][h] = gm_operand<gm_row_bytes<KIND>, BN, PS, PAIRS>(lp + h * PLP, 4 * wp + t, 0, lane);
 #pragma unroll
         for (int q = 0; q < TQ; ++q) {
             gm_i4 b[3];
 #pragma unroll
-            for (int h = 0; h < 3; ++h) b[h] = gm_operand<gm_row_bytes<KIND>, BM, QS, false>(lq + h * PLQ, 0, tq0 + q, 0, lane);
+            for (int h = 0; h < 3; ++h) b[h] = gm_operand<gm_row_bytes<KIND>, BM, QS, false>(lq + h * PLQ, tq0 + q, 0, lane);
             // the small products first
 #pragma unroll
             for (int s = 2; s >= 0; --s)
@@ -249,14 +314,71 @@ __device__ __forceinline__ void gm_slab(const char *lq, const char *lp, int wp, 
         for (int s = 0; s < 2; ++s) {
             gm_i4 a[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) a[t] = gm_operand<gm_row_bytes<KIND>, BN, PS, true>(lp, wp, t, s, lane);
+            for (int t = 0; t < 4; ++t) a[t] = gm_operand<gm_row_bytes<KIND>, BN, PS, PAIRS>(lp, 4 * wp + t, s, lane);
 #pragma unroll
             for (int q = 0; q < TQ; ++q) {
-                const gm_i4 b = gm_operand<gm_row_bytes<KIND>, BM, QS, false>(lq, 0, tq0 + q, s, lane);
+                const gm_i4 b = gm_operand<gm_row_bytes<KIND>, BM, QS, false>(lq, tq0 + q, s, lane);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) acc[q][t] = gm_mfma<KIND>(a[t], b, acc[q][t]);
             }
         }
+    }
+}
+
+// What becomes of W sums a lane, as the kernels take it: LinearEpi for linear maps.  ROWS: rows whose reads are asked for together.
+template <typename E>
+struct LinearEpi {
+    static constexpr int W = fe_width<E>, ROWS = 4;
+    GemmEpi e;
+    typedef GemmCols<W> Cols;
+    typedef typename GemmVec<E, W>::type Ahead;
+    __device__ __forceinline__ void columns(int n, Cols &c) const { gm_columns(e, n, c); }
+    __device__ __forceinline__ Ahead ahead(int64_t, int64_t m, int n) const { return gm_ahead<E, W>(e, m, n); }
+    __device__ __forceinline__ void finish(const Cols &c, const Ahead &a, int64_t, int64_t m, int n, float (&v)[W]) const { gm_finish<E, W>(e, c, a, m, n, v); }
+};
+
+// A wave's results: 16 TQ rows from m0 on, 64 columns from n0 on.
+template <int TQ, typename F, typename A>
+__device__ __forceinline__ void gm_results(const GemmP &p, const F &f, int64_t batch, int split, int64_t m0, int n0, int lane, const A (&acc)[TQ][4])
+{
+    constexpr int W = F::W, J = 16 / W, ROWS = F::ROWS < TQ ? F::ROWS : TQ;
+    const int r = lane & 15, g = lane >> 4;
+    auto sums = [&](int i, int j, float (&v)[W]) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[k] = (float)acc[i][j * (W / 4) + k / 4][k % 4];
+    };
+    auto column = [&](int j) { return n0 + 4 * W * j + W * g; };
+    if (p.splits > 1) {
+#pragma unroll
+        for (int i = 0; i < TQ; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int64_t m = m0 + 16 * i + r;
+                float v[W];
+                sums(i, j, v);
+                if (m < p.m && column(j) < p.n) gm_store<float, W>(v, p.part + ((batch * p.splits + split) * p.m + m) * p.n + column(j), p.n - column(j));
+            }
+        return;
+    }
+    typename F::Cols cols[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) f.columns(column(j), cols[j]);
+    // a row's parts one after the other: lines of the caches that are written whole leave them whole
+#pragma unroll
+    for (int i0 = 0; i0 < TQ; i0 += ROWS) {
+        typename F::Ahead a[ROWS][J];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) a[i][j] = f.ahead(batch, m0 + 16 * (i0 + i) + r, column(j));
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                float v[W];
+                sums(i0 + i, j, v);
+                f.finish(cols[j], a[i][j], batch, m0 + 16 * (i0 + i) + r, column(j), v);
+            }
     }
 }
 
@@ -354,17 +476,17 @@ struct GemmLoader {
         }
         base += S ? (int64_t)SLAB * ld : (int64_t)SLAB * SIZE;
     }
-    template <bool INTERLEAVED>
+    template <bool PAIRS>
     __device__ __forceinline__ void store(char *tile)
     {
 #pragma unroll
         for (int c = 0; c < COUNT; ++c) {
-            const int o = outer + c * STEP, at = S ? gm_at_s<ROWS, INTERLEAVED>(o, inner) : gm_at_c<gm_row_bytes<KIND>, INTERLEAVED>(o, inner);
+            const int o = outer + c * STEP, at = S ? gm_at_s<ROWS, PAIRS>(o, inner) : gm_at_c<gm_row_bytes<KIND>, PAIRS>(o, inner);
             if constexpr (KIND == FGNN_E4M3) {
                 gm_i4 half[2];
                 gm_widen(w[c], half);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) *reinterpret_cast<gm_i4 *>(tile + gm_at_c<gm_row_bytes<KIND>, INTERLEAVED>(o, 2 * inner + h)) = half[h];
+                for (int h = 0; h < 2; ++h) *reinterpret_cast<gm_i4 *>(tile + gm_at_c<gm_row_bytes<KIND>, PAIRS>(o, 2 * inner + h)) = half[h];
             } else if constexpr (KIND == FGNN_F32) {
                 gm_i4 part[3];
                 gm_split(w[c], part);
@@ -398,7 +520,7 @@ __device__ __forceinline__ void gm_repair(const GemmP &p, int64_t m0, int n0, in
             const float b = in ? ((const float *)p.q)[QS ? kk * p.ldq + m : m * p.ldq + kk] : 0.f;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const int64_t n = min(n0 + 16 * (r >> 2) + 4 * t + (r & 3), p.n - 1);
+                const int64_t n = min(n0 + 16 * t + r, p.n - 1);
                 const float a = in ? ((const float *)p.p)[PS ? kk * p.ldp + n : n * p.ldp + kk] : 0.f;
                 sum[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, sum[t], 0, 0, 0);
             }
@@ -415,7 +537,8 @@ __device__ __forceinline__ void gm_repair(const GemmP &p, int64_t m0, int n0, in
 template <int KIND, typename E, bool QS, bool PS>
 __global__ __launch_bounds__(256, 2) void gemm_any_kernel(GemmP p)
 {
-    constexpr int BM = 128, BN = 128, SLAB = GemmKind<KIND>::slab, TQ = 4;
+    constexpr int BM = 128, BN = 128, SLAB = GemmKind<KIND>::slab, TQ = 4, W = fe_width<E>;
+    constexpr bool PAIRS = W == 8;
     constexpr int BYTES = 128 * gm_row_bytes<KIND> * GemmKind<KIND>::planes;
     __shared__ __attribute__((aligned(16))) char lds[2 * BYTES];
     char *lq = lds, *lp = lds + BYTES;
@@ -436,50 +559,49 @@ __global__ __launch_bounds__(256, 2) void gemm_any_kernel(GemmP p)
     for (int64_t k = k0; k < k1; k += SLAB) {
         __syncthreads();                    // the slab before has been read
         q.template store<false>(lq);
-        b.template store<true>(lp);
+        b.template store<PAIRS>(lp);
         __syncthreads();
         if (k + SLAB < k1) {
             q.fetch(k1 - k - SLAB);
             b.fetch(k1 - k - SLAB);
         }
-        gm_slab<KIND, BM, BN, QS, PS, TQ>(lq, lp, wp, tq0, lane, acc);
+        gm_slab<KIND, BM, BN, QS, PS, PAIRS, TQ>(lq, lp, wp, tq0, lane, acc);
     }
     if constexpr (KIND == FGNN_F32) gm_repair<QS, PS, TQ>(p, (int64_t)tm * BM + 16 * tq0, tn * BN + 64 * wp, k0, k1, lane, acc);
-    const int n = tn * BN + 64 * wp + 16 * (lane >> 4);
-    GemmCols<16> cols;
-    if (p.splits == 1) gm_columns(p.epi, n, cols);
-#pragma unroll
-    for (int i = 0; i < TQ; ++i) {
-        const int64_t m = (int64_t)tm * BM + 16 * (tq0 + i) + (lane & 15);
-        float v[16];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * t + j] = (float)acc[i][t][j];
-        if (p.splits == 1) gm_finish<E, 16>(p.epi, cols, m, n, v);
-        else if (m < p.m && n < p.n) gm_store<float, 16>(v, p.part + ((int64_t)split * p.m + m) * p.n + n, p.n - n);
-    }
+    gm_results<TQ>(p, LinearEpi<E>{p.epi}, 0, split, (int64_t)tm * BM + 16 * tq0, tn * BN + 64 * wp, lane, acc);
 }
 
-// The partial sums of a reduction cut into `splits`, added up in their order; four columns a thread.
-template <typename E>
+// The partial sums of a reduction cut into `splits`, added up in a fixed order: four columns a thread, or a part of their sums where few columns have many.
+template <typename E, int SHARE>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmP p)
 {
-    const int quads = (p.n + 3) / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / quads;
-    if (m >= p.m) return;
+    __shared__ gm_f4 sums[SHARE > 1 ? 256 : 1];
+    const int quads = (p.n + 3) / 4, share = (int)threadIdx.x / (256 / SHARE);
+    const int64_t i = (int64_t)blockIdx.x * (256 / SHARE) + threadIdx.x % (256 / SHARE), m = i / quads;
     const int n = (int)(i - m * quads) * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (m < p.m) {
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-        float u[4];
-        gm_load<float, 4>(u, p.part + ((int64_t)s * p.m + m) * p.n + n, p.n - n);
+        for (int s = share; s < p.splits; s += SHARE) {
+            float u[4];
+            gm_load<float, 4>(u, p.part + ((int64_t)s * p.m + m) * p.n + n, p.n - n);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += u[j];
+            for (int j = 0; j < 4; ++j) v[j] += u[j];
+        }
     }
+    if constexpr (SHARE > 1) {
+        sums[threadIdx.x] = gm_f4{v[0], v[1], v[2], v[3]};
+        __syncthreads();
+        if (share) return;
+#pragma unroll
+        for (int s = 1; s < SHARE; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += sums[s * (256 / SHARE) + threadIdx.x][j];
+    }
+    if (m >= p.m) return;
     GemmCols<4> cols;
     gm_columns(p.epi, n, cols);
-    gm_finish<E, 4>(p.epi, cols, m, n, v);
+    gm_finish<E, 4>(p.epi, cols, gm_ahead<E, 4>(p.epi, m, n), m, n, v);
 }
 
 // ------------------------------------------------------------------------------------------------ aligned operands, from memory to LDS
@@ -497,7 +619,7 @@ struct GemmMover {
     int along[COUNT];                       // their first reduction element in the slab
     const char *base; int64_t step;
 
-    template <bool INTERLEAVED>
+    template <bool PAIRS>
     __device__ __forceinline__ void init(const void *p, int64_t ld, int64_t row0, int64_t rows, int lane, int wave)
     {
         const int left = (int)min((int64_t)ROWS, rows - row0);
@@ -508,12 +630,12 @@ struct GemmMover {
             const int pos = (c * WAVES + wave) * 64 + lane;                 // 16-byte place in the LDS tile
             if constexpr (S) {
                 constexpr int PER = ROWS / 8;
-                const int k = pos / PER, chunk = (gm_at_s<ROWS, INTERLEAVED>(k, pos % PER) - k * (ROWS * 2)) >> 4;
+                const int k = pos / PER, chunk = (gm_at_s<ROWS, PAIRS>(k, pos % PER) - k * (ROWS * 2)) >> 4;
                 // columns past the operand's last are never stored: any of its values will do
                 at[c] = (uint32_t)(k * ld * SIZE) + 16 * min(chunk, left / CH - 1);
                 along[c] = k;
             } else {
-                const int row = pos / 8, chunk = (gm_at_c<128, INTERLEAVED>(row, pos % 8) - row * 128) >> 4;
+                const int row = pos / 8, chunk = (gm_at_c<128, PAIRS>(row, pos % 8) - row * 128) >> 4;
                 at[c] = (uint32_t)(min(row, left - 1) * ld * SIZE) + 16 * chunk;
                 along[c] = chunk * CH;
             }
@@ -550,11 +672,12 @@ __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(Ge
     const int64_t once = (p.k + SLAB - 1) / SLAB, small = PLANES == 2 ? 2 * once : 0;       // slabs of the reduction, and of the small parts
     const int64_t per = p.slabs * (PLANES == 2 ? 3 : 1), s0 = split * per;
     const int slabs = (int)max((int64_t)0, min(once + small, s0 + per) - s0);
+    constexpr bool PAIRS = F::W == 8;
     typename GemmKind<KIND>::acc acc[TQ][4] = {};
     GemmMover<SIZE, BM, QS, WAVES> q;
     GemmMover<SIZE, BN, PS, WAVES> b;
     q.template init<false>((const char *)p.q + batch * p.batch_q, p.ldq, (int64_t)tm * BM, p.rows_q, lane, wave);
-    b.template init<true>((const char *)p.p + batch * p.batch_p, p.ldp, (int64_t)tn * BN, p.rows_p, lane, wave);
+    b.template init<PAIRS>((const char *)p.p + batch * p.batch_p, p.ldp, (int64_t)tn * BN, p.rows_p, lane, wave);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     // transfer c of slab i
     auto move = [&](int i, int c) {
@@ -573,8 +696,8 @@ __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(Ge
     // operand j of half h of slab i: four of P, then Q's
     auto read = [&](int i, int h, int j, Operands &o) {
         const char *from = lds + (i & 1) * HALF;
-        if (j < 4) o.a[j] = gm_operand<128, BN, PS, true>(from + BM * 128, wp, j, h, lane);
-        else o.b[j - 4] = gm_operand<128, BM, QS, false>(from, 0, tq0 + j - 4, h, lane);
+        if (j < 4) o.a[j] = gm_operand<128, BN, PS, PAIRS>(from + BM * 128, 4 * wp + j, h, lane);
+        else o.b[j - 4] = gm_operand<128, BM, QS, false>(from, tq0 + j - 4, h, lane);
     };
     auto read_all = [&](int i, int h, Operands &o) {
 #pragma unroll
@@ -637,29 +760,8 @@ __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(Ge
         half.template operator()<false>(i + 1, 0, second, first);
     }
     if (PLANES == 2 && s0 + slabs <= small) scale();
-    const int n = tn * BN + 64 * wp + 16 * (lane >> 4);
-    typename F::Cols cols;
-    if (p.splits == 1) f.columns(n, cols);
-#pragma unroll
-    for (int i = 0; i < TQ; ++i) {
-        const int64_t m = (int64_t)tm * BM + 16 * (tq0 + i) + (lane & 15);
-        float v[16];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * t + j] = (float)acc[i][t][j];
-        if (p.splits == 1) f.finish(cols, batch, m, n, v);
-        else if (m < p.m && n < p.n) gm_store<float, 16>(v, p.part + ((int64_t)split * p.m + m) * p.n + n, p.n - n);
-    }
+    gm_results<TQ>(p, f, batch, split, (int64_t)tm * BM + 16 * tq0, tn * BN + 64 * wp, lane, acc);
 }
-
-template <typename E>
-struct LinearEpi {
-    GemmEpi e;
-    typedef GemmCols<16> Cols;
-    __device__ __forceinline__ void columns(int n, Cols &c) const { gm_columns(e, n, c); }
-    __device__ __forceinline__ void finish(const Cols &c, int64_t, int64_t m, int n, float (&v)[16]) const { gm_finish<E, 16>(e, c, m, n, v); }
-};
 
 // ------------------------------------------------------------------------------------------------ few rows
 // Products of at most 16 RT rows, bound by reading P once: a workgroup takes 16 CT columns of D, its waves share the reduction (blocks of four instructions' worth,
@@ -769,6 +871,6 @@ __global__ __launch_bounds__(64 * GR_WAVES) void gemm_rows_kernel(GemmP p)
         GemmCols<4> cols;
         gm_columns(p.epi, min(n, p.n - 1), cols);
         float v[4] = {(float)s[0], (float)s[1], (float)s[2], (float)s[3]};
-        gm_finish<E, 4>(p.epi, cols, 16 * (j / CT) + r, n, v);
+        gm_finish<E, 4>(p.epi, cols, gm_ahead<E, 4>(p.epi, 16 * (j / CT) + r, n), 16 * (j / CT) + r, n, v);
     }
 }

@@ -7,12 +7,13 @@
 static int gm_units() { const int cus = fgnn_current_device_compute_units(); return cus > 0 ? cus : 256; }
 static int gm_slab_of(int kind) { return kind == FGNN_F32 ? 32 : kind == FGNN_I8 ? 128 : 64; }
 
-// How a reduction is cut so that a small result still fills the device: two workgroups a compute unit (one of 256 x 256), four slabs each at the least.
-static void gm_cut(GemmP *p, int tile, int kind)
+// How a reduction is cut so that a small result still fills the device, four slabs a part at the least.  The kernel that moves its operands to LDS by itself
+// fills a compute unit with one workgroup (2048^3 bf16 26.7 us, cut in two for two workgroups 39.5), the one that converts them wants two (fp32 118 / 97).
+static void gm_cut(GemmP *p, int tile, int kind, bool moved)
 {
     p->tiles_m = (int)((p->m + tile - 1) / tile);
     p->tiles_n = (p->n + tile - 1) / tile;
-    const int slab = gm_slab_of(kind), fill = (tile == 256 ? 1 : 2) * gm_units();
+    const int slab = gm_slab_of(kind), fill = (moved ? 1 : 2) * gm_units();
     const int64_t tiles = (int64_t)p->tiles_m * p->tiles_n, slabs = (p->k + slab - 1) / slab;
     int64_t splits = 1;
     if (tiles > 0 && tiles < fill) splits = std::max<int64_t>(1, std::min<int64_t>({fill / tiles, slabs / 4, 256}));
@@ -89,7 +90,7 @@ static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool strided)
     if (m <= 16 && !strided) return 0;
     GemmP p{};
     p.m = m; p.n = n; p.k = k;
-    gm_cut(&p, 128, kind);
+    gm_cut(&p, 128, kind, false);          // (what moves its operands is cut into fewer)
     return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
 }
 
@@ -100,7 +101,7 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
     const bool moved = p.k > 0 && gm_movable(p.q, p.ldq, qs ? p.m : p.k, kind) && gm_movable(p.p, p.ldp, ps ? p.n : p.k, kind);
     const bool few = !qs && !ps && gm_few(p, kind, moved);
     const int tile = moved ? gm_tile_for(p.m, p.n) : 128;
-    gm_cut(&p, tile, kind);
+    gm_cut(&p, tile, kind, moved);
     if (few) p.splits = 1;
     FGNN_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1ll << 31) && (p.m * ((p.n + 3) / 4) + 255) / 256 < (1ll << 31), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
     FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * p.m * p.n * sizeof(float)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
@@ -114,7 +115,10 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
             else if (moved) gm_launch_moved<KIND, E, 128>(p, qs, ps, st);
             else gm_launch_any<KIND, E>(p, qs, ps, st);
         } else gm_launch_any<KIND, E>(p, qs, ps, st);
-        if (p.splits > 1) hipLaunchKernelGGL((gemm_join_kernel<E>), dim3((unsigned)((p.m * ((p.n + 3) / 4) + 255) / 256)), dim3(256), 0, st, p);
+        if (p.splits == 1) return;
+        const int64_t quads = p.m * ((p.n + 3) / 4);
+        if (p.splits >= 16 && quads < 256 * 256) hipLaunchKernelGGL((gemm_join_kernel<E, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((gemm_join_kernel<E, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p);
     };
     if (kind == FGNN_F32) launch.template operator()<FGNN_F32, float>();
     else if (kind == FGNN_BF16) launch.template operator()<FGNN_BF16, __bf16>();
@@ -226,8 +230,7 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(SlopeP p)
             if (p.act) {
                 float z[V];
                 gm_load<E, V>(z, (const E *)p.z + row * p.n + c, count);
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[i] *= gm_act_slope(z[i], p.act, p.slope);
+                gm_act_slope(g, z, p.act, p.slope);
             }
             if (p.dz) gm_store<E, V>(g, (E *)p.dz + row * p.n + c, count);
 #pragma unroll

@@ -25,48 +25,82 @@ static int64_t om_plane(const OrthM &m) { return m.rows * m.ld; }
 
 // D = alpha sums + beta C as two planes, or as values of a floating type (`out`, contiguous).
 struct OrthEpi {
+    static constexpr int W = 8, ROWS = 2;
     OrthM c, d;
     void *out; int type;
     float alpha, beta;
+    int mirror;                             // D is symmetric, and what lies further than a tile of so many rows above the diagonal is written from below it; 0: it is not
     struct Cols {};
     __device__ __forceinline__ void columns(int, Cols &) const {}
-    __device__ __forceinline__ void finish(const Cols &, int64_t batch, int64_t m, int n, float (&v)[16]) const
+    struct Ahead { or_h8 hi, lo; };
+    __device__ __forceinline__ Ahead ahead(int64_t batch, int64_t m, int n) const
+    {
+        Ahead a = {};
+        if (beta != 0.f) {
+            const int64_t plane = d.rows * d.ld, at = batch * 2 * plane + (m < d.rows && n < d.ld ? m * d.ld + n : 0);
+            a.hi = *reinterpret_cast<const or_h8 *>(c.p + at);
+            a.lo = *reinterpret_cast<const or_h8 *>(c.p + plane + at);
+        }
+        return a;
+    }
+    __device__ __forceinline__ void finish(const Cols &, const Ahead &a, int64_t batch, int64_t m, int n, float (&v)[W]) const
     {
         const int64_t plane = d.rows * d.ld;
-        const int count = (out ? d.cols : (int)d.ld) - n;
-        if (m >= d.rows || count <= 0) return;
+        if (m >= d.rows || n >= d.ld) return;                   // (rows are whole chunks of eight)
         const int64_t at = batch * 2 * plane + m * d.ld + n;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= alpha;
+        for (int i = 0; i < W; ++i) v[i] *= alpha;
         if (beta != 0.f) {
-            float hi[16], lo[16];
-            gm_load<_Float16, 16>(hi, c.p + at, (int)d.ld - n);
-            gm_load<_Float16, 16>(lo, c.p + plane + at, (int)d.ld - n);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = fmaf(beta, fmaf(lo[i], 0x1p-11f, hi[i]), v[i]);
+            for (int i = 0; i < W; ++i) v[i] = fmaf(beta, fmaf((float)a.lo[i], 0x1p-11f, (float)a.hi[i]), v[i]);
         }
         const int64_t to = (batch * d.rows + m) * d.cols + n;
-        if (out && type == FGNN_F32) gm_store<float, 16>(v, (float *)out + to, count);
-        else if (out && type == FGNN_BF16) gm_store<__bf16, 16>(v, (__bf16 *)out + to, count);
-        else if (out) gm_store<_Float16, 16>(v, (_Float16 *)out + to, count);
+        if (out && type == FGNN_F32) gm_store<float, W>(v, (float *)out + to, d.cols - n);
+        else if (out && type == FGNN_BF16) gm_store<__bf16, W>(v, (__bf16 *)out + to, d.cols - n);
+        else if (out) gm_store<_Float16, W>(v, (_Float16 *)out + to, d.cols - n);
         else {
-            or_h8 hi[2], lo[2];
+            or_h8 hi, lo;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < W; ++i) {
                 _Float16 a, b;
                 or_split(n + i < d.cols ? v[i] : 0.f, a, b);
-                hi[i / 8][i % 8] = a; lo[i / 8][i % 8] = b;
+                hi[i] = a; lo[i] = b;
             }
-            // (rows are whole chunks of eight)
+            *reinterpret_cast<or_h8 *>(d.p + at) = hi;
+            *reinterpret_cast<or_h8 *>(d.p + plane + at) = lo;
+            if (mirror && n / mirror < m / mirror) {
+                // 16 lanes have 16 consecutive m: 32 bytes of a row at a time
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (8 * j < count) {
-                    *reinterpret_cast<or_h8 *>(d.p + at + 8 * j) = hi[j];
-                    *reinterpret_cast<or_h8 *>(d.p + plane + at + 8 * j) = lo[j];
-                }
+                for (int i = 0; i < W; ++i)
+                    if (n + i < d.cols) {
+                        _Float16 *to = d.p + batch * 2 * plane + (n + i) * d.ld + m;
+                        to[0] = hi[i];
+                        to[plane] = lo[i];
+                        if (m == d.rows - 1)                // and the row's padding
+                            for (int64_t c = 1; m + c < d.ld; ++c) to[c] = to[plane + c] = (_Float16)0.f;
+                    }
+            }
         }
     }
 };
+
+// The partial sums of a cut reduction, added up in their order: eight columns a thread, 16 rows side by side.
+__global__ __launch_bounds__(256) void orth_join_kernel(GemmP p, OrthEpi f)
+{
+    const int64_t batch = blockIdx.z, m = (int64_t)blockIdx.y * 16 + (threadIdx.x & 15);
+    const int n = (int)blockIdx.x * 128 + ((int)threadIdx.x >> 4) * 8;
+    if (m >= p.m || n >= p.n || (f.mirror && n / f.mirror > m / f.mirror)) return;
+    const OrthEpi::Ahead a = f.ahead(batch, m, n);
+    float v[8] = {};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        float u[8];
+        gm_load<float, 8>(u, p.part + ((batch * p.splits + s) * p.m + m) * p.n + n, p.n - n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += u[i];
+    }
+    f.finish({}, a, batch, m, n, v);
+}
 
 // ------------------------------------------------------------------------------------------------ norm and planes of X_0
 #define OR_PARTS 256                        // most workgroups that share a matrix's norm
@@ -157,27 +191,60 @@ static OrthShape or_shape(int64_t m, int64_t n)
     return s;
 }
 
+// How a product of D [m, n] over k is laid out: tiles of 256 x 256 where they fill the device or the reduction is long enough to be cut for it, of 128 x 128 else.
+struct OrthPlan { int tile, splits; int64_t slabs; };
+static OrthPlan or_plan(int64_t m, int64_t n, int64_t k, int batch, bool lower)
+{
+    const int cus = fgnn_current_device_compute_units(), units = cus > 0 ? cus : 256;
+    auto tiles = [&](int64_t t) { const int64_t a = (m + t - 1) / t, b = (n + t - 1) / t; return batch * (lower ? a * (a + 1) / 2 : a * b); };
+    const int64_t slabs = (k + 63) / 64;
+    auto cut = [&](int64_t t) {
+        // (a slab of the reduction is three of the kernel's)
+        const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({units / tiles(t), slabs / 4, 16})), each = (slabs + splits - 1) / splits;
+        return OrthPlan{(int)t, (int)((slabs + each - 1) / each), each};
+    };
+    if (tiles(256) >= units) return OrthPlan{256, 1, slabs};
+    const OrthPlan big = cut(256);
+    return tiles(256) * big.splits * 4 >= units * 3 ? big : cut(128);
+}
+
+template <bool QS, bool PS>
+static void or_product(GemmP p, OrthEpi f, int batch, bool lower, float *part, hipStream_t st)
+{
+    const OrthPlan plan = or_plan(p.m, p.n, p.k, batch, lower);
+    p.splits = plan.splits; p.slabs = plan.slabs; p.part = part; p.lower = lower;
+    f.mirror = lower ? plan.tile : 0;
+    auto go = [&]<int TILE>() {
+        p.tiles_m = (int)((p.m + TILE - 1) / TILE);
+        p.tiles_n = (p.n + TILE - 1) / TILE;
+        const int64_t tiles = lower ? (int64_t)p.tiles_m * (p.tiles_m + 1) / 2 : (int64_t)p.tiles_m * p.tiles_n;
+        hipLaunchKernelGGL((gemm_moved_kernel<FGNN_F16, OrthEpi, QS, PS, TILE, TILE, 2>), dim3((unsigned)(tiles * p.splits), (unsigned)batch), dim3(64 * gm_waves(TILE, TILE)),
+                           gm_moved_lds(TILE, TILE), st, p, f);
+    };
+    if (plan.tile == 256) go.template operator()<256>();
+    else go.template operator()<128>();
+    if (p.splits > 1) hipLaunchKernelGGL(orth_join_kernel, dim3((unsigned)((p.n + 127) / 128), (unsigned)((p.m + 15) / 16), (unsigned)batch), dim3(256), 0, st, p, f);
+}
+
+// Partial sums of the product that needs the most of them.
+static size_t or_part_bytes(int batch, const OrthShape &s, int m, int n)
+{
+    size_t most = 0;
+    auto see = [&](int64_t rows, int64_t cols, int64_t k, bool lower) {
+        const OrthPlan p = or_plan(rows, cols, k, batch, lower);
+        if (p.splits > 1) most = std::max(most, (size_t)batch * p.splits * rows * cols * sizeof(float));
+    };
+    see(s.small, s.small, s.tall ? m : s.ld_x, true);
+    see(s.small, s.small, s.ld_s, true);
+    see(m, n, s.tall ? s.ld_s : s.small, false);
+    return most;
+}
+
 extern "C" size_t fgnn_orthogonalize_workspace_bytes(int batch, int m, int n)
 {
     if (batch < 1 || m < 1 || n < 1) return 0;
     const OrthShape s = or_shape(m, n);
-    return (size_t)batch * ((size_t)s.parts * sizeof(float) + 2 * 2 * sizeof(_Float16) * ((size_t)m * s.ld_x + (size_t)s.small * s.ld_s)) + 5 * 256;
-}
-
-template <bool QS, bool PS>
-static void or_product(GemmP p, const OrthEpi &f, int batch, hipStream_t st)
-{
-    p.splits = 1;
-    p.slabs = (p.k + 63) / 64;
-    auto go = [&]<int TILE>() {
-        p.tiles_m = (int)((p.m + TILE - 1) / TILE);
-        p.tiles_n = (p.n + TILE - 1) / TILE;
-        hipLaunchKernelGGL((gemm_moved_kernel<FGNN_F16, OrthEpi, QS, PS, TILE, TILE, 2>), dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)batch),
-                           dim3(64 * gm_waves(TILE, TILE)), gm_moved_lds(TILE, TILE), st, p, f);
-    };
-    const int cus = fgnn_current_device_compute_units();
-    if (((p.m + 255) / 256) * ((p.n + 255) / 256) * batch >= (cus > 0 ? cus : 256)) go.template operator()<256>();
-    else go.template operator()<128>();
+    return (size_t)batch * ((size_t)s.parts * sizeof(float) + 2 * 2 * sizeof(_Float16) * ((size_t)m * s.ld_x + (size_t)s.small * s.ld_s)) + or_part_bytes(batch, s, m, n) + 7 * 256;
 }
 
 static GemmP or_operands(const OrthM &q, bool qs, const OrthM &p, bool ps, int64_t m, int n, int64_t k)
@@ -210,14 +277,14 @@ extern "C" int fgnn_orthogonalize(int batch, int m, int n, int type, const void 
     auto take = [&](size_t bytes) { char *p = at; at += fgnn_align256(bytes); return p; };
     auto matrix = [&](int64_t rows, int cols, int64_t ld) { return OrthM{(_Float16 *)take((size_t)batch * 2 * rows * ld * sizeof(_Float16)), rows, ld, cols}; };
     OrthM x = matrix(m, n, s.ld_x), y = matrix(m, n, s.ld_x), a = matrix(s.small, (int)s.small, s.ld_s), b = matrix(s.small, (int)s.small, s.ld_s);
-    float *part = (float *)take((size_t)batch * s.parts * sizeof(float));
+    float *norms = (float *)take((size_t)batch * s.parts * sizeof(float)), *part = (float *)take(or_part_bytes(batch, s, m, n));
 
     double top = 1.001;
     float sx = or_scale(top);
     fe_dispatch(type, [&]<typename E>() {
-        hipLaunchKernelGGL((orth_norm_kernel<E>), dim3(s.parts, batch), dim3(256), 0, st, (const E *)g, (int64_t)m * n, part);
+        hipLaunchKernelGGL((orth_norm_kernel<E>), dim3(s.parts, batch), dim3(256), 0, st, (const E *)g, (int64_t)m * n, norms);
         const unsigned blocks = (unsigned)std::min<int64_t>((om_plane(x) / 8 + 255) / 256, 4096);
-        hipLaunchKernelGGL((orth_planes_kernel<E>), dim3(blocks, batch), dim3(256), 0, st, (const E *)g, (const float *)part, s.parts, eps, sx, x);
+        hipLaunchKernelGGL((orth_planes_kernel<E>), dim3(blocks, batch), dim3(256), 0, st, (const E *)g, (const float *)norms, s.parts, eps, sx, x);
     });
     for (int i = 0; i < steps; ++i) {
         const float *c = coefficients + 3 * i;
@@ -225,15 +292,15 @@ extern "C" int fgnn_orthogonalize(int batch, int m, int n, int type, const void 
         top = or_reach(c[0], c[1], c[2], top) * 1.001;
         const float sy = or_scale(top);
         const int small = (int)s.small;
-        OrthEpi f{{}, a, nullptr, type, sa / (sx * sx), 0.f};
-        if (s.tall) or_product<true, true>(or_operands(x, true, x, true, small, small, m), f, batch, st);
-        else or_product<false, false>(or_operands(x, false, x, false, small, small, s.ld_x), f, batch, st);
-        f = OrthEpi{a, b, nullptr, type, sb * c[2] / (sa * sa), sb * c[1] / sa};
-        or_product<false, false>(or_operands(a, false, a, false, small, small, s.ld_s), f, batch, st);
+        OrthEpi f{{}, a, nullptr, type, sa / (sx * sx), 0.f, 0};
+        if (s.tall) or_product<true, true>(or_operands(x, true, x, true, small, small, m), f, batch, true, part, st);
+        else or_product<false, false>(or_operands(x, false, x, false, small, small, s.ld_x), f, batch, true, part, st);
+        f = OrthEpi{a, b, nullptr, type, sb * c[2] / (sa * sa), sb * c[1] / sa, 0};
+        or_product<false, false>(or_operands(a, false, a, false, small, small, s.ld_s), f, batch, true, part, st);
         const bool last = i == steps - 1;
-        f = OrthEpi{x, y, last ? out : nullptr, type, (last ? 1.f : sy) / (sb * sx), (last ? 1.f : sy) * c[0] / sx};
-        if (s.tall) or_product<false, false>(or_operands(x, false, b, false, m, small, s.ld_s), f, batch, st);
-        else or_product<false, true>(or_operands(b, false, x, true, small, n, small), f, batch, st);
+        f = OrthEpi{x, y, last ? out : nullptr, type, (last ? 1.f : sy) / (sb * sx), (last ? 1.f : sy) * c[0] / sx, 0};
+        if (s.tall) or_product<false, false>(or_operands(x, false, b, false, m, small, s.ld_s), f, batch, false, part, st);
+        else or_product<false, true>(or_operands(b, false, x, true, small, n, small), f, batch, false, part, st);
         std::swap(x, y);
         sx = sy;
     }
