@@ -77,16 +77,17 @@ _SIGNATURES = {
     "fgnn_rms_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "fgnn_rms_norm_backward": (c_int, [c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_size_t, c_void_p]),
-    "fgnn_linear_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "fgnn_linear_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int]),
     "fgnn_linear": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_int, c_float, c_void_p,
                             c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_linear_q8": (c_int, [c_int64, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64,
                                c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_linear_slope_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
-    "fgnn_linear_slope": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
-    "fgnn_linear_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
-    "fgnn_linear_dx": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "fgnn_linear_dw": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fgnn_linear_slope": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_float, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_size_t,
+                                  c_void_p]),
+    "fgnn_linear_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int]),
+    "fgnn_linear_dx": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fgnn_linear_dw": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_orthogonalize_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "fgnn_orthogonalize": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_knn_graph": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),

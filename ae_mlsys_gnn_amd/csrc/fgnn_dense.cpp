@@ -58,6 +58,12 @@ Rows rows_of(const Tensor &t)
     if ((cols > 1 && r.stride(1) != 1) || (rows > 1 && r.stride(0) < cols)) r = r.contiguous();
     return {r, rows, cols, rows > 1 ? r.stride(0) : cols};
 }
+// Whether rows do not all start at 16 bytes and hold whole 16 bytes.
+bool loose(const Rows &r)
+{
+    const int64_t size = r.t.element_size();
+    return ((uintptr_t)r.t.data_ptr() | r.ld * size | r.cols * size) & 15;
+}
 Tensor like(const Tensor &t, at::IntArrayRef shape) { return at::empty(shape, t.options()); }
 Tensor like(const Tensor &t, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, t.options().dtype(type)); }
 Tensor scratch(const Tensor &t, size_t bytes) { return bytes ? at::empty({(int64_t)bytes}, t.options().dtype(at::kByte)) : Tensor(); }
@@ -237,7 +243,7 @@ LinearOut linear_forward(const Tensor &x, const Tensor &w, const Tensor &bias, c
     const c10::OptionalDeviceGuard guard(x.device());
     LinearOut out{like(x, with_last(x, n)), {}};
     if (keep) out.z = like(x, {a.rows, n});
-    const size_t bytes = fgnn_linear_workspace_bytes(a.rows, n, k, type);
+    const size_t bytes = fgnn_linear_workspace_bytes(a.rows, n, k, type, loose(a) || loose(b));
     const Tensor ws = scratch(x, bytes);
     check(fgnn_linear(a.rows, n, k, type, address(a.t), a.ld, address(b.t), b.ld, address(e.bias), e.btype, address(e.res.t), e.res.ld, (int)act, (float)slope, address(out.z), address(out.y),
                       address(ws), bytes, stream_of(x)), "fgnn_linear");
@@ -273,22 +279,25 @@ struct Linear : torch::autograd::Function<Linear> {
         if (need & 4) db = like(x.t, {n}, bias);
         if (n && (sloped || (need & 4))) {
             const Rows g = dz;
-            if (sloped) dz = Rows{like(x.t, {x.rows, n}), x.rows, n, n};
+            if (sloped) {
+                const int64_t width = 16 / x.t.element_size(), ld = (n + width - 1) / width * width;
+                dz = Rows{like(x.t, {x.rows, ld}), x.rows, n, ld};
+            }
             const size_t bytes = need & 4 ? fgnn_linear_slope_workspace_bytes(x.rows, n, type) : 0;
             const Tensor ws = scratch(x.t, bytes);
-            check(fgnn_linear_slope(x.rows, n, type, address(g.t), g.ld, address(saved[2]), act, (float)ctx->saved_data["slope"].toDouble(), sloped ? address(dz.t) : nullptr, address(db),
+            check(fgnn_linear_slope(x.rows, n, type, address(g.t), g.ld, address(saved[2]), act, (float)ctx->saved_data["slope"].toDouble(), sloped ? address(dz.t) : nullptr, dz.ld, address(db),
                                     db.defined() ? float_type(db) : type, address(ws), bytes, stream), "fgnn_linear_slope");
         }
         if (need & 3) {
-            const size_t bytes = fgnn_linear_backward_workspace_bytes(x.rows, n, k, type);
+            const size_t bytes = fgnn_linear_backward_workspace_bytes(x.rows, n, k, type, loose(x) || loose(w) || (!sloped && loose(dz)));
             const Tensor ws = scratch(x.t, bytes);
             if (need & 1) {
                 dx = like(x.t, saved[0].sizes());
-                check(fgnn_linear_dx(x.rows, n, k, type, address(dz.t), dz.ld, address(w.t), w.ld, address(dx), address(ws), bytes, stream), "fgnn_linear_dx");
+                check(fgnn_linear_dx(x.rows, n, k, type, address(dz.t), dz.ld, sloped, address(w.t), w.ld, address(dx), address(ws), bytes, stream), "fgnn_linear_dx");
             }
             if (need & 2) {
                 dw = like(x.t, {n, k});
-                check(fgnn_linear_dw(x.rows, n, k, type, address(dz.t), dz.ld, address(x.t), x.ld, address(dw), address(ws), bytes, stream), "fgnn_linear_dw");
+                check(fgnn_linear_dw(x.rows, n, k, type, address(dz.t), dz.ld, sloped, address(x.t), x.ld, address(dw), address(ws), bytes, stream), "fgnn_linear_dw");
             }
         }
         return final_gradients("linear_act", {dx, dw, db, need & 8 ? up[0] : Tensor(), Tensor(), Tensor()});
@@ -321,7 +330,7 @@ Tensor linear_q8(const Tensor &q, const Tensor &scale, const Tensor &w, const Te
     const Tensor s = scale.contiguous(), ws = wscale.contiguous();
     const c10::OptionalDeviceGuard guard(q.device());
     const Tensor y = like(q, with_last(q, n), to);
-    const size_t bytes = fgnn_linear_workspace_bytes(x.rows, n, k, eight);
+    const size_t bytes = fgnn_linear_workspace_bytes(x.rows, n, k, eight, loose(x) || loose(p));
     const Tensor work = scratch(q, bytes);
     check(fgnn_linear_q8(x.rows, n, k, eight, type, address(x.t), x.ld, (const float *)address(s), address(p.t), p.ld, (const float *)address(ws), address(e.bias), e.btype, address(e.res.t),
                          e.res.ld, (int)act, (float)slope, address(y), address(work), bytes, stream_of(q)), "fgnn_linear_q8");

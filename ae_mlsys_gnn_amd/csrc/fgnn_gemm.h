@@ -659,15 +659,12 @@ template <int LEFT> __device__ __forceinline__ void gm_arrive() { asm volatile("
 // Waves of 64 columns by 128 rows in tiles of 256 x 256, by 64 rows in smaller ones.
 constexpr int gm_waves(int bm, int bn) { return bm * bn / 64 / (bm >= 256 ? 128 : 64); }
 constexpr size_t gm_moved_lds(int bm, int bn) { return (size_t)2 * (bm + bn) * 128; }
+// One tile of D.  lds: [2][BM + BN][128], which no wave reads any more.
 template <int KIND, typename F, bool QS, bool PS, int BM, int BN, int PLANES>
-__global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(GemmP p, F f)
+__device__ __forceinline__ void gm_moved_tile(const GemmP &p, const F &f, int tm, int tn, int split, int64_t batch, char *lds)
 {
     constexpr int WAVES = gm_waves(BM, BN), WP = BN / 64, TQ = BM / 16 / (WAVES / WP), SIZE = GemmKind<KIND>::size, SLAB = 128 / SIZE;
     constexpr int MOVES = (BM + BN) * 128 / 1024 / WAVES, HALF = (BM + BN) * 128;          // transfers of a wave, and bytes, a slab
-    extern __shared__ __attribute__((aligned(16))) char lds[];                              // [2][BM + BN][128]
-    int tm, tn, split;
-    gm_tile(p, tm, tn, split);
-    const int64_t batch = blockIdx.y;
     const int lane = fg_lane(), wave = fg_wave(), wp = wave % WP, tq0 = wave / WP * TQ;
     const int64_t once = (p.k + SLAB - 1) / SLAB, small = PLANES == 2 ? 2 * once : 0;       // slabs of the reduction, and of the small parts
     const int64_t per = p.slabs * (PLANES == 2 ? 3 : 1), s0 = split * per;
@@ -761,6 +758,91 @@ __global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(Ge
     }
     if (PLANES == 2 && s0 + slabs <= small) scale();
     gm_results<TQ>(p, f, batch, split, (int64_t)tm * BM + 16 * tq0, tn * BN + 64 * wp, lane, acc);
+}
+template <int KIND, typename F, bool QS, bool PS, int BM, int BN, int PLANES>
+__global__ __launch_bounds__(64 * gm_waves(BM, BN), 2) void gemm_moved_kernel(GemmP p, F f)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    int tm, tn, split;
+    gm_tile(p, tm, tn, split);
+    gm_moved_tile<KIND, F, QS, PS, BM, BN, PLANES>(p, f, tm, tn, split, blockIdx.y, lds);
+}
+
+// The same for two planes on a tile of 128 x 128, eight waves of 64 columns by 32 rows: a slab holds both planes of both operands and gives all three products (four
+// parts moved for six), with sums of their own for the small ones.  Reductions that are short, or tiles that are few, wait for memory once a slab: a third
+// as often.  lds: [2][4][128][128], which no wave reads any more.
+constexpr size_t GM_PLANES_LDS = 2 * 4 * 128 * 128;
+#define GM_PLANES_WAVES 8
+template <typename F, bool QS, bool PS>
+__device__ __forceinline__ void gm_planes_tile(const GemmP &p, const F &f, int tm, int tn, int split, int64_t batch, char *lds)
+{
+    constexpr int WAVES = GM_PLANES_WAVES, TQ = 2, PART = 128 * 128, HALF = 4 * PART;       // parts: Q hi, Q lo, P hi, P lo
+    constexpr bool PAIRS = F::W == 8;
+    const int lane = fg_lane(), wave = fg_wave(), wp = wave & 1, tq0 = (wave >> 1) * TQ;
+    const int64_t s0 = split * p.slabs;
+    const int slabs = (int)max((int64_t)0, min((p.k + 63) / 64, s0 + p.slabs) - s0);
+    GemmMover<2, 128, QS, WAVES> q;
+    GemmMover<2, 128, PS, WAVES> b;
+    q.template init<false>((const char *)p.q + batch * p.batch_q, p.ldq, (int64_t)tm * 128, p.rows_q, lane, wave);
+    b.template init<PAIRS>((const char *)p.p + batch * p.batch_p, p.ldp, (int64_t)tn * 128, p.rows_p, lane, wave);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    auto move = [&](int i) {
+        const int64_t at = s0 + i, left = p.k - at * 64;
+        const uint32_t to = lds0 + (i & 1) * HALF;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < q.COUNT; ++c) {
+                q.move(c, at, h * p.plane_q, left, to + h * PART, wave);
+                b.move(c, at, h * p.plane_p, left, to + (2 + h) * PART, wave);
+            }
+    };
+    constexpr int MOVES = 4 * GemmMover<2, 128, QS, WAVES>::COUNT;
+    gm_f4 acc[TQ][4] = {}, low[TQ][4] = {};
+    if (slabs > 0) move(0);
+    if (slabs > 1) move(1);
+#pragma unroll 1
+    for (int i = 0; i < slabs; ++i) {
+        if (i + 1 < slabs) gm_arrive<MOVES>();
+        else gm_arrive<0>();
+        const char *from = lds + (i & 1) * HALF;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            gm_i4 a[2][4], x[2][TQ];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) a[e][u] = gm_operand<128, 128, PS, PAIRS>(from + (2 + e) * PART, 4 * wp + u, h, lane);
+#pragma unroll
+                for (int t = 0; t < TQ; ++t) x[e][t] = gm_operand<128, 128, QS, false>(from + e * PART, tq0 + t, h, lane);
+            }
+#pragma unroll
+            for (int t = 0; t < TQ; ++t)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    acc[t][u] = gm_mfma<FGNN_F16>(a[0][u], x[0][t], acc[t][u]);
+                    low[t][u] = gm_mfma<FGNN_F16>(a[1][u], x[0][t], low[t][u]);
+                    low[t][u] = gm_mfma<FGNN_F16>(a[0][u], x[1][t], low[t][u]);
+                }
+        }
+        if (i + 2 < slabs) {
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");     // this slab has been read everywhere
+            move(i + 2);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TQ; ++t)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[t][u] += 0x1p-11f * low[t][u];
+    gm_results<TQ>(p, f, batch, split, (int64_t)tm * 128 + 16 * tq0, tn * 128 + 64 * wp, lane, acc);
+}
+template <typename F, bool QS, bool PS>
+__global__ __launch_bounds__(64 * GM_PLANES_WAVES, 2) void gemm_planes_kernel(GemmP p, F f)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    int tm, tn, split;
+    gm_tile(p, tm, tn, split);
+    gm_planes_tile<F, QS, PS>(p, f, tm, tn, split, blockIdx.y, lds);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows

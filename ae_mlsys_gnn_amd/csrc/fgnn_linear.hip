@@ -21,11 +21,61 @@ static void gm_cut(GemmP *p, int tile, int kind, bool moved)
     p->splits = (int)std::max<int64_t>(1, (slabs + p->slabs - 1) / p->slabs);
 }
 
+// ------------------------------------------------------------------------------------------------ operands laid out anew
+// Rows of 16-bit values, or of 8-bit floats as fp16, copied to rows of whole 16-byte chunks with zeros behind: a chunk a thread.
+template <bool E4M3>
+__global__ __launch_bounds__(256) void linear_pack_kernel(const char *from, int64_t ld, int64_t rows, int cols, char *to)
+{
+    const int chunks = (cols + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / chunks;
+    if (row >= rows) return;
+    const int c = (int)(i - row * chunks) * 8, count = cols - c;
+    gm_i4 v = {0, 0, 0, 0};
+    if constexpr (E4M3) {
+        const uint8_t *p = (const uint8_t *)from + row * ld + c;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (count >= 8) __builtin_memcpy(w, p, 8);
+        else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) if (k < count) w[k / 4] |= (uint32_t)p[k] << (8 * (k % 4));
+        }
+        gm_i4 half[2];
+        gm_widen(w, half);
+        v = half[0];
+    } else {
+        const uint16_t *p = (const uint16_t *)from + row * ld + c;
+        if (count >= 8) __builtin_memcpy(&v, p, 16);
+        else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) if (k < count) v[k / 2] |= (int)p[k] << (16 * (k % 2));
+        }
+    }
+    reinterpret_cast<gm_i4 *>(to)[i] = v;
+}
+static size_t gm_packed_bytes(int64_t rows, int64_t cols) { return fgnn_align256((size_t)rows * ((cols + 7) / 8) * 16); }
+static void gm_pack(const void *from, int64_t ld, int64_t rows, int cols, char *to, bool e4m3, hipStream_t st)
+{
+    const dim3 g((unsigned)((rows * ((cols + 7) / 8) + 255) / 256));
+    if (e4m3) hipLaunchKernelGGL(linear_pack_kernel<true>, g, dim3(256), 0, st, (const char *)from, ld, rows, cols, to);
+    else hipLaunchKernelGGL(linear_pack_kernel<false>, g, dim3(256), 0, st, (const char *)from, ld, rows, cols, to);
+}
+// Whether a product is large enough for operands that cannot be moved as they lie to be laid out anew first.  us, through registers / laid out and moved,
+// forward, input and weights' gradient: 1003^3 (1e9 products) 21 / 27, 24 / 28, 27 / 27; 2049 x 513 -> 2049 (2e9) 27 / 29, 33 / 30, 34 / 30; 5003 x 602 -> 1433
+// (4e9) 30 / 29, 54 / 35, 51 / 37; 169,343 x 129 -> 257 (6e9) 101 / 108, 94 / 89, 150 / 101; 8191 x 4097 -> 4095 399 / 270, 546 / 325, 1106 / 408; 8-bit
+// floats 8192 x 4096 -> 8192 577 / 407.
+static bool gm_worth_packing(int64_t m, int64_t n, int64_t k, int kind)
+{
+    const double most = (double)std::max(m, n) * ((k + 7) / 8 + 1);       // chunks of an operand: a launch's threads
+    return (kind == FGNN_BF16 || kind == FGNN_F16 || kind == FGNN_E4M3) && most < 2e11 && (double)m * n * k >= 3e9;
+}
+
 // Whether rows of an operand are whole 16-byte chunks at 16-byte addresses, and near enough for 32-bit offsets in a tile.
-static bool gm_movable(const void *p, int64_t ld, int64_t inner, int kind)
+// (padded: zeros follow a row up to whole chunks)
+static bool gm_movable(const void *p, int64_t ld, int64_t inner, int kind, bool padded)
 {
     const int ch = 16 / fe_size(kind);
-    return kind != FGNN_F32 && kind != FGNN_E4M3 && fgnn_aligned16(p) && ld % ch == 0 && inner % ch == 0 && inner > 0 && ld * fe_size(kind) * 256 < (1ll << 31);
+    return kind != FGNN_F32 && kind != FGNN_E4M3 && fgnn_aligned16(p) && ld % ch == 0 && (padded ? ld >= (inner + ch - 1) / ch * ch : inner % ch == 0) && inner > 0
+        && ld * fe_size(kind) * 256 < (1ll << 31);
 }
 
 template <int KIND, typename E>
@@ -37,13 +87,22 @@ static void gm_launch_any(const GemmP &p, bool qs, bool ps, hipStream_t st)
     else if (ps) hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, true>), g, b, 0, st, p);
     else hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, false>), g, b, 0, st, p);
 }
-template <int KIND, typename E, int TILE>
+template <typename E>
+static void gm_join(const GemmP &p, hipStream_t st)
+{
+    if (p.splits == 1) return;
+    // eight threads a column where it has many parts and there are few columns (256 x 128 of 128 parts 67 / 12 us)
+    const int64_t quads = p.m * ((p.n + 3) / 4);
+    if (p.splits >= 16 && quads < 256 * 256) hipLaunchKernelGGL((gemm_join_kernel<E, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((gemm_join_kernel<E, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p);
+}
+template <int KIND, typename E, int TILE, bool FORWARD = false>
 static void gm_launch_moved(const GemmP &p, bool qs, bool ps, hipStream_t st)
 {
     const dim3 g((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), b(64 * gm_waves(TILE, TILE));
     const size_t lds = gm_moved_lds(TILE, TILE);
     const LinearEpi<E> f{p.epi};
-    if constexpr (fe_size_of<KIND> == 1) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, false, TILE, TILE, 1>), g, b, lds, st, p, f);
+    if constexpr (fe_size_of<KIND> == 1 || FORWARD) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, false, TILE, TILE, 1>), g, b, lds, st, p, f);
     else if (qs) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, true, true, TILE, TILE, 1>), g, b, lds, st, p, f);
     else if (ps) hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, true, TILE, TILE, 1>), g, b, lds, st, p, f);
     else hipLaunchKernelGGL((gemm_moved_kernel<KIND, LinearEpi<E>, false, false, TILE, TILE, 1>), g, b, lds, st, p, f);
@@ -85,20 +144,47 @@ static int gm_tile_for(int64_t m, int n)
     return ((m + 255) / 256) * ((n + 255) / 256) >= gm_units() ? 256 : 128;
 }
 
-static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool strided)
+// Partial sums and operands laid out anew; loose: an operand may not be movable as it lies.
+static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool qs, bool ps, bool loose)
 {
-    if (m <= 16 && !strided) return 0;
+    if (m <= 16 && !qs && !ps) return 0;
     GemmP p{};
     p.m = m; p.n = n; p.k = k;
     gm_cut(&p, 128, kind, false);          // (what moves its operands is cut into fewer)
-    return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
+    size_t bytes = p.splits > 1 ? fgnn_align256((size_t)p.splits * m * n * sizeof(float)) : 0;
+    if (loose && gm_worth_packing(m, n, k, kind)) bytes += (qs ? gm_packed_bytes(k, m) : gm_packed_bytes(m, k)) + (ps ? gm_packed_bytes(k, n) : gm_packed_bytes(n, k)) + 256;
+    return bytes;
 }
 
 // D [m, n] of type `type` from operands of kind `kind`; qs: Q is strided along the reduction (and P then too).
-static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, bool ps, void *workspace, size_t workspace_bytes, hipStream_t st)
+static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, bool ps, bool q_padded, void *workspace, size_t workspace_bytes, hipStream_t st)
 {
     if (p.m == 0 || p.n == 0) return 0;
-    const bool moved = p.k > 0 && gm_movable(p.q, p.ldq, qs ? p.m : p.k, kind) && gm_movable(p.p, p.ldp, ps ? p.n : p.k, kind);
+    const int64_t inner_q = qs ? p.m : p.k, inner_p = ps ? p.n : p.k;
+    const bool q_moves = p.k > 0 && gm_movable(p.q, p.ldq, inner_q, kind, q_padded), p_moves = p.k > 0 && gm_movable(p.p, p.ldp, inner_p, kind, false);
+    bool moved = q_moves && p_moves;
+    p.rows_q = qs ? (p.m + 7) / 8 * 8 : p.m;                   // (strided operands hold whole chunks of rows, or are made to)
+    p.rows_p = ps ? (p.n + 7) / 8 * 8 : p.n;
+    if (!moved && p.k > 0 && gm_worth_packing(p.m, p.n, p.k, kind) && !(!qs && !ps && gm_few(p, kind, false))) {
+        const int64_t outer_q = qs ? p.k : p.m, outer_p = ps ? p.k : p.n;
+        const size_t bytes_q = q_moves ? 0 : gm_packed_bytes(outer_q, inner_q), bytes_p = p_moves ? 0 : gm_packed_bytes(outer_p, inner_p);
+        char *to = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+        FGNN_REQUIRE(workspace && (size_t)(to - (char *)workspace) + bytes_q + bytes_p <= workspace_bytes, FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who, workspace_bytes);
+        if (!q_moves) {
+            gm_pack(p.q, p.ldq, outer_q, (int)inner_q, to, kind == FGNN_E4M3, st);
+            p.q = to;
+            p.ldq = (inner_q + 7) / 8 * 8;
+        }
+        if (!p_moves) {
+            gm_pack(p.p, p.ldp, outer_p, (int)inner_p, to + bytes_q, kind == FGNN_E4M3, st);
+            p.p = to + bytes_q;
+            p.ldp = (inner_p + 7) / 8 * 8;
+        }
+        workspace_bytes -= (size_t)(to - (char *)workspace) + bytes_q + bytes_p;
+        workspace = to + bytes_q + bytes_p;
+        if (kind == FGNN_E4M3) kind = FGNN_F16;
+        moved = true;
+    }
     const bool few = !qs && !ps && gm_few(p, kind, moved);
     const int tile = moved ? gm_tile_for(p.m, p.n) : 128;
     gm_cut(&p, tile, kind, moved);
@@ -107,7 +193,7 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
     FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * p.m * p.n * sizeof(float)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
                  workspace_bytes);
     p.part = (float *)workspace;
-    p.epi.m = p.rows_q = p.m; p.epi.n = (int)(p.rows_p = p.n);
+    p.epi.m = p.m; p.epi.n = p.n;
     auto launch = [&]<int KIND, typename E>() {
         if (few) return gm_launch_rows<KIND, E>(p, st);
         if constexpr (KIND != FGNN_F32 && KIND != FGNN_E4M3) {
@@ -115,14 +201,19 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
             else if (moved) gm_launch_moved<KIND, E, 128>(p, qs, ps, st);
             else gm_launch_any<KIND, E>(p, qs, ps, st);
         } else gm_launch_any<KIND, E>(p, qs, ps, st);
-        if (p.splits == 1) return;
-        const int64_t quads = p.m * ((p.n + 3) / 4);
-        if (p.splits >= 16 && quads < 256 * 256) hipLaunchKernelGGL((gemm_join_kernel<E, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((gemm_join_kernel<E, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p);
+        gm_join<E>(p, st);
+    };
+    // 8-bit floats as fp16: forward products of moved operands alone
+    auto launch_widened = [&]<typename E>() {
+        if (tile == 256) gm_launch_moved<FGNN_F16, E, 256, true>(p, false, false, st);
+        else gm_launch_moved<FGNN_F16, E, 128, true>(p, false, false, st);
+        gm_join<E>(p, st);
     };
     if (kind == FGNN_F32) launch.template operator()<FGNN_F32, float>();
     else if (kind == FGNN_BF16) launch.template operator()<FGNN_BF16, __bf16>();
-    else if (kind == FGNN_F16) launch.template operator()<FGNN_F16, _Float16>();
+    else if (kind == FGNN_F16 && type == FGNN_F16) launch.template operator()<FGNN_F16, _Float16>();
+    else if (kind == FGNN_F16 && type == FGNN_BF16) launch_widened.template operator()<__bf16>();
+    else if (kind == FGNN_F16) launch_widened.template operator()<float>();
     else fe_dispatch(type, [&]<typename E>() {
         if (kind == FGNN_I8) launch.template operator()<FGNN_I8, E>();
         else launch.template operator()<FGNN_E4M3, E>();
@@ -138,10 +229,10 @@ static int gm_check_epilogue(const char *who, int type, const void *bias, int bt
     return 0;
 }
 
-extern "C" size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind)
+extern "C" size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind, int loose)
 {
     if (rows < 1 || n < 1 || k < 0 || kind < FGNN_F32 || kind > FGNN_E4M3) return 0;
-    return gm_workspace(rows, n, k, kind, false);
+    return gm_workspace(rows, n, k, kind, false, false, loose || kind == FGNN_E4M3);
 }
 
 extern "C" int fgnn_linear(int64_t rows, int n, int k, int type, const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int btype,
@@ -155,7 +246,7 @@ extern "C" int fgnn_linear(int64_t rows, int n, int k, int type, const void *x, 
     GemmP p{};
     p.m = rows; p.n = n; p.k = k; p.q = x; p.ldq = ldx; p.p = weight; p.ldp = ldw;
     p.epi.bias = bias; p.epi.btype = btype; p.epi.res = residual; p.epi.ldr = ldr; p.epi.act = act; p.epi.slope = slope; p.epi.z = z; p.epi.y = y;
-    return gm_product("fgnn_linear", p, type, type, false, false, workspace, workspace_bytes, (hipStream_t)stream);
+    return gm_product("fgnn_linear", p, type, type, false, false, false, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 extern "C" int fgnn_linear_q8(int64_t rows, int n, int k, int eight, int type, const void *q, int64_t ldq, const float *scale, const void *weight, int64_t ldw,
@@ -173,10 +264,10 @@ extern "C" int fgnn_linear_q8(int64_t rows, int n, int k, int eight, int type, c
     p.m = rows; p.n = n; p.k = k; p.q = q; p.ldq = ldq; p.p = weight; p.ldp = ldw;
     p.epi.sx = scale; p.epi.sw = weight_scale;
     p.epi.bias = bias; p.epi.btype = btype; p.epi.res = residual; p.epi.ldr = ldr; p.epi.act = act; p.epi.slope = slope; p.epi.y = y;
-    return gm_product("fgnn_linear_q8", p, eight, type, false, false, workspace, workspace_bytes, (hipStream_t)stream);
+    return gm_product("fgnn_linear_q8", p, eight, type, false, false, false, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-extern "C" int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *weight, int64_t ldw, void *dx, void *workspace,
+extern "C" int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, int padded, const void *weight, int64_t ldw, void *dx, void *workspace,
                               size_t workspace_bytes, void *stream)
 {
     FGNN_REQUIRE(rows >= 0 && n >= 0 && k >= 0 && ldz >= n && ldw >= k && fe_is_float(type), FGNN_ERR_SHAPE, "fgnn_linear_dx: bad sizes rows=%lld n=%d k=%d ldz=%lld ldw=%lld type=%d",
@@ -185,10 +276,10 @@ extern "C" int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *
     GemmP p{};
     p.m = rows; p.n = k; p.k = n; p.q = dz; p.ldq = ldz; p.p = weight; p.ldp = ldw;
     p.epi.y = dx;
-    return gm_product("fgnn_linear_dx", p, type, type, false, true, workspace, workspace_bytes, (hipStream_t)stream);
+    return gm_product("fgnn_linear_dx", p, type, type, false, true, padded != 0, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-extern "C" int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *x, int64_t ldx, void *dw, void *workspace,
+extern "C" int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, int padded, const void *x, int64_t ldx, void *dw, void *workspace,
                               size_t workspace_bytes, void *stream)
 {
     FGNN_REQUIRE(rows >= 0 && n >= 0 && k >= 0 && ldz >= n && ldx >= k && fe_is_float(type), FGNN_ERR_SHAPE, "fgnn_linear_dw: bad sizes rows=%lld n=%d k=%d ldz=%lld ldx=%lld type=%d",
@@ -197,13 +288,13 @@ extern "C" int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *
     GemmP p{};
     p.m = n; p.n = k; p.k = rows; p.q = dz; p.ldq = ldz; p.p = x; p.ldp = ldx;
     p.epi.y = dw;
-    return gm_product("fgnn_linear_dw", p, type, type, true, true, workspace, workspace_bytes, (hipStream_t)stream);
+    return gm_product("fgnn_linear_dw", p, type, type, true, true, padded != 0, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-extern "C" size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type)
+extern "C" size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type, int loose)
 {
     if (rows < 1 || n < 1 || k < 1 || !fe_is_float(type)) return 0;
-    return std::max(gm_workspace(rows, k, n, type, true), gm_workspace(n, k, rows, type, true));
+    return std::max(gm_workspace(rows, k, n, type, false, true, loose), gm_workspace(n, k, rows, type, true, true, loose));
 }
 
 // ------------------------------------------------------------------------------------------------ slope and column sums
@@ -213,7 +304,7 @@ struct SlopeP {
     int64_t rows; int n;
     const void *gy; int64_t ldg; const void *z;
     int act; float slope;
-    void *dz;                               // contiguous; NULL: not wanted
+    void *dz; int64_t ldz;                  // ldz: n, or more with zeros behind n; NULL: not wanted
     float *part;                            // [grid.y][n]; NULL: not wanted
 };
 template <typename E, int TX>
@@ -232,7 +323,7 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(SlopeP p)
                 gm_load<E, V>(z, (const E *)p.z + row * p.n + c, count);
                 gm_act_slope(g, z, p.act, p.slope);
             }
-            if (p.dz) gm_store<E, V>(g, (E *)p.dz + row * p.n + c, count);
+            if (p.dz) gm_store<E, V>(g, (E *)p.dz + row * p.ldz + c, p.ldz == p.n ? count : V);          // (values past a row's end were read as zeros)
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[i] += g[i];
         }
@@ -269,12 +360,14 @@ extern "C" size_t fgnn_linear_slope_workspace_bytes(int64_t rows, int n, int typ
     return (size_t)sl_grid(rows, n, type).y * n * sizeof(float);
 }
 
-extern "C" int fgnn_linear_slope(int64_t rows, int n, int type, const void *gy, int64_t ldg, const void *z, int act, float slope, void *dz, void *dbias, int btype,
+extern "C" int fgnn_linear_slope(int64_t rows, int n, int type, const void *gy, int64_t ldg, const void *z, int act, float slope, void *dz, int64_t ldz, void *dbias, int btype,
                                  void *workspace, size_t workspace_bytes, void *stream)
 {
     FGNN_REQUIRE(rows >= 0 && n >= 1 && ldg >= n && fe_is_float(type) && act >= GM_NONE && act <= GM_LEAKY, FGNN_ERR_SHAPE,
                  "fgnn_linear_slope: bad sizes rows=%lld n=%d ldg=%lld type=%d act=%d", (long long)rows, n, (long long)ldg, type, act);
     FGNN_REQUIRE(!dbias || btype == type || btype == FGNN_F32, FGNN_ERR_SHAPE, "fgnn_linear_slope: bias of type %d", btype);
+    const int width = fe_is_float(type) ? 16 / fe_size(type) : 1;
+    FGNN_REQUIRE(!dz || ldz == n || ldz == (n + width - 1) / width * width, FGNN_ERR_SHAPE, "fgnn_linear_slope: rows of %lld for %d columns", (long long)ldz, n);
     FGNN_REQUIRE(rows == 0 || (gy && (act == GM_NONE || z)), FGNN_ERR_NULL, "fgnn_linear_slope: NULL argument");
     FGNN_REQUIRE(!dbias || rows == 0 || (workspace && workspace_bytes >= fgnn_linear_slope_workspace_bytes(rows, n, type)), FGNN_ERR_WORKSPACE,
                  "fgnn_linear_slope: workspace of %zu bytes", workspace_bytes);
@@ -283,7 +376,7 @@ extern "C" int fgnn_linear_slope(int64_t rows, int n, int type, const void *gy, 
     if (rows > 0 && (dz || dbias)) {
         const dim3 g = sl_grid(rows, n, type);
         parts = (int)g.y;
-        SlopeP p{rows, n, gy, ldg, z, act, slope, dz, dbias ? (float *)workspace : nullptr};
+        SlopeP p{rows, n, gy, ldg, z, act, slope, dz, ldz, dbias ? (float *)workspace : nullptr};
         fe_dispatch(type, [&]<typename E>() {
             switch (sl_width(n, type)) {
             case 8: hipLaunchKernelGGL((linear_slope_kernel<E, 8>), g, dim3(256), 0, st, p); break;

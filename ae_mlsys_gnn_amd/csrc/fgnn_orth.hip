@@ -21,7 +21,7 @@ __device__ __forceinline__ void or_split(float v, _Float16 &hi, _Float16 &lo)
 
 // One matrix of the iteration in memory: `rows` rows of `cols` columns, padded with zeros to `ld` (whole 16-byte chunks), two planes, a batch of them.
 struct OrthM { _Float16 *p; int64_t rows, ld; int cols; };
-static int64_t om_plane(const OrthM &m) { return m.rows * m.ld; }
+static __host__ __device__ __forceinline__ int64_t om_plane(const OrthM &m) { return m.rows * m.ld; }
 
 // D = alpha sums + beta C as two planes, or as values of a floating type (`out`, contiguous).
 struct OrthEpi {
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void orth_join_kernel(GemmP p, OrthEpi f)
 }
 
 // ------------------------------------------------------------------------------------------------ norm and planes of X_0
-#define OR_PARTS 256                        // most workgroups that share a matrix's norm
+#define OR_PARTS 1024                       // most workgroups that share a matrix's norm
 template <typename E>
 __global__ __launch_bounds__(256) void orth_norm_kernel(const E *g, int64_t size, float *part)
 {
@@ -111,6 +111,7 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(const E *g, int64_t size
     __shared__ float red[4];
     g += (int64_t)blockIdx.y * size;
     float ss = 0.f;
+#pragma unroll 4
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < size; i += (int64_t)gridDim.x * 256 * V) {
         float v[V];
         gm_load<E, V>(v, g + i, (int)min((int64_t)V, size - i));
@@ -153,6 +154,74 @@ __global__ __launch_bounds__(256) void orth_planes_kernel(const E *g, const floa
         _Float16 *to = x.p + (int64_t)blockIdx.y * 2 * plane + row * x.ld + col;
         *reinterpret_cast<or_h8 *>(to) = hi;
         *reinterpret_cast<or_h8 *>(to + plane) = lo;
+    }
+}
+
+static __host__ __device__ __forceinline__ GemmP or_operands(const OrthM &q, bool qs, const OrthM &p, bool ps, int64_t m, int n, int64_t k)
+{
+    GemmP g{};
+    g.m = m; g.n = n; g.k = k;
+    g.q = q.p; g.ldq = q.ld; g.rows_q = qs ? (m + 7) / 8 * 8 : m; g.plane_q = om_plane(q) * 2; g.batch_q = 2 * g.plane_q;
+    g.p = p.p; g.ldp = p.ld; g.rows_p = ps ? (n + 7) / 8 * 8 : n; g.plane_p = om_plane(p) * 2; g.batch_p = 2 * g.plane_p;
+    return g;
+}
+
+// ------------------------------------------------------------------------------------------------ small matrices
+// All steps of a matrix with a side of at most 128 in one launch: a workgroup goes through the three products of a step, tile by tile, and meets itself in between;
+// what it wrote comes back through its own caches.  Bound by the latency of that way, 7 us a tile.
+#define OR_STEPS 16
+struct OrthFactors { float a, b, b_c, x, x_c; };             // of the epilogues of A, B and X: of the sums, and of what is added
+struct OrthSmall {
+    OrthM x, y, a, b;
+    void *out; int type, steps;
+    OrthFactors k[OR_STEPS];
+};
+// Step i's, chosen among the arguments value by value: a copy of the table would live in memory.
+template <int J = 0>
+__device__ __forceinline__ void or_factors(const OrthSmall &s, int i, float &a, float &b, float &b_c, float &x, float &x_c)
+{
+    if constexpr (J < OR_STEPS) {
+        const float va = s.k[J].a, vb = s.k[J].b, vbc = s.k[J].b_c, vx = s.k[J].x, vxc = s.k[J].x_c;
+        a = i == J ? va : a;
+        b = i == J ? vb : b;
+        b_c = i == J ? vbc : b_c;
+        x = i == J ? vx : x;
+        x_c = i == J ? vxc : x_c;
+        or_factors<J + 1>(s, i, a, b, b_c, x, x_c);
+    }
+}
+template <bool TALL>
+__global__ __launch_bounds__(64 * GM_PLANES_WAVES, 2) void orth_small_kernel(OrthSmall s)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int64_t batch = blockIdx.x;
+    const int small = s.a.cols, tiles = (int)(((TALL ? s.x.rows : s.x.cols) + 127) / 128);
+#pragma unroll 1
+    for (int i = 0; i < s.steps; ++i) {
+        OrthM x = s.x, y = s.x;
+        x.p = i & 1 ? s.y.p : s.x.p;
+        y.p = i & 1 ? s.x.p : s.y.p;
+        OrthFactors k{};
+        or_factors(s, i, k.a, k.b, k.b_c, k.x, k.x_c);
+        GemmP p = TALL ? or_operands(x, true, x, true, small, small, x.rows) : or_operands(x, false, x, false, small, small, x.ld);
+        p.splits = 1;
+        p.slabs = (p.k + 63) / 64;
+        gm_planes_tile<OrthEpi, TALL, TALL>(p, OrthEpi{{}, s.a, nullptr, 0, k.a, 0.f, 0}, 0, 0, 0, batch, lds);
+        __syncthreads();
+        p = or_operands(s.a, false, s.a, false, small, small, s.a.ld);
+        p.splits = 1;
+        p.slabs = (p.k + 63) / 64;
+        gm_planes_tile<OrthEpi, false, false>(p, OrthEpi{s.a, s.b, nullptr, 0, k.b, k.b_c, 0}, 0, 0, 0, batch, lds);
+        __syncthreads();
+        const OrthEpi f{x, y, i == s.steps - 1 ? s.out : nullptr, s.type, k.x, k.x_c, 0};
+        p = TALL ? or_operands(x, false, s.b, false, x.rows, small, s.b.ld) : or_operands(s.b, false, x, true, small, x.cols, small);
+        p.splits = 1;
+        p.slabs = (p.k + 63) / 64;
+#pragma unroll 1
+        for (int t = 0; t < tiles; ++t) {
+            gm_planes_tile<OrthEpi, false, !TALL>(p, f, TALL ? t : 0, TALL ? 0 : t, 0, batch, lds);
+            __syncthreads();
+        }
     }
 }
 
@@ -214,15 +283,13 @@ static void or_product(GemmP p, OrthEpi f, int batch, bool lower, float *part, h
     const OrthPlan plan = or_plan(p.m, p.n, p.k, batch, lower);
     p.splits = plan.splits; p.slabs = plan.slabs; p.part = part; p.lower = lower;
     f.mirror = lower ? plan.tile : 0;
-    auto go = [&]<int TILE>() {
-        p.tiles_m = (int)((p.m + TILE - 1) / TILE);
-        p.tiles_n = (p.n + TILE - 1) / TILE;
-        const int64_t tiles = lower ? (int64_t)p.tiles_m * (p.tiles_m + 1) / 2 : (int64_t)p.tiles_m * p.tiles_n;
-        hipLaunchKernelGGL((gemm_moved_kernel<FGNN_F16, OrthEpi, QS, PS, TILE, TILE, 2>), dim3((unsigned)(tiles * p.splits), (unsigned)batch), dim3(64 * gm_waves(TILE, TILE)),
-                           gm_moved_lds(TILE, TILE), st, p, f);
-    };
-    if (plan.tile == 256) go.template operator()<256>();
-    else go.template operator()<128>();
+    p.tiles_m = (int)((p.m + plan.tile - 1) / plan.tile);
+    p.tiles_n = (p.n + plan.tile - 1) / plan.tile;
+    const int64_t tiles = lower ? (int64_t)p.tiles_m * (p.tiles_m + 1) / 2 : (int64_t)p.tiles_m * p.tiles_n;
+    const dim3 grid((unsigned)(tiles * p.splits), (unsigned)batch);
+    if (plan.tile == 256)
+        hipLaunchKernelGGL((gemm_moved_kernel<FGNN_F16, OrthEpi, QS, PS, 256, 256, 2>), grid, dim3(64 * gm_waves(256, 256)), gm_moved_lds(256, 256), st, p, f);
+    else hipLaunchKernelGGL((gemm_planes_kernel<OrthEpi, QS, PS>), grid, dim3(64 * GM_PLANES_WAVES), GM_PLANES_LDS, st, p, f);
     if (p.splits > 1) hipLaunchKernelGGL(orth_join_kernel, dim3((unsigned)((p.n + 127) / 128), (unsigned)((p.m + 15) / 16), (unsigned)batch), dim3(256), 0, st, p, f);
 }
 
@@ -245,15 +312,6 @@ extern "C" size_t fgnn_orthogonalize_workspace_bytes(int batch, int m, int n)
     if (batch < 1 || m < 1 || n < 1) return 0;
     const OrthShape s = or_shape(m, n);
     return (size_t)batch * ((size_t)s.parts * sizeof(float) + 2 * 2 * sizeof(_Float16) * ((size_t)m * s.ld_x + (size_t)s.small * s.ld_s)) + or_part_bytes(batch, s, m, n) + 7 * 256;
-}
-
-static GemmP or_operands(const OrthM &q, bool qs, const OrthM &p, bool ps, int64_t m, int n, int64_t k)
-{
-    GemmP g{};
-    g.m = m; g.n = n; g.k = k;
-    g.q = q.p; g.ldq = q.ld; g.rows_q = qs ? (m + 7) / 8 * 8 : m; g.plane_q = om_plane(q) * 2; g.batch_q = 2 * g.plane_q;
-    g.p = p.p; g.ldp = p.ld; g.rows_p = ps ? (n + 7) / 8 * 8 : n; g.plane_p = om_plane(p) * 2; g.batch_p = 2 * g.plane_p;
-    return g;
 }
 
 extern "C" int fgnn_orthogonalize(int batch, int m, int n, int type, const void *g, int steps, const float *coefficients, float eps, void *out, void *workspace,
@@ -286,23 +344,34 @@ extern "C" int fgnn_orthogonalize(int batch, int m, int n, int type, const void 
         const unsigned blocks = (unsigned)std::min<int64_t>((om_plane(x) / 8 + 255) / 256, 4096);
         hipLaunchKernelGGL((orth_planes_kernel<E>), dim3(blocks, batch), dim3(256), 0, st, (const E *)g, (const float *)norms, s.parts, eps, sx, x);
     });
+    // One launch for all steps where a workgroup's way through the tiles of X is no longer than the launches, or there are many matrices (us, launches / one: one of
+    // 64 x 64 94 / 65, four of 128 x 256 155 / 154, one of 128 x 512 167 / 248, 100 of them 345 / 276, 300 of 100 x 128 629 / 219).
+    const bool one = s.small <= 128 && steps <= OR_STEPS && (s.wide <= 256 || (s.wide <= 512 && batch >= 64));
+    OrthSmall all{x, y, a, b, out, type, steps, {}};
     for (int i = 0; i < steps; ++i) {
         const float *c = coefficients + 3 * i;
+        const bool last = i == steps - 1;
         const float sa = or_scale(top * top), sb = or_scale(or_reach_b(c[1], c[2], top * top));
         top = or_reach(c[0], c[1], c[2], top) * 1.001;
-        const float sy = or_scale(top);
+        const float sy = last ? 1.f : or_scale(top);
+        const float alpha[3] = {sa / (sx * sx), sb * c[2] / (sa * sa), sy / (sb * sx)}, beta[3] = {0.f, sb * c[1] / sa, sy * c[0] / sx};
+        sx = sy;
+        if (one) {
+            all.k[i] = OrthFactors{alpha[0], alpha[1], beta[1], alpha[2], beta[2]};
+            continue;
+        }
         const int small = (int)s.small;
-        OrthEpi f{{}, a, nullptr, type, sa / (sx * sx), 0.f, 0};
+        OrthEpi f{{}, a, nullptr, type, alpha[0], beta[0], 0};
         if (s.tall) or_product<true, true>(or_operands(x, true, x, true, small, small, m), f, batch, true, part, st);
         else or_product<false, false>(or_operands(x, false, x, false, small, small, s.ld_x), f, batch, true, part, st);
-        f = OrthEpi{a, b, nullptr, type, sb * c[2] / (sa * sa), sb * c[1] / sa, 0};
+        f = OrthEpi{a, b, nullptr, type, alpha[1], beta[1], 0};
         or_product<false, false>(or_operands(a, false, a, false, small, small, s.ld_s), f, batch, true, part, st);
-        const bool last = i == steps - 1;
-        f = OrthEpi{x, y, last ? out : nullptr, type, (last ? 1.f : sy) / (sb * sx), (last ? 1.f : sy) * c[0] / sx, 0};
+        f = OrthEpi{x, y, last ? out : nullptr, type, alpha[2], beta[2], 0};
         if (s.tall) or_product<false, false>(or_operands(x, false, b, false, m, small, s.ld_s), f, batch, false, part, st);
         else or_product<false, true>(or_operands(b, false, x, true, small, n, small), f, batch, false, part, st);
         std::swap(x, y);
-        sx = sy;
     }
+    if (one && s.tall) hipLaunchKernelGGL(orth_small_kernel<true>, dim3(batch), dim3(64 * GM_PLANES_WAVES), GM_PLANES_LDS, st, all);
+    else if (one) hipLaunchKernelGGL(orth_small_kernel<false>, dim3(batch), dim3(64 * GM_PLANES_WAVES), GM_PLANES_LDS, st, all);
     return fgnn_launch_status("gemm_moved_kernel");
 }

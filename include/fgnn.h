@@ -338,10 +338,12 @@ int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const void *gy, con
  * receives the activation's argument for the backward pass.  y, z contiguous.  fp32 products are summed from parts of 8 significant bits, to about
  * 2^-23 of the sum of magnitudes.
  * _q8: operands in 8 bits (eight: FGNN_I8, k <= 131072, or FGNN_E4M3) with scale [rows] and weight_scale [n]; bias, residual and y are of type `type`.
- * _slope: dz = gy act'(z) (NULL: not wanted) and dbias = its column sums (NULL: not wanted), summed before dz is rounded.
- * _dx: dx [rows, k] = dz weight;  _dw: dw [n, k] = dz^T x.  All are deterministic.  Workspaces: fgnn_linear and _q8 fgnn_linear_workspace_bytes (kind: type or
- * eight), _dx and _dw fgnn_linear_backward_workspace_bytes. */
-size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind);
+ * _slope: dz = gy act'(z) (NULL: not wanted; rows of ldz = n, or of the next whole 16 bytes with zeros behind n) and dbias = its column sums (NULL: not
+ * wanted), summed before dz is rounded.
+ * _dx: dx [rows, k] = dz weight;  _dw: dw [n, k] = dz^T x; padded: zeros follow the rows of dz up to whole 16 bytes.  All are deterministic.
+ * Workspaces: fgnn_linear and _q8 fgnn_linear_workspace_bytes (kind: type or eight), _dx and _dw fgnn_linear_backward_workspace_bytes; loose: nonzero where rows
+ * of an operand (dz apart, where it is padded) may not start at 16 bytes each and hold whole 16 bytes: large products lay them out anew. */
+size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind, int loose);
 int fgnn_linear(int64_t rows, int n, int k, int type, const void *x, int64_t ldx, const void *weight, int64_t ldw,
                 const void *bias, int btype, const void *residual, int64_t ldr, int act, float slope, void *z, void *y,
                 void *workspace, size_t workspace_bytes, void *stream);
@@ -351,11 +353,11 @@ int fgnn_linear_q8(int64_t rows, int n, int k, int eight, int type, const void *
                    size_t workspace_bytes, void *stream);
 size_t fgnn_linear_slope_workspace_bytes(int64_t rows, int n, int type);
 int fgnn_linear_slope(int64_t rows, int n, int type, const void *gy, int64_t ldg, const void *z, int act, float slope,
-                      void *dz, void *dbias, int btype, void *workspace, size_t workspace_bytes, void *stream);
-size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type);
-int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *weight, int64_t ldw,
-                   void *dx, void *workspace, size_t workspace_bytes, void *stream);
-int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, const void *x, int64_t ldx,
+                      void *dz, int64_t ldz, void *dbias, int btype, void *workspace, size_t workspace_bytes, void *stream);
+size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type, int loose);
+int fgnn_linear_dx(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, int padded, const void *weight,
+                   int64_t ldw, void *dx, void *workspace, size_t workspace_bytes, void *stream);
+int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *dz, int64_t ldz, int padded, const void *x, int64_t ldx,
                    void *dw, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Orthogonalised updates of `batch` weight matrices g [m, n] (contiguous, fp32, bf16 or fp16; out of the same type): X = g / (|g| + eps) by the Frobenius

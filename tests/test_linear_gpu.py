@@ -96,6 +96,11 @@ def test_larger_products(dtype):
     check_all(1030, 1100, 1290, dtype, "silu")
     check_all(20011, 128, 256, dtype, "relu")
     check_all(2048, 1024, 2048, dtype, None)
+    # rows at odd addresses, with and without an activation in between
+    check_all(1501, 1003, 1201, dtype, "gelu")
+    check_all(1501, 1003, 1201, dtype, None)
+    check_all(1504, 1001, 1208, dtype, "relu")
+    check_all(1501, 1008, 1204, dtype, None)
 
 
 @pytest.mark.gpu
@@ -200,7 +205,7 @@ def test_infinities_and_nan_stay_in_their_rows(dtype, size):
 @pytest.mark.gpu
 @pytest.mark.parametrize("eight", [torch.int8, torch.float8_e4m3fn])
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("size", SIZES + [(700, 512, 384)])
+@pytest.mark.parametrize("size", SIZES + [(700, 512, 384), (1100, 1010, 1030), (1500, 1024, 1024)])
 def test_eight_bits(eight, dtype, size):
     rows, k, n = size
     x, w, b, r, _ = operands(rows, k, n, torch.float32)
@@ -269,9 +274,10 @@ def test_refusals():
     assert l.fgnn_linear(2, 6, 8, 1, p, 8, None, 8, None, 0, None, 0, 0, 0.0, None, p, None, 0, None) == -1
     assert l.fgnn_linear_q8(2, 6, 131073, 3, 1, p, 131073, p, p, 131073, p, None, 1, None, 0, 0, 0.0, p, None, 0, None) == -4
     assert l.fgnn_linear_q8(2, 6, 8, 1, 1, p, 8, p, p, 8, p, None, 1, None, 0, 0, 0.0, p, None, 0, None) == -2
-    assert l.fgnn_linear_slope(2, 6, 0, p, 6, None, 1, 0.0, p, None, 0, None, 0, None) == -1                     # an activation without its argument
-    assert l.fgnn_linear_slope(2, 6, 0, p, 6, p, 1, 0.0, p, p, 0, None, 0, None) == -5                           # no workspace for the sums
-    big = l.fgnn_linear_workspace_bytes(100, 16, 100000, 1)
+    assert l.fgnn_linear_slope(2, 6, 0, p, 6, p, 1, 0.0, p, 7, None, 0, None, 0, None) == -2                     # rows of dz neither n nor whole 16 bytes
+    assert l.fgnn_linear_slope(2, 6, 0, p, 6, None, 1, 0.0, p, 6, None, 0, None, 0, None) == -1                     # an activation without its argument
+    assert l.fgnn_linear_slope(2, 6, 0, p, 6, p, 1, 0.0, p, 6, p, 0, None, 0, None) == -5                           # no workspace for the sums
+    big = l.fgnn_linear_workspace_bytes(100, 16, 100000, 1, 0)
     assert big > 0 and l.fgnn_linear(100, 16, 100000, 1, p, 100000, p, 100000, None, 0, None, 0, 0, 0.0, None, p, p, big - 4, None) == -5
 
 
