@@ -3,7 +3,7 @@
 // written as values, or in 8 bits with a scale a row (scale = max_j |y_j| / Q, q_j = round(y_j / scale), Q = 127 or 448), and its gradient
 //   g = gy w,   dx = dr = gh + s g - h s^3 mean_j(g h),   dw_j = sum_i gy_ij h_ij s_i .
 // All three are bound by memory: a row is read once into registers, its statistics (32 bits) are taken from there, and it is written
-// once.  T threads share a row, R 16-byte vectors each, so that a row of 16 bytes and one of 64 KB keep about as many loads in flight.
+// once (16,384 x 4096 bf16 with residual, forward and backward 4.8 TB/s; a copy of 1 GiB reaches 5.1).  T threads share a row, R 16-byte vectors each, so that a row of 16 bytes and one of 64 KB keep about as many loads in flight.
 #include <algorithm>
 #include "fgnn_elem.h"
 
@@ -273,13 +273,16 @@ int fgnn_sum_parts(const float *part, int rows, int cols, void *out, int type, h
     return fgnn_launch_status("norm_sum_kernel");
 }
 
-// Threads a row and vectors a thread; columns that are no multiple of the vector take part of one.
+// Threads a row and vectors a thread; columns that are no multiple of the vector take part of one.  Rows of 65 to 96 vectors that become 8 bits take half a
+// wave: their two reductions and short stores cost more than idle lanes in the loads (100,000 rows of fp16, us, 64 threads / 32: 520 columns 117 / 105, 602 157 / 130, 768
+// 142 / 121; as values 86 / 114, 112 / 145, 117 / 141; backward 130 / 176, 187 / 228, 148 / 190).
 template <typename Fn>
-static bool nm_shape(int64_t vectors, Fn &&f)
+static bool nm_shape(int64_t vectors, bool eight, Fn &&f)
 {
     if (vectors <= 16) f.template operator()<16, 1>();
     else if (vectors <= 32) f.template operator()<16, 2>();
     else if (vectors <= 64) f.template operator()<64, 1>();
+    else if (vectors <= 96 && eight) f.template operator()<32, 3>();
     else if (vectors <= 128) f.template operator()<64, 2>();
     else if (vectors <= 256) f.template operator()<256, 1>();
     else if (vectors <= 512) f.template operator()<256, 2>();
@@ -309,7 +312,7 @@ static int nm_forward(const char *who, NormP p, int type, int eight, hipStream_t
 {
     if (p.rows == 0) return 0;
     fe_dispatch(type, [&]<typename E>() {
-        nm_shape(nm_vectors(p.cols, type), [&]<int T, int R>() {
+        nm_shape(nm_vectors(p.cols, type), eight != 0, [&]<int T, int R>() {
             const dim3 b(T > NM_TPB ? T : NM_TPB), g(nm_grid(p.rows, T, 8));
             if (eight == FGNN_I8) hipLaunchKernelGGL((norm_kernel<E, T, R, FGNN_I8>), g, b, 0, st, p);
             else if (eight == FGNN_E4M3) hipLaunchKernelGGL((norm_kernel<E, T, R, FGNN_E4M3>), g, b, 0, st, p);
@@ -353,7 +356,7 @@ extern "C" int fgnn_quantize_rows(int64_t rows, int cols, int type, const void *
 static unsigned nm_backward_grid(int64_t rows, int cols, int type)
 {
     unsigned grid = 1;
-    nm_shape(nm_vectors(cols, type), [&]<int T, int R>() { grid = nm_grid(rows, T, 4); });
+    nm_shape(nm_vectors(cols, type), false, [&]<int T, int R>() { grid = nm_grid(rows, T, 4); });
     return grid;
 }
 
@@ -377,7 +380,7 @@ extern "C" int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const vo
         NormB p{rows, cols, gy, gh, h, ldh, weight, wtype, rstd, dx, dweight ? (float *)workspace : nullptr};
         parts = (int)nm_backward_grid(rows, cols, type);
         fe_dispatch(type, [&]<typename E>() {
-            nm_shape(nm_vectors(cols, type), [&]<int T, int R>() {
+            nm_shape(nm_vectors(cols, type), false, [&]<int T, int R>() {
                 hipLaunchKernelGGL((norm_backward_kernel<E, T, R>), dim3(parts), dim3(T > NM_TPB ? T : NM_TPB), 0, st, p);
             });
         });
