@@ -301,3 +301,25 @@ def test_second_order_gradients_are_refused():
     (dx,) = torch.autograd.grad(linear_act(x, w, activation="gelu").sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="second order"):
         dx.sum().backward()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    from ae_mlsys_gnn_amd.operators import rms_norm
+    rows, k = 2200003, 1000                                      # 2.2e9 values
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda")
+    for part in x.split(200000):
+        part.normal_()
+    w = torch.randn(24, k, device="cuda").to(torch.bfloat16)
+    y = linear_act(x, w)
+    picks = torch.tensor([0, 1, 2147483, 2147484, rows - 130, rows - 2, rows - 1], device="cuda")
+    z = x[picks].double() @ w.double().t()
+    within(y[picks], z, allowance(torch.bfloat16, z, x[picks].double().abs() @ w.double().abs().t()), "rows")
+    g = torch.zeros(rows, 24, dtype=torch.bfloat16, device="cuda")
+    g[picks] = 1
+    wl = w.clone().requires_grad_(True)
+    (dw,) = torch.autograd.grad(linear_act(x, wl), wl, g)
+    ref = x[picks].double().sum(0).expand(24, k)
+    within(dw, ref, allowance(torch.bfloat16, ref, x[picks].double().abs().sum(0).expand(24, k)), "dw")
+    n = rms_norm(x)
+    assert torch.equal(n[picks], rms_norm(x[picks]))
