@@ -275,27 +275,39 @@ int fgnn_sum_parts(const float *part, int rows, int cols, void *out, int type, h
 
 // Threads a row and vectors a thread; columns that are no multiple of the vector take part of one.  Rows of 65 to 96 vectors that become 8 bits take half a
 // wave: their two reductions and short stores cost more than idle lanes in the loads (100,000 rows of fp16, us, 64 threads / 32: 520 columns 117 / 105, 602 157 / 130, 768
-// 142 / 121; as values 86 / 114, 112 / 145, 117 / 141; backward 130 / 176, 187 / 228, 148 / 190).
-template <typename Fn>
-static bool nm_shape(int64_t vectors, bool eight, Fn &&f)
+// 142 / 121; as values 86 / 114, 112 / 145, 117 / 141; backward 130 / 176, 187 / 228, 148 / 190).  Above 512 vectors registers decide, the backward pass's
+// most (14,000 rows of fp16, us, 256 threads / as below: 4736 columns as values 131 / 104, 8 bits 143 / 126, backward 232 / 198; 8192 187 / 171, 174 / 174, 295 / 217; with
+// 1024 threads of four vectors / of two: 12,000 374 / 283, 533 / 324, 1815 / 348).
+enum { NM_FORWARD, NM_EIGHT, NM_BACKWARD };
+template <int PASS, typename Fn>
+static bool nm_shape(int64_t vectors, Fn &&f)
 {
     if (vectors <= 16) f.template operator()<16, 1>();
     else if (vectors <= 32) f.template operator()<16, 2>();
     else if (vectors <= 64) f.template operator()<64, 1>();
-    else if (vectors <= 96 && eight) f.template operator()<32, 3>();
-    else if (vectors <= 128) f.template operator()<64, 2>();
-    else if (vectors <= 256) f.template operator()<256, 1>();
+    else if (vectors <= 128) {
+        if constexpr (PASS == NM_EIGHT) {
+            if (vectors <= 96) f.template operator()<32, 3>();
+            else f.template operator()<64, 2>();
+        } else f.template operator()<64, 2>();
+    } else if (vectors <= 256) f.template operator()<256, 1>();
     else if (vectors <= 512) f.template operator()<256, 2>();
-    else if (vectors <= 1024) f.template operator()<256, 4>();
+    else if (vectors <= 1024) {
+        if constexpr (PASS == NM_FORWARD) f.template operator()<512, 2>();
+        else if constexpr (PASS == NM_BACKWARD) f.template operator()<1024, 1>();
+        else if (vectors <= 768) f.template operator()<256, 3>();
+        else f.template operator()<256, 4>();
+    } else if (vectors <= 2048) f.template operator()<1024, 2>();
     else if (vectors <= 4096) f.template operator()<1024, 4>();
     else return false;
     return true;
 }
 static inline int nm_vectors(int cols, int type) { const int v = 16 / fe_size(type); return (cols + v - 1) / v; }
+// per_unit: workgroups of 256 threads a compute unit
 static unsigned nm_grid(int64_t rows, int T, int per_unit)
 {
     const int cus = fgnn_current_device_compute_units(), groups = T >= NM_TPB ? 1 : NM_TPB / T;
-    return (unsigned)std::min<int64_t>((rows + groups - 1) / groups, (int64_t)(cus > 0 ? cus : 256) * per_unit);
+    return (unsigned)std::min<int64_t>((rows + groups - 1) / groups, (int64_t)(cus > 0 ? cus : 256) * std::max(1, per_unit * NM_TPB / std::max(T, NM_TPB)));
 }
 
 static int nm_check(const char *who, int64_t rows, int cols, int type, const void *x, int64_t ldx, const void *r, int64_t ldr, const void *w, int wtype)
@@ -311,13 +323,14 @@ static int nm_check(const char *who, int64_t rows, int cols, int type, const voi
 static int nm_forward(const char *who, NormP p, int type, int eight, hipStream_t st)
 {
     if (p.rows == 0) return 0;
+    const int vectors = nm_vectors(p.cols, type);
     fe_dispatch(type, [&]<typename E>() {
-        nm_shape(nm_vectors(p.cols, type), eight != 0, [&]<int T, int R>() {
-            const dim3 b(T > NM_TPB ? T : NM_TPB), g(nm_grid(p.rows, T, 8));
-            if (eight == FGNN_I8) hipLaunchKernelGGL((norm_kernel<E, T, R, FGNN_I8>), g, b, 0, st, p);
-            else if (eight == FGNN_E4M3) hipLaunchKernelGGL((norm_kernel<E, T, R, FGNN_E4M3>), g, b, 0, st, p);
-            else hipLaunchKernelGGL((norm_kernel<E, T, R, 0>), g, b, 0, st, p);
-        });
+        auto launch = [&]<int Q, int T, int R>() {
+            hipLaunchKernelGGL((norm_kernel<E, T, R, Q>), dim3(nm_grid(p.rows, T, 8)), dim3(T > NM_TPB ? T : NM_TPB), 0, st, p);
+        };
+        if (eight == FGNN_I8) nm_shape<NM_EIGHT>(vectors, [&]<int T, int R>() { launch.template operator()<FGNN_I8, T, R>(); });
+        else if (eight == FGNN_E4M3) nm_shape<NM_EIGHT>(vectors, [&]<int T, int R>() { launch.template operator()<FGNN_E4M3, T, R>(); });
+        else nm_shape<NM_FORWARD>(vectors, [&]<int T, int R>() { launch.template operator()<0, T, R>(); });
     });
     return fgnn_launch_status(who);
 }
@@ -356,7 +369,7 @@ extern "C" int fgnn_quantize_rows(int64_t rows, int cols, int type, const void *
 static unsigned nm_backward_grid(int64_t rows, int cols, int type)
 {
     unsigned grid = 1;
-    nm_shape(nm_vectors(cols, type), false, [&]<int T, int R>() { grid = nm_grid(rows, T, 4); });
+    nm_shape<NM_BACKWARD>(nm_vectors(cols, type), [&]<int T, int R>() { grid = nm_grid(rows, T, 4); });
     return grid;
 }
 
@@ -380,7 +393,7 @@ extern "C" int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const vo
         NormB p{rows, cols, gy, gh, h, ldh, weight, wtype, rstd, dx, dweight ? (float *)workspace : nullptr};
         parts = (int)nm_backward_grid(rows, cols, type);
         fe_dispatch(type, [&]<typename E>() {
-            nm_shape(nm_vectors(cols, type), false, [&]<int T, int R>() {
+            nm_shape<NM_BACKWARD>(nm_vectors(cols, type), [&]<int T, int R>() {
                 hipLaunchKernelGGL((norm_backward_kernel<E, T, R>), dim3(parts), dim3(T > NM_TPB ? T : NM_TPB), 0, st, p);
             });
         });

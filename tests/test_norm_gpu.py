@@ -9,7 +9,7 @@ from ae_mlsys_gnn_amd.operators import quantize_rows, rms_norm, rms_norm_q8
 UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 TYPES = list(UNIT)
 # either side of every change of threads and vectors a row, odd widths, one column, the widest rows
-COLS = [1, 3, 8, 64, 65, 128, 129, 255, 602, 1000, 1433, 4096, 8191, 16384]
+COLS = [1, 3, 8, 64, 65, 128, 129, 255, 602, 1000, 1433, 2049, 4096, 4736, 8191, 8200, 16384]
 TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 
 
