@@ -69,13 +69,22 @@ static bool gm_worth_packing(int64_t m, int64_t n, int64_t k, int kind)
     return (kind == FGNN_BF16 || kind == FGNN_F16 || kind == FGNN_E4M3) && most < 2e11 && (double)m * n * k >= 3e9;
 }
 
-// Whether rows of an operand are whole 16-byte chunks at 16-byte addresses, and near enough for 32-bit offsets in a tile.
+// Whether rows `ld` bytes apart are near enough for the 32-bit offsets of the kernel that moves them: a tile takes up to 256 rows of an operand whose reduction
+// is contiguous, 64 of a strided one.
+static bool gm_near(int64_t ld, bool strided) { return ld * (strided ? 64 : 256) < (1ll << 31); }
+// Whether operands that cannot be moved as they lie are laid out anew: where it is worth it, and their new rows are near enough.
+static bool gm_packs(int64_t m, int64_t n, int64_t k, int kind, bool qs, bool ps)
+{
+    return gm_worth_packing(m, n, k, kind) && gm_near(((qs ? m : k) + 7) / 8 * 16, qs) && gm_near(((ps ? n : k) + 7) / 8 * 16, ps);
+}
+
+// Whether rows of an operand are whole 16-byte chunks at 16-byte addresses, and near enough.
 // (padded: zeros follow a row up to whole chunks)
-static bool gm_movable(const void *p, int64_t ld, int64_t inner, int kind, bool padded)
+static bool gm_movable(const void *p, int64_t ld, int64_t inner, int kind, bool strided, bool padded)
 {
     const int ch = 16 / fe_size(kind);
     return kind != FGNN_F32 && kind != FGNN_E4M3 && fgnn_aligned16(p) && ld % ch == 0 && (padded ? ld >= (inner + ch - 1) / ch * ch : inner % ch == 0) && inner > 0
-        && ld * fe_size(kind) * 256 < (1ll << 31);
+        && gm_near(ld * fe_size(kind), strided);
 }
 
 template <int KIND, typename E>
@@ -152,7 +161,7 @@ static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool qs, bool 
     p.m = m; p.n = n; p.k = k;
     gm_cut(&p, 128, kind, false);          // (what moves its operands is cut into fewer)
     size_t bytes = p.splits > 1 ? fgnn_align256((size_t)p.splits * m * n * sizeof(float)) : 0;
-    if (loose && gm_worth_packing(m, n, k, kind)) bytes += (qs ? gm_packed_bytes(k, m) : gm_packed_bytes(m, k)) + (ps ? gm_packed_bytes(k, n) : gm_packed_bytes(n, k)) + 256;
+    if (loose && gm_packs(m, n, k, kind, qs, ps)) bytes += (qs ? gm_packed_bytes(k, m) : gm_packed_bytes(m, k)) + (ps ? gm_packed_bytes(k, n) : gm_packed_bytes(n, k)) + 256;
     return bytes;
 }
 
@@ -161,11 +170,11 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
 {
     if (p.m == 0 || p.n == 0) return 0;
     const int64_t inner_q = qs ? p.m : p.k, inner_p = ps ? p.n : p.k;
-    const bool q_moves = p.k > 0 && gm_movable(p.q, p.ldq, inner_q, kind, q_padded), p_moves = p.k > 0 && gm_movable(p.p, p.ldp, inner_p, kind, false);
+    const bool q_moves = p.k > 0 && gm_movable(p.q, p.ldq, inner_q, kind, qs, q_padded), p_moves = p.k > 0 && gm_movable(p.p, p.ldp, inner_p, kind, ps, false);
     bool moved = q_moves && p_moves;
     p.rows_q = qs ? (p.m + 7) / 8 * 8 : p.m;                   // (strided operands hold whole chunks of rows, or are made to)
     p.rows_p = ps ? (p.n + 7) / 8 * 8 : p.n;
-    if (!moved && p.k > 0 && gm_worth_packing(p.m, p.n, p.k, kind) && !(!qs && !ps && gm_few(p, kind, false))) {
+    if (!moved && p.k > 0 && gm_packs(p.m, p.n, p.k, kind, qs, ps) && !(!qs && !ps && gm_few(p, kind, false))) {
         const int64_t outer_q = qs ? p.k : p.m, outer_p = ps ? p.k : p.n;
         const size_t bytes_q = q_moves ? 0 : gm_packed_bytes(outer_q, inner_q), bytes_p = p_moves ? 0 : gm_packed_bytes(outer_p, inner_p);
         char *to = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
