@@ -58,11 +58,12 @@ Rows rows_of(const Tensor &t)
     if ((cols > 1 && r.stride(1) != 1) || (rows > 1 && r.stride(0) < cols)) r = r.contiguous();
     return {r, rows, cols, rows > 1 ? r.stride(0) : cols};
 }
-// Whether rows do not all start at 16 bytes and hold whole 16 bytes.
-bool loose(const Rows &r)
+// Whether rows do not all start at 16 bytes and hold whole 16 bytes, or lie too far apart to be moved as they are: 2^23 bytes, 2^25 where the reduction goes
+// from row to row (`strided`).
+bool loose(const Rows &r, bool strided = false)
 {
     const int64_t size = r.t.element_size();
-    return ((uintptr_t)r.t.data_ptr() | r.ld * size | r.cols * size) & 15;
+    return (((uintptr_t)r.t.data_ptr() | r.ld * size | r.cols * size) & 15) || r.ld * size >= (strided ? 1 << 25 : 1 << 23);
 }
 Tensor like(const Tensor &t, at::IntArrayRef shape) { return at::empty(shape, t.options()); }
 Tensor like(const Tensor &t, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, t.options().dtype(type)); }
@@ -289,7 +290,7 @@ struct Linear : torch::autograd::Function<Linear> {
                                     db.defined() ? float_type(db) : type, address(ws), bytes, stream), "fgnn_linear_slope");
         }
         if (need & 3) {
-            const size_t bytes = fgnn_linear_backward_workspace_bytes(x.rows, n, k, type, loose(x) || loose(w) || (!sloped && loose(dz)));
+            const size_t bytes = fgnn_linear_backward_workspace_bytes(x.rows, n, k, type, loose(x, true) || loose(w, true) || (!sloped && loose(dz)));
             const Tensor ws = scratch(x.t, bytes);
             if (need & 1) {
                 dx = like(x.t, saved[0].sizes());

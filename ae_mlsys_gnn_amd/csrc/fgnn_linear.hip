@@ -153,6 +153,7 @@ static int gm_tile_for(int64_t m, int n)
     return ((m + 255) / 256) * ((n + 255) / 256) >= gm_units() ? 256 : 128;
 }
 
+static size_t gm_part_bytes(const GemmP &p) { return p.splits > 1 ? (size_t)p.splits * p.m * p.n * sizeof(float) : 0; }
 // Partial sums and operands laid out anew; loose: an operand may not be movable as it lies.
 static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool qs, bool ps, bool loose)
 {
@@ -160,7 +161,7 @@ static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool qs, bool 
     GemmP p{};
     p.m = m; p.n = n; p.k = k;
     gm_cut(&p, 128, kind, false);          // (what moves its operands is cut into fewer)
-    size_t bytes = p.splits > 1 ? fgnn_align256((size_t)p.splits * m * n * sizeof(float)) : 0;
+    size_t bytes = fgnn_align256(gm_part_bytes(p));
     if (loose && gm_packs(m, n, k, kind, qs, ps)) bytes += (qs ? gm_packed_bytes(k, m) : gm_packed_bytes(m, k)) + (ps ? gm_packed_bytes(k, n) : gm_packed_bytes(n, k)) + 256;
     return bytes;
 }
@@ -177,29 +178,32 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
     if (!moved && p.k > 0 && gm_packs(p.m, p.n, p.k, kind, qs, ps) && !(!qs && !ps && gm_few(p, kind, false))) {
         const int64_t outer_q = qs ? p.k : p.m, outer_p = ps ? p.k : p.n;
         const size_t bytes_q = q_moves ? 0 : gm_packed_bytes(outer_q, inner_q), bytes_p = p_moves ? 0 : gm_packed_bytes(outer_p, inner_p);
-        char *to = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
-        FGNN_REQUIRE(workspace && (size_t)(to - (char *)workspace) + bytes_q + bytes_p <= workspace_bytes, FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who, workspace_bytes);
-        if (!q_moves) {
-            gm_pack(p.q, p.ldq, outer_q, (int)inner_q, to, kind == FGNN_E4M3, st);
-            p.q = to;
-            p.ldq = (inner_q + 7) / 8 * 8;
+        char *to = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255), *after = to + bytes_q + bytes_p;
+        gm_cut(&p, gm_tile_for(p.m, p.n), kind, true);
+        // (a caller who did not say that an operand may be loose has brought no room for it: then through registers)
+        if (workspace && (size_t)(after - (char *)workspace) + gm_part_bytes(p) <= workspace_bytes) {
+            if (!q_moves) {
+                gm_pack(p.q, p.ldq, outer_q, (int)inner_q, to, kind == FGNN_E4M3, st);
+                p.q = to;
+                p.ldq = (inner_q + 7) / 8 * 8;
+            }
+            if (!p_moves) {
+                gm_pack(p.p, p.ldp, outer_p, (int)inner_p, to + bytes_q, kind == FGNN_E4M3, st);
+                p.p = to + bytes_q;
+                p.ldp = (inner_p + 7) / 8 * 8;
+            }
+            workspace_bytes -= (size_t)(after - (char *)workspace);
+            workspace = after;
+            if (kind == FGNN_E4M3) kind = FGNN_F16;
+            moved = true;
         }
-        if (!p_moves) {
-            gm_pack(p.p, p.ldp, outer_p, (int)inner_p, to + bytes_q, kind == FGNN_E4M3, st);
-            p.p = to + bytes_q;
-            p.ldp = (inner_p + 7) / 8 * 8;
-        }
-        workspace_bytes -= (size_t)(to - (char *)workspace) + bytes_q + bytes_p;
-        workspace = to + bytes_q + bytes_p;
-        if (kind == FGNN_E4M3) kind = FGNN_F16;
-        moved = true;
     }
     const bool few = !qs && !ps && gm_few(p, kind, moved);
     const int tile = moved ? gm_tile_for(p.m, p.n) : 128;
     gm_cut(&p, tile, kind, moved);
     if (few) p.splits = 1;
     FGNN_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1ll << 31) && (p.m * ((p.n + 3) / 4) + 255) / 256 < (1ll << 31), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
-    FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * p.m * p.n * sizeof(float)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
+    FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= gm_part_bytes(p)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
                  workspace_bytes);
     p.part = (float *)workspace;
     p.epi.m = p.m; p.epi.n = p.n;

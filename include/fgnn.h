@@ -342,7 +342,8 @@ int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const void *gy, con
  * wanted), summed before dz is rounded.
  * _dx: dx [rows, k] = dz weight;  _dw: dw [n, k] = dz^T x; padded: zeros follow the rows of dz up to whole 16 bytes.  All are deterministic.
  * Workspaces: fgnn_linear and _q8 fgnn_linear_workspace_bytes (kind: type or eight), _dx and _dw fgnn_linear_backward_workspace_bytes; loose: nonzero where rows
- * of an operand (dz apart, where it is padded) may not start at 16 bytes each and hold whole 16 bytes: large products lay them out anew. */
+ * of an operand may not start at 16 bytes each and hold whole 16 bytes (rows of dz, where it is padded, hold them), or may lie 2^23 bytes apart or more
+ * (x and weight in _dx and _dw 2^25): large products lay them out anew.  Without that room they run all the same, more slowly. */
 size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind, int loose);
 int fgnn_linear(int64_t rows, int n, int k, int type, const void *x, int64_t ldx, const void *weight, int64_t ldw,
                 const void *bias, int btype, const void *residual, int64_t ldr, int act, float slope, void *z, void *y,

@@ -35,3 +35,39 @@ def test_odd_reduction_past_32_bit_offsets():
         xd = x[i:i + 1].double()
         ref = (xd * wd).sum(-1)
         within(y[i], ref, allowance(torch.bfloat16, ref, (xd * wd).abs().sum(-1)), "row %d" % i)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up: without a device nothing is launched")
+def test_long_row_strides_need_no_room_that_was_not_asked_for():
+    l, p = _lib.lib(), 4096
+    # (rows, n, k, row stride of x): aligned 16-bit rows, so far apart that they are not moved as they lie
+    for rows, n, k, ldx in ((512, 32000, 4096, 4194304), (300, 32000, 4096, 4194304), (200, 128256, 4096, 8388608), (128, 64, 4194304, 4194304)):
+        told = l.fgnn_linear_workspace_bytes(rows, n, k, BF16, 0)
+        assert l.fgnn_linear(rows, n, k, BF16, p, ldx, p, k, None, 0, None, 0, 0, 0.0, None, p, p, told, None) not in (0, -5), (rows, n, k)
+    # the same by an address that is not said to be loose, and in a gradient
+    told = l.fgnn_linear_workspace_bytes(2048, 2048, 1024, BF16, 0)
+    assert l.fgnn_linear(2048, 2048, 1024, BF16, p + 2, 1024, p, 1024, None, 0, None, 0, 0, 0.0, None, p, p, told, None) not in (0, -5)
+    told = l.fgnn_linear_backward_workspace_bytes(512, 2048, 4096, BF16, 0)
+    assert l.fgnn_linear_dw(512, 2048, 4096, BF16, p, 2048, 0, p, 33554432, p, p, told, None) not in (0, -5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_far_apart(dtype):
+    # the last of 1024 positions of every sequence, before a wide layer
+    rows, k, n, ld = 512, 4096, 1536, 4194304
+    g = torch.Generator(device="cuda").manual_seed(1)
+    space = torch.empty((rows - 1) * ld + k, dtype=dtype, device="cuda")
+    x = space.as_strided((rows, k), (ld, 1))
+    x.normal_(generator=g)
+    w = torch.empty(n, k, dtype=dtype, device="cuda").normal_(0, k ** -0.5, generator=g)
+    gy = torch.empty(rows, n, dtype=dtype, device="cuda").normal_(generator=g)
+    xl, wl = x.detach().requires_grad_(True), w.clone().requires_grad_(True)
+    assert xl.stride() == (ld, 1)
+    y = linear_act(xl, wl)
+    dx, dw = torch.autograd.grad(y, (xl, wl), gy)
+    xd, wd, gd = x.double(), w.double(), gy.double()
+    for got, a, b, what in ((y, xd, wd.t(), "y"), (dx, gd, wd, "dx"), (dw, gd.t(), xd, "dw")):
+        b = b.contiguous()
+        ref = a @ b
+        within(got, ref, allowance(dtype, ref, a.abs() @ b.abs()), what)
