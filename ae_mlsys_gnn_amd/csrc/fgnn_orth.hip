@@ -4,18 +4,21 @@
 //
 // A step multiplies rounding errors of small singular values by a (3.4 at the usual coefficients, 490 in five steps), so the products have to carry more than
 // 16-bit values do.  X, A and B are kept as two fp16 planes, 22 significant bits, and a product is hi hi + hi lo + lo hi, summed in 32 bits: three
-// instructions of the fast kind where fp32 takes sixteen.  The low plane is kept 2^11 times as large, since the instructions take subnormal operands for
-// zeros.  fp16 has no exponents to spare, so each matrix is scaled by a power of two that its largest
-// possible element allows: the singular values of X_0 are at most 1, and what a step makes of the bound is known on the host.
+// instructions of the fast kind where fp32 takes sixteen.  The low plane is kept 2^11 times as large: as it is, it would often lie where fp16's step is 2^-24
+// whatever the value, with few bits or none (the instructions take subnormal operands as they are).  fp16 has no exponents to spare, so each matrix is scaled
+// by a power of two that its largest possible element allows: the singular values of X_0 are at most 1, and what a step makes of the bound is known on the host.
 #include <cmath>
 #include "fgnn_gemm.h"
 
 typedef _Float16 or_h8 __attribute__((ext_vector_type(8)));
 
-// v = hi + 2^-11 lo, to 2^-23 of v and 2^-36; nothing is left to a subnormal hi.
+// v = hi + 2^-11 lo, to 2^-23 of v and 2^-36.
 __device__ __forceinline__ void or_split(float v, _Float16 &hi, _Float16 &lo)
 {
-    hi = fabsf(v) < 0x1p-14f ? (_Float16)0.f : (_Float16)v;
+    // v is one value of 32 bits from here on: of a product that was still to be rounded the compiler would form hi twice, for memory from the value of 32 bits and for the
+    // difference straight from the product, and one element in 2^13 would get the remainder of another hi
+    asm("" : "+v"(v));
+    hi = (_Float16)v;
     lo = (_Float16)((v - (float)hi) * 0x1p11f);
 }
 

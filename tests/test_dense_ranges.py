@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from ae_mlsys_gnn_amd import _lib
-from ae_mlsys_gnn_amd.operators import linear_act
+from ae_mlsys_gnn_amd.operators import linear_act, orthogonalize
 
 from .test_linear_gpu import allowance, within
 
@@ -71,3 +71,29 @@ def test_rows_far_apart(dtype):
         b = b.contiguous()
         ref = a @ b
         within(got, ref, allowance(dtype, ref, a.abs() @ b.abs()), what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(100, 90), (300, 520), (1100, 700)])
+def test_planes_of_every_element(dtype, shape):
+    # one step with a = 1, b = c = 0 hands X_0 back as its two planes hold it, to 2^-23 of each element; X_0 itself and the result are four roundings in 32 bits
+    g = torch.Generator().manual_seed(3)
+    m = (1 + torch.rand(shape, generator=g)).to(dtype)
+    got = orthogonalize(m.cuda(), steps=1, coefficients=(1.0, 0.0, 0.0)).double().cpu()
+    ref = m.double() / (m.double().norm() + 1e-7)
+    own = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    assert ((got - ref).abs() <= (2.0 ** -23 + 4 * 2.0 ** -24 + 1.01 * own) * ref.abs() + 2.0 ** -50 + (2.0 ** -25 if dtype is torch.float16 else 0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 40), (40, 2), (300, 520)])
+def test_planes_of_small_elements(shape):
+    # one step with a = 1, b = c = 0 hands X_0 back as its two planes hold it: elements of 2^-16 to 2^-32 of the norm beside one that is the norm.  The planes of
+    # an X_0 scaled by 2^14 hold 2^-23 of an element, and 2^-36 where that is less; X_0 itself and the result are four roundings in 32 bits
+    g = torch.Generator().manual_seed(2)
+    m = torch.randn(shape, generator=g) * torch.exp2(-16.0 * (1 + torch.rand(shape, generator=g)))
+    m[0, 0] = 1.0
+    got = orthogonalize(m.cuda(), steps=1, coefficients=(1.0, 0.0, 0.0)).double().cpu()
+    ref = m.double() / (m.double().norm() + 1e-7)
+    assert ((got - ref).abs() <= (2.0 ** -23 + 4 * 2.0 ** -24) * ref.abs() + 2.0 ** -50).all()
