@@ -97,3 +97,32 @@ def test_planes_of_small_elements(shape):
     got = orthogonalize(m.cuda(), steps=1, coefficients=(1.0, 0.0, 0.0)).double().cpu()
     ref = m.double() / (m.double().norm() + 1e-7)
     assert ((got - ref).abs() <= (2.0 ** -23 + 4 * 2.0 ** -24) * ref.abs() + 2.0 ** -50).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 64), (1, 61, 33), (40, 128, 96), (40, 129, 97), (300, 128, 256), (300, 129, 257), (1501, 1003, 1201)])
+def test_operands_below_fp16s_normal_range(rows, k, n):
+    # 1e-5 to 6e-5 lies below 2^-14: as rows, as weights and as gradients, beside values that keep the results within range
+    g = torch.Generator().manual_seed(4)
+
+    def small(*shape):
+        return ((1e-5 + 5e-5 * torch.rand(shape, generator=g)) * torch.randn(shape, generator=g).sign()).half().cuda()
+
+    def large(*shape):
+        return (64 * torch.randn(shape, generator=g)).half().cuda()
+
+    def product(got, a, b, what):
+        a, b = a.double(), b.double().contiguous()
+        ref = a @ b
+        within(got, ref, allowance(torch.float16, ref, a.abs() @ b.abs()), what)
+
+    x, w, gy = small(rows, k), small(n, k), small(rows, n)
+    xs, ws = large(rows, k), large(n, k)
+    product(linear_act(x, ws), x, ws.t(), "small rows")
+    product(linear_act(xs, w), xs, w.t(), "small weights")
+    # gradients straight into the products, and by way of an activation's slope (1 here: all that goes into the sums is positive)
+    for name in (None, "relu"):
+        leaves = (xs.abs() / 64).requires_grad_(True), ws.abs().requires_grad_(True)
+        dx, dw = torch.autograd.grad(linear_act(*leaves, activation=name), leaves, gy)
+        product(dx, gy, leaves[1].detach(), "dx")
+        product(dw, gy.t(), leaves[0].detach(), "dw")
