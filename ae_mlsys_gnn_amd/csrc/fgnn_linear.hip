@@ -269,7 +269,7 @@ extern "C" int fgnn_linear_q8(int64_t rows, int n, int k, int eight, int type, c
     FGNN_REQUIRE(rows >= 0 && n >= 0 && k >= 0 && ldq >= k && ldw >= k, FGNN_ERR_SHAPE, "fgnn_linear_q8: bad sizes rows=%lld n=%d k=%d ldq=%lld ldw=%lld",
                  (long long)rows, n, k, (long long)ldq, (long long)ldw);
     FGNN_REQUIRE(fe_is_eight(eight), FGNN_ERR_SHAPE, "fgnn_linear_q8: operand type %d", eight);
-    FGNN_REQUIRE(eight != FGNN_I8 || k <= 131072, FGNN_ERR_LIMIT, "fgnn_linear_q8: sums of %d products of 8-bit integers do not fit 32 bits", k);
+    FGNN_REQUIRE(eight != FGNN_I8 || k <= 131071, FGNN_ERR_LIMIT, "fgnn_linear_q8: sums of %d products of 8-bit integers do not fit 32 bits", k);
     const int rc = gm_check_epilogue("fgnn_linear_q8", type, bias, btype, residual, ldr, n, act);
     if (rc) return rc;
     FGNN_REQUIRE(rows == 0 || n == 0 || (y && scale && weight_scale && (k == 0 || (q && weight))), FGNN_ERR_NULL, "fgnn_linear_q8: NULL argument");

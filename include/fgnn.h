@@ -337,7 +337,7 @@ int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const void *gy, con
  * that type or FGNN_F32).  act: 0 none, 1 relu, 2 gelu (by the error function), 3 silu, 4 leaky relu with `slope`.  bias, residual, z NULL: none; z
  * receives the activation's argument for the backward pass.  y, z contiguous.  fp32 products are summed from parts of 8 significant bits, to about
  * 2^-23 of the sum of magnitudes.
- * _q8: operands in 8 bits (eight: FGNN_I8, k <= 131072, or FGNN_E4M3) with scale [rows] and weight_scale [n]; bias, residual and y are of type `type`.
+ * _q8: operands in 8 bits (eight: FGNN_I8, k <= 131071, or FGNN_E4M3) with scale [rows] and weight_scale [n]; bias, residual and y are of type `type`.
  * _slope: dz = gy act'(z) (NULL: not wanted; rows of ldz = n, or of the next whole 16 bytes with zeros behind n) and dbias = its column sums (NULL: not
  * wanted), summed before dz is rounded.
  * _dx: dx [rows, k] = dz weight;  _dw: dw [n, k] = dz^T x; padded: zeros follow the rows of dz up to whole 16 bytes.  All are deterministic.

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from ae_mlsys_gnn_amd import _lib
-from ae_mlsys_gnn_amd.operators import linear_act, orthogonalize
+from ae_mlsys_gnn_amd.operators import linear_act, linear_q8, orthogonalize
 
 from .test_linear_gpu import allowance, within
 
@@ -126,3 +126,17 @@ def test_operands_below_fp16s_normal_range(rows, k, n):
         dx, dw = torch.autograd.grad(linear_act(*leaves, activation=name), leaves, gy)
         product(dx, gy, leaves[1].detach(), "dx")
         product(dw, gy.t(), leaves[0].detach(), "dw")
+
+
+def test_sums_of_8_bit_integers_fit_32_bits():
+    # 131,072 products of -128 by -128 are 2^31
+    l, p = _lib.lib(), 4096
+    assert l.fgnn_linear_q8(2, 6, 131072, I8, BF16, p, 131072, p, p, 131072, p, None, 1, None, 0, 0, 0.0, p, None, 0, None) == -4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 200])
+def test_largest_sums_of_8_bit_integers(rows):
+    q, w = (torch.full((n, 131071), -128, dtype=torch.int8, device="cuda") for n in (rows, 20))
+    y = linear_q8(q, torch.ones(rows, device="cuda"), w, torch.ones(20, device="cuda"), dtype=torch.float32)
+    assert (y == 131071 * 16384).all()
