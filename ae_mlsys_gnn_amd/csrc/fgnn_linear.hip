@@ -4,6 +4,8 @@
 // by that rounding.
 #include "fgnn_gemm.h"
 
+// Columns of a result are counted in 32 bits, up to the end of the tile or strip (of 2048) that holds the last.
+#define GM_MOST_COLUMNS (INT32_MAX - 4095)
 static int gm_units() { const int cus = fgnn_current_device_compute_units(); return cus > 0 ? cus : 256; }
 static int gm_slab_of(int kind) { return kind == FGNN_F32 ? 32 : kind == FGNN_I8 ? 128 : 64; }
 
@@ -169,6 +171,7 @@ static size_t gm_workspace(int64_t m, int n, int64_t k, int kind, bool qs, bool 
 // D [m, n] of type `type` from operands of kind `kind`; qs: Q is strided along the reduction (and P then too).
 static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, bool ps, bool q_padded, void *workspace, size_t workspace_bytes, hipStream_t st)
 {
+    FGNN_REQUIRE(p.n <= GM_MOST_COLUMNS, FGNN_ERR_LIMIT, "%s: %d columns", who, p.n);
     if (p.m == 0 || p.n == 0) return 0;
     const int64_t inner_q = qs ? p.m : p.k, inner_p = ps ? p.n : p.k;
     const bool q_moves = p.k > 0 && gm_movable(p.q, p.ldq, inner_q, kind, qs, q_padded), p_moves = p.k > 0 && gm_movable(p.p, p.ldp, inner_p, kind, ps, false);
@@ -244,7 +247,7 @@ static int gm_check_epilogue(const char *who, int type, const void *bias, int bt
 
 extern "C" size_t fgnn_linear_workspace_bytes(int64_t rows, int n, int k, int kind, int loose)
 {
-    if (rows < 1 || n < 1 || k < 0 || kind < FGNN_F32 || kind > FGNN_E4M3) return 0;
+    if (rows < 1 || n < 1 || n > GM_MOST_COLUMNS || k < 0 || kind < FGNN_F32 || kind > FGNN_E4M3) return 0;
     return gm_workspace(rows, n, k, kind, false, false, loose || kind == FGNN_E4M3);
 }
 
@@ -306,7 +309,7 @@ extern "C" int fgnn_linear_dw(int64_t rows, int n, int k, int type, const void *
 
 extern "C" size_t fgnn_linear_backward_workspace_bytes(int64_t rows, int n, int k, int type, int loose)
 {
-    if (rows < 1 || n < 1 || k < 1 || !fe_is_float(type)) return 0;
+    if (rows < 1 || n < 1 || k < 1 || k > GM_MOST_COLUMNS || !fe_is_float(type)) return 0;
     return std::max(gm_workspace(rows, k, n, type, false, true, loose), gm_workspace(n, k, rows, type, true, true, loose));
 }
 
@@ -369,7 +372,7 @@ static dim3 sl_grid(int64_t rows, int n, int type)
 
 extern "C" size_t fgnn_linear_slope_workspace_bytes(int64_t rows, int n, int type)
 {
-    if (rows < 1 || n < 1 || !fe_is_float(type)) return 0;
+    if (rows < 1 || n < 1 || n > GM_MOST_COLUMNS || !fe_is_float(type)) return 0;
     return (size_t)sl_grid(rows, n, type).y * n * sizeof(float);
 }
 
@@ -378,6 +381,7 @@ extern "C" int fgnn_linear_slope(int64_t rows, int n, int type, const void *gy, 
 {
     FGNN_REQUIRE(rows >= 0 && n >= 1 && ldg >= n && fe_is_float(type) && act >= GM_NONE && act <= GM_LEAKY, FGNN_ERR_SHAPE,
                  "fgnn_linear_slope: bad sizes rows=%lld n=%d ldg=%lld type=%d act=%d", (long long)rows, n, (long long)ldg, type, act);
+    FGNN_REQUIRE(n <= GM_MOST_COLUMNS, FGNN_ERR_LIMIT, "fgnn_linear_slope: %d columns", n);
     FGNN_REQUIRE(!dbias || btype == type || btype == FGNN_F32, FGNN_ERR_SHAPE, "fgnn_linear_slope: bias of type %d", btype);
     const int width = fe_is_float(type) ? 16 / fe_size(type) : 1;
     FGNN_REQUIRE(!dz || ldz == n || ldz == (n + width - 1) / width * width, FGNN_ERR_SHAPE, "fgnn_linear_slope: rows of %lld for %d columns", (long long)ldz, n);

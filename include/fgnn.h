@@ -336,7 +336,7 @@ int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const void *gy, con
 /* Linear maps with the epilogue in the product: y [rows, n] = act(x [rows, k] weight [n, k]^T + bias) + residual, all of one floating type (bias of
  * that type or FGNN_F32).  act: 0 none, 1 relu, 2 gelu (by the error function), 3 silu, 4 leaky relu with `slope`.  bias, residual, z NULL: none; z
  * receives the activation's argument for the backward pass.  y, z contiguous.  fp32 products are summed from parts of 8 significant bits, to about
- * 2^-23 of the sum of magnitudes.
+ * 2^-23 of the sum of magnitudes.  Results of up to 2^31 - 4096 columns.
  * _q8: operands in 8 bits (eight: FGNN_I8, k <= 131071, or FGNN_E4M3) with scale [rows] and weight_scale [n]; bias, residual and y are of type `type`.
  * _slope: dz = gy act'(z) (NULL: not wanted; rows of ldz = n, or of the next whole 16 bytes with zeros behind n) and dbias = its column sums (NULL: not
  * wanted), summed before dz is rounded.

@@ -140,3 +140,17 @@ def test_largest_sums_of_8_bit_integers(rows):
     q, w = (torch.full((n, 131071), -128, dtype=torch.int8, device="cuda") for n in (rows, 20))
     y = linear_q8(q, torch.ones(rows, device="cuda"), w, torch.ones(20, device="cuda"), dtype=torch.float32)
     assert (y == 131071 * 16384).all()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up: without a device nothing is launched")
+def test_columns_that_32_bits_cannot_count_are_refused():
+    # the last tile of columns ends past 2^31
+    l, p = _lib.lib(), 4096
+    n, most = 2 ** 31 - 100, 2 ** 31 - 4096
+    for rows in (1, 100):
+        assert l.fgnn_linear(rows, n, 1, BF16, p, 1, p, 1, None, 0, None, 0, 0, 0.0, None, p, None, 0, None) == -4
+        assert l.fgnn_linear(rows, most, 1, BF16, p, 1, p, 1, None, 0, None, 0, 0, 0.0, None, p, None, 0, None) != 0
+    assert l.fgnn_linear_q8(1, n, 1, I8, BF16, p, 1, p, p, 1, p, None, 1, None, 0, 0, 0.0, p, None, 0, None) == -4
+    assert l.fgnn_linear_dx(1, 1, n, BF16, p, 1, 0, p, n, p, None, 0, None) == -4
+    assert l.fgnn_linear_dw(1, 1, n, BF16, p, 1, 0, p, n, p, None, 0, None) == -4
+    assert l.fgnn_linear_slope(1, n, BF16, p, n, p, 1, 0.0, p, n, None, 0, None, 0, None) == -4
