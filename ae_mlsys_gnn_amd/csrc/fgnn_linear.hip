@@ -6,6 +6,8 @@
 
 // Columns of a result are counted in 32 bits, up to the end of the tile or strip (of 2048) that holds the last.
 #define GM_MOST_COLUMNS (INT32_MAX - 4095)
+// A launch has fewer than 2^32 threads.
+static bool gm_launches(int64_t workgroups, int threads) { return workgroups < (1ll << 32) / threads; }
 static int gm_units() { const int cus = fgnn_current_device_compute_units(); return cus > 0 ? cus : 256; }
 static int gm_slab_of(int kind) { return kind == FGNN_F32 ? 32 : kind == FGNN_I8 ? 128 : 64; }
 
@@ -55,9 +57,10 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const char *from, int6
     reinterpret_cast<gm_i4 *>(to)[i] = v;
 }
 static size_t gm_packed_bytes(int64_t rows, int64_t cols) { return fgnn_align256((size_t)rows * ((cols + 7) / 8) * 16); }
+static int64_t gm_pack_workgroups(int64_t rows, int64_t cols) { return (rows * ((cols + 7) / 8) + 255) / 256; }
 static void gm_pack(const void *from, int64_t ld, int64_t rows, int cols, char *to, bool e4m3, hipStream_t st)
 {
-    const dim3 g((unsigned)((rows * ((cols + 7) / 8) + 255) / 256));
+    const dim3 g((unsigned)gm_pack_workgroups(rows, cols));
     if (e4m3) hipLaunchKernelGGL(linear_pack_kernel<true>, g, dim3(256), 0, st, (const char *)from, ld, rows, cols, to);
     else hipLaunchKernelGGL(linear_pack_kernel<false>, g, dim3(256), 0, st, (const char *)from, ld, rows, cols, to);
 }
@@ -67,17 +70,17 @@ static void gm_pack(const void *from, int64_t ld, int64_t rows, int cols, char *
 // floats 8192 x 4096 -> 8192 577 / 407.
 static bool gm_worth_packing(int64_t m, int64_t n, int64_t k, int kind)
 {
-    const double most = (double)std::max(m, n) * ((k + 7) / 8 + 1);       // chunks of an operand: a launch's threads
-    return (kind == FGNN_BF16 || kind == FGNN_F16 || kind == FGNN_E4M3) && most < 2e11 && (double)m * n * k >= 3e9;
+    return (kind == FGNN_BF16 || kind == FGNN_F16 || kind == FGNN_E4M3) && (double)m * n * k >= 3e9;
 }
 
 // Whether rows `ld` bytes apart are near enough for the 32-bit offsets of the kernel that moves them: a tile takes up to 256 rows of an operand whose reduction
 // is contiguous, 64 of a strided one.
 static bool gm_near(int64_t ld, bool strided) { return ld * (strided ? 64 : 256) < (1ll << 31); }
-// Whether operands that cannot be moved as they lie are laid out anew: where it is worth it, and their new rows are near enough.
+// Whether operands that cannot be moved as they lie are laid out anew: where it is worth it, their new rows are near enough, and a launch has the threads.
 static bool gm_packs(int64_t m, int64_t n, int64_t k, int kind, bool qs, bool ps)
 {
-    return gm_worth_packing(m, n, k, kind) && gm_near(((qs ? m : k) + 7) / 8 * 16, qs) && gm_near(((ps ? n : k) + 7) / 8 * 16, ps);
+    return gm_worth_packing(m, n, k, kind) && gm_near(((qs ? m : k) + 7) / 8 * 16, qs) && gm_near(((ps ? n : k) + 7) / 8 * 16, ps)
+        && gm_launches(qs ? gm_pack_workgroups(k, m) : gm_pack_workgroups(m, k), 256) && gm_launches(ps ? gm_pack_workgroups(k, n) : gm_pack_workgroups(n, k), 256);
 }
 
 // Whether rows of an operand are whole 16-byte chunks at 16-byte addresses, and near enough.
@@ -128,6 +131,7 @@ static int gm_rows_ct(int64_t m, int n) { return m > 16 && n >= 32 * gm_units() 
 static bool gm_few(const GemmP &p, int kind, bool moved)
 {
     const int64_t again = (p.m + 15) / 16 * p.k * p.n * fe_size(kind) / gm_rows_ct(p.m, p.n);
+    if (!gm_launches(p.n / 16 + 1, 64 * GR_WAVES)) return false;
     return p.m <= 16 || (p.m <= 64 && again <= (moved ? 100000000 : 300000000));
 }
 template <int KIND, typename E>
@@ -205,7 +209,7 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
     const int tile = moved ? gm_tile_for(p.m, p.n) : 128;
     gm_cut(&p, tile, kind, moved);
     if (few) p.splits = 1;
-    FGNN_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (1ll << 31) && (p.m * ((p.n + 3) / 4) + 255) / 256 < (1ll << 31), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
+    FGNN_REQUIRE(few || gm_launches((p.m + tile - 1) / tile * p.tiles_n * p.splits, tile == 256 ? 512 : 256), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
     FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= gm_part_bytes(p)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
                  workspace_bytes);
     p.part = (float *)workspace;

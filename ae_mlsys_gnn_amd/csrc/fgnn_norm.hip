@@ -247,29 +247,35 @@ __global__ __launch_bounds__(T > NM_TPB ? T : NM_TPB) void norm_backward_kernel(
     }
 }
 
-// out [cols] = the column sums of part [rows, cols], in a type known at run time: 16 columns a workgroup, 64 rows side by side.
+// out [cols] = the column sums of part [rows, cols], in a type known at run time: 16 columns a workgroup at a time, 64 rows side by side.
+#define NM_SUM_GRID (1 << 20)               // most workgroups: a launch has fewer than 2^32 threads
 __global__ __launch_bounds__(1024) void norm_sum_kernel(const float *__restrict__ part, int rows, int cols, void *out, int type)
 {
     __shared__ float red[64][17];
-    const int c = (int)threadIdx.x & 15, q = (int)threadIdx.x >> 4, col = (int)blockIdx.x * 16 + c;
-    float v = 0.f;
-    if (col < cols) {
+    const int c = (int)threadIdx.x & 15, q = (int)threadIdx.x >> 4;
+    for (int64_t first = (int64_t)blockIdx.x * 16; first < cols; first += (int64_t)gridDim.x * 16) {
+        const int64_t col = first + c;
+        float v = 0.f;
+        if (col < cols) {
 #pragma unroll 4
-        for (int i = q; i < rows; i += 64) v += part[(int64_t)i * cols + col];
-    }
-    red[q][c] = v;
-    __syncthreads();
-    if (q == 0 && col < cols) {
-        v = 0.f;
+            for (int i = q; i < rows; i += 64) v += part[(int64_t)i * cols + col];
+        }
+        __syncthreads();                    // the sums before are read
+        red[q][c] = v;
+        __syncthreads();
+        if (q == 0 && col < cols) {
+            v = 0.f;
 #pragma unroll 8
-        for (int i = 0; i < 64; ++i) v += red[i][c];
-        fe_store(out, col, type, v);
+            for (int i = 0; i < 64; ++i) v += red[i][c];
+            fe_store(out, col, type, v);
+        }
     }
 }
 
 int fgnn_sum_parts(const float *part, int rows, int cols, void *out, int type, hipStream_t st)
 {
-    hipLaunchKernelGGL(norm_sum_kernel, dim3((cols + 15) / 16), dim3(1024), 0, st, part, rows, cols, out, type);
+    const unsigned groups = (unsigned)(((int64_t)cols + 15) / 16);
+    hipLaunchKernelGGL(norm_sum_kernel, dim3(std::min<unsigned>(groups, NM_SUM_GRID)), dim3(1024), 0, st, part, rows, cols, out, type);
     return fgnn_launch_status("norm_sum_kernel");
 }
 

@@ -154,3 +154,24 @@ def test_columns_that_32_bits_cannot_count_are_refused():
     assert l.fgnn_linear_dx(1, 1, n, BF16, p, 1, 0, p, n, p, None, 0, None) == -4
     assert l.fgnn_linear_dw(1, 1, n, BF16, p, 1, 0, p, n, p, None, 0, None) == -4
     assert l.fgnn_linear_slope(1, n, BF16, p, n, p, 1, 0.0, p, n, None, 0, None, 0, None) == -4
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up: without a device nothing is launched")
+def test_more_tiles_than_a_launch_takes_are_refused():
+    # 2^24 tiles of 256 threads are 2^32 threads
+    l, p = _lib.lib(), 4096
+    assert l.fgnn_linear(2 ** 31, 1, 1, BF16, p, 1, p, 1, None, 0, None, 0, 0, 0.0, None, p, None, 0, None) == -4
+    assert l.fgnn_linear(2 ** 31 - 128, 1, 1, BF16, p, 1, p, 1, None, 0, None, 0, 0, 0.0, None, p, None, 0, None) not in (0, -4)
+
+
+@pytest.mark.gpu
+def test_a_row_of_many_columns():
+    # more columns than a launch of the kernel for few rows, or one of the bias gradient's last sum, has threads for
+    n = 2 ** 28 + 40
+    x = torch.randn(2, 1).cuda().bfloat16()
+    w = torch.randn(n, 1, device="cuda").bfloat16()
+    b = torch.zeros(n, device="cuda", requires_grad=True)
+    y = linear_act(x, w, b)
+    assert torch.equal(y.detach(), (x.float() * w.float().t()).bfloat16())
+    (db,) = torch.autograd.grad(y, b, y.detach())
+    assert torch.equal(db, y.detach().float().sum(0))
