@@ -652,7 +652,7 @@ struct GemmMover {
         const uint64_t from = (uint64_t)(base + index * step + plane);
         const gm_i4 buffer = {(int)(uint32_t)from, (int)((uint32_t)(from >> 32) & 0xffffu), (int)0x80000000u, 0x00027000};
         const uint32_t v = along[c] < left ? at[c] : 0x80000000u;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(tile + (c * WAVES + wave) * 1024), "v"(v), "s"(buffer));
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(tile + (c * WAVES + wave) * 1024), "v"(v), "s"(buffer) : "m0");
     }
 };
 

@@ -1,4 +1,8 @@
 """The dense operators at the ends of their ranges: long rows and row strides, small and large values, sums of integers, what they refuse."""
+import glob
+import os
+import re
+
 import pytest
 import torch
 
@@ -8,6 +12,7 @@ from ae_mlsys_gnn_amd.operators import linear_act, linear_q8, orthogonalize
 from .test_linear_gpu import allowance, within
 
 F32, BF16, F16, I8, E4M3 = range(5)
+CSRC = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
 
 
 def test_rows_past_32_bit_offsets_are_not_laid_out_anew():
@@ -175,3 +180,15 @@ def test_a_row_of_many_columns():
     assert torch.equal(y.detach(), (x.float() * w.float().t()).bfloat16())
     (db,) = torch.autograd.grad(y, b, y.detach())
     assert torch.equal(db, y.detach().float().sum(0))
+
+
+def test_assembly_declares_what_it_writes():
+    # a scalar register that a statement names as its first operand, and that is no operand of the statement itself, is among what it says it changes
+    seen = 0
+    for path in glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.hip")):
+        for body in re.findall(r"\basm(?:\s+volatile)?\s*\((.*?)\);", open(path).read(), flags=re.S):
+            parts = re.split(r":(?=(?:[^\"]*\"[^\"]*\")*[^\"]*$)", body)
+            for written in re.findall(r"\bs_\w+\s+(m0|vcc|exec|s\d+)\b", parts[0]):
+                seen += 1
+                assert len(parts) == 4 and '"%s"' % written in parts[3], (os.path.basename(path), written)
+    assert seen >= 1
