@@ -646,13 +646,13 @@ struct GemmMover {
     // Transfer c of slab `index` of a plane that starts `plane` bytes after the first; `left` reduction elements exist from its first on.  What lies past them
     // is read as zeros: out of the buffer's range.  Written out (it has no output registers), because the compiler would have every transposing read wait
     // for all transfers before it, whatever their place; gm_arrive waits for the ones that matter, and orders reads against them.  Five wait states
-    // between whatever wrote the descriptor (a spilled scalar comes back by a vector instruction) and its use, which nobody else counts here.
+    // between whatever wrote the descriptor (a spilled scalar comes back by a vector instruction) or m0, the place in LDS, and their use, which nobody else counts here.
     __device__ __forceinline__ void move(int c, int64_t index, int64_t plane, int64_t left, uint32_t tile, int wave) const
     {
         const uint64_t from = (uint64_t)(base + index * step + plane);
         const gm_i4 buffer = {(int)(uint32_t)from, (int)((uint32_t)(from >> 32) & 0xffffu), (int)0x80000000u, 0x00027000};
         const uint32_t v = along[c] < left ? at[c] : 0x80000000u;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(tile + (c * WAVES + wave) * 1024), "v"(v), "s"(buffer) : "m0");
+        asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v), "s"(buffer), "{m0}"(tile + (c * WAVES + wave) * 1024));
     }
 };
 

@@ -183,12 +183,12 @@ def test_a_row_of_many_columns():
 
 
 def test_assembly_declares_what_it_writes():
-    # a scalar register that a statement names as its first operand, and that is no operand of the statement itself, is among what it says it changes
+    # a scalar register that an instruction of a statement names as its first operand is among what the statement says it changes
     seen = 0
     for path in glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.hip")):
         for body in re.findall(r"\basm(?:\s+volatile)?\s*\((.*?)\);", open(path).read(), flags=re.S):
             parts = re.split(r":(?=(?:[^\"]*\"[^\"]*\")*[^\"]*$)", body)
+            seen += 1
             for written in re.findall(r"\bs_\w+\s+(m0|vcc|exec|s\d+)\b", parts[0]):
-                seen += 1
                 assert len(parts) == 4 and '"%s"' % written in parts[3], (os.path.basename(path), written)
-    assert seen >= 1
+    assert seen >= 3
