@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from ae_mlsys_gnn_amd import _lib
-from ae_mlsys_gnn_amd.operators import linear_act, linear_q8, orthogonalize
+from ae_mlsys_gnn_amd.operators import linear_act, linear_q8, orthogonalize, rms_norm
 
 from .test_linear_gpu import allowance, within
 
@@ -192,3 +192,27 @@ def test_assembly_declares_what_it_writes():
             for written in re.findall(r"\bs_\w+\s+(m0|vcc|exec|s\d+)\b", parts[0]):
                 assert len(parts) == 4 and '"%s"' % written in parts[3], (os.path.basename(path), written)
     assert seen >= 3
+
+
+@pytest.mark.gpu
+def test_last_sums_of_column_sums():
+    # 2^24 beside 63 ones: each part of the sum is exact, and 32 bits would drop every one added to it alone.  Rows are dealt out in turns of 32, so that the
+    # ones stand in other parts than the large value
+    gy = torch.zeros(2048, 32)
+    gy[0] = 2.0 ** 24
+    gy[32::32] = 1.0
+    b = torch.zeros(32, device="cuda", requires_grad=True)
+    x, w = torch.zeros(2048, 8, device="cuda"), torch.zeros(32, 8, device="cuda")
+    (db,) = torch.autograd.grad(linear_act(x, w, b), b, gy.cuda())
+    ref = gy.double().sum(0)
+    assert ((db.cpu().double() - ref).abs() <= 4 * 2.0 ** -24 * ref).all(), db
+    # the norm's weights: as exact as 32 bits in each workgroup and one rounding
+    for rows, cols in ((2708, 128), (20000, 64)):
+        g = torch.Generator().manual_seed(5)
+        x, gy = torch.randn(rows, cols, generator=g), torch.randn(rows, cols, generator=g)
+        wl = torch.ones(cols).cuda().requires_grad_(True)
+        (dw,) = torch.autograd.grad(rms_norm(x.cuda(), wl), wl, gy.cuda())
+        terms = gy.double() * x.double() * (x.double().square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+        # errors of the terms (a handful of roundings each) and of the workgroups' sums of at most 16 rows side by side add up like a walk
+        off = (dw.cpu().double() - terms.sum(0)).norm() / terms.sum(0).norm()
+        assert off <= 4 * 2.0 ** -24, off
