@@ -8,11 +8,12 @@
 // one store instruction writes 64 bytes of each of 16 rows, as do reads of the residual (with 16 columns a lane, in four stores of 16 bytes each 64
 // apart, the L2 saw four times the requests: 169,343 x 128 -> 256 fp32 with gelu and residual 226 us).
 //
-// Element kinds: 16-bit values (products of 8 significant bits and sums in 32 bits), 8-bit integers (sums in integers: exact), 8-bit floats, and
-// fp32.  fp32 operands are cut into three parts of 8 significant bits (truncated, so that the three are exact), and the six products that reach above
+// Element kinds: 16-bit values (exact products, summed in 32 bits), 8-bit integers (summed in integers, over the parts of a cut reduction too: exact), 8-bit
+// floats, and fp32.  fp32 operands are cut into three parts of 8 significant bits (truncated, so that the three are exact), and the six products that reach above
 // 2^-24 of the result are summed in 32 bits: the matrix unit does 16 of them in the time of one fp32 product.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 #include "fgnn_elem.h"
 
 typedef float gm_f4 __attribute__((ext_vector_type(4)));
@@ -101,8 +102,8 @@ struct GemmEpi {
 };
 
 // W consecutive elements of a row, the first `count` of them where fewer are left.
-template <typename E, int W>
-__device__ __forceinline__ void gm_load(float (&v)[W], const E *p, int count)
+template <typename E, int W, typename U>
+__device__ __forceinline__ void gm_load(U (&v)[W], const E *p, int count)
 {
     constexpr int V = fe_width<E> < W ? fe_width<E> : W;
     typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
@@ -111,15 +112,15 @@ __device__ __forceinline__ void gm_load(float (&v)[W], const E *p, int count)
         for (int j = 0; j < W / V; ++j) {
             const vec u = *reinterpret_cast<const vec *>(p + j * V);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[j * V + i] = (float)u[i];
+            for (int i = 0; i < V; ++i) v[j * V + i] = (U)u[i];
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = i < count ? (float)p[i] : 0.f;
+        for (int i = 0; i < W; ++i) v[i] = i < count ? (U)p[i] : (U)0;
     }
 }
-template <typename E, int W>
-__device__ __forceinline__ void gm_store(const float (&v)[W], E *p, int count)
+template <typename E, int W, typename U>
+__device__ __forceinline__ void gm_store(const U (&v)[W], E *p, int count)
 {
     constexpr int V = fe_width<E> < W ? fe_width<E> : W;
     typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
@@ -194,7 +195,7 @@ struct GemmP {
     int tiles_m, tiles_n, splits;
     int lower;                              // only tiles on and below the diagonal: D is symmetric, and the epilogue writes the rest
     int64_t slabs;                          // slabs of the reduction a split takes
-    float *part;                            // [splits][m][n] where splits > 1
+    void *part;                             // [splits][m][n] where splits > 1, in the type of the sums: fp32, or int32 of 8-bit integers
     int64_t rows_q, rows_p;                 // rows that the operands have (more than D has where a strided one is padded to whole chunks)
     int64_t batch_q, batch_p, plane_q, plane_p;                                // bytes between the batch's matrices, and between planes
     GemmEpi epi;
@@ -343,20 +344,21 @@ __device__ __forceinline__ void gm_results(const GemmP &p, const F &f, int64_t b
 {
     constexpr int W = F::W, J = 16 / W, ROWS = F::ROWS < TQ ? F::ROWS : TQ;
     const int r = lane & 15, g = lane >> 4;
-    auto sums = [&](int i, int j, float (&v)[W]) {
+    auto sums = [&]<typename U>(int i, int j, U (&v)[W]) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) v[k] = (float)acc[i][j * (W / 4) + k / 4][k % 4];
+        for (int k = 0; k < W; ++k) v[k] = (U)acc[i][j * (W / 4) + k / 4][k % 4];
     };
     auto column = [&](int j) { return n0 + 4 * W * j + W * g; };
     if (p.splits > 1) {
+        typedef std::remove_reference_t<decltype(acc[0][0][0] + acc[0][0][0])> S;           // float, or int of 8-bit integers
 #pragma unroll
         for (int i = 0; i < TQ; ++i)
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 const int64_t m = m0 + 16 * i + r;
-                float v[W];
+                S v[W];
                 sums(i, j, v);
-                if (m < p.m && column(j) < p.n) gm_store<float, W>(v, p.part + ((batch * p.splits + split) * p.m + m) * p.n + column(j), p.n - column(j));
+                if (m < p.m && column(j) < p.n) gm_store<S, W>(v, (S *)p.part + ((batch * p.splits + split) * p.m + m) * p.n + column(j), p.n - column(j));
             }
         return;
     }
@@ -573,25 +575,26 @@ __global__ __launch_bounds__(256, 2) void gemm_any_kernel(GemmP p)
 }
 
 // The partial sums of a reduction cut into `splits`, added up in a fixed order: four columns a thread, or a part of their sums where few columns have many.
-template <typename E, int SHARE>
+template <typename E, typename S, int SHARE>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmP p)
 {
-    __shared__ gm_f4 sums[SHARE > 1 ? 256 : 1];
+    typedef S quad __attribute__((ext_vector_type(4)));
+    __shared__ quad sums[SHARE > 1 ? 256 : 1];
     const int quads = (p.n + 3) / 4, share = (int)threadIdx.x / (256 / SHARE);
     const int64_t i = (int64_t)blockIdx.x * (256 / SHARE) + threadIdx.x % (256 / SHARE), m = i / quads;
     const int n = (int)(i - m * quads) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    S v[4] = {0, 0, 0, 0};
     if (m < p.m) {
 #pragma unroll 4
         for (int s = share; s < p.splits; s += SHARE) {
-            float u[4];
-            gm_load<float, 4>(u, p.part + ((int64_t)s * p.m + m) * p.n + n, p.n - n);
+            S u[4];
+            gm_load<S, 4>(u, (const S *)p.part + ((int64_t)s * p.m + m) * p.n + n, p.n - n);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] += u[j];
         }
     }
     if constexpr (SHARE > 1) {
-        sums[threadIdx.x] = gm_f4{v[0], v[1], v[2], v[3]};
+        sums[threadIdx.x] = quad{v[0], v[1], v[2], v[3]};
         __syncthreads();
         if (share) return;
 #pragma unroll
@@ -602,7 +605,8 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmP p)
     if (m >= p.m) return;
     GemmCols<4> cols;
     gm_columns(p.epi, n, cols);
-    gm_finish<E, 4>(p.epi, cols, gm_ahead<E, 4>(p.epi, m, n), m, n, v);
+    float z[4] = {(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+    gm_finish<E, 4>(p.epi, cols, gm_ahead<E, 4>(p.epi, m, n), m, n, z);
 }
 
 // ------------------------------------------------------------------------------------------------ aligned operands, from memory to LDS

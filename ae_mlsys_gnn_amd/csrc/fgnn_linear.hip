@@ -101,14 +101,14 @@ static void gm_launch_any(const GemmP &p, bool qs, bool ps, hipStream_t st)
     else if (ps) hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, true>), g, b, 0, st, p);
     else hipLaunchKernelGGL((gemm_any_kernel<KIND, E, false, false>), g, b, 0, st, p);
 }
-template <typename E>
+template <typename E, typename S>
 static void gm_join(const GemmP &p, hipStream_t st)
 {
     if (p.splits == 1) return;
     // eight threads a column where it has many parts and there are few columns (256 x 128 of 128 parts 67 / 12 us)
     const int64_t quads = p.m * ((p.n + 3) / 4);
-    if (p.splits >= 16 && quads < 256 * 256) hipLaunchKernelGGL((gemm_join_kernel<E, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((gemm_join_kernel<E, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p);
+    if (p.splits >= 16 && quads < 256 * 256) hipLaunchKernelGGL((gemm_join_kernel<E, S, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((gemm_join_kernel<E, S, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p);
 }
 template <int KIND, typename E, int TILE, bool FORWARD = false>
 static void gm_launch_moved(const GemmP &p, bool qs, bool ps, hipStream_t st)
@@ -212,7 +212,7 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
     FGNN_REQUIRE(few || gm_launches((p.m + tile - 1) / tile * p.tiles_n * p.splits, tile == 256 ? 512 : 256), FGNN_ERR_LIMIT, "%s: more tiles than a launch takes", who);
     FGNN_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= gm_part_bytes(p)), FGNN_ERR_WORKSPACE, "%s: workspace of %zu bytes", who,
                  workspace_bytes);
-    p.part = (float *)workspace;
+    p.part = workspace;
     p.epi.m = p.m; p.epi.n = p.n;
     auto launch = [&]<int KIND, typename E>() {
         if (few) return gm_launch_rows<KIND, E>(p, st);
@@ -221,13 +221,13 @@ static int gm_product(const char *who, GemmP p, int kind, int type, bool qs, boo
             else if (moved) gm_launch_moved<KIND, E, 128>(p, qs, ps, st);
             else gm_launch_any<KIND, E>(p, qs, ps, st);
         } else gm_launch_any<KIND, E>(p, qs, ps, st);
-        gm_join<E>(p, st);
+        gm_join<E, std::conditional_t<KIND == FGNN_I8, int, float>>(p, st);
     };
     // 8-bit floats as fp16: forward products of moved operands alone
     auto launch_widened = [&]<typename E>() {
         if (tile == 256) gm_launch_moved<FGNN_F16, E, 256, true>(p, false, false, st);
         else gm_launch_moved<FGNN_F16, E, 128, true>(p, false, false, st);
-        gm_join<E>(p, st);
+        gm_join<E, float>(p, st);
     };
     if (kind == FGNN_F32) launch.template operator()<FGNN_F32, float>();
     else if (kind == FGNN_BF16) launch.template operator()<FGNN_BF16, __bf16>();

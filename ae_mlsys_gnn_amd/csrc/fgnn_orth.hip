@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void orth_join_kernel(GemmP p, OrthEpi f)
 #pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
         float u[8];
-        gm_load<float, 8>(u, p.part + ((batch * p.splits + s) * p.m + m) * p.n + n, p.n - n);
+        gm_load<float, 8>(u, (const float *)p.part + ((batch * p.splits + s) * p.m + m) * p.n + n, p.n - n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += u[i];
     }

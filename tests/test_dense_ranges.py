@@ -216,3 +216,14 @@ def test_last_sums_of_column_sums():
         # errors of the terms (a handful of roundings each) and of the workgroups' sums of at most 16 rows side by side add up like a walk
         off = (dw.cpu().double() - terms.sum(0)).norm() / terms.sum(0).norm()
         assert off <= 4 * 2.0 ** -24, off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(100, 40000, 24), (300, 6000, 200), (257, 9001, 130), (70, 131071, 9), (1500, 1024, 1024), (40, 5000, 48)])
+def test_sums_of_8_bit_integers_are_exact(rows, k, n):
+    # sums past 2^24 in every part of a cut reduction, and past it altogether: one rounding to fp32, at the end
+    g = torch.Generator().manual_seed(6)
+    q, w = (torch.randint(90, 128, (m, k), dtype=torch.int8, generator=g) for m in (rows, n))
+    w[::3] *= -1
+    got = linear_q8(q.cuda(), torch.ones(rows).cuda(), w.cuda(), torch.ones(n).cuda(), dtype=torch.float32)
+    assert torch.equal(got.cpu(), (q.double() @ w.double().t()).float())
