@@ -60,6 +60,9 @@ __device__ __forceinline__ void gm_act(float (&z)[W], int act, float slope)
         break;
     }
 }
+// Far out gelu and silu are straight: what is outside +-128 has the slope that is there, 0 or 1 in 32 bits.  (z comes rounded to the rows' type: of fp16 an infinity
+// may stand for an argument that the forward pass had as a finite number.)  A NaN stays one.
+__device__ __forceinline__ float gm_within(float z) { return z > 128.f ? 128.f : z < -128.f ? -128.f : z; }
 // g times the slope at z
 template <int W>
 __device__ __forceinline__ void gm_act_slope(float (&g)[W], const float (&z)[W], int act, float slope)
@@ -73,15 +76,15 @@ __device__ __forceinline__ void gm_act_slope(float (&g)[W], const float (&z)[W],
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             float bell;
-            const float p = gm_normal(z[i], bell);
-            g[i] *= fmaf(z[i], 0.39894228f * bell, p);
+            const float u = gm_within(z[i]), p = gm_normal(u, bell);
+            g[i] *= fmaf(u, 0.39894228f * bell, p);
         }
         break;
     case GM_SILU:
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            const float p = gm_logistic(z[i]);
-            g[i] *= fmaf(p * z[i], 1.f - p, p);
+            const float u = gm_within(z[i]), p = gm_logistic(u);
+            g[i] *= fmaf(p * u, 1.f - p, p);
         }
         break;
     case GM_LEAKY:

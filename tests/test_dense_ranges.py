@@ -9,7 +9,7 @@ import torch
 from ae_mlsys_gnn_amd import _lib
 from ae_mlsys_gnn_amd.operators import linear_act, linear_q8, orthogonalize, rms_norm
 
-from .test_linear_gpu import allowance, within
+from .test_linear_gpu import act, allowance, within
 
 F32, BF16, F16, I8, E4M3 = range(5)
 CSRC = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
@@ -227,3 +227,35 @@ def test_sums_of_8_bit_integers_are_exact(rows, k, n):
     w[::3] *= -1
     got = linear_q8(q.cuda(), torch.ones(rows).cuda(), w.cuda(), torch.ones(n).cuda(), dtype=torch.float32)
     assert torch.equal(got.cpu(), (q.double() @ w.double().t()).float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["relu", "gelu", "silu", "leaky_relu"])
+@pytest.mark.parametrize("n", [16, 33])
+def test_gradients_where_an_argument_leaves_fp16(name, n):
+    # z of +-90,000 and +-60,000, and what lies between: the activation's slope is 0 or 1 (0.2 where the rows leak) whatever z is rounded to
+    x = torch.tensor([[300.0], [200.0], [-200.0], [-300.0], [1.0]]).half()
+    w = torch.full((n, 1), 300.0).half()
+    xl, wl = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    y = linear_act(xl, wl, activation=name)
+    low = 0.2 if name == "leaky_relu" else 0.0
+    assert torch.equal(y[1].cpu().float(), torch.full((n,), 60000.0)) and ((y[3].cpu().float() + 0.0 - low * -90000.0).abs() <= 16).all()
+    gy = torch.full((5, n), 2.0 ** -10)
+    dx, dw = torch.autograd.grad(y, (xl, wl), gy.half().cuda())
+    slope = torch.tensor([1.0, 1.0, low, low, 1.0]).half().double()[:, None]
+    dz = (gy.double() * slope).half().double()
+    within(dx, dz @ w.double(), allowance(torch.float16, dz @ w.double(), dz.abs() @ w.double().abs(), 2.0 ** -11 * (dz.abs() @ w.double().abs())), "dx")
+    within(dw, dz.t() @ x.double(), allowance(torch.float16, dz.t() @ x.double(), dz.abs().t() @ x.double().abs(), 2.0 ** -11 * (dz.abs().t() @ x.double().abs())), "dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", ["gelu", "silu"])
+def test_slopes_far_out(dtype, name):
+    z = torch.tensor([-3e38, -1e20, -1000.0, -129.0, -100.0, -30.0, -9.0, -1.0, 0.0, 1.0, 9.0, 30.0, 100.0, 129.0, 1000.0, 1e20, 3e38], dtype=torch.float64).to(dtype)
+    x = z[:, None].cuda().requires_grad_(True)
+    (dx,) = torch.autograd.grad(linear_act(x, torch.ones(1, 1, device="cuda", dtype=dtype), activation=name), x, torch.ones(len(z), 1, device="cuda", dtype=dtype))
+    zd = z.double().requires_grad_(True)
+    (ref,) = torch.autograd.grad(act(zd, name).sum(), zd)
+    # one rounding of dz, one of dx, and the approximation's own 1e-6 (exponentials of up to 128 in 32 bits: 2^-17 of what is left there)
+    assert ((dx[:, 0].double().cpu() - ref).abs() <= 2.02 * {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}[dtype] * ref.abs() + 1e-6).all()
