@@ -212,7 +212,7 @@ __global__ __launch_bounds__(T > NM_TPB ? T : NM_TPB) void norm_backward_kernel(
         }
         if (!p.dx) continue;
         dot = nm_all<T, false>(dot, red);
-        const float k = s * s * s * dot * inv;
+        const float k = s * s * (s * dot * inv);           // (s dot is of the gradient's size, where s^3 leaves 32 bits for rows of 1e13 or 1e-13)
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int c = (r * T + lane) * V;

@@ -259,3 +259,20 @@ def test_slopes_far_out(dtype, name):
     (ref,) = torch.autograd.grad(act(zd, name).sum(), zd)
     # one rounding of dz, one of dx, and the approximation's own 1e-6 (exponentials of up to 128 in 32 bits: 2^-17 of what is left there)
     assert ((dx[:, 0].double().cpu() - ref).abs() <= 2.02 * {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}[dtype] * ref.abs() + 1e-6).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-17, 1e-14, 1e-10, 1.0, 1e10, 1e14, 1e17])
+def test_gradient_of_the_norm_of_large_and_small_rows(dtype, size):
+    g = torch.Generator().manual_seed(7)
+    x = (torch.randn(9, 300, generator=g).double() * size).to(dtype)
+    gy = (torch.randn(9, 300, generator=g) + x.double().float() / size).to(dtype)       # with a part along the row, which the second term takes away
+    xl = x.cuda().requires_grad_(True)
+    (dx,) = torch.autograd.grad(rms_norm(xl, eps=0.0), xl, gy.cuda())
+    xd = x.double().requires_grad_(True)
+    (ref,) = torch.autograd.grad(xd * xd.square().mean(-1, keepdim=True).rsqrt(), xd, gy.double())
+    s, hd, gd = xd.detach().square().mean(-1, keepdim=True).rsqrt(), xd.detach(), gy.double()
+    parts = (s * gd).abs() + (hd * s).abs() * s * (gd * hd * s).abs().mean(-1, keepdim=True)
+    unit = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}[dtype]
+    assert ((dx.double().cpu() - ref).abs() <= 1.01 * unit * ref.abs() + 16 * 2.0 ** -24 * parts).all()
