@@ -3,10 +3,12 @@
 // most of the rest to the thread that runs backward passes).  The kernels are those of libfgnn_hip.so; there is no CPU path here either.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <sstream>
 #include "fgnn.h"
 
@@ -42,9 +44,22 @@ int float_type(const Tensor &t)
 int eight_type(at::ScalarType t) { return t == at::kChar ? FGNN_I8 : t == at::kFloat8_e4m3fn ? FGNN_E4M3 : -1; }
 void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
-void on_gpu(const Tensor &t)
+// Operands are on the GPU, and torch's own operations are not being recorded or transformed: a kernel launched past jit.trace, make_fx or export would be missing from the
+// record (its output a constant of it), and one launched past forward mode would drop the tangents, with no error from anyone.  torch.compile breaks its graph at
+// the call and runs it as it is; functorch's tensors have no memory and are refused for that by torch.
+void usable_one(const char *who, const Tensor &t)
 {
-    if (t.defined() && !t.is_cuda()) refuse("fgnn operators run on the GPU only (got a ", t.device(), " tensor); there is no CPU path");
+    if (!t.defined()) return;
+    if (!t.is_cuda()) refuse("fgnn operators run on the GPU only (got a ", t.device(), " tensor); there is no CPU path");
+    if (t._fw_grad(0).defined()) refuse(who, ": derivatives in forward mode are not recorded");
+}
+template <typename... T> void usable(const char *who, const T &...operands)
+{
+    (usable_one(who, operands), ...);
+    typedef c10::impl::TorchDispatchModeTLS Modes;
+    typedef c10::impl::TorchDispatchModeKey Mode;
+    if (torch::jit::tracer::isTracing() || (Modes::any_modes_set() && (Modes::get_mode(Mode::PROXY) || Modes::get_mode(Mode::FAKE) || Modes::get_mode(Mode::FUNCTIONAL))))
+        refuse(who, ": calls are not recorded by jit.trace, make_fx or export");
 }
 Tensor given(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
 
@@ -99,7 +114,7 @@ variable_list final_gradients(const char *what, variable_list grads)
 struct NormOperands { Rows x, r; Tensor w; int type, wtype; };
 NormOperands norm_operands(const char *who, const Tensor &x, const Tensor &w, const Tensor &r)
 {
-    on_gpu(x); on_gpu(w); on_gpu(r);
+    usable(who, x, w, r);
     const int type = float_type(x);
     if (type < 0) refuse(who, ": rows of ", x.scalar_type(), "; fp32, bf16 and fp16 are supported");
     if (x.dim() == 0 || x.size(-1) == 0) refuse(who, ": no features in ", x.sizes());
@@ -233,7 +248,7 @@ Epilogue epilogue(const char *who, const Tensor &x, int64_t n, at::ScalarType dt
 struct LinearOut { Tensor y, z; };
 LinearOut linear_forward(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, int64_t act, double slope, bool keep)
 {
-    on_gpu(x); on_gpu(w); on_gpu(bias); on_gpu(residual);
+    usable("linear_act", x, w, bias, residual);
     const int type = float_type(x);
     if (type < 0 || w.scalar_type() != x.scalar_type())
         refuse("linear_act: rows of ", x.scalar_type(), " with weights of ", w.scalar_type(), "; fp32, bf16 and fp16, both the same, are supported");
@@ -317,7 +332,7 @@ Tensor linear_q8(const Tensor &q, const Tensor &scale, const Tensor &w, const Te
                  at::ScalarType to)
 {
     const Tensor b = given(bias), r = given(residual);
-    for (const Tensor &t : {q, scale, w, wscale, b, r}) on_gpu(t);
+    usable("linear_q8", q, scale, w, wscale, b, r);
     const int eight = eight_type(q.scalar_type()), type = to == at::kFloat ? FGNN_F32 : to == at::kBFloat16 ? FGNN_BF16 : to == at::kHalf ? FGNN_F16 : -1;
     if (eight < 0 || w.scalar_type() != q.scalar_type() || type < 0)
         refuse("linear_q8: ", q.scalar_type(), " with weights of ", w.scalar_type(), " to ", to, "; int8 or float8_e4m3fn, both the same, to fp32, bf16 or fp16 are supported");
@@ -341,7 +356,7 @@ Tensor linear_q8(const Tensor &q, const Tensor &scale, const Tensor &w, const Te
 // ------------------------------------------------------------------------------------------------ orthogonalised updates
 Tensor orthogonalize(const Tensor &given_g, const std::vector<float> &coefficients, double eps)
 {
-    on_gpu(given_g);
+    usable("orthogonalize", given_g);
     const int type = float_type(given_g);
     if (type < 0 || given_g.dim() < 2) refuse("orthogonalize: matrices ", given_g.sizes(), " of ", given_g.scalar_type(), "; fp32, bf16 and fp16 are supported");
     const Tensor g = given_g.detach().contiguous();
