@@ -70,15 +70,18 @@ def build_parser():
     p.add_argument("--warmup", type=int, default=10)
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--residual-blocks", type=int, default=0, help="residual blocks (norm, two products) behind every hidden layer")
-    p.add_argument("--optimizer", choices=("adam", "muon"), default="adam", help="muon: the blocks' matrices by orthogonalised updates, the rest by Adam")
+    p.add_argument("--optimizer", choices=("adam", "muon"), default="adam", help="muon: the residual blocks' matrices by orthogonalised updates, the rest by Adam")
     p.add_argument("--muon-lr", type=float, default=0.02)
-    p.add_argument("--eight-bit", choices=sorted(EIGHT), default=None, help="evaluate with the blocks in 8 bits as well")
+    p.add_argument("--eight-bit", choices=sorted(EIGHT), default=None, help="evaluate with the residual blocks in 8 bits as well")
     p.add_argument("--hip-graph", action="store_true", help="capture the training step into a HIP graph and replay it (pays off on small graphs)")
     return p
 
 
 def main(argv=None):
-    args = build_parser().parse_args(argv)
+    parser = build_parser()
+    args = parser.parse_args(argv)
+    if (args.optimizer == "muon" or args.eight_bit) and min(args.residual_blocks, args.num_layers) < 1:
+        parser.error("--optimizer muon and --eight-bit are for residual blocks: give --residual-blocks, and hidden layers for them to follow")
     dev = torch.device("cuda", args.gpu)
     torch.cuda.set_device(dev)
     data = datasets.load_node_dataset(args.dataset, dev, root=args.data_root, seed=args.seed, scale=args.scale, cache_dir=args.cache_dir)

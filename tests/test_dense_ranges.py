@@ -316,3 +316,12 @@ def test_transforms_that_would_drop_derivatives_are_refused():
             torch.func.grad(lambda v: call(v).sum())(x)
         with pytest.raises(RuntimeError):
             torch.func.vmap(call)(torch.stack([x, x]))
+
+
+@pytest.mark.parametrize("flags", [["--optimizer", "muon"], ["--eight-bit", "int8"], ["--eight-bit", "e4m3", "--residual-blocks", "0"],
+                                   ["--optimizer", "muon", "--residual-blocks", "2", "--num-layers", "0"]])
+def test_flags_for_blocks_that_are_not_there(flags, capsys):
+    from ae_mlsys_gnn_amd.train import train_gatconv
+    with pytest.raises(SystemExit):
+        train_gatconv.main(["--dataset", "cora"] + flags)
+    assert "residual" in capsys.readouterr().err
