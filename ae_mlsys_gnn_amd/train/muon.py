@@ -9,7 +9,9 @@ from ..operators.newton_schulz import COEFFICIENTS, orthogonalize
 
 class Muon(torch.optim.Optimizer):
     """For matrices [rows, columns]: b <- momentum b + g, then w <- (1 - lr weight_decay) w - lr max(1, rows / columns)^0.5 O, where O is g + momentum b (b without
-    `nesterov`) orthogonalised.  Matrices of the same shape and type go through the same launches.  Vectors and scalars belong to another optimizer."""
+    `nesterov`) orthogonalised.  Matrices of the same shape and type go through the same launches.  Vectors and scalars belong to another optimizer.
+    States are 32 bits.  bf16 and fp16 matrices have 32-bit weights among them, of which the parameter is the rounded form: updates and decay below its own step add
+    up there.  A parameter that something else has changed is taken as it is, element by element."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=coefficients))
@@ -17,6 +19,16 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.dim() != 2:
                     raise FgnnError("Muon: a parameter of shape %s is no matrix" % (tuple(p.shape),))
+                if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                    raise FgnnError("Muon: a parameter of %s; fp32, bf16 and fp16 are supported" % p.dtype)
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # torch has cast the states to the parameters' types
+        names = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(names, (p for group in self.param_groups for p in group["params"])):
+            for name, value in state_dict["state"].get(i, {}).items():
+                self.state[p][name] = value.detach().to(p.device, torch.float32, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -29,17 +41,27 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is not None:
                     alike.setdefault((tuple(p.shape), p.dtype, p.device), []).append(p)
-            for (shape, _, _), ps in alike.items():
-                grads = [p.grad for p in ps]
+            for (shape, dtype, _), ps in alike.items():
+                grads = [p.grad.float() for p in ps]
                 for p in ps:
-                    if "momentum" not in self.state[p]:
-                        self.state[p]["momentum"] = torch.zeros_like(p)
+                    state = self.state[p]
+                    if "momentum" not in state:
+                        state["momentum"] = torch.zeros_like(p, dtype=torch.float32)
+                    if dtype is not torch.float32 and "weights" not in state:
+                        state["weights"] = p.detach().float()
                 kept = [self.state[p]["momentum"] for p in ps]
                 torch._foreach_mul_(kept, group["momentum"])
                 torch._foreach_add_(kept, grads)
                 updates = torch._foreach_add(grads, kept, alpha=group["momentum"]) if group["nesterov"] else kept
                 out = orthogonalize(torch.stack(updates), steps=group["steps"], coefficients=group["coefficients"])
+                ws = ps if dtype is torch.float32 else [self.state[p]["weights"] for p in ps]
+                if ws is not ps:
+                    for w, p in zip(ws, ps):
+                        w.copy_(torch.where(w.to(dtype) == p, w, p.float()))
                 if group["weight_decay"]:
-                    torch._foreach_mul_(ps, 1.0 - group["lr"] * group["weight_decay"])
-                torch._foreach_add_(ps, list(out.unbind(0)), alpha=-group["lr"] * max(1.0, shape[0] / shape[1]) ** 0.5)
+                    torch._foreach_mul_(ws, 1.0 - group["lr"] * group["weight_decay"])
+                torch._foreach_add_(ws, list(out.unbind(0)), alpha=-group["lr"] * max(1.0, shape[0] / shape[1]) ** 0.5)
+                if ws is not ps:
+                    for w, p in zip(ws, ps):
+                        p.copy_(w)
         return loss

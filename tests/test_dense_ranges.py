@@ -9,6 +9,7 @@ from torch.utils.flop_counter import FlopCounterMode
 
 from ae_mlsys_gnn_amd import _lib
 from ae_mlsys_gnn_amd.operators import linear_act, linear_q8, orthogonalize, quantize_rows, rms_norm, rms_norm_q8
+from ae_mlsys_gnn_amd.train.muon import Muon
 
 from .test_linear_gpu import act, allowance, within
 
@@ -325,3 +326,65 @@ def test_flags_for_blocks_that_are_not_there(flags, capsys):
     with pytest.raises(SystemExit):
         train_gatconv.main(["--dataset", "cora"] + flags)
     assert "residual" in capsys.readouterr().err
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nesterov", [False, True])
+def test_muon_of_16_bit_matrices(dtype, nesterov):
+    g = torch.Generator().manual_seed(8)
+    shapes = [(40, 64), (64, 40), (40, 64), (100, 7)]
+    ws = [torch.nn.Parameter(torch.randn(s, generator=g).to(dtype).cuda()) for s in shapes]
+    ref = [w.detach().double().cpu() for w in ws]
+    buf = [torch.zeros_like(w) for w in ref]
+    opt = Muon(ws, lr=0.1, momentum=0.9, nesterov=nesterov, weight_decay=0.01)
+    a, b, c = 3.4445, -4.7750, 2.0315
+    for step in range(6):
+        for i, w in enumerate(ws):
+            grad = torch.randn(shapes[i], generator=g).to(dtype)
+            w.grad = grad.cuda()
+            buf[i] = 0.9 * buf[i] + grad.double()
+            u = grad.double() + 0.9 * buf[i] if nesterov else buf[i]
+            u = u / (u.norm() + 1e-7)
+            for _ in range(5):
+                gram = u @ u.t()
+                u = a * u + (b * gram + c * gram @ gram) @ u
+            ref[i] = ref[i] * (1 - 0.1 * 0.01) - 0.1 * max(1.0, shapes[i][0] / shapes[i][1]) ** 0.5 * u
+        opt.step()
+        if step == 2:
+            # another optimizer goes on from what this one wrote down
+            saved = opt.state_dict()
+            opt = Muon(ws, lr=0.5)
+            opt.load_state_dict(saved)
+    unit = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    for w, r in zip(ws, ref):
+        assert all(v.dtype is torch.float32 for v in opt.state[w].values())
+        # the 32-bit weights as those of fp32 matrices, and the parameter one rounding from them
+        assert float((opt.state[w]["weights"].double().cpu() - r).norm()) <= 1e-4 * float(r.norm())
+        assert ((w.detach().double() - opt.state[w]["weights"].double()).abs() <= unit * opt.state[w]["weights"].double().abs() + 2.0 ** -24).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_decay_of_16_bit_matrices_adds_up(dtype):
+    w = torch.nn.Parameter(torch.randn(16, 24, generator=torch.Generator().manual_seed(9)).to(dtype).cuda())
+    first = w.detach().double()
+    w.grad = torch.zeros_like(w)
+    opt = Muon([w], lr=0.02, weight_decay=0.01)             # 2e-4 a step, below half a step of either type
+    for _ in range(400):
+        opt.step()
+    unit = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    want = first * (1 - 2e-4) ** 400
+    assert ((w.detach().double() - want).abs() <= (unit + 400 * 2.0 ** -23) * want.abs()).all()
+    # weights that something else has written are what the next step starts from
+    with torch.no_grad():
+        w[3:7].fill_(2.0)
+    opt.step()
+    want[3:7] = 2.0
+    want = want * (1 - 2e-4)
+    assert ((w.detach().double() - want).abs() <= (unit + 401 * 2.0 ** -23) * want.abs()).all()
+
+
+def test_muon_refuses_other_types():
+    with pytest.raises(_lib.FgnnError, match="float64"):
+        Muon([torch.nn.Parameter(torch.randn(5, 4, dtype=torch.float64))])
