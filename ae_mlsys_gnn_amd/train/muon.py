@@ -15,20 +15,25 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=coefficients))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() != 2:
-                    raise FgnnError("Muon: a parameter of shape %s is no matrix" % (tuple(p.shape),))
-                if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-                    raise FgnnError("Muon: a parameter of %s; fp32, bf16 and fp16 are supported" % p.dtype)
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                del self.param_groups[-1]
+                raise FgnnError("Muon: a parameter of shape %s is no matrix" % (tuple(p.shape),))
+            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                del self.param_groups[-1]
+                raise FgnnError("Muon: a parameter of %s; fp32, bf16 and fp16 are supported" % p.dtype)
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
         # torch has cast the states to the parameters' types
         names = [i for group in state_dict["param_groups"] for i in group["params"]]
         for i, p in zip(names, (p for group in self.param_groups for p in group["params"])):
-            for name, value in state_dict["state"].get(i, {}).items():
-                self.state[p][name] = value.detach().to(p.device, torch.float32, copy=True)
+            saved = state_dict["state"].get(i, {})
+            for name in saved.keys() & {"momentum", "weights"}:
+                self.state[p][name] = saved[name].detach().to(p.device, torch.float32, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -39,7 +44,7 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             alike = {}
             for p in group["params"]:
-                if p.grad is not None:
+                if p.grad is not None and p.numel():
                     alike.setdefault((tuple(p.shape), p.dtype, p.device), []).append(p)
             for (shape, dtype, _), ps in alike.items():
                 grads = [p.grad.float() for p in ps]

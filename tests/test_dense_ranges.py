@@ -388,3 +388,16 @@ def test_decay_of_16_bit_matrices_adds_up(dtype):
 def test_muon_refuses_other_types():
     with pytest.raises(_lib.FgnnError, match="float64"):
         Muon([torch.nn.Parameter(torch.randn(5, 4, dtype=torch.float64))])
+
+
+def test_muon_refuses_what_is_no_matrix_in_later_groups_too():
+    opt = Muon([torch.nn.Parameter(torch.randn(5, 4))])
+    for bad in (torch.randn(5), torch.randn(2, 5, 4), torch.randn(5, 4, dtype=torch.float64)):
+        with pytest.raises(_lib.FgnnError):
+            opt.add_param_group({"params": [torch.nn.Parameter(bad)]})
+    assert len(opt.param_groups) == 1
+    # matrices without elements have nothing to learn
+    for shape in ((0, 4), (4, 0)):
+        w = torch.nn.Parameter(torch.empty(shape))
+        w.grad = torch.empty(shape)
+        Muon([w]).step()
