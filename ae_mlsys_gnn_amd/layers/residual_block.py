@@ -55,6 +55,15 @@ class QuantizedResidualBlock(nn.Module):
             self.register_buffer(name, q)
             self.register_buffer(name + "_scale", scale)
 
+    def _apply(self, fn, recurse=True):
+        # .half(), .to(dtype): the norm's weights and the bias follow the features, what is laid out in 8 bits and its scales stay as they are
+        laid_out = {name: getattr(self, name) for name in ("w1", "w1_scale", "w2", "w2_scale")}
+        super()._apply(fn, recurse)
+        for name, t in laid_out.items():
+            if getattr(self, name).dtype is not t.dtype:
+                setattr(self, name, t.to(getattr(self, name).device))
+        return self
+
     @torch.no_grad()
     def forward(self, x, residual=None):
         if residual is None:

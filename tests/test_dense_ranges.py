@@ -8,6 +8,7 @@ import torch
 from torch.utils.flop_counter import FlopCounterMode
 
 from ae_mlsys_gnn_amd import _lib
+from ae_mlsys_gnn_amd.layers import ResidualBlock
 from ae_mlsys_gnn_amd.operators import linear_act, linear_q8, orthogonalize, quantize_rows, rms_norm, rms_norm_q8
 from ae_mlsys_gnn_amd.train.muon import Muon
 
@@ -401,3 +402,23 @@ def test_muon_refuses_what_is_no_matrix_in_later_groups_too():
         w = torch.nn.Parameter(torch.empty(shape))
         w.grad = torch.empty(shape)
         Muon([w]).step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_eight_bit_blocks_follow_the_type_of_the_features(eight, dtype):
+    torch.manual_seed(10)
+    block = ResidualBlock(96, 200).cuda()
+    served = block.quantized(eight)
+    kept = {name: t.clone() for name, t in served.state_dict().items()}
+    served = torch.nn.Sequential(served).to(dtype)
+    for name, t in served[0].state_dict().items():
+        same = name in ("w1", "w2", "w1_scale", "w2_scale")
+        assert t.dtype is (kept[name].dtype if same else dtype) and t.is_cuda
+        assert not same or torch.equal(t.float(), kept[name].float())
+    x = torch.randn(40, 96).cuda().to(dtype)
+    got, ref = served(x), block(x.float())
+    assert got.dtype is dtype and float((got.float() - ref).norm()) <= 0.1 * float(ref.norm())
+    # to other memory and back
+    assert served.cpu()[0].w1.device.type == "cpu" and torch.equal(served.cuda()(x), got)
