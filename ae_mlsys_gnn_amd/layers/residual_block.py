@@ -43,7 +43,7 @@ class ResidualBlock(nn.Module):
 
 class QuantizedResidualBlock(nn.Module):
     """A ResidualBlock whose two products take operands in 8 bits (torch.int8 or torch.float8_e4m3fn) with a scale a row.  The features between blocks, the
-    bias and what is added stay in the type of the features."""
+    bias and what is added are in the type of the features, and follow the module's conversions to another."""
 
     def __init__(self, block, dtype=torch.int8):
         super().__init__()

@@ -17,8 +17,11 @@ def _activation(who, activation):
 
 def linear_act(x, weight, bias=None, residual=None, activation=None, negative_slope=0.2):
     """act(x weight^T + bias) + residual for x [..., k], weight [n, k]: one pass over the result.  activation: None, "relu", "gelu" (by the error
-    function), "silu" or "leaky_relu" (with negative_slope).  fp32, bf16 or fp16 (bias of that type or fp32), sums in 32 bits; fp32 products are formed from
-    parts of 8 significant bits to fp32's accuracy.  Gradients of x, weight, bias and residual; those of second order are not recorded."""
+    function), "silu" or "leaky_relu" (with negative_slope).  fp32, bf16 or fp16, the same for x, weight and residual under autocast too (bias of that type or fp32),
+    sums in 32 bits; fp32 products are formed from parts of 8 significant bits, to fp32's accuracy for operands from 2^-110 on.
+    Gradients of x, weight, bias and residual; those of second order are not recorded, and calls are refused in forward mode and by jit.trace, make_fx and export.
+    The backward pass reads the activation's argument as rounded to the rows' type (where that is 0, relu's slope is 0) and rounds the argument's gradient to it before
+    the two products; the bias gradient is summed before that.  For 16-bit rows gradients are off by about 1.4 roundings of the exact result."""
     return dense().linear_act(x, weight, bias, residual, _activation("linear_act", activation), negative_slope)
 
 

@@ -336,10 +336,10 @@ int fgnn_rms_norm_backward(int64_t rows, int cols, int type, const void *gy, con
 /* Linear maps with the epilogue in the product: y [rows, n] = act(x [rows, k] weight [n, k]^T + bias) + residual, all of one floating type (bias of
  * that type or FGNN_F32).  act: 0 none, 1 relu, 2 gelu (by the error function), 3 silu, 4 leaky relu with `slope`.  bias, residual, z NULL: none; z
  * receives the activation's argument for the backward pass.  y, z contiguous.  fp32 products are summed from parts of 8 significant bits, to about
- * 2^-23 of the sum of magnitudes.  Results of up to 2^31 - 4096 columns.
+ * 2^-23 of the sum of magnitudes (operands below 2^-110 count to 2^-133 each).  Results of up to 2^31 - 4096 columns.
  * _q8: operands in 8 bits (eight: FGNN_I8, k <= 131071, or FGNN_E4M3) with scale [rows] and weight_scale [n]; bias, residual and y are of type `type`.
- * _slope: dz = gy act'(z) (NULL: not wanted; rows of ldz = n, or of the next whole 16 bytes with zeros behind n) and dbias = its column sums (NULL: not
- * wanted), summed before dz is rounded.
+ * _slope: dz = gy act'(z), of z as it was rounded to the rows' type (NULL: not wanted; rows of ldz = n, or of the next whole 16 bytes with zeros behind
+ * n) and dbias = its column sums (NULL: not wanted), summed before dz is rounded.
  * _dx: dx [rows, k] = dz weight;  _dw: dw [n, k] = dz^T x; padded: zeros follow the rows of dz up to whole 16 bytes.  All are deterministic.
  * Workspaces: fgnn_linear and _q8 fgnn_linear_workspace_bytes (kind: type or eight), _dx and _dw fgnn_linear_backward_workspace_bytes; loose: nonzero where rows
  * of an operand may not start at 16 bytes each and hold whole 16 bytes (rows of dz, where it is padded, hold them), or may lie 2^23 bytes apart or more

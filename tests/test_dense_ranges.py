@@ -422,3 +422,17 @@ def test_eight_bit_blocks_follow_the_type_of_the_features(eight, dtype):
     assert got.dtype is dtype and float((got.float() - ref).norm()) <= 0.1 * float(ref.norm())
     # to other memory and back
     assert served.cpu()[0].w1.device.type == "cpu" and torch.equal(served.cuda()(x), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(5, 70, 33), (300, 128, 256), (300, 129, 257)])
+def test_small_fp32_operands(rows, k, n):
+    # the parts of an operand from 2^-110 on lie in the range that holds all of their bits; below, the last part's step of 2^-133 is what each may be off by
+    g = torch.Generator().manual_seed(11)
+    w = torch.randn(n, k, generator=g)
+    for exponent, step in ((-109, 0.0), (-120, 2.0 ** -133), (-126, 2.0 ** -133)):
+        x = torch.randn(rows, k, generator=g).sign() * (1 + torch.rand(rows, k, generator=g)) * 2.0 ** exponent
+        for a, b in ((x, w), (w, x)):
+            ref, terms = a.double() @ b.double().t(), a.double().abs() @ b.double().abs().t()
+            off = step * (w.double().abs().sum(-1) if b is w else w.double().abs().sum(-1)[:, None])
+            within(linear_act(a.cuda(), b.cuda()), ref, allowance(torch.float32, ref, terms, off), "2^%d" % exponent)
