@@ -88,6 +88,15 @@ _SIGNATURES = {
     "fgnn_linear_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int]),
     "fgnn_linear_dx": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_linear_dw": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fgnn_group_norm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int, c_int]),
+    "fgnn_group_norm": (c_int, [c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_float, c_int, c_float]
+                        + [c_void_p] * 4 + [c_size_t, c_void_p]),
+    "fgnn_group_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int, c_int]),
+    "fgnn_group_norm_backward": (c_int, [c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_float]
+                                 + [c_void_p] * 6 + [c_size_t, c_void_p]),
+    "fgnn_embedding": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_float, c_void_p, c_void_p]),
+    "fgnn_embedding_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "fgnn_embedding_backward": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_int64, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_orthogonalize_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "fgnn_orthogonalize": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_knn_graph": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),

@@ -353,6 +353,150 @@ Tensor linear_q8(const Tensor &q, const Tensor &scale, const Tensor &w, const Te
     return y;
 }
 
+// ------------------------------------------------------------------------------------------------ group norm
+// t as [samples, points, channels] with unit channel stride; copied only where no view of that kind exists.
+struct Points { Tensor t; int64_t batch, points, cols, ld, stride; };
+Points points_of(const Tensor &t)
+{
+    const int64_t b = t.size(0), cols = t.size(-1), n = c10::multiply_integers(t.sizes().slice(1, t.dim() - 2));
+    Tensor r = t.reshape({b, n, cols});
+    if ((cols > 1 && r.stride(2) != 1) || (n > 1 && r.stride(1) < cols)) r = r.contiguous();
+    return {r, b, n, cols, n > 1 ? r.stride(1) : cols, b > 1 ? r.stride(0) : 0};
+}
+struct GroupNormOperands { Points x; Tensor w, b; int type, wtype, btype, groups; };
+GroupNormOperands group_norm_operands(const Tensor &x, int64_t groups, const Tensor &w, const Tensor &b)
+{
+    usable("group_norm", x, w, b);
+    const int type = float_type(x);
+    if (type < 0) refuse("group_norm: features of ", x.scalar_type(), "; fp32, bf16 and fp16 are supported");
+    if (x.dim() < 2 || x.size(-1) == 0) refuse("group_norm: features ", x.sizes(), "; [samples, ..., channels] is wanted");
+    if (groups < 1 || groups > x.size(-1) || x.size(-1) % groups) refuse("group_norm: ", groups, " groups of ", x.size(-1), " channels");
+    GroupNormOperands o{{}, {}, {}, type, type, type, as_int(groups, "groups")};
+    const auto vector = [&](const Tensor &v, const char *what, Tensor &to, int &to_type) {
+        if (!v.defined()) return;
+        if (v.dim() != 1 || v.size(0) != x.size(-1) || (v.scalar_type() != x.scalar_type() && v.scalar_type() != at::kFloat) || v.device() != x.device())
+            refuse("group_norm: ", what, " ", v.sizes(), " of ", v.scalar_type(), " for features ", x.sizes(), " of ", x.scalar_type());
+        to = v.contiguous();
+        to_type = float_type(v);
+    };
+    vector(w, "weights", o.w, o.wtype);
+    vector(b, "bias", o.b, o.btype);
+    o.x = points_of(x);
+    return o;
+}
+struct GroupNormOut { Tensor y, mean, rstd; };
+GroupNormOut group_norm_forward(const Tensor &x, int64_t groups, const Tensor &w, const Tensor &b, double eps, int64_t act, double slope)
+{
+    const GroupNormOperands o = group_norm_operands(x, groups, w, b);
+    const c10::OptionalDeviceGuard guard(x.device());
+    const int cols = as_int(o.x.cols, "features");
+    GroupNormOut out{like(x, x.sizes()), like(x, {o.x.batch, groups}, at::kFloat), like(x, {o.x.batch, groups}, at::kFloat)};
+    const size_t bytes = fgnn_group_norm_workspace_bytes(o.x.batch, o.x.points, cols, o.groups, o.type);
+    const Tensor ws = scratch(x, bytes);
+    check(fgnn_group_norm(o.x.batch, o.x.points, cols, o.groups, o.type, address(o.x.t), o.x.ld, o.x.stride, address(o.w), o.wtype, address(o.b), o.btype, (float)eps, (int)act, (float)slope,
+                          address(out.y), (float *)address(out.mean), (float *)address(out.rstd), address(ws), bytes, stream_of(x)), "fgnn_group_norm");
+    return out;
+}
+
+// Kept for the backward pass: x, weights, bias, and two numbers a sample and group.
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, int64_t groups, double eps, int64_t act, double slope)
+    {
+        const Tensor w = given(weight), b = given(bias);
+        const GroupNormOut o = group_norm_forward(x, groups, w, b, eps, act, slope);
+        ctx->saved_data["need"] = (int64_t)(wanted(x) | wanted(w) << 1 | wanted(b) << 2);
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["slope"] = slope;
+        ctx->save_for_backward({x, w, b, o.mean, o.rstd});
+        return o.y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list up)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const int64_t need = ctx->saved_data["need"].toInt();
+        const Points x = points_of(saved[0]);
+        const Tensor w = saved[1].defined() ? saved[1].contiguous() : Tensor(), b = saved[2].defined() ? saved[2].contiguous() : Tensor(), gy = up[0].contiguous();
+        const int type = float_type(x.t), wtype = w.defined() ? float_type(w) : type, btype = b.defined() ? float_type(b) : type, cols = (int)x.cols,
+                  groups = (int)ctx->saved_data["groups"].toInt();
+        const c10::OptionalDeviceGuard guard(x.t.device());
+        Tensor dx, dw, db;
+        if (need & 1) dx = like(x.t, saved[0].sizes());
+        if (need & 2) dw = like(w, w.sizes());
+        if (need & 4) db = like(b, b.sizes());
+        const size_t bytes = fgnn_group_norm_backward_workspace_bytes(x.batch, x.points, cols, groups, type);
+        const Tensor ws = scratch(x.t, bytes);
+        check(fgnn_group_norm_backward(x.batch, x.points, cols, groups, type, address(gy), address(x.t), x.ld, x.stride, address(w), wtype, address(b), btype,
+                                       (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["slope"].toDouble(), (const float *)address(saved[3]), (const float *)address(saved[4]),
+                                       address(dx), address(dw), address(db), address(ws), bytes, stream_of(x.t)), "fgnn_group_norm_backward");
+        return final_gradients("group_norm", {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+Tensor group_norm(const Tensor &x, int64_t groups, const MaybeTensor &weight, const MaybeTensor &bias, double eps, int64_t act, double slope)
+{
+    py::gil_scoped_release off;
+    const Tensor w = given(weight), b = given(bias);
+    if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b))) return GroupNorm::apply(x, weight, bias, groups, eps, act, slope);
+    return group_norm_forward(x, groups, w, b, eps, act, slope).y;
+}
+
+// ------------------------------------------------------------------------------------------------ embeddings
+struct Lookup { Tensor tokens; Rows w; int type, wide; };
+Lookup lookup_operands(const Tensor &tokens, const Tensor &weight, const std::optional<int64_t> &padding)
+{
+    usable("embedding", tokens, weight);
+    const int type = float_type(weight);
+    if (type < 0 || weight.dim() != 2 || weight.size(1) == 0) refuse("embedding: a table ", weight.sizes(), " of ", weight.scalar_type(), "; rows of fp32, bf16 and fp16 are supported");
+    if ((tokens.scalar_type() != at::kInt && tokens.scalar_type() != at::kLong) || tokens.device() != weight.device())
+        refuse("embedding: tokens of ", tokens.scalar_type(), " on ", tokens.device(), "; int32 and int64 on the table's device are supported");
+    if (padding && (*padding < 0 || *padding >= weight.size(0))) refuse("embedding: padding ", *padding, " in a table of ", weight.size(0), " rows");
+    as_int(weight.size(0), "rows of a table; columns");
+    return {tokens.contiguous(), rows_of(weight), type, tokens.scalar_type() == at::kLong};
+}
+Tensor lookup_forward(const Tensor &tokens, const Tensor &weight, double scale, const std::optional<int64_t> &padding)
+{
+    const Lookup o = lookup_operands(tokens, weight, padding);
+    const c10::OptionalDeviceGuard guard(weight.device());
+    std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+    shape.push_back(o.w.cols);
+    const Tensor y = like(weight, shape);
+    check(fgnn_embedding(tokens.numel(), (int)o.w.rows, as_int(o.w.cols, "a table"), o.type, address(o.tokens), o.wide, address(o.w.t), o.w.ld, (float)scale, address(y), stream_of(weight)),
+          "fgnn_embedding");
+    return y;
+}
+
+// Kept for the backward pass: the tokens.
+struct Embedding : torch::autograd::Function<Embedding> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &weight, const Tensor &tokens, double scale, std::optional<int64_t> padding)
+    {
+        const Tensor y = lookup_forward(tokens, weight, scale, padding);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding ? *padding : (int64_t)-1;
+        ctx->saved_data["rows"] = weight.size(0);
+        ctx->save_for_backward({tokens});
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list up)
+    {
+        const Tensor tokens = ctx->get_saved_variables()[0].contiguous();
+        const Rows gy = rows_of(up[0]);
+        const int rows = (int)ctx->saved_data["rows"].toInt(), cols = (int)gy.cols, type = float_type(gy.t);
+        const c10::OptionalDeviceGuard guard(gy.t.device());
+        const Tensor dw = like(gy.t, {rows, cols});
+        const size_t bytes = fgnn_embedding_backward_workspace_bytes(gy.rows, rows, cols, type);
+        const Tensor ws = scratch(gy.t, bytes);
+        check(fgnn_embedding_backward(gy.rows, rows, cols, type, address(tokens), tokens.scalar_type() == at::kLong, ctx->saved_data["padding"].toInt(), address(gy.t), gy.ld,
+                                      (float)ctx->saved_data["scale"].toDouble(), address(dw), address(ws), bytes, stream_of(gy.t)), "fgnn_embedding_backward");
+        return final_gradients("embedding", {dw, Tensor(), Tensor(), Tensor()});
+    }
+};
+Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale, std::optional<int64_t> padding)
+{
+    py::gil_scoped_release off;
+    if (at::GradMode::is_enabled() && wanted(weight)) return Embedding::apply(weight, tokens, scale, padding);
+    return lookup_forward(tokens, weight, scale, padding);
+}
+
 // ------------------------------------------------------------------------------------------------ orthogonalised updates
 Tensor orthogonalize(const Tensor &given_g, const std::vector<float> &coefficients, double eps)
 {
@@ -388,4 +532,6 @@ PYBIND11_MODULE(_dense, m)
     m.def("linear_act", &linear_act);
     m.def("linear_q8", &linear_q8);
     m.def("orthogonalize", &orthogonalize);
+    m.def("group_norm", &group_norm);
+    m.def("embedding", &embedding);
 }

@@ -596,6 +596,31 @@ int    fgnn_coo2csr(int n_rows, int n_cols, int64_t E, const int32_t *dst, const
                     int32_t *row_ptr, int32_t *col_ind, int64_t *n_out, int32_t *edge_pos,
                     void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------- operators of conditioned blocks
+ * Group norm with an activation of x [batch, points, cols], channels last (sample stride sx, point stride ldx, in elements): per sample and group of cols / groups
+ * channels, u = (x - mean) rstd over points and channels, y = act(u weight + bias).  Types and act as above; weight and bias of the rows' type or FGNN_F32, NULL: ones,
+ * zeros.  y contiguous; mean, rstd [batch, groups] are for the backward pass.  _backward: gy, dx contiguous; dx, dweight, dbias (of the types of weight and bias; of the
+ * rows' where those are NULL) may each be NULL.  Deterministic. */
+size_t fgnn_group_norm_workspace_bytes(int64_t batch, int64_t points, int cols, int groups, int type);
+int fgnn_group_norm(int64_t batch, int64_t points, int cols, int groups, int type, const void *x, int64_t ldx, int64_t sx,
+                    const void *weight, int wtype, const void *bias, int btype, float eps, int act, float slope, void *y,
+                    float *mean, float *rstd, void *workspace, size_t workspace_bytes, void *stream);
+size_t fgnn_group_norm_backward_workspace_bytes(int64_t batch, int64_t points, int cols, int groups, int type);
+int fgnn_group_norm_backward(int64_t batch, int64_t points, int cols, int groups, int type, const void *gy, const void *x,
+                             int64_t ldx, int64_t sx, const void *weight, int wtype, const void *bias, int btype, int act,
+                             float slope, const float *mean, const float *rstd, void *dx, void *dweight, void *dbias,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* y [n, cols] = scale weight[tokens] (y contiguous, weight [vocabulary, cols] with row stride ldw; tokens int32, or int64 where wide is 1).  A token outside
+ * [0, vocabulary) reads nothing and gives a row of NaN.  _backward: dw [vocabulary, cols] (contiguous) = scale times the sums of gy's rows by token, zeros for
+ * tokens that are not met; `padding` (-1: none) and tokens outside the table give no gradient.  Deterministic. */
+int fgnn_embedding(int64_t n, int vocabulary, int cols, int type, const void *tokens, int wide, const void *weight, int64_t ldw,
+                   float scale, void *y, void *stream);
+size_t fgnn_embedding_backward_workspace_bytes(int64_t n, int vocabulary, int cols, int type);
+int fgnn_embedding_backward(int64_t n, int vocabulary, int cols, int type, const void *tokens, int wide, int64_t padding,
+                            const void *gy, int64_t ldg, float scale, void *dw, void *workspace, size_t workspace_bytes,
+                            void *stream);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }
