@@ -97,6 +97,10 @@ _SIGNATURES = {
     "fgnn_embedding": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_float, c_void_p, c_void_p]),
     "fgnn_embedding_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "fgnn_embedding_backward": (c_int, [c_int64, c_int, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_int64, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fgnn_attention_workspace_bytes": (c_size_t, [c_int] * 7 + [c_void_p] * 3),
+    "fgnn_attention": (c_int, [c_int] * 7 + [c_void_p] * 5 + [c_int, c_void_p, c_float] + [c_void_p] * 3 + [c_size_t, c_void_p]),
+    "fgnn_attention_backward_workspace_bytes": (c_size_t, [c_int] * 7 + [c_void_p] * 5),
+    "fgnn_attention_backward": (c_int, [c_int] * 7 + [c_void_p] * 7 + [c_int, c_void_p, c_float] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     "fgnn_orthogonalize_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "fgnn_orthogonalize": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fgnn_knn_graph": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),

@@ -1,0 +1,523 @@
+// Attention of queries to keys and values of another length, softmax over the keys that are seen:
+//   S = scale Q K^T,   P = exp(S - lse),   Y = P V,   lse = log sum exp S over the keys that are seen,
+// and its gradient,  dV = P^T G,   dP = G V^T,   dS = P (dP - delta),   delta = rowsum(G Y),   dQ = scale dS K,   dK = scale dS^T Q.
+// Nothing of the size of S is written: scores are formed tile by tile, and again in the backward pass.
+//
+// Every product is a matrix instruction of 32 x 32 sums whose second operand waits in registers. A wave owns 32 columns (queries in the forward pass and in that of dQ, keys
+// in that of dK and dV) and walks tiles of the other side, which the workgroup's waves share in LDS.  Its scores come out with a lane per column and 16 of 32 rows in
+// its registers (row 8 (i / 4) + 4 (lane / 32) + i % 4 in register i), so that a softmax is a matter of the lane and the one 32 lanes away, and the scores are,
+// rounded, the second operand of the next product as they lie: the order of a reduction is free as long as both operands have the same, and the first operand, the tile
+// transposed, is read from LDS in that order.
+//
+// 16-bit types: products of 16-bit values, P and dS rounded to the type (as the values they are multiplied with are), sums, statistics and results in 32 bits.  fp32: the
+// matrix instruction of fp32, everything in 32 bits.
+#pragma once
+#include "fgnn_gemm.h"
+
+typedef float at_f16 __attribute__((ext_vector_type(16)));
+
+struct AttentionP {
+    int batch, nq, nk, heads, kv_heads, share, dim;             // share: heads that use the same keys
+    int rows;                                                   // queries of one head of keys: nq share, row = position share + head
+    uint32_t share_mul; int share_shift;                        // row / share
+    const void *q, *k, *v, *g; int64_t qb, qn, qh, kb, kn, kh, vb, vn, vh, gb, gn, gh;      // strides of samples, positions and heads, in elements
+    const void *lengths; int wide; const uint8_t *mask;         // keys seen: the first lengths[b], and those with mask[b][key]; NULL: all
+    float scale, log2_scale;                                    // log2_scale = scale log2 e
+    void *y; float *lse, *delta;                                // y [batch][nq][heads][dim]; [batch][heads][nq], lse in powers of two; +inf of rows that see nothing
+    void *dq, *dk, *dv;                                         // contiguous, as y
+    int tiles, splits, per;                                     // tiles of 32 waves columns; parts of the other side, and tiles of each
+    float *part, *part_lse;                                     // sums of the parts
+};
+
+template <typename E> struct AtKind { static constexpr int V = fe_width<E>, SIZE = (int)sizeof(E); };
+// Rows of a tile that lies in LDS.
+template <typename E> constexpr int at_tile = sizeof(E) == 4 ? 32 : 64;
+
+// 16-byte chunk `ch` of row `row` in a tile of ROW bytes a row.  Chunks are exchanged so that both ways of reading meet different banks: eight rows at one
+// chunk, and four rows at two neighbouring chunks.
+template <int ROW>
+__device__ __forceinline__ int at_place(int row, int ch)
+{
+    const int f = ROW % 128 ? (row >> 1) & 3 : (row & 3) << 1 | ((row >> 2) & 1);
+    return row * ROW + ((ch ^ f) << 4);
+}
+
+template <typename E>
+__device__ __forceinline__ at_f16 at_multiply(gm_i4 a, gm_i4 b, at_f16 c)
+{
+    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__int_as_float(a[j]), __int_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    } else if constexpr (std::is_same_v<E, _Float16>) return __builtin_amdgcn_mfma_f32_32x32x16_f16(*(gm_h8 *)&a, *(gm_h8 *)&b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(gm_b8 *)&a, *(gm_b8 *)&b, c, 0, 0, 0);
+}
+
+// The scores of 32 rows of a tile (from row0 on) with the wave's columns.
+template <typename E, int DP>
+__device__ __forceinline__ at_f16 at_scores(const char *tile, int row0, const gm_i4 (&cols)[DP * (int)sizeof(E) / 32], int lane)
+{
+    constexpr int ROW = DP * (int)sizeof(E);
+    at_f16 s = {};
+#pragma unroll
+    for (int j = 0; j < ROW / 32; ++j) s = at_multiply<E>(*reinterpret_cast<const gm_i4 *>(tile + at_place<ROW>(row0 + (lane & 31), 2 * j + (lane >> 5))), cols[j], s);
+    return s;
+}
+
+// acc[t] (32 components from 32 t on, by the wave's columns) += (32 rows of a tile, from row0 on)^T w
+template <typename E, int DP>
+__device__ __forceinline__ void at_gather(const char *tile, int row0, const float (&w)[16], at_f16 (&acc)[DP / 32], int lane)
+{
+    constexpr int ROW = DP * (int)sizeof(E);
+    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int row = row0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t) {
+                const float a = *reinterpret_cast<const float *>(tile + at_place<ROW>(row, 8 * t + ((lane & 31) >> 2)) + (lane & 3) * 4);
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[i], acc[t], 0, 0, 0);
+            }
+        }
+    } else {
+        const int r = lane & 15;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            typedef E e8 __attribute__((ext_vector_type(8)));
+            e8 b;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = (E)w[8 * s + i];
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t) {
+                // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
+                typedef __attribute__((address_space(3))) gm_s4 *lds_p;
+                typedef short s8 __attribute__((ext_vector_type(8)));
+                const int row = row0 + 16 * s + 4 * (lane >> 5) + (r >> 2), d = 32 * t + 16 * ((lane >> 4) & 1) + 4 * (r & 3);
+                const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + at_place<ROW>(row, d >> 3) + (d & 4) * 2));
+                const gm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + at_place<ROW>(row + 8, d >> 3) + (d & 4) * 2));
+                const s8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[t] = at_multiply<E>(*(const gm_i4 *)&a, *(const gm_i4 *)&b, acc[t]);
+            }
+        }
+    }
+}
+
+// A tile on its way from memory to LDS.  Rows that are not wanted (bit not set) and components past the last are zeros: out of the buffer's range.
+template <typename E, int ROWS, int DP, int THREADS>
+struct AtLoader {
+    static constexpr int SIZE = (int)sizeof(E), CH = DP * SIZE / 16, COUNT = ROWS * CH / THREADS;
+    static_assert(ROWS * CH % THREADS == 0, "threads share a tile evenly");
+    gm_i4 w[COUNT];
+    __device__ __forceinline__ void fetch(const E *base, int64_t stride, uint64_t bits, int dim)
+    {
+        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, 0x80000000u, 0x00027000);
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) {
+            const int pos = c * THREADS + (int)threadIdx.x, row = pos / CH, ch = pos % CH;
+            const bool there = ((bits >> row) & 1) && ch * (16 / SIZE) < dim;
+            w[c] = __builtin_amdgcn_raw_buffer_load_b128(from, there ? (uint32_t)row * (uint32_t)(stride * SIZE) + ch * 16 : 0x80000000u, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void store(char *tile) const
+    {
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) {
+            const int pos = c * THREADS + (int)threadIdx.x;
+            *reinterpret_cast<gm_i4 *>(tile + at_place<DP * SIZE>(pos / CH, pos % CH)) = w[c];
+        }
+    }
+};
+
+// One row as the second operand of products: its chunks 2 j + (lane / 32).  Any alignment.
+template <typename E, int DP>
+__device__ __forceinline__ void at_row(gm_i4 (&cols)[DP * (int)sizeof(E) / 32], const E *row, bool there, int dim, int lane)
+{
+    constexpr int V = fe_width<E>;
+#pragma unroll
+    for (int j = 0; j < DP * (int)sizeof(E) / 32; ++j) {
+        const int at = (2 * j + (lane >> 5)) * V;
+        E v[V];
+        gm_load<E, V>(v, row + (there && at < dim ? at : 0), there ? dim - at : 0);
+#pragma unroll
+        for (int i = 0; i < V; ++i) ((E *)&cols[j])[i] = v[i];
+    }
+}
+
+// The value of the lane that holds the same column's other rows.
+__device__ __forceinline__ float at_other_max(float v)
+{
+    const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
+}
+__device__ __forceinline__ float at_other_sum(float v)
+{
+    const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(u[0]) + __uint_as_float(u[1]);
+}
+
+// fp16 has 2^-14 as its smallest number of all significant bits, where softmax weights of long rows and gradients lie below: weights are rounded times 2^15
+// (they are 1 at the most), gradients of scores times a power of two of the column's own that brings its largest so far to 2^14 .. 2^15.
+template <typename E> constexpr float at_lift = std::is_same_v<E, _Float16> ? 15.f : 0.f;      // as an exponent
+template <typename E, int STEPS>
+struct AtRange {
+    float f = std::is_same_v<E, _Float16> ? 0x1p96f : 1.f;
+    __device__ __forceinline__ void fit(float (&w)[16], at_f16 (&acc)[STEPS])
+    {
+        if constexpr (std::is_same_v<E, _Float16>) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(w[i]));
+            top = at_other_max(top);
+            const bool over = top * f > 32768.f;
+            if (__ballot(over)) {
+                const float now = over ? __builtin_ldexpf(1.f, min(96, 15 - __builtin_amdgcn_frexp_expf(top))) : f, r = now / f;
+                f = now;
+#pragma unroll
+                for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[t][i] *= r;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] *= f;
+        }
+    }
+};
+
+// Which keys of a tile are seen.  The mask's bytes are asked for a tile ahead.
+template <int TILE>
+struct AtSeen {
+    const uint8_t *mask; int64_t length; int lane;
+    bool next;
+    __device__ __forceinline__ void init(const AttentionP &p, int b, int lane_)
+    {
+        lane = lane_;
+        length = p.nk;
+        if (p.lengths) {
+            const int64_t n = p.wide ? ((const int64_t *)p.lengths)[b] : ((const int32_t *)p.lengths)[b];
+            length = n < 0 ? 0 : n < p.nk ? n : p.nk;
+        }
+        mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
+    }
+    __device__ __forceinline__ void ask(int64_t key0) { next = mask && lane < TILE && key0 + lane < length && mask[key0 + lane]; }
+    __device__ __forceinline__ uint64_t take(int64_t key0) const
+    {
+        if (mask) return __ballot(next);
+        const int64_t left = length - key0;
+        return left >= TILE ? (TILE == 64 ? ~0ull : (1ull << TILE) - 1) : left > 0 ? (1ull << left) - 1 : 0;
+    }
+};
+
+// A workgroup's place: neighbouring tiles of one head run on one XCD, whose L2 holds what they share.
+struct AtPlace { int tile, split, head, b; };
+__device__ __forceinline__ AtPlace at_block(const AttentionP &p)
+{
+    const int total = (int)gridDim.x, i = (int)blockIdx.x, xcd = i % FGNN_NUM_XCD, q = total / FGNN_NUM_XCD, r = total % FGNN_NUM_XCD;
+    int t = xcd * q + min(xcd, r) + i / FGNN_NUM_XCD;
+    AtPlace o;
+    o.tile = t % p.tiles;
+    t /= p.tiles;
+    o.split = t % p.splits;
+    t /= p.splits;
+    o.head = t % p.kv_heads;
+    o.b = t / p.kv_heads;
+    return o;
+}
+// Position and head of a row of queries.
+__device__ __forceinline__ void at_query(const AttentionP &p, int row, int &pos, int &sub)
+{
+    pos = (int)((__umulhi((uint32_t)row, p.share_mul) + (uint32_t)row) >> p.share_shift);
+    sub = row - pos * p.share;
+}
+// 32 components a step of a wave's sums, times `f`, to a row of `dim`.
+template <typename E, int DP, typename F>
+__device__ __forceinline__ void at_store(const at_f16 (&acc)[DP / 32], E *row, int dim, int lane, F f)
+{
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 32 * t + 8 * i + 4 * (lane >> 5);
+            const float v[4] = {f(acc[t][4 * i]), f(acc[t][4 * i + 1]), f(acc[t][4 * i + 2]), f(acc[t][4 * i + 3])};
+            if (d < dim) gm_store<E, 4>(v, row + d, dim - d);
+        }
+}
+
+constexpr int at_lds(int dim, int size, int rows) { return 2 * rows * dim * size; }
+
+// Y and lse.  With `splits` parts of the keys, normalised sums and lse of each to `part`.
+template <typename E, int DP, int WAVES, int TILE>
+__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_kernel(AttentionP p)
+{
+    constexpr int ROW = DP * (int)sizeof(E);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *lk = lds, *lv = lds + TILE * ROW;
+    const AtPlace o = at_block(p);
+    const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
+    int pos, sub;
+    at_query(p, min(row, p.rows - 1), pos, sub);
+    const int head = o.head * p.share + sub;
+    AtSeen<TILE> seen;
+    seen.init(p, o.b, lane);
+    const E *k = (const E *)p.k + o.b * p.kb + o.head * p.kh, *v = (const E *)p.v + o.b * p.vb + o.head * p.vh;
+    gm_i4 q[ROW / 32];
+    at_row<E, DP>(q, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, row < p.rows, p.dim, lane);
+    const int64_t first = (int64_t)o.split * p.per * TILE, last = min(seen.length, first + (int64_t)p.per * TILE);
+
+    at_f16 acc[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) acc[t] = at_f16{};
+    float most = -__builtin_inff(), sum = 0.f;
+    AtLoader<E, TILE, DP, 64 * WAVES> fk, fv;
+    seen.ask(first);
+    uint64_t bits = seen.take(first), coming = 0;
+    if (first < last) {
+        fk.fetch(k + first * p.kn, p.kn, bits, p.dim);
+        fv.fetch(v + first * p.vn, p.vn, bits, p.dim);
+        seen.ask(first + TILE);
+    }
+#pragma unroll 1
+    for (int64_t key = first; key < last; key += TILE, bits = coming) {
+        __syncthreads();                    // the tile before has been read
+        fk.store(lk);
+        fv.store(lv);
+        __syncthreads();
+        if (key + TILE < last) {
+            coming = seen.take(key + TILE);
+            fk.fetch(k + (key + TILE) * p.kn, p.kn, coming, p.dim);
+            fv.fetch(v + (key + TILE) * p.vn, p.vn, coming, p.dim);
+            seen.ask(key + 2 * TILE);
+        }
+        if (bits == 0) continue;
+        at_f16 s[TILE / 32];
+#pragma unroll
+        for (int t = 0; t < TILE / 32; ++t) s[t] = at_scores<E, DP>(lk, 32 * t, q, lane);
+        if (bits != (TILE == 64 ? ~0ull : (1ull << TILE) - 1)) {
+#pragma unroll
+            for (int t = 0; t < TILE / 32; ++t) {
+                const uint32_t own = (uint32_t)(bits >> (32 * t)) >> (4 * (lane >> 5));
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = (own >> (8 * (i / 4) + i % 4)) & 1 ? s[t][i] : -__builtin_inff();
+            }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int t = 0; t < TILE / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+        top = at_other_max(top) * p.log2_scale;
+        if (__ballot(top > most)) {
+            const float now = fmaxf(top, most), f = most > -__builtin_inff() ? __builtin_amdgcn_exp2f(most - now) : 0.f;
+            most = now;
+            sum *= f;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][i] *= f;
+        }
+        const float base = (most > -__builtin_inff() ? most : 0.f) - at_lift<E>;
+#pragma unroll
+        for (int t = 0; t < TILE / 32; ++t) {
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], p.log2_scale, -base));
+                sum += w[i];
+            }
+            at_gather<E, DP>(lv, 32 * t, w, acc, lane);
+        }
+    }
+    sum = at_other_sum(sum);
+    const bool none = sum == 0.f;
+    const float inv = none ? 0.f : 1.f / sum;
+    if (row >= p.rows) return;
+    const auto norm = [&](float x) { return none ? 0.f : x * inv; };
+    if (p.splits > 1) {
+        const int64_t at = (((int64_t)o.b * p.kv_heads + o.head) * p.splits + o.split) * p.rows + row;
+        at_store<float, DP>(acc, p.part + at * p.dim, p.dim, lane, norm);
+        if (lane < 32) p.part_lse[at] = none ? -__builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
+        return;
+    }
+    at_store<E, DP>(acc, (E *)p.y + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, p.dim, lane, norm);
+    if (p.lse && lane < 32) p.lse[((int64_t)o.b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
+}
+
+// dQ: as the forward pass, with P from lse.  With parts of the keys, their sums to `part`.
+template <typename E, int DP, int WAVES, int TILE>
+__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_dq_kernel(AttentionP p)
+{
+    constexpr int ROW = DP * (int)sizeof(E);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *lk = lds, *lv = lds + TILE * ROW;
+    const AtPlace o = at_block(p);
+    const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
+    int pos, sub;
+    at_query(p, min(row, p.rows - 1), pos, sub);
+    const int head = o.head * p.share + sub;
+    AtSeen<TILE> seen;
+    seen.init(p, o.b, lane);
+    const E *k = (const E *)p.k + o.b * p.kb + o.head * p.kh, *v = (const E *)p.v + o.b * p.vb + o.head * p.vh;
+    gm_i4 q[ROW / 32], g[ROW / 32];
+    at_row<E, DP>(q, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, row < p.rows, p.dim, lane);
+    at_row<E, DP>(g, (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, row < p.rows, p.dim, lane);
+    const int64_t stat = ((int64_t)o.b * p.heads + head) * p.nq + pos;
+    const float lse = p.lse[stat] - at_lift<E>, delta = p.delta[stat];
+    AtRange<E, DP / 32> range;
+    const int64_t first = (int64_t)o.split * p.per * TILE, last = min(seen.length, first + (int64_t)p.per * TILE);
+
+    at_f16 acc[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) acc[t] = at_f16{};
+    AtLoader<E, TILE, DP, 64 * WAVES> fk, fv;
+    seen.ask(first);
+    uint64_t bits = seen.take(first), coming = 0;
+    if (first < last) {
+        fk.fetch(k + first * p.kn, p.kn, bits, p.dim);
+        fv.fetch(v + first * p.vn, p.vn, bits, p.dim);
+        seen.ask(first + TILE);
+    }
+#pragma unroll 1
+    for (int64_t key = first; key < last; key += TILE, bits = coming) {
+        __syncthreads();
+        fk.store(lk);
+        fv.store(lv);
+        __syncthreads();
+        if (key + TILE < last) {
+            coming = seen.take(key + TILE);
+            fk.fetch(k + (key + TILE) * p.kn, p.kn, coming, p.dim);
+            fv.fetch(v + (key + TILE) * p.vn, p.vn, coming, p.dim);
+            seen.ask(key + 2 * TILE);
+        }
+#pragma unroll
+        for (int t = 0; t < TILE / 32; ++t) {
+            const uint32_t part = (uint32_t)(bits >> (32 * t));
+            if (part == 0) continue;
+            const at_f16 s = at_scores<E, DP>(lk, 32 * t, q, lane), dp = at_scores<E, DP>(lv, 32 * t, g, lane);
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.log2_scale, -lse)) * (dp[i] - delta);
+            if (part != ~0u) {
+                const uint32_t own = part >> (4 * (lane >> 5));
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = (own >> (8 * (i / 4) + i % 4)) & 1 ? w[i] : 0.f;
+            }
+            range.fit(w, acc);
+            at_gather<E, DP>(lk, 32 * t, w, acc, lane);
+        }
+    }
+    if (row >= p.rows) return;
+    const float f = p.scale / range.f * __builtin_amdgcn_exp2f(-at_lift<E>);
+    const auto scaled = [&](float x) { return x * f; };
+    if (p.splits > 1) {
+        const int64_t at = (((int64_t)o.b * p.kv_heads + o.head) * p.splits + o.split) * p.rows + row;
+        at_store<float, DP>(acc, p.part + at * p.dim, p.dim, lane, scaled);
+    } else at_store<E, DP>(acc, (E *)p.dq + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, p.dim, lane, scaled);
+}
+
+// dK and dV: a wave owns 32 keys and walks the queries of every head that uses them, tile by tile.  PARTS: the components are taken in that many passes
+// over the scores (of wide fp32 heads one pass's sums and operands do not fit the registers).
+template <typename E, int DP, int WAVES, int TILE, int PARTS>
+__global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP p)
+{
+    constexpr int ROW = DP * (int)sizeof(E), STEPS = DP / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *lq = lds, *lg = lds + TILE * ROW;
+    float *stats = (float *)(lds + 2 * TILE * ROW);             // lse, delta of the tile's rows
+    const AtPlace o = at_block(p);
+    const int lane = fg_lane(), key = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
+    AtSeen<64> seen;
+    seen.init(p, o.b, lane);
+    const bool there = key < seen.length && (!p.mask || seen.mask[min(key, p.nk - 1)]), any = __ballot(there) != 0;
+    gm_i4 k[ROW / 32], v[ROW / 32];
+    const int64_t at = min(key, p.nk - 1);
+    at_row<E, DP>(k, (const E *)p.k + o.b * p.kb + at * p.kn + o.head * p.kh, there, p.dim, lane);
+    at_row<E, DP>(v, (const E *)p.v + o.b * p.vb + at * p.vn + o.head * p.vh, there, p.dim, lane);
+    // tiles of every head's positions, one head after the other
+    const int per_head = (p.nq + TILE - 1) / TILE, first = o.split * p.per, last = min(per_head * p.share, first + p.per);
+
+    at_f16 dk[STEPS], dv[STEPS];
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) dk[t] = dv[t] = at_f16{};
+    AtRange<E, STEPS> range;
+    AtLoader<E, TILE, DP, 64 * WAVES> fq, fg;
+    float stat = 0.f;
+    auto fetch = [&](int i) {
+        const int sub = i / per_head, pos = (i - sub * per_head) * TILE, head = o.head * p.share + sub, left = p.nq - pos;
+        const uint64_t bits = left >= TILE ? (TILE == 64 ? ~0ull : (1ull << TILE) - 1) : (1ull << left) - 1;
+        fq.fetch((const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, p.qn, bits, p.dim);
+        fg.fetch((const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, p.gn, bits, p.dim);
+        // rows past the last weigh nothing
+        const int r = (int)threadIdx.x % TILE, which = (int)threadIdx.x / TILE;
+        if (which < 2) stat = r < left ? (which ? p.delta : p.lse)[((int64_t)o.b * p.heads + head) * p.nq + pos + r] - (which ? 0.f : at_lift<E>) : which ? 0.f : __builtin_inff();
+    };
+    static_assert(64 * WAVES >= 2 * TILE, "a thread for every row's lse and delta");
+    if (first < last) fetch(first);
+#pragma unroll 1
+    for (int i = first; i < last; ++i) {
+        __syncthreads();
+        fq.store(lq);
+        fg.store(lg);
+        if (threadIdx.x < 2 * TILE) stats[threadIdx.x] = stat;
+        __syncthreads();
+        if (i + 1 < last) fetch(i + 1);
+        if (!any) continue;
+#pragma unroll
+        for (int t = 0; t < TILE / 32; ++t) {
+            const at_f16 s = at_scores<E, DP>(lq, 32 * t, k, lane), dp = at_scores<E, DP>(lg, 32 * t, v, lane);
+            float w[16], ds[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const gm_f4 lse = *reinterpret_cast<const gm_f4 *>(stats + 32 * t + 8 * j + 4 * (lane >> 5)),
+                            delta = *reinterpret_cast<const gm_f4 *>(stats + TILE + 32 * t + 8 * j + 4 * (lane >> 5));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    w[4 * j + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + c], p.log2_scale, -lse[c]));
+                    ds[4 * j + c] = w[4 * j + c] * (dp[4 * j + c] - delta[c]);
+                }
+            }
+            at_gather<E, DP>(lg, 32 * t, w, dv, lane);
+            range.fit(ds, dk);
+            at_gather<E, DP>(lq, 32 * t, ds, dk, lane);
+        }
+    }
+    if (key >= p.nk) return;
+    // keys that are not seen were zeros in every product: what a score of 0 made of them is dropped
+    const float down = __builtin_amdgcn_exp2f(-at_lift<E>), f = p.scale / range.f * down;
+    const auto sk = [&](float x) { return there ? x * f : 0.f; };
+    const auto sv = [&](float x) { return there ? x * down : 0.f; };
+    if (p.splits > 1) {
+        const int64_t n = (int64_t)p.batch * p.nk * p.kv_heads * p.dim, to = o.split * 2 * n + (((int64_t)o.b * p.nk + key) * p.kv_heads + o.head) * p.dim;
+        at_store<float, DP>(dk, p.part + to, p.dim, lane, sk);
+        at_store<float, DP>(dv, p.part + to + n, p.dim, lane, sv);
+    } else {
+        const int64_t to = (((int64_t)o.b * p.nk + key) * p.kv_heads + o.head) * p.dim;
+        at_store<E, DP>(dk, (E *)p.dk + to, p.dim, lane, sk);
+        at_store<E, DP>(dv, (E *)p.dv + to, p.dim, lane, sv);
+    }
+}
+
+// The kernels of a type, by what they are for: one file each (fgnn_attention_*.hip).
+enum { AT_FORWARD, AT_DQ, AT_DKV };
+struct AtShape { int waves, tile, dim; };                       // waves a workgroup, rows of a tile in LDS, padded components
+template <typename E> void at_launch(int what, const AtShape &shape, const AttentionP &p, unsigned grid, hipStream_t st);
+
+template <typename E, int DP>
+static void at_launch_dim(int what, const AtShape &s, const AttentionP &p, unsigned grid, hipStream_t st)
+{
+    constexpr int T = at_tile<E>;
+    const size_t lds = at_lds(DP, (int)sizeof(E), s.tile);
+    if (what == AT_DKV) hipLaunchKernelGGL((attention_dkv_kernel<E, DP, 4, T, 1>), dim3(grid), dim3(256), lds + 2 * T * sizeof(float), st, p);
+    else if (what == AT_DQ) {
+        if (s.waves == 4) hipLaunchKernelGGL((attention_dq_kernel<E, DP, 4, T>), dim3(grid), dim3(256), lds, st, p);
+        else hipLaunchKernelGGL((attention_dq_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), lds, st, p);
+    } else {
+        if (s.waves == 4) hipLaunchKernelGGL((attention_kernel<E, DP, 4, T>), dim3(grid), dim3(256), lds, st, p);
+        else hipLaunchKernelGGL((attention_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), lds, st, p);
+    }
+}
+template <typename E>
+void at_launch(int what, const AtShape &s, const AttentionP &p, unsigned grid, hipStream_t st)
+{
+    if (s.dim == 64) at_launch_dim<E, 64>(what, s, p, grid, st);
+    else if (s.dim == 128) at_launch_dim<E, 128>(what, s, p, grid, st);
+    else at_launch_dim<E, 256>(what, s, p, grid, st);
+}

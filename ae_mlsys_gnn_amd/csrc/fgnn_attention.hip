@@ -1,0 +1,301 @@
+// Attention: the C entries, the choice of tiles and parts, and the small kernels around those of fgnn_attention.h.
+#include <algorithm>
+#include "fgnn_attention.h"
+
+#define AT_TPB 256
+extern template void at_launch<float>(int, const AtShape &, const AttentionP &, unsigned, hipStream_t);
+extern template void at_launch<__bf16>(int, const AtShape &, const AttentionP &, unsigned, hipStream_t);
+extern template void at_launch<_Float16>(int, const AtShape &, const AttentionP &, unsigned, hipStream_t);
+
+// delta = rowsum(G Y): `lanes` threads a row.
+template <typename E>
+__global__ __launch_bounds__(AT_TPB) void attention_delta_kernel(AttentionP p, int lanes)
+{
+    constexpr int V = fe_width<E>;
+    const int lane = (int)threadIdx.x % lanes;
+    const int64_t rows = (int64_t)p.batch * p.nq * p.heads, step = (int64_t)gridDim.x * (AT_TPB / lanes);
+    for (int64_t first = (int64_t)blockIdx.x * (AT_TPB / lanes); first < rows; first += step) {
+        const int64_t row = first + threadIdx.x / lanes;
+        float sum = 0.f;
+        const int head = (int)(row % p.heads);
+        const int64_t pos = row / p.heads % p.nq, b = row / p.heads / p.nq;
+        if (row < rows) {
+            const int left = p.dim - lane * V;
+            if (left > 0) {
+                float y[V], g[V];
+                gm_load<E, V>(y, (const E *)p.y + row * p.dim + lane * V, left);
+                gm_load<E, V>(g, (const E *)p.g + b * p.gb + pos * p.gn + head * p.gh + lane * V, left);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum = fmaf(y[i], g[i], sum);
+            }
+        }
+        for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (row < rows && lane == 0) p.delta[(b * p.heads + head) * p.nq + pos] = sum;
+    }
+}
+
+// Parts of the keys joined: Y = sum 2^(lse_s - lse) Y_s over the parts, in their order.  Four components a thread.
+template <typename E>
+__global__ __launch_bounds__(AT_TPB) void attention_join_kernel(AttentionP p)
+{
+    const int quads = (p.dim + 3) / 4;
+    const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows, total = rows * quads;
+    for (int64_t i = (int64_t)blockIdx.x * AT_TPB + threadIdx.x; i < total; i += (int64_t)gridDim.x * AT_TPB) {
+        const int64_t r = i / quads, group = r / p.rows;
+        const int d = (int)(i - r * quads) * 4, row = (int)(r - group * p.rows), pos = row / p.share, head = (int)(group % p.kv_heads) * p.share + row % p.share;
+        const int64_t at = group * p.splits * p.rows + row, b = group / p.kv_heads;
+        float most = -__builtin_inff();
+        for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.part_lse[at + (int64_t)s * p.rows]);
+        float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) {
+            const float lse = p.part_lse[at + (int64_t)s * p.rows];
+            if (lse == -__builtin_inff()) continue;             // a part that sees nothing
+            const float w = __builtin_amdgcn_exp2f(lse - most);
+            float u[4];
+            gm_load<float, 4>(u, p.part + (at + (int64_t)s * p.rows) * p.dim + d, p.dim - d);
+            sum += w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = fmaf(w, u[j], v[j]);
+        }
+        const bool none = sum == 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = none ? 0.f : v[j] / sum;
+        gm_store<E, 4>(v, (E *)p.y + ((b * p.nq + pos) * p.heads + head) * p.dim + d, p.dim - d);
+        if (p.lse && d == 0) p.lse[(b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum);
+    }
+}
+
+// Sums of parts [splits][n], in their order, to `out`; dQ's come by head of keys and row.
+template <typename E, bool DQ>
+__global__ __launch_bounds__(AT_TPB) void attention_sum_kernel(AttentionP p)
+{
+    const int quads = (p.dim + 3) / 4;
+    const int64_t rows = DQ ? (int64_t)p.batch * p.kv_heads * p.rows : 2 * (int64_t)p.batch * p.nk * p.kv_heads, total = rows * quads;
+    for (int64_t i = (int64_t)blockIdx.x * AT_TPB + threadIdx.x; i < total; i += (int64_t)gridDim.x * AT_TPB) {
+        const int64_t r = i / quads;
+        const int d = (int)(i - r * quads) * 4;
+        int64_t from, step;
+        E *to;
+        if constexpr (DQ) {
+            const int64_t group = r / p.rows, b = group / p.kv_heads;
+            const int row = (int)(r - group * p.rows), pos = row / p.share, head = (int)(group % p.kv_heads) * p.share + row % p.share;
+            from = group * p.splits * p.rows + row;
+            step = p.rows;
+            to = (E *)p.dq + ((b * p.nq + pos) * p.heads + head) * p.dim;
+        } else {
+            from = r;
+            step = rows;
+            to = r < rows / 2 ? (E *)p.dk + r * p.dim : (E *)p.dv + (r - rows / 2) * p.dim;
+        }
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) {
+            float u[4];
+            gm_load<float, 4>(u, p.part + (from + s * step) * p.dim + d, p.dim - d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += u[j];
+        }
+        gm_store<E, 4>(v, to + d, p.dim - d);
+    }
+}
+
+// Rows [batch][n][heads][dim] of any strides and alignment laid out anew, with `wide` components, zeros behind dim.
+struct PackP { int64_t rows, sb, sn, sh; int n, heads, dim, wide; const void *from; void *to; };
+template <typename E>
+__global__ __launch_bounds__(AT_TPB) void attention_pack_kernel(PackP p)
+{
+    constexpr int V = fe_width<E>;
+    const int chunks = p.wide / V;
+    const int64_t total = p.rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * AT_TPB + threadIdx.x; i < total; i += (int64_t)gridDim.x * AT_TPB) {
+        const int64_t r = i / chunks, head = r % p.heads, pos = r / p.heads % p.n, b = r / p.heads / p.n;
+        const int d = (int)(i - r * chunks) * V;
+        E v[V];
+        gm_load<E, V>(v, (const E *)p.from + b * p.sb + pos * p.sn + head * p.sh + d, p.dim - d);
+        gm_store<E, V>(v, (E *)p.to + r * p.wide + d, V);
+    }
+}
+
+static unsigned at_flat(int64_t items) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + AT_TPB - 1) / AT_TPB, 8192)); }
+static int at_units() { const int n = fgnn_current_device_compute_units(); return n > 0 ? n : 256; }
+static int at_wide(int dim, int type) { const int v = 16 / fe_size(type); return (dim + v - 1) / v * v; }
+// Whether rows do not all start at 16 bytes and hold whole 16 bytes, or lie 2^24 bytes apart or more.
+static bool at_loose(const void *p, const int64_t *strides, int dim, int type)
+{
+    const int64_t size = fe_size(type);
+    return (((uintptr_t)p | strides[0] * size | strides[1] * size | strides[2] * size | dim * size) & 15) || strides[1] * size >= 1 << 24;
+}
+static size_t at_pack_bytes(int64_t batch, int64_t n, int64_t heads, int dim, int type) { return fgnn_align256((size_t)batch * n * heads * at_wide(dim, type) * fe_size(type)); }
+static int at_pack(const void *&p, int64_t &sb, int64_t &sn, int64_t &sh, int batch, int n, int heads, int dim, int type, char *&space, hipStream_t st)
+{
+    PackP k{(int64_t)batch * n * heads, sb, sn, sh, n, heads, dim, at_wide(dim, type), p, space};
+    space += at_pack_bytes(batch, n, heads, dim, type);
+    p = k.to;
+    sh = k.wide;
+    sn = (int64_t)heads * sh;
+    sb = n * sn;
+    if (k.rows == 0) return 0;
+    fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_pack_kernel<E>), dim3(at_flat(k.rows * (k.wide / fe_width<E>))), dim3(AT_TPB), 0, st, k); });
+    return fgnn_launch_status("attention_pack_kernel");
+}
+
+// Waves and tiles of a pass, and the parts that its long side is cut into where there are too few workgroups for the device.
+static AtShape at_shape(AttentionP &p, int what, int type)
+{
+    AtShape s;
+    s.dim = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
+    s.tile = fe_size(type) == 4 ? 32 : 64;
+    s.waves = what != AT_DKV && p.rows <= 64 ? 1 : 4;
+    if (s.waves == 1) s.tile = 32;
+    const int64_t columns = what == AT_DKV ? p.nk : p.rows, walked = what == AT_DKV ? (int64_t)((p.nq + s.tile - 1) / s.tile) * p.share : (p.nk + s.tile - 1) / s.tile;
+    p.tiles = (int)((columns + 32 * s.waves - 1) / (32 * s.waves));
+    const int64_t groups = std::max<int64_t>(1, (int64_t)p.tiles * p.kv_heads * p.batch), wanted = (int64_t)at_units() * (s.waves == 1 ? 8 : 2);
+    const int64_t most = std::max<int64_t>(1, walked / 4);
+    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, wanted / groups), most, 256});
+    p.per = (int)((walked + p.splits - 1) / p.splits);
+    p.splits = p.per ? (int)((walked + p.per - 1) / p.per) : 1;
+    if (p.splits < 1) p.splits = 1;
+    return s;
+}
+static size_t at_part_bytes(const AttentionP &p, int what)
+{
+    if (p.splits < 2) return 0;
+    if (what == AT_DKV) return fgnn_align256((size_t)p.splits * 2 * p.batch * p.nk * p.kv_heads * p.dim * sizeof(float));
+    return fgnn_align256((size_t)p.batch * p.kv_heads * p.splits * p.rows * (p.dim + 1) * sizeof(float));
+}
+static int64_t at_grid(const AttentionP &p) { return (int64_t)p.tiles * p.splits * p.kv_heads * p.batch; }
+
+static int at_check(const char *who, int batch, int nq, int nk, int heads, int kv_heads, int dim, int type)
+{
+    FGNN_REQUIRE(batch >= 0 && nq >= 0 && nk >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && dim >= 1, FGNN_ERR_SHAPE,
+                 "%s: bad sizes batch=%d queries=%d keys=%d heads=%d kv_heads=%d dim=%d", who, batch, nq, nk, heads, kv_heads, dim);
+    FGNN_REQUIRE(fe_is_float(type), FGNN_ERR_SHAPE, "%s: element type %d", who, type);
+    FGNN_REQUIRE(dim <= 256, FGNN_ERR_LIMIT, "%s: heads of %d components, more than 256", who, dim);
+    FGNN_REQUIRE((int64_t)nq * (heads / kv_heads) < 1LL << 31 && nk < (1LL << 31) - 128 && nq < (1LL << 31) - 128, FGNN_ERR_LIMIT, "%s: queries=%d keys=%d", who, nq, nk);
+    return 0;
+}
+static AttentionP at_problem(int batch, int nq, int nk, int heads, int kv_heads, int dim)
+{
+    AttentionP p = {};
+    p.batch = batch; p.nq = nq; p.nk = nk; p.heads = heads; p.kv_heads = kv_heads; p.dim = dim;
+    p.share = heads / kv_heads;
+    p.rows = nq * p.share;
+    // row / share by a multiplication (for rows below 2^31)
+    while ((1LL << p.share_shift) < p.share) ++p.share_shift;
+    p.share_mul = (uint32_t)(((1ULL << 32) * ((1ULL << p.share_shift) - p.share)) / p.share + 1);
+    return p;
+}
+static int at_run(int what, int type, const AtShape &s, const AttentionP &p, hipStream_t st)
+{
+    const int64_t grid = at_grid(p);
+    if (grid == 0) return 0;
+    FGNN_REQUIRE(grid < 1LL << 24, FGNN_ERR_LIMIT, "attention: %lld workgroups", (long long)grid);
+    fe_dispatch(type, [&]<typename E>() { at_launch<E>(what, s, p, (unsigned)grid, st); });
+    return fgnn_launch_status(what == AT_FORWARD ? "attention_kernel" : what == AT_DQ ? "attention_dq_kernel" : "attention_dkv_kernel");
+}
+
+extern "C" size_t fgnn_attention_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *k, const void *v, const int64_t *strides)
+{
+    if (batch < 1 || nq < 1 || nk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > 256 || !fe_is_float(type) || !strides) return 0;
+    AttentionP p = at_problem(batch, nq, nk, heads, kv_heads, dim);
+    at_shape(p, AT_FORWARD, type);
+    const size_t pack = at_pack_bytes(batch, nk, kv_heads, dim, type);
+    return (at_loose(k, strides + 3, dim, type) ? pack : 0) + (at_loose(v, strides + 6, dim, type) ? pack : 0) + at_part_bytes(p, AT_FORWARD);
+}
+
+extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const int64_t *strides,
+                              const void *lengths, int wide, const uint8_t *mask, float scale, void *y, float *lse, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = at_check("fgnn_attention", batch, nq, nk, heads, kv_heads, dim, type);
+    if (rc || batch == 0 || nq == 0) return rc;
+    FGNN_REQUIRE(scale > 0.f && scale < __builtin_inff(), FGNN_ERR_SHAPE, "fgnn_attention: scale %g", (double)scale);
+    FGNN_REQUIRE(q && y && strides && (nk == 0 || (k && v)), FGNN_ERR_NULL, "fgnn_attention: NULL argument");
+    const size_t bytes = fgnn_attention_workspace_bytes(batch, nq, nk, heads, kv_heads, dim, type, k, v, strides);
+    FGNN_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), FGNN_ERR_WORKSPACE, "fgnn_attention: workspace of %zu bytes", workspace_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    AttentionP p = at_problem(batch, nq, nk, heads, kv_heads, dim);
+    p.q = q; p.k = k; p.v = v;
+    p.qb = strides[0]; p.qn = strides[1]; p.qh = strides[2]; p.kb = strides[3]; p.kn = strides[4]; p.kh = strides[5]; p.vb = strides[6]; p.vn = strides[7]; p.vh = strides[8];
+    p.lengths = lengths; p.wide = wide; p.mask = mask;
+    p.scale = scale; p.log2_scale = scale * 1.44269504f;
+    p.y = y; p.lse = lse;
+    char *space = (char *)workspace;
+    if (nk && at_loose(k, strides + 3, dim, type) && (rc = at_pack(p.k, p.kb, p.kn, p.kh, batch, nk, kv_heads, dim, type, space, st))) return rc;
+    if (nk && at_loose(v, strides + 6, dim, type) && (rc = at_pack(p.v, p.vb, p.vn, p.vh, batch, nk, kv_heads, dim, type, space, st))) return rc;
+    const AtShape s = at_shape(p, AT_FORWARD, type);
+    p.part = (float *)space;
+    p.part_lse = p.part + (size_t)batch * kv_heads * p.splits * p.rows * dim;
+    if ((rc = at_run(AT_FORWARD, type, s, p, st)) || p.splits < 2) return rc;
+    fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_join_kernel<E>), dim3(at_flat((int64_t)batch * nq * heads * ((dim + 3) / 4))), dim3(AT_TPB), 0, st, p); });
+    return fgnn_launch_status("attention_join_kernel");
+}
+
+extern "C" size_t fgnn_attention_backward_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const void *g,
+                                                          const int64_t *strides)
+{
+    if (batch < 1 || nq < 1 || nk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > 256 || !fe_is_float(type) || !strides) return 0;
+    AttentionP p = at_problem(batch, nq, nk, heads, kv_heads, dim);
+    at_shape(p, AT_DQ, type);
+    size_t part = at_part_bytes(p, AT_DQ);
+    at_shape(p, AT_DKV, type);
+    part = std::max(part, at_part_bytes(p, AT_DKV));
+    const size_t keys = at_pack_bytes(batch, nk, kv_heads, dim, type), queries = at_pack_bytes(batch, nq, heads, dim, type);
+    return fgnn_align256((size_t)batch * heads * nq * sizeof(float)) + part + (at_loose(q, strides, dim, type) ? queries : 0) + (at_loose(k, strides + 3, dim, type) ? keys : 0) +
+           (at_loose(v, strides + 6, dim, type) ? keys : 0) + (at_loose(g, strides + 9, dim, type) ? queries : 0);
+}
+
+extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const void *y, const void *g,
+                                       const int64_t *strides, const void *lengths, int wide, const uint8_t *mask, float scale, const float *lse, void *dq, void *dk, void *dv, void *workspace,
+                                       size_t workspace_bytes, void *stream)
+{
+    int rc = at_check("fgnn_attention_backward", batch, nq, nk, heads, kv_heads, dim, type);
+    if (rc || batch == 0) return rc;
+    FGNN_REQUIRE(scale > 0.f && scale < __builtin_inff(), FGNN_ERR_SHAPE, "fgnn_attention_backward: scale %g", (double)scale);
+    FGNN_REQUIRE((dk == nullptr) == (dv == nullptr), FGNN_ERR_NULL, "fgnn_attention_backward: dk and dv are formed together");
+    FGNN_REQUIRE(strides && (nq == 0 || (q && y && g && lse)) && (nk == 0 || (k && v)), FGNN_ERR_NULL, "fgnn_attention_backward: NULL argument");
+    const size_t bytes = fgnn_attention_backward_workspace_bytes(batch, nq, nk, heads, kv_heads, dim, type, q, k, v, g, strides);
+    FGNN_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), FGNN_ERR_WORKSPACE, "fgnn_attention_backward: workspace of %zu bytes", workspace_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    AttentionP p = at_problem(batch, nq, nk, heads, kv_heads, dim);
+    p.q = q; p.k = k; p.v = v; p.g = g;
+    p.qb = strides[0]; p.qn = strides[1]; p.qh = strides[2]; p.kb = strides[3]; p.kn = strides[4]; p.kh = strides[5]; p.vb = strides[6]; p.vn = strides[7]; p.vh = strides[8];
+    p.gb = strides[9]; p.gn = strides[10]; p.gh = strides[11];
+    p.lengths = lengths; p.wide = wide; p.mask = mask;
+    p.scale = scale; p.log2_scale = scale * 1.44269504f;
+    p.y = const_cast<void *>(y); p.lse = const_cast<float *>(lse);
+    p.dq = dq; p.dk = dk; p.dv = dv;
+    char *space = (char *)workspace;
+    if (nq) {
+        p.delta = (float *)space;
+        space += fgnn_align256((size_t)batch * heads * nq * sizeof(float));
+        int lanes = 1;
+        while (lanes * (16 / fe_size(type)) < dim) lanes *= 2;
+        fe_dispatch(type, [&]<typename E>() {
+            hipLaunchKernelGGL((attention_delta_kernel<E>), dim3(at_flat((int64_t)batch * nq * heads * lanes)), dim3(AT_TPB), 0, st, p, lanes);
+        });
+        if ((rc = fgnn_launch_status("attention_delta_kernel"))) return rc;
+        if (at_loose(q, strides, dim, type) && (rc = at_pack(p.q, p.qb, p.qn, p.qh, batch, nq, heads, dim, type, space, st))) return rc;
+        if (at_loose(k, strides + 3, dim, type) && (rc = at_pack(p.k, p.kb, p.kn, p.kh, batch, nk, kv_heads, dim, type, space, st))) return rc;
+        if (at_loose(v, strides + 6, dim, type) && (rc = at_pack(p.v, p.vb, p.vn, p.vh, batch, nk, kv_heads, dim, type, space, st))) return rc;
+        if (at_loose(g, strides + 9, dim, type) && (rc = at_pack(p.g, p.gb, p.gn, p.gh, batch, nq, heads, dim, type, space, st))) return rc;
+    }
+    p.part = (float *)space;
+    if (dq && nq) {
+        const AtShape s = at_shape(p, AT_DQ, type);
+        if ((rc = at_run(AT_DQ, type, s, p, st))) return rc;
+        if (p.splits > 1) {
+            fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_sum_kernel<E, true>), dim3(at_flat((int64_t)batch * nq * heads * ((dim + 3) / 4))), dim3(AT_TPB), 0, st, p); });
+            if ((rc = fgnn_launch_status("attention_sum_kernel"))) return rc;
+        }
+    }
+    if (dk && nk) {
+        const AtShape s = at_shape(p, AT_DKV, type);
+        if ((rc = at_run(AT_DKV, type, s, p, st))) return rc;
+        if (p.splits > 1) {
+            fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_sum_kernel<E, false>), dim3(at_flat(2LL * batch * nk * kv_heads * ((dim + 3) / 4))), dim3(AT_TPB), 0, st, p); });
+            return fgnn_launch_status("attention_sum_kernel");
+        }
+    }
+    return 0;
+}

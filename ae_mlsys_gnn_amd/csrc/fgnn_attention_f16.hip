@@ -1,0 +1,3 @@
+// The attention kernels of one element type.
+#include "fgnn_attention.h"
+template void at_launch<_Float16>(int what, const AtShape &shape, const AttentionP &p, unsigned grid, hipStream_t st);

@@ -9,6 +9,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <cmath>
 #include <sstream>
 #include "fgnn.h"
 
@@ -497,6 +498,93 @@ Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale, std::
     return lookup_forward(tokens, weight, scale, padding);
 }
 
+// ------------------------------------------------------------------------------------------------ attention
+// t [samples, positions, heads, components] with unit component stride and no negative ones; copied only where no view of that kind exists.
+Tensor heads_of(const Tensor &t) { return t.size(3) > 1 && t.stride(3) != 1 ? t.contiguous() : t; }
+struct AttentionOperands { Tensor q, k, v, lengths, mask; int type, batch, nq, nk, heads, kv_heads, dim, wide; float scale; };
+void strides_to(int64_t *to, const Tensor &t)
+{
+    for (int i = 0; i < 3; ++i) to[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+AttentionOperands attention_operands(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lengths, const Tensor &mask, const std::optional<double> &scale)
+{
+    usable("cross_attention", q, k, v, lengths, mask);
+    const int type = float_type(q);
+    if (type < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
+        refuse("cross_attention: queries of ", q.scalar_type(), " with keys of ", k.scalar_type(), " and values of ", v.scalar_type(), "; fp32, bf16 and fp16, all the same, are supported");
+    if (q.dim() != 4 || k.dim() != 4 || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(3) != k.size(3) || k.device() != q.device() || v.device() != q.device())
+        refuse("cross_attention: queries ", q.sizes(), ", keys ", k.sizes(), ", values ", v.sizes(), "; [samples, positions, heads, components] are wanted");
+    if (k.size(2) == 0 || q.size(2) == 0 || q.size(2) % k.size(2)) refuse("cross_attention: ", q.size(2), " heads over ", k.size(2), " of keys");
+    if (q.size(3) < 1 || q.size(3) > 256) refuse("cross_attention: heads of ", q.size(3), " components; up to 256 are supported");
+    if (lengths.defined() && (lengths.dim() != 1 || lengths.size(0) != q.size(0) || (lengths.scalar_type() != at::kInt && lengths.scalar_type() != at::kLong) || lengths.device() != q.device()))
+        refuse("cross_attention: lengths ", lengths.sizes(), " of ", lengths.scalar_type(), "; one int32 or int64 for each of ", q.size(0), " samples is wanted");
+    if (mask.defined() && (mask.dim() != 2 || mask.size(0) != q.size(0) || mask.size(1) != k.size(1) || mask.scalar_type() != at::kBool || mask.device() != q.device()))
+        refuse("cross_attention: mask ", mask.sizes(), " of ", mask.scalar_type(), "; a truth value for each of ", q.size(0), " x ", k.size(1), " keys is wanted");
+    const double s = scale ? *scale : 1. / std::sqrt((double)q.size(3));
+    if (!(s >= 1e-30 && s <= 1e30)) refuse("cross_attention: scale ", s, "; a positive number is wanted");
+    return {heads_of(q), heads_of(k), heads_of(v), lengths.defined() ? lengths.contiguous() : Tensor(), mask.defined() ? mask.contiguous() : Tensor(), type, as_int(q.size(0), "samples;"),
+            as_int(q.size(1), "queries;"), as_int(k.size(1), "keys;"), as_int(q.size(2), "heads;"), (int)k.size(2), (int)q.size(3), lengths.defined() && lengths.scalar_type() == at::kLong, (float)s};
+}
+struct AttentionOut { Tensor y, lse; };
+AttentionOut attention_forward(const AttentionOperands &o, bool keep)
+{
+    const c10::OptionalDeviceGuard guard(o.q.device());
+    int64_t strides[9];
+    strides_to(strides, o.q);
+    strides_to(strides + 3, o.k);
+    strides_to(strides + 6, o.v);
+    AttentionOut out{like(o.q, o.q.sizes()), keep ? like(o.q, {o.batch, o.heads, o.nq}, at::kFloat) : Tensor()};
+    const size_t bytes = fgnn_attention_workspace_bytes(o.batch, o.nq, o.nk, o.heads, o.kv_heads, o.dim, o.type, address(o.k), address(o.v), strides);
+    const Tensor ws = scratch(o.q, bytes);
+    check(fgnn_attention(o.batch, o.nq, o.nk, o.heads, o.kv_heads, o.dim, o.type, address(o.q), address(o.k), address(o.v), strides, address(o.lengths), o.wide,
+                         (const uint8_t *)address(o.mask), o.scale, address(out.y), (float *)address(out.lse), address(ws), bytes, stream_of(o.q)), "fgnn_attention");
+    return out;
+}
+
+// Kept for the backward pass: q, k, v, y, the logarithm of every query's sum, and what is seen.
+struct Attention : torch::autograd::Function<Attention> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const MaybeTensor &lengths, const MaybeTensor &mask, std::optional<double> scale)
+    {
+        const AttentionOperands o = attention_operands(q, k, v, given(lengths), given(mask), scale);
+        const AttentionOut out = attention_forward(o, true);
+        ctx->saved_data["need"] = (int64_t)(wanted(q) | wanted(k) << 1 | wanted(v) << 2);
+        ctx->saved_data["scale"] = (double)o.scale;
+        ctx->save_for_backward({q, k, v, out.y, out.lse, o.lengths, o.mask});
+        return out.y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list up)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const int64_t need = ctx->saved_data["need"].toInt();
+        const Tensor q = heads_of(saved[0]), k = heads_of(saved[1]), v = heads_of(saved[2]), &y = saved[3], &lengths = saved[5], &mask = saved[6], g = heads_of(up[0]);
+        const int type = float_type(q), batch = (int)q.size(0), nq = (int)q.size(1), nk = (int)k.size(1), heads = (int)q.size(2), kv_heads = (int)k.size(2), dim = (int)q.size(3);
+        const c10::OptionalDeviceGuard guard(q.device());
+        int64_t strides[12];
+        strides_to(strides, q);
+        strides_to(strides + 3, k);
+        strides_to(strides + 6, v);
+        strides_to(strides + 9, g);
+        Tensor dq, dk, dv;
+        if (need & 1) dq = like(q, q.sizes());
+        if (need & 6) {
+            dk = like(k, k.sizes());
+            dv = like(v, v.sizes());
+        }
+        const size_t bytes = fgnn_attention_backward_workspace_bytes(batch, nq, nk, heads, kv_heads, dim, type, address(q), address(k), address(v), address(g), strides);
+        const Tensor ws = scratch(q, bytes);
+        check(fgnn_attention_backward(batch, nq, nk, heads, kv_heads, dim, type, address(q), address(k), address(v), address(y), address(g), strides, address(lengths),
+                                      lengths.defined() && lengths.scalar_type() == at::kLong, (const uint8_t *)address(mask), (float)ctx->saved_data["scale"].toDouble(),
+                                      (const float *)address(saved[4]), address(dq), address(dk), address(dv), address(ws), bytes, stream_of(q)), "fgnn_attention_backward");
+        return final_gradients("cross_attention", {dq, need & 2 ? dk : Tensor(), need & 4 ? dv : Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+Tensor cross_attention(const Tensor &q, const Tensor &k, const Tensor &v, const MaybeTensor &lengths, const MaybeTensor &mask, std::optional<double> scale)
+{
+    py::gil_scoped_release off;
+    if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v))) return Attention::apply(q, k, v, lengths, mask, scale);
+    return attention_forward(attention_operands(q, k, v, given(lengths), given(mask), scale), false).y;
+}
+
 // ------------------------------------------------------------------------------------------------ orthogonalised updates
 Tensor orthogonalize(const Tensor &given_g, const std::vector<float> &coefficients, double eps)
 {
@@ -534,4 +622,5 @@ PYBIND11_MODULE(_dense, m)
     m.def("orthogonalize", &orthogonalize);
     m.def("group_norm", &group_norm);
     m.def("embedding", &embedding);
+    m.def("cross_attention", &cross_attention);
 }

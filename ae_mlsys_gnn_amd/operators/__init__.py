@@ -1,5 +1,6 @@
 """Python mirror of the reference's ``operators/`` package for the fused sparse-operator path.
 Same callables and signatures; the work is done by libfgnn_hip.so."""
+from .attention import cross_attention  # noqa: F401
 from .csr2csc import sparsetrans  # noqa: F401  (the csr2csc function lives in the csr2csc submodule)
 from .edge_proj import EdgeLinearTanhFunction, edge_linear_tanh  # noqa: F401
 from .edge_softmax import EdgeSoftmaxFunction, csr_edge_softmax  # noqa: F401
