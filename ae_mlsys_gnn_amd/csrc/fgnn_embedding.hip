@@ -1,13 +1,14 @@
 // Rows of a table by tokens, y_i = s W[t_i], and the table's gradient dW[v] = s sum_{i: t_i = v} gy_i, summed in the tokens' order.
-// Both are bound by memory.  The forward pass reads a row for every token.  For the gradient the tokens are sorted (stably, with their positions); the sorted
+// Both are bound by memory.  The forward pass reads a row for every token.  For the gradient the tokens are sorted (stably, with their positions), and the sorted
 // positions are cut into tiles of one length whatever the tokens, so that a token met a hundred thousand times is summed by as many workgroups as a hundred
-// thousand tokens met once.  A token whose positions lie in one tile is written from there; parts of the others are added up by the kernel that
-// also writes the rows of tokens that are not met.  Sums are 32 bits, in a fixed order.
+// thousand tokens met once.  A token whose positions lie in one tile is written from there, beside workgroups that write zeros for the tokens that are not met; the parts of
+// the others, two a tile at the most, are added up in a second launch.  Sums are 32 bits, in a fixed order.
 #include <algorithm>
 #include "fgnn_gemm.h"
 
 #define EM_TPB 256
 #define EM_GRID (1 << 20)
+#define EM_FEW 4096                         // tokens that are sorted by their ranks
 struct EmbeddingP {
     int64_t n; int vocabulary, cols;
     const void *tokens; int wide;           // wide: int64
@@ -16,9 +17,9 @@ struct EmbeddingP {
     void *y;
     const void *gy; int64_t ldg; void *dw;
     int lanes, groups, tiles_c;             // threads a row, rows a workgroup, parts of a row
-    int length; int64_t tiles;              // sorted positions a tile
-    const int *keys, *order, *start;        // sorted tokens, their positions, where each token's begin [vocabulary + 1]
-    float *part;                            // [tiles][2][cols]: sums of the tile's first token and of its last
+    int length, tile; int64_t tiles;        // sorted positions of a group of threads and of a workgroup, workgroups' tiles
+    const int *keys, *order;                // sorted tokens, their positions
+    float *part;                            // [tiles][2][cols]: sums of the tile's first token (where it began before) and of its last (where it goes on)
 };
 
 __device__ __forceinline__ int64_t em_token(const EmbeddingP &p, int64_t i) { return p.wide ? ((const int64_t *)p.tokens)[i] : ((const int32_t *)p.tokens)[i]; }
@@ -26,133 +27,254 @@ __device__ __forceinline__ int64_t em_token(const EmbeddingP &p, int64_t i) { re
 template <typename E>
 __global__ __launch_bounds__(EM_TPB) void embedding_kernel(EmbeddingP p)
 {
-    constexpr int V = fe_width<E>;
+    constexpr int V = fe_width<E>, U = 4;
     const int lane = (int)threadIdx.x % p.lanes, group = (int)threadIdx.x / p.lanes;
-    const int64_t items = (p.n + p.groups - 1) / p.groups * p.tiles_c;
+    const int64_t rows = (int64_t)p.groups * U, items = (p.n + rows - 1) / rows * p.tiles_c;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t i = item / p.tiles_c * p.groups + group;
+        const int64_t i = item / p.tiles_c * rows + group;
         const int c = ((int)(item % p.tiles_c) * p.lanes + lane) * V;
-        if (group >= p.groups || i >= p.n || c >= p.cols) continue;
-        const int64_t t = em_token(p, i);
-        float v[V];
-        if (t >= 0 && t < p.vocabulary) {
-            gm_load<E, V>(v, (const E *)p.w + t * p.ldw + c, p.cols - c);
+        if (group >= p.groups || c >= p.cols) continue;
+        float v[U][V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] *= p.scale;
-        } else {
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = i + (int64_t)u * p.groups, t = at < p.n ? em_token(p, at) : 0;
+            if (t >= 0 && t < p.vocabulary) gm_load<E, V>(v[u], (const E *)p.w + t * p.ldw + c, p.cols - c);
+            else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = __builtin_nanf("");
+                for (int j = 0; j < V; ++j) v[u][j] = __builtin_nanf("");
+            }
         }
-        gm_store<E, V>(v, (E *)p.y + i * p.cols + c, p.cols - c);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = i + (int64_t)u * p.groups;
+            if (at >= p.n) break;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[u][j] *= p.scale;
+            gm_store<E, V>(v[u], (E *)p.y + at * p.cols + c, p.cols - c);
+        }
     }
 }
 
 // Tokens as 32-bit keys; those without a gradient (padding, outside the table) come last.
+__device__ __forceinline__ int em_key(const EmbeddingP &p, int64_t i, int64_t padding)
+{
+    const int64_t t = em_token(p, i);
+    return t >= 0 && t < p.vocabulary && t != padding ? (int)t : p.vocabulary;
+}
 __global__ __launch_bounds__(EM_TPB) void embedding_keys_kernel(EmbeddingP p, int64_t padding, int *__restrict__ keys)
 {
-    for (int64_t i = (int64_t)blockIdx.x * EM_TPB + threadIdx.x; i < p.n; i += (int64_t)gridDim.x * EM_TPB) {
-        const int64_t t = em_token(p, i);
-        keys[i] = t >= 0 && t < p.vocabulary && t != padding ? (int)t : p.vocabulary;
-    }
+    for (int64_t i = (int64_t)blockIdx.x * EM_TPB + threadIdx.x; i < p.n; i += (int64_t)gridDim.x * EM_TPB) keys[i] = em_key(p, i, padding);
 }
-// start[v] = the first sorted position of a key >= v
-__global__ __launch_bounds__(EM_TPB) void embedding_start_kernel(const int *__restrict__ keys, int64_t n, int vocabulary, int *__restrict__ start)
+// Few tokens are sorted by their ranks: a thread counts what comes before its token, four comparisons a read of LDS.
+__global__ __launch_bounds__(EM_TPB) void embedding_rank_kernel(EmbeddingP p, int64_t padding, int *__restrict__ keys, int *__restrict__ order)
 {
-    const int v = (int)(blockIdx.x * EM_TPB + threadIdx.x);
-    if (v > vocabulary) return;
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < v) lo = mid + 1; else hi = mid;
+    __shared__ __attribute__((aligned(16))) int all[EM_FEW];
+    const int n = (int)p.n, padded = (n + 3) & ~3;
+    for (int i = threadIdx.x; i < padded; i += EM_TPB) all[i] = i < n ? em_key(p, i, padding) : 0x7fffffff;
+    __syncthreads();
+    const int i = (int)(blockIdx.x * EM_TPB + threadIdx.x);
+    if (i >= n) return;
+    const int key = all[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < padded; j += 4) {
+        const gm_i4 k = *reinterpret_cast<const gm_i4 *>(all + j);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) rank += k[u] < key || (k[u] == key && j + u < i);
     }
-    start[v] = (int)lo;
+    keys[rank] = key;
+    order[rank] = i;
+}
+// The first sorted position of a key >= v, seven probes a step.
+__device__ __forceinline__ int64_t em_bound(const int *__restrict__ keys, int64_t n, int v)
+{
+    int64_t lo = 0, hi = n;                 // keys[lo - 1] < v <= keys[hi]
+    while (lo < hi) {
+        const int64_t step = (hi - lo + 7) / 8;
+        int below = 0;
+#pragma unroll
+        for (int j = 1; j < 8; ++j) {
+            const int64_t at = lo + j * step - 1;
+            below += at < hi && keys[at] < v;
+        }
+        // (keys are sorted: the first `below` probes are below v)
+        hi = min(hi, below < 7 ? lo + (below + 1) * step - 1 : hi);
+        lo += below * step;
+    }
+    return lo;
 }
 
+// The first `tiles` x tiles_c workgroups sum tiles, the others write zeros for tokens that are not met, EM_ROWS of them each.
+#define EM_ROWS 64
+enum { EM_CLOSE = 1, EM_WHOLE = 2, EM_ON = 4 };
 template <typename E>
 __global__ __launch_bounds__(EM_TPB) void embedding_sum_kernel(EmbeddingP p)
 {
     constexpr int V = fe_width<E>, U = 8;
+    __shared__ float ends[2][EM_TPB * V];                       // a group's first token's sum, where it began before, and its last one's, where it goes on
+    __shared__ int flags[EM_TPB], firsts[EM_TPB], lasts[EM_TPB];
     const int lane = (int)threadIdx.x % p.lanes, group = (int)threadIdx.x / p.lanes;
-    const int64_t items = (p.tiles + p.groups - 1) / p.groups * p.tiles_c;
-    const int64_t end = p.start[p.vocabulary];                  // what lies behind has no gradient
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t tile = item / p.tiles_c * p.groups + group;
-        const int c = ((int)(item % p.tiles_c) * p.lanes + lane) * V, left = p.cols - c;
-        const int64_t first = tile * p.length, last = min(end, first + p.length);
-        if (group >= p.groups || left <= 0 || first >= last) continue;
-        float sum[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum[j] = 0.f;
-        int now = p.keys[first];
-        bool open = first > 0 && p.keys[first - 1] == now;      // the token's positions began in a tile before
-        auto leave = [&](bool on) {                             // on: they go on behind this tile
-            if (open || on) {
-                gm_store<float, V>(sum, p.part + (2 * tile + (open ? 0 : 1)) * p.cols + c, left);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) sum[j] *= p.scale;
-                gm_store<E, V>(sum, (E *)p.dw + (int64_t)now * p.cols + c, left);
+    if (blockIdx.x >= p.tiles * p.tiles_c) {
+        const int row0 = (int)(blockIdx.x - p.tiles * p.tiles_c) * EM_ROWS, row = row0 + (int)threadIdx.x;
+        if (threadIdx.x < EM_ROWS) {
+            const int64_t at = row < p.vocabulary ? em_bound(p.keys, p.n, row) : 0;
+            flags[threadIdx.x] = row < p.vocabulary && (at == p.n || p.keys[at] != row);
+        }
+        __syncthreads();
+        const float zero[V] = {};
+        for (int tile = 0; tile < p.tiles_c; ++tile)
+            for (int r = group; r < EM_ROWS && group < p.groups; r += p.groups) {
+                const int c = (tile * p.lanes + lane) * V;
+                if (flags[r] && c < p.cols) gm_store<E, V>(zero, (E *)p.dw + (int64_t)(row0 + r) * p.cols + c, p.cols - c);
             }
+        return;
+    }
+    const int64_t tile = blockIdx.x / p.tiles_c;
+    const int c = ((int)(blockIdx.x % p.tiles_c) * p.lanes + lane) * V, left = p.cols - c;
+    const int64_t first = tile * p.tile + (int64_t)group * p.length, last = min(p.n, first + p.length);
+    auto write = [&](float (&sum)[V], int key) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] *= p.scale;
+        gm_store<E, V>(sum, (E *)p.dw + (int64_t)key * p.cols + c, left);
+    };
+    if (group < p.groups) {
+        int flag = 0, now = first < last ? p.keys[first] : p.vocabulary;
+        const int head = now;
+        if (now < p.vocabulary) {
+            bool open = first > 0 && p.keys[first - 1] == now;
+            float sum[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] = 0.f;
-            open = false;
-        };
-        for (int64_t i = first; i < last; i += U) {
-            float g[U][V];
-            int key[U];
+            auto keep = [&](int which) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t at = min(i + u, last - 1);
-                key[u] = p.keys[at];
-                gm_load<E, V>(g[u], (const E *)p.gy + (int64_t)p.order[at] * p.ldg + c, left);
-            }
+                for (int j = 0; j < V; ++j) ends[which][threadIdx.x * V + j] = sum[j];
+            };
+            for (int64_t i = first; i < last; i += U) {
+                float g[U][V];
+                int key[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i + u >= last) break;
-                if (key[u] != now) {
-                    leave(false);
-                    now = key[u];
+                for (int u = 0; u < U; ++u) {
+                    const int64_t at = min(i + u, last - 1);
+                    key[u] = p.keys[at];
+                    gm_load<E, V>(g[u], (const E *)p.gy + (int64_t)p.order[at] * p.ldg + c, left);
                 }
 #pragma unroll
-                for (int j = 0; j < V; ++j) sum[j] += g[u][j];
+                for (int u = 0; u < U; ++u) {
+                    if (i + u >= last || now == p.vocabulary) break;
+                    if (key[u] != now) {
+                        if (open) {
+                            keep(0);
+                            flag |= EM_CLOSE;
+                        } else if (left > 0) write(sum, now);
+                        open = false;
+                        now = key[u];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) sum[j] = 0.f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < V; ++j) sum[j] += g[u][j];
+                }
+            }
+            if (now < p.vocabulary) {
+                const bool on = last < p.n && p.keys[last] == now;
+                if (open || on) {
+                    keep(open ? 0 : 1);
+                    flag |= !open ? EM_ON : on ? EM_WHOLE : EM_CLOSE;
+                } else if (left > 0) write(sum, now);
             }
         }
-        leave(last < end && p.keys[last] == now);
+        if (lane == 0) {
+            flags[group] = flag;
+            firsts[group] = head;
+            lasts[group] = now;
+        }
     }
+    __syncthreads();
+    if (group != 0 || left <= 0) return;
+    // the groups' ends in their order: a token that begins and ends in the workgroup's tile is written, the others' parts are kept
+    float sum[V];
+    int key = 0, have = 0;                  // have: 1 begun here, 2 before
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.f;
+    for (int g = 0; g < p.groups; ++g) {
+        const int flag = flags[g], from = (g * p.lanes + lane) * V;
+        if (flag & (EM_CLOSE | EM_WHOLE)) {
+            if (!have) {
+                have = 2;
+                key = firsts[g];
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += ends[0][from + j];
+            if (flag & EM_CLOSE) {
+                if (have == 2) gm_store<float, V>(sum, p.part + 2 * tile * p.cols + c, left);
+                else write(sum, key);
+                have = 0;
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] = 0.f;
+            }
+        }
+        if (flag & EM_ON) {
+            have = 1;
+            key = lasts[g];
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] = ends[1][from + j];
+        }
+    }
+    if (have) gm_store<float, V>(sum, p.part + (2 * tile + (have == 1)) * p.cols + c, left);
 }
 
-// Rows of tokens that are not met, and of those whose positions lie in more than one tile: the first one's sum is its last token's, the others' their first's.
+// The same by a whole wave, 64 probes a step.
+__device__ __forceinline__ int64_t em_bound_wave(const int *__restrict__ keys, int64_t n, int v)
+{
+    const int lane = fg_lane();
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t step = (hi - lo + 64) / 65, at = lo + (lane + 1) * step - 1;
+        const int below = __popcll(__ballot(at < hi && keys[at < hi ? at : lo] < v));
+        hi = min(hi, below < 64 ? lo + (below + 1) * step - 1 : hi);
+        lo += below * step;
+    }
+    return lo;
+}
+
+// Tokens whose positions lie in more than one tile: the workgroup of the tile where they begin adds up their parts, its groups every so many of them, then those
+// sums (one group for all of them: 124 parts of 128 fp32 took 40 us).
 template <typename E>
-__global__ __launch_bounds__(EM_TPB) void embedding_rows_kernel(EmbeddingP p)
+__global__ __launch_bounds__(EM_TPB) void embedding_join_kernel(EmbeddingP p)
 {
     constexpr int V = fe_width<E>;
+    __shared__ float sums[EM_TPB * V];
     const int lane = (int)threadIdx.x % p.lanes, group = (int)threadIdx.x / p.lanes;
-    const int64_t items = ((int64_t)p.vocabulary + p.groups - 1) / p.groups * p.tiles_c;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t row = item / p.tiles_c * p.groups + group;
-        const int c = ((int)(item % p.tiles_c) * p.lanes + lane) * V, left = p.cols - c;
-        if (group >= p.groups || left <= 0 || row >= p.vocabulary) continue;
-        const int64_t a = p.n ? p.start[row] : 0, b = p.n ? p.start[row + 1] : 0;
-        float sum[V];
+    const int64_t tile = blockIdx.x / p.tiles_c;
+    const int c = ((int)(blockIdx.x % p.tiles_c) * p.lanes + lane) * V, left = p.cols - c;
+    const int64_t first = tile * p.tile, end = first + p.tile;
+    if (end >= p.n) return;
+    const int key = p.keys[end - 1];
+    if (key == p.vocabulary || p.keys[end] != key || (first > 0 && p.keys[first - 1] == key)) return;
+    const int64_t last = (em_bound_wave(p.keys, p.n, key + 1) - 1) / p.tile;
+    float sum[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[j] = 0.f;
-        if (b > a) {
-            const int64_t t0 = a / p.length, t1 = (b - 1) / p.length;
-            if (t0 == t1) continue;
-            // (it begins its first tile where a is the tile's first position: then that tile's sum is of its first token, and not open; see leave)
-            gm_load<float, V>(sum, p.part + (2 * t0 + 1) * p.cols + c, left);
-#pragma unroll 4
-            for (int64_t t = t0 + 1; t <= t1; ++t) {
-                float v[V];
-                gm_load<float, V>(v, p.part + 2 * t * p.cols + c, left);
+    for (int j = 0; j < V; ++j) sum[j] = 0.f;
+    if (group < p.groups && left > 0) {
+        if (group == 0) gm_load<float, V>(sum, p.part + (2 * tile + 1) * p.cols + c, left);
+#pragma unroll 8
+        for (int64_t t = tile + 1 + group; t <= last; t += p.groups) {
+            float v[V];
+            gm_load<float, V>(v, p.part + 2 * t * p.cols + c, left);
 #pragma unroll
-                for (int j = 0; j < V; ++j) sum[j] += v[j];
-            }
-#pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] *= p.scale;
+            for (int j = 0; j < V; ++j) sum[j] += v[j];
         }
-        gm_store<E, V>(sum, (E *)p.dw + row * p.cols + c, left);
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = sum[j];
+    __syncthreads();
+    if (group != 0 || left <= 0) return;
+    for (int g = 1; g < p.groups; ++g)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += sums[(g * p.lanes + lane) * V + j];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] *= p.scale;
+    gm_store<E, V>(sum, (E *)p.dw + (int64_t)key * p.cols + c, left);
 }
 
 static void em_cut(EmbeddingP &p, int type)
@@ -162,9 +284,9 @@ static void em_cut(EmbeddingP &p, int type)
     p.lanes = (vectors + p.tiles_c - 1) / p.tiles_c;
     p.groups = EM_TPB / p.lanes;
     p.length = 32;
-    p.tiles = (p.n + p.length - 1) / p.length;
+    p.tile = p.length * p.groups;
+    p.tiles = (p.n + p.tile - 1) / p.tile;
 }
-static unsigned em_grid(int64_t rows, const EmbeddingP &p) { return (unsigned)std::min<int64_t>((rows + p.groups - 1) / p.groups * p.tiles_c, EM_GRID); }
 
 static int em_check(const char *who, int64_t n, int vocabulary, int cols, int type, const void *tokens, int wide)
 {
@@ -183,20 +305,19 @@ extern "C" int fgnn_embedding(int64_t n, int vocabulary, int cols, int type, con
     FGNN_REQUIRE(y && (weight || vocabulary == 0), FGNN_ERR_NULL, "fgnn_embedding: NULL argument");
     EmbeddingP p = {n, vocabulary, cols, tokens, wide, weight, ldw, scale, y};
     em_cut(p, type);
-    fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((embedding_kernel<E>), dim3(em_grid(n, p)), dim3(EM_TPB), 0, (hipStream_t)stream, p); });
+    fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((embedding_kernel<E>), dim3((unsigned)std::min<int64_t>((n + 4 * p.groups - 1) / (4 * p.groups) * p.tiles_c, EM_GRID)), dim3(EM_TPB), 0, (hipStream_t)stream, p); });
     return fgnn_launch_status("embedding_kernel");
 }
 
-// keys, order, start, the sums of the tiles' ends, the sort's own
-struct EmbeddingSpace { size_t keys, start, part, sort; int bits; size_t all() const { return 2 * keys + start + part + sort; } };
+// keys, order, the sums of the tiles' ends, the sort's own
+struct EmbeddingSpace { size_t keys, part, sort; int bits; size_t all() const { return 3 * keys + part + sort; } };
 static EmbeddingSpace em_space(const EmbeddingP &p)
 {
     EmbeddingSpace s;
     s.bits = fgnn_rs_key_bits(p.vocabulary + 1);
     s.keys = fgnn_align256((size_t)p.n * sizeof(int));
-    s.start = fgnn_align256(((size_t)p.vocabulary + 1) * sizeof(int));
     s.part = fgnn_align256((size_t)p.tiles * 2 * p.cols * sizeof(float));
-    s.sort = fgnn_rs_sort_workspace(p.n, s.bits);
+    s.sort = p.n > EM_FEW ? fgnn_rs_sort_workspace(p.n, s.bits) : 0;
     return s;
 }
 extern "C" size_t fgnn_embedding_backward_workspace_bytes(int64_t n, int vocabulary, int cols, int type)
@@ -216,28 +337,27 @@ extern "C" int fgnn_embedding_backward(int64_t n, int vocabulary, int cols, int 
     FGNN_REQUIRE(dw && (n == 0 || gy), FGNN_ERR_NULL, "fgnn_embedding_backward: NULL argument");
     EmbeddingP p = {n, vocabulary, cols, tokens, wide, nullptr, 0, scale, nullptr, gy, ldg, dw};
     em_cut(p, type);
-    hipStream_t st = (hipStream_t)stream;
-    if (n == 0) {
-        fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((embedding_rows_kernel<E>), dim3(em_grid(vocabulary, p)), dim3(EM_TPB), 0, st, p); });
-        return fgnn_launch_status("embedding_rows_kernel");
-    }
     const EmbeddingSpace s = em_space(p);
-    FGNN_REQUIRE(workspace && workspace_bytes >= s.all(), FGNN_ERR_WORKSPACE, "fgnn_embedding_backward: workspace of %zu bytes", workspace_bytes);
+    FGNN_REQUIRE(n == 0 || (workspace && workspace_bytes >= s.all()), FGNN_ERR_WORKSPACE, "fgnn_embedding_backward: workspace of %zu bytes", workspace_bytes);
+    const int64_t summed = p.tiles * p.tiles_c, zeroed = ((int64_t)vocabulary + EM_ROWS - 1) / EM_ROWS;
+    FGNN_REQUIRE(summed + zeroed < 1 << 24, FGNN_ERR_LIMIT, "fgnn_embedding_backward: n=%lld vocabulary=%d cols=%d", (long long)n, vocabulary, cols);
+    hipStream_t st = (hipStream_t)stream;
     char *at = (char *)workspace;
-    int *keys = (int *)at, *order = (int *)(at + s.keys), *start = (int *)(at + 2 * s.keys);
-    p.part = (float *)(at + 2 * s.keys + s.start);
-    const unsigned flat = (unsigned)std::min<int64_t>((n + EM_TPB - 1) / EM_TPB, EM_GRID);
-    hipLaunchKernelGGL(embedding_keys_kernel, dim3(flat), dim3(EM_TPB), 0, st, p, padding, keys);
-    int launched = fgnn_launch_status("embedding_keys_kernel");
-    if (launched) return launched;
-    launched = fgnn_rs_sort_pairs(keys, nullptr, n, s.bits, order, &p.keys, at + 2 * s.keys + s.start + s.part, st);
-    if (launched) return launched;
+    int *keys = (int *)at, *order = (int *)(at + s.keys);
+    p.part = (float *)(at + 3 * s.keys);
     p.order = order;
-    p.start = start;
-    hipLaunchKernelGGL(embedding_start_kernel, dim3((unsigned)(vocabulary / EM_TPB + 1)), dim3(EM_TPB), 0, st, p.keys, n, vocabulary, start);
+    p.keys = keys;
+    if (n > EM_FEW) {
+        int *loose = (int *)(at + 2 * s.keys);
+        hipLaunchKernelGGL(embedding_keys_kernel, dim3((unsigned)std::min<int64_t>((n + EM_TPB - 1) / EM_TPB, EM_GRID)), dim3(EM_TPB), 0, st, p, padding, loose);
+        int launched = fgnn_launch_status("embedding_keys_kernel");
+        if (launched) return launched;
+        launched = fgnn_rs_sort_pairs(loose, nullptr, n, s.bits, order, &p.keys, at + 3 * s.keys + s.part, st);
+        if (launched) return launched;
+    } else if (n) hipLaunchKernelGGL(embedding_rank_kernel, dim3((unsigned)((n + EM_TPB - 1) / EM_TPB)), dim3(EM_TPB), 0, st, p, padding, keys, order);
     fe_dispatch(type, [&]<typename E>() {
-        hipLaunchKernelGGL((embedding_sum_kernel<E>), dim3(em_grid(p.tiles, p)), dim3(EM_TPB), 0, st, p);
-        hipLaunchKernelGGL((embedding_rows_kernel<E>), dim3(em_grid(vocabulary, p)), dim3(EM_TPB), 0, st, p);
+        hipLaunchKernelGGL((embedding_sum_kernel<E>), dim3((unsigned)(summed + zeroed)), dim3(EM_TPB), 0, st, p);
+        if (p.tiles > 1) hipLaunchKernelGGL((embedding_join_kernel<E>), dim3((unsigned)summed), dim3(EM_TPB), 0, st, p);
     });
-    return fgnn_launch_status("embedding_rows_kernel");
+    return fgnn_launch_status("embedding_join_kernel");
 }
