@@ -24,12 +24,33 @@ struct GroupNormP {
     float *sums, *group;                    // backward: [batch][2][cols] A and B, [batch][groups][2] means
 };
 
-template <typename E, int V>
-__device__ __forceinline__ void gn_load(float (&v)[V], const E *row, int left)
+// Vectors that would end behind the last channel begin earlier, where there is room: the channels that they share with the vector before are summed there alone,
+// and written twice, the same values (element by element, 86-byte groups of fp16 took three times as long).
+struct GnVector { int c, shared, left; };   // first channel, how many of them are the vector's before, channels from the first on
+template <int V>
+__device__ __forceinline__ GnVector gn_vector(int c, int end, int first)
 {
-    gm_load<E, V>(v, row, left);
+    const int from = max(min(c, end - V), first);
+    return {from, c - from, end - from};
 }
-// The statistics, weights and bias of a thread's V channels.
+template <typename E>
+__device__ __forceinline__ typename fe_vec<E>::type gn_read(const E *p, int left)
+{
+    typedef typename fe_vec<E>::type vec;
+    if (left >= fe_width<E>) return *reinterpret_cast<const vec *>(p);
+    vec v = {};
+#pragma unroll
+    for (int i = 0; i < fe_width<E>; ++i) if (i < left) v[i] = p[i];
+    return v;
+}
+template <typename E, int V>
+__device__ __forceinline__ void gn_floats(float (&v)[V], typename fe_vec<E>::type u)
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)u[i];
+}
+// The statistics, weights and bias of a thread's V channels; mean: -mean rstd, so that u = x rstd + mean in one operation, which is off by a rounding of the mean in
+// deviations, as the mean itself is.
 template <int V> struct GnCols { float mean[V], rstd[V], w[V], b[V]; };
 template <int V>
 __device__ __forceinline__ void gn_columns(const GroupNormP &p, int64_t sample, int c, GnCols<V> &o)
@@ -38,27 +59,28 @@ __device__ __forceinline__ void gn_columns(const GroupNormP &p, int64_t sample, 
     for (int i = 0; i < V; ++i) {
         const int j = min(c + i, p.cols - 1);
         const int64_t g = sample * p.groups + j / p.width;
-        o.mean[i] = p.mean[g];
         o.rstd[i] = p.rstd[g];
+        o.mean[i] = -p.mean[g] * o.rstd[i];
         o.w[i] = p.w ? fe_load(p.w, j, p.wtype) : 1.f;
         o.b[i] = p.b ? fe_load(p.b, j, p.btype) : 0.f;
     }
 }
-// d and u of V elements, from x and gy
-template <int V>
+// d and u of V elements, from x and gy.  ACT: the activation, or GN_ANY: p.act.
+#define GN_ANY (-1)
+template <int ACT, int V>
 __device__ __forceinline__ void gn_slope(const GroupNormP &p, const GnCols<V> &o, float (&x)[V], float (&g)[V])
 {
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        x[i] = (x[i] - o.mean[i]) * o.rstd[i];
+        x[i] = fmaf(x[i], o.rstd[i], o.mean[i]);
         z[i] = fmaf(x[i], o.w[i], o.b[i]);
     }
-    gm_act_slope(g, z, p.act, p.slope);
+    gm_act_slope(g, z, ACT == GN_ANY ? p.act : ACT, p.slope);
 }
 
 // A workgroup's place: sample, chunk of points, tile of channels.
-struct GnPlace { int64_t sample, first, last; int chunk, c, left, row, step; bool on; };
+struct GnPlace { int64_t sample, first, last; int chunk, tile0, c, shared, left, row, step; bool on; };
 template <int V>
 __device__ __forceinline__ GnPlace gn_place(const GroupNormP &p, int64_t item)
 {
@@ -71,18 +93,22 @@ __device__ __forceinline__ GnPlace gn_place(const GroupNormP &p, int64_t item)
     o.last = min(p.points, o.first + p.rows);
     o.step = GN_TPB / p.lanes;
     o.row = (int)threadIdx.x / p.lanes;
-    o.c = (tile * p.lanes + (int)threadIdx.x % p.lanes) * V;
-    o.left = p.cols - o.c;
-    o.on = o.row < o.step && o.left > 0;
+    o.tile0 = tile * p.lanes * V;
+    const int c = o.tile0 + (int)threadIdx.x % p.lanes * V;
+    const GnVector v = gn_vector<V>(c, p.cols, 0);
+    o.c = v.c;
+    o.shared = v.shared;
+    o.left = v.left;
+    o.on = o.row < o.step && c < p.cols;
     return o;
 }
 
 // Sums over a chunk of points, a channel each: of x - k and its square, with k the channel's first value in the sample (squares of what is far from 0
 // would lose the variance), or of d and d u.
-template <typename E, bool BACKWARD>
+template <typename E, bool BACKWARD, int ACT>
 __global__ __launch_bounds__(GN_TPB) void gn_sums_kernel(GroupNormP p)
 {
-    constexpr int V = fe_width<E>, U = BACKWARD ? 2 : 4;
+    constexpr int V = fe_width<E>, U = 4;
     __shared__ float red[2][GN_TPB * V];
     const int64_t items = p.batch * p.chunks * p.tiles;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
@@ -96,10 +122,14 @@ __global__ __launch_bounds__(GN_TPB) void gn_sums_kernel(GroupNormP p)
             float k[V];
             GnCols<V> cols;
             if constexpr (BACKWARD) gn_columns<V>(p, o.sample, o.c, cols);
-            else gn_load<E, V>(k, x, o.left);
-            auto add = [&](float (&v)[V], float (&g)[V]) {
+            else gm_load<E, V>(k, x, o.left);
+            typedef typename fe_vec<E>::type vec;
+            auto add = [&](vec vx, vec vg) {
+                float v[V], g[V];
+                gn_floats<E, V>(v, vx);
+                if constexpr (BACKWARD) gn_floats<E, V>(g, vg);
                 if constexpr (BACKWARD) {
-                    gn_slope<V>(p, cols, v, g);
+                    gn_slope<ACT, V>(p, cols, v, g);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         a[i] += g[i];
@@ -116,30 +146,32 @@ __global__ __launch_bounds__(GN_TPB) void gn_sums_kernel(GroupNormP p)
             };
             int64_t r = o.first + o.row;
             for (; r + (U - 1) * o.step < o.last; r += U * o.step) {
-                float v[U][V], g[U][V];
+                vec v[U], g[U];
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
-                    gn_load<E, V>(v[j], x + (r + j * o.step) * p.ldx, o.left);
-                    if constexpr (BACKWARD) gn_load<E, V>(g[j], gy + (r + j * o.step) * p.cols, o.left);
+                    v[j] = gn_read<E>(x + (r + j * o.step) * p.ldx, o.left);
+                    if constexpr (BACKWARD) g[j] = gn_read<E>(gy + (r + j * o.step) * p.cols, o.left);
                 }
 #pragma unroll
                 for (int j = 0; j < U; ++j) add(v[j], g[j]);
             }
             for (; r < o.last; r += o.step) {
-                float v[V], g[V];
-                gn_load<E, V>(v, x + r * p.ldx, o.left);
-                if constexpr (BACKWARD) gn_load<E, V>(g, gy + r * p.cols, o.left);
+                vec v = gn_read<E>(x + r * p.ldx, o.left), g = {};
+                if constexpr (BACKWARD) g = gn_read<E>(gy + r * p.cols, o.left);
                 add(v, g);
             }
         }
         __syncthreads();                    // the sums before are read
+        const int tile0 = o.tile0, n = min(p.lanes * V, p.cols - tile0);
+        if (o.on) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            red[0][threadIdx.x * V + i] = a[i];
-            red[1][threadIdx.x * V + i] = b[i];
+            for (int i = 0; i < V; ++i)
+                if (i >= o.shared && i < o.left) {
+                    red[0][o.row * p.lanes * V + o.c - tile0 + i] = a[i];
+                    red[1][o.row * p.lanes * V + o.c - tile0 + i] = b[i];
+                }
         }
         __syncthreads();
-        const int tile0 = o.c - (int)(threadIdx.x % p.lanes) * V, n = min(p.lanes * V, p.cols - tile0);
         for (int t = threadIdx.x; t < 2 * n; t += GN_TPB) {
             const int which = t >= n, c = t - which * n;
             float v = 0.f;
@@ -240,13 +272,14 @@ __global__ __launch_bounds__(GN_TPB) void gn_group_kernel(GroupNormP p)
 }
 
 // y, or dx, of a chunk of points.
-template <typename E, bool BACKWARD>
+template <typename E, bool BACKWARD, int ACT>
 __global__ __launch_bounds__(GN_TPB) void gn_apply_kernel(GroupNormP p)
 {
-    constexpr int V = fe_width<E>, U = BACKWARD ? 2 : 4;
+    constexpr int V = fe_width<E>, U = 4;
     const int64_t items = p.batch * p.chunks * p.tiles;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const GnPlace o = gn_place<V>(p, item);
+        // the last chunks first: they are the ones that the sums have left in the caches
+        const GnPlace o = gn_place<V>(p, items - 1 - item);
         if (!o.on) continue;
         const E *x = (const E *)p.x + o.sample * p.sx + o.c;
         const int64_t base = o.sample * p.points * p.cols + o.c;
@@ -261,36 +294,252 @@ __global__ __launch_bounds__(GN_TPB) void gn_apply_kernel(GroupNormP p)
                 mb[i] = p.group[2 * g + 1];
             }
         }
-        auto finish = [&](float (&v)[V], float (&g)[V], int64_t r) {
+        typedef typename fe_vec<E>::type vec;
+        auto finish = [&](vec vx, vec vg, int64_t r) {
+            float v[V], g[V];
+            gn_floats<E, V>(v, vx);
+            if constexpr (BACKWARD) gn_floats<E, V>(g, vg);
             if constexpr (BACKWARD) {
-                gn_slope<V>(p, cols, v, g);
+                gn_slope<ACT, V>(p, cols, v, g);
 #pragma unroll
                 for (int i = 0; i < V; ++i) g[i] = cols.rstd[i] * (fmaf(g[i], cols.w[i], -ma[i]) - v[i] * mb[i]);
                 gm_store<E, V>(g, (E *)p.dx + base + r * p.cols, o.left);
             } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = fmaf((v[i] - cols.mean[i]) * cols.rstd[i], cols.w[i], cols.b[i]);
-                gm_act(v, p.act, p.slope);
+                for (int i = 0; i < V; ++i) v[i] = fmaf(fmaf(v[i], cols.rstd[i], cols.mean[i]), cols.w[i], cols.b[i]);
+                gm_act(v, ACT, p.slope);
                 gm_store<E, V>(v, (E *)p.y + base + r * p.cols, o.left);
             }
         };
         int64_t r = o.first + o.row;
         for (; r + (U - 1) * o.step < o.last; r += U * o.step) {
-            float v[U][V], g[U][V];
+            vec v[U], g[U];
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                gn_load<E, V>(v[j], x + (r + j * o.step) * p.ldx, o.left);
-                if constexpr (BACKWARD) gn_load<E, V>(g[j], (const E *)p.gy + base + (r + j * o.step) * p.cols, o.left);
+                v[j] = gn_read<E>(x + (r + j * o.step) * p.ldx, o.left);
+                if constexpr (BACKWARD) g[j] = gn_read<E>((const E *)p.gy + base + (r + j * o.step) * p.cols, o.left);
             }
 #pragma unroll
             for (int j = 0; j < U; ++j) finish(v[j], g[j], r + j * o.step);
         }
         for (; r < o.last; r += o.step) {
-            float v[V], g[V];
-            gn_load<E, V>(v, x + r * p.ldx, o.left);
-            if constexpr (BACKWARD) gn_load<E, V>(g, (const E *)p.gy + base + r * p.cols, o.left);
+            vec v = gn_read<E>(x + r * p.ldx, o.left), g = {};
+            if constexpr (BACKWARD) g = gn_read<E>((const E *)p.gy + base + r * p.cols, o.left);
             finish(v, g, r);
         }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ samples that fit a workgroup's registers
+// T threads hold the points of a slab (a few whole groups) of one sample, 16 bytes in each of R registers quads a thread, so that everything is read
+// once; sums go over the threads through LDS, deviations are taken from the mean itself.  Thread t holds vector t % lanes of points t / lanes + i T / lanes.
+struct GroupHeldP { GroupNormP p; int slab, slabs, lanes; int64_t items, rows; };      // slab: channels; rows: thread groups a slab, and rows of `part`
+template <typename E, int T, int SUMS>
+constexpr int gn_held_floats() { return SUMS * (T * fe_width<E> + T) + 2 * T; }        // LDS of T threads
+
+// Sums of v over the points, [threads a channel][the slab's channels] of them to part; K: threads a channel; o: the vector, in the slab.
+template <int T, int V>
+__device__ __forceinline__ void gn_held_points(const float (&v)[V], float *red, float *part, int t, const GnVector &o, int row, int wide, int steps, int K)
+{
+    if (row < steps) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (i >= o.shared && i < o.left) red[row * wide + o.c + i] = v[i];
+    }
+    __syncthreads();
+    if (t < K * wide) {
+        const int at = t, c = at % wide, k = at / wide;
+        float sum = 0.f;
+        for (int r = k; r < steps; r += K) sum += red[r * wide + c];
+        part[at] = sum;
+    }
+}
+// Sums over the groups' channels (times w where given) to `group`, one wave a group, or one thread where groups are narrow.
+template <int T, typename F>
+__device__ __forceinline__ void gn_held_groups(const float *part, float *group, int t, int wide, int K, int width, int groups, F f)
+{
+    if (width * K <= 32) {
+        for (int g = t; g < groups; g += T) {
+            float sum = 0.f;
+            for (int c = 0; c < width; ++c)
+                for (int k = 0; k < K; ++k) sum += f(g * width + c) * part[k * wide + g * width + c];
+            group[g] = sum;
+        }
+    } else {
+        for (int g = t >> 6; g < groups; g += T / 64) {
+            float sum = 0.f;
+            for (int i = t & 63; i < width * K; i += 64) sum += f(g * width + i % width) * part[i / width * wide + g * width + i % width];
+            sum = fg_wave_sum(sum);
+            if ((t & 63) == 0) group[g] = sum;
+        }
+    }
+}
+
+template <typename E, int T, int R, bool BACKWARD>
+__global__ __launch_bounds__(T > GN_TPB ? T : GN_TPB) void gn_held_kernel(GroupHeldP h)
+{
+    typedef typename fe_vec<E>::type vec;
+    constexpr int V = fe_width<E>, TPB = T > GN_TPB ? T : GN_TPB, G = TPB / T, SUMS = BACKWARD ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const GroupNormP &p = h.p;
+    const int t = (int)threadIdx.x % T, steps = T / h.lanes, r0 = t / h.lanes;
+    float *red = lds + (threadIdx.x / T) * gn_held_floats<E, T, SUMS>(), *part = red + SUMS * T * V, *group = part + SUMS * T;
+    // neighbouring slabs run on one XCD, whose L2 holds the lines that they share
+    const int total = (int)gridDim.x, b = (int)blockIdx.x, xcd = b % FGNN_NUM_XCD, each = total / FGNN_NUM_XCD, rest = total % FGNN_NUM_XCD;
+    const int64_t place = ((int64_t)xcd * each + min(xcd, rest) + b / FGNN_NUM_XCD) * G + threadIdx.x / T;
+    const int slab = (int)(place % h.slabs), c0 = slab * h.slab, wide = min(p.cols - c0, h.slab), groups = wide / p.width, g0 = c0 / p.width, K = min(steps, T / wide);
+    const GnVector own_v = gn_vector<V>(t % h.lanes * V, wide, 0);
+    const int c = c0 + own_v.c, left = own_v.left;
+    const bool on = r0 < steps && t % h.lanes * V < wide;
+    const float inv = 1.f / ((float)p.points * (float)p.width);
+    float w[V], bias[V];
+    int in[V];                              // the channels' groups, in the slab
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int j = min(c + i, c0 + wide - 1);
+        w[i] = p.w ? fe_load(p.w, j, p.wtype) : 1.f;
+        bias[i] = p.b ? fe_load(p.b, j, p.btype) : 0.f;
+        in[i] = (j - c0) / p.width;
+    }
+    float own[2] = {0.f, 0.f};              // sums of A and B of the slab's channel t over this place's samples
+    const int64_t rounds = (p.batch + h.rows - 1) / h.rows;
+    for (int64_t round = 0; round < rounds; ++round) {
+        const int64_t sample = place / h.slabs + round * h.rows;
+        // (formed again in every round, and before the results: offsets of all points kept over the loop would take the registers of as many points)
+        int at = r0;
+        asm volatile("" : "+v"(at));
+        const bool there = sample < p.batch && place / h.slabs < h.rows;
+        const E *x = (const E *)p.x + sample * p.sx + c;
+        int64_t base = sample * p.points * p.cols + c;
+        const int points = there && on ? (int)p.points : 0;
+        vec vx[R], vg[BACKWARD ? R : 1];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            const int r = at + i * steps;
+            vx[i] = vec{};
+            if constexpr (BACKWARD) vg[i] = vec{};
+            if (r < points) {
+                vx[i] = gn_read<E>(x + r * p.ldx, left);
+                if constexpr (BACKWARD) vg[i] = gn_read<E>((const E *)p.gy + base + (int64_t)r * p.cols, left);
+            }
+        }
+        asm volatile("" : "+v"(base), "+v"(at));
+        if constexpr (!BACKWARD) {
+            float mean[V], rstd[V];
+#pragma unroll
+            for (int pass = 0; pass < 2; ++pass) {
+                float sum[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+                    if (at + i * steps < points) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            const float v = (float)vx[i][j] - (pass ? mean[j] : 0.f);
+                            sum[j] = pass ? fmaf(v, v, sum[j]) : sum[j] + v;
+                        }
+                    }
+                __syncthreads();            // the sums before are read
+                gn_held_points<T, V>(sum, red, part, t, own_v, on ? r0 : steps, wide, steps, K);
+                __syncthreads();
+                gn_held_groups<T>(part, group, t, wide, K, p.width, groups, [](int) { return 1.f; });
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float v = group[in[j]] * inv;
+                    if (pass) rstd[j] = 1.f / sqrtf(v + p.eps);
+                    else mean[j] = v;
+                }
+                if (there)
+                    for (int g = t; g < groups; g += T) {
+                        const float v = group[g] * inv;
+                        if (pass) p.rstd[sample * p.groups + g0 + g] = 1.f / sqrtf(v + p.eps);
+                        else p.mean[sample * p.groups + g0 + g] = v;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int r = at + i * steps;
+                if (r < points) {
+                    float v[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[j] = fmaf(((float)vx[i][j] - mean[j]) * rstd[j], w[j], bias[j]);
+                    gm_act(v, p.act, p.slope);
+                    gm_store<E, V>(v, (E *)p.y + base + (int64_t)r * p.cols, left);
+                }
+            }
+        } else {
+            GnCols<V> cols;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int64_t g = (there ? sample : 0) * p.groups + g0 + in[j];
+                cols.rstd[j] = p.rstd[g];
+                cols.mean[j] = -p.mean[g] * cols.rstd[j];
+                cols.w[j] = w[j];
+                cols.b[j] = bias[j];
+            }
+            float sum[2][V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[0][j] = sum[1][j] = 0.f;
+            auto terms = [&](int i, float (&u)[V], float (&d)[V]) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    u[j] = (float)vx[i][j];
+                    d[j] = (float)vg[i][j];
+                }
+                gn_slope<GN_ANY, V>(p, cols, u, d);
+            };
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                __builtin_amdgcn_sched_barrier(0);      // one point's terms at a time: the registers are full of points
+                if (at + i * steps < points) {
+                    float u[V], d[V];
+                    terms(i, u, d);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        sum[0][j] += d[j];
+                        sum[1][j] = fmaf(d[j], u[j], sum[1][j]);
+                    }
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) gn_held_points<T, V>(sum[k], red + k * T * V, part + k * T, t, own_v, on ? r0 : steps, wide, steps, K);
+            __syncthreads();
+            const auto weight = [&](int j) { return p.w ? fe_load(p.w, c0 + j, p.wtype) : 1.f; };
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                gn_held_groups<T>(part + k * T, group + k * T, t, wide, K, p.width, groups, weight);
+                if (t < wide)
+                    for (int i = 0; i < K; ++i) own[k] += part[k * T + i * wide + t];
+            }
+            __syncthreads();
+            float ma[V], mb[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                ma[j] = group[in[j]] * inv;
+                mb[j] = group[T + in[j]] * inv;
+            }
+            if (p.dx) {
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int r = at + i * steps;
+                    if (r < points) {
+                        float u[V], d[V];
+                        terms(i, u, d);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d[j] = cols.rstd[j] * (fmaf(d[j], cols.w[j], -ma[j]) - u[j] * mb[j]);
+                        gm_store<E, V>(d, (E *)p.dx + base + (int64_t)r * p.cols, left);
+                    }
+                }
+            }
+        }
+    }
+    if (BACKWARD && place / h.slabs < h.rows && t < wide) {
+        p.sums[(place / h.slabs * 2) * p.cols + c0 + t] = own[0];
+        p.sums[(place / h.slabs * 2 + 1) * p.cols + c0 + t] = own[1];
     }
 }
 
@@ -329,6 +578,70 @@ static void gn_cut(GroupNormP &p, int type)
     p.rows = std::max<int64_t>({(p.points + wanted - 1) / wanted, 8 * step, 1});
     p.chunks = (int)((p.points + p.rows - 1) / p.rows);
 }
+// Whether a sample's slab fits a workgroup: slabs are whole groups, 128 bytes (a cache line) of a point where that fits and more where a wave would hold little, no more
+// channels than threads.  T, R: threads and vectors a thread, 0 where nothing fits.
+struct GnHeld { GroupHeldP h; int T, R, grid; };
+template <typename Fn>
+static void gn_held_shape(int T, int R, Fn &&f)
+{
+    if (T == 64) {
+        if (R == 1) f.template operator()<64, 1>();
+        else f.template operator()<64, 4>();
+    } else if (T == 256) {
+        if (R == 2) f.template operator()<256, 2>();
+        else if (R == 4) f.template operator()<256, 4>();
+        else f.template operator()<256, 8>();
+    } else if (R == 8) f.template operator()<512, 8>();
+    else if (R == 16) f.template operator()<512, 16>();
+    else f.template operator()<512, 18>();
+}
+static GnHeld gn_held(const GroupNormP &p, int type)
+{
+    GnHeld o = {};
+    const int v = 16 / fe_size(type), width = p.cols / p.groups;
+    if (width > 512 || p.points > 18 * 512) return o;
+    const auto lanes = [&](int groups) { return ((int64_t)groups * width + v - 1) / v; };
+    // vectors a thread, for T threads: the points that they hold at a time are whole
+    const auto deep = [&](int groups, int T) { return lanes(groups) > T ? (int64_t)1 << 30 : (p.points + T / lanes(groups) - 1) / (T / lanes(groups)); };
+    int n = (int)std::min<int64_t>(p.groups, (128 / fe_size(type) + width - 1) / width);
+    while (n > 1 && (n * width > 512 || deep(n, 512) > 18)) --n;
+    if (deep(n, 512) > 18) return o;
+    while (2 * n <= p.groups && 2 * n * width <= 64 && deep(2 * n, 64) <= 1) n *= 2;
+    const int64_t d64 = n * width <= 64 ? deep(n, 64) : 1 << 30, d256 = n * width <= 256 ? deep(n, 256) : 1 << 30, d512 = deep(n, 512);
+    o.T = d64 <= 4 ? 64 : d256 <= 8 ? 256 : 512;
+    o.R = o.T == 64 ? (d64 <= 1 ? 1 : 4) : o.T == 256 ? (d256 <= 2 ? 2 : d256 <= 4 ? 4 : 8) : d512 <= 8 ? 8 : d512 <= 16 ? 16 : 18;
+    o.h.slab = n * width;
+    o.h.slabs = (p.groups + n - 1) / n;
+    o.h.lanes = (int)lanes(n);
+    // every place keeps its slab: as many workgroups as give each slab the same number of places, four times what the device holds at the most
+    const int G = std::max(1, GN_TPB / o.T), cus = fgnn_current_device_compute_units();
+    const int64_t wanted = (int64_t)(cus > 0 ? cus : 256) * (o.T == 512 ? 4 : 16) * G;
+    o.h.rows = std::max<int64_t>(1, std::min<int64_t>(p.batch, wanted / o.h.slabs));
+    o.grid = (int)((o.h.rows * o.h.slabs + G - 1) / G);
+    return o;
+}
+template <bool BACKWARD>
+static void gn_held_launch(GnHeld &o, const GroupNormP &p, int type, hipStream_t st)
+{
+    o.h.p = p;
+    o.h.p.width = p.cols / p.groups;
+    fe_dispatch(type, [&]<typename E>() {
+        gn_held_shape(o.T, o.R, [&]<int T, int R>() {
+            constexpr int G = std::max(1, GN_TPB / T), SUMS = BACKWARD ? 2 : 1;
+            constexpr size_t bytes = G * gn_held_floats<E, T, SUMS>() * sizeof(float);
+            hipLaunchKernelGGL((gn_held_kernel<E, T, R, BACKWARD>), dim3(o.grid), dim3(std::max(T, GN_TPB)), bytes, st, o.h);
+        });
+    });
+}
+template <typename Fn>
+static void gn_act(int act, Fn &&f)
+{
+    if (act == GM_RELU) f.template operator()<GM_RELU>();
+    else if (act == GM_GELU) f.template operator()<GM_GELU>();
+    else if (act == GM_SILU) f.template operator()<GM_SILU>();
+    else if (act == GM_LEAKY) f.template operator()<GM_LEAKY>();
+    else f.template operator()<GM_NONE>();
+}
 static unsigned gn_grid(int64_t items) { return (unsigned)std::min<int64_t>(items, GN_GRID); }
 
 static int gn_check(const char *who, int64_t batch, int64_t points, int cols, int groups, int type, const void *x, int64_t ldx, int64_t sx, const void *w, int wtype, const void *b,
@@ -352,6 +665,8 @@ static size_t gn_workspace(int64_t batch, int64_t points, int cols, int groups, 
     if (batch < 1 || points < 1 || cols < 1 || groups < 1 || !fe_is_float(type)) return 0;
     GroupNormP p = {};
     p.batch = batch; p.points = points; p.cols = cols; p.groups = groups;
+    const GnHeld held = gn_held(p, type);
+    if (held.T) return backward ? fgnn_align256((size_t)held.h.rows * 2 * cols * sizeof(float)) : 0;
     gn_cut(p, type);
     return gn_part_bytes(p) + (backward ? gn_sums_bytes(p) + fgnn_align256((size_t)batch * groups * 2 * sizeof(float)) : 0);
 }
@@ -366,15 +681,20 @@ extern "C" int fgnn_group_norm(int64_t batch, int64_t points, int cols, int grou
     if (batch == 0 || points == 0) return 0;
     FGNN_REQUIRE(y && mean && rstd, FGNN_ERR_NULL, "fgnn_group_norm: NULL argument");
     GroupNormP p = {batch, points, cols, groups, 0, x, ldx, sx, weight, bias, wtype, btype, eps, slope, act, y, mean, rstd};
+    hipStream_t st = (hipStream_t)stream;
+    GnHeld held = gn_held(p, type);
+    if (held.T) {
+        gn_held_launch<false>(held, p, type, st);
+        return fgnn_launch_status("gn_held_kernel");
+    }
     gn_cut(p, type);
     FGNN_REQUIRE(workspace && workspace_bytes >= gn_workspace(batch, points, cols, groups, type, 0), FGNN_ERR_WORKSPACE, "fgnn_group_norm: workspace of %zu bytes", workspace_bytes);
-    hipStream_t st = (hipStream_t)stream;
     p.part = (float *)workspace;
     const unsigned grid = gn_grid(batch * p.chunks * p.tiles);
     fe_dispatch(type, [&]<typename E>() {
-        hipLaunchKernelGGL((gn_sums_kernel<E, false>), dim3(grid), dim3(GN_TPB), 0, st, p);
+        hipLaunchKernelGGL((gn_sums_kernel<E, false, GM_NONE>), dim3(grid), dim3(GN_TPB), 0, st, p);
         hipLaunchKernelGGL((gn_stats_kernel<E>), dim3(gn_grid(batch * groups)), dim3(GN_TPB), 0, st, p);
-        hipLaunchKernelGGL((gn_apply_kernel<E, false>), dim3(grid), dim3(GN_TPB), 0, st, p);
+        gn_act(act, [&]<int ACT>() { hipLaunchKernelGGL((gn_apply_kernel<E, false, ACT>), dim3(grid), dim3(GN_TPB), 0, st, p); });
     });
     return fgnn_launch_status("gn_apply_kernel");
 }
@@ -387,6 +707,7 @@ extern "C" int fgnn_group_norm_backward(int64_t batch, int64_t points, int cols,
     if (rc) return rc;
     hipStream_t st = (hipStream_t)stream;
     const bool empty = batch == 0 || points == 0;
+    int64_t rows = empty ? 0 : batch;       // of the sums of dw and db
     GroupNormP p = {batch, points, cols, groups, 0, x, ldx, sx, weight, bias, wtype, btype, 0.f, slope, act, nullptr, const_cast<float *>(mean), const_cast<float *>(rstd), gy, dx};
     if (!weight) p.wtype = type;
     if (!bias) p.btype = type;
@@ -394,21 +715,28 @@ extern "C" int fgnn_group_norm_backward(int64_t batch, int64_t points, int cols,
         FGNN_REQUIRE(gy && mean && rstd, FGNN_ERR_NULL, "fgnn_group_norm_backward: NULL argument");
         FGNN_REQUIRE(workspace && workspace_bytes >= gn_workspace(batch, points, cols, groups, type, 1), FGNN_ERR_WORKSPACE, "fgnn_group_norm_backward: workspace of %zu bytes",
                      workspace_bytes);
-        gn_cut(p, type);
-        p.part = (float *)workspace;
-        p.sums = (float *)((char *)workspace + gn_part_bytes(p));
-        p.group = (float *)((char *)p.sums + gn_sums_bytes(p));
-        const unsigned grid = gn_grid(batch * p.chunks * p.tiles);
-        fe_dispatch(type, [&]<typename E>() {
-            hipLaunchKernelGGL((gn_sums_kernel<E, true>), dim3(grid), dim3(GN_TPB), 0, st, p);
-            hipLaunchKernelGGL(gn_group_kernel, dim3(gn_grid(batch * groups)), dim3(GN_TPB), 0, st, p);
-            if (dx) hipLaunchKernelGGL((gn_apply_kernel<E, true>), dim3(grid), dim3(GN_TPB), 0, st, p);
-        });
+        GnHeld held = gn_held(p, type);
+        if (held.T) {
+            p.sums = (float *)workspace;
+            rows = held.h.rows;
+            gn_held_launch<true>(held, p, type, st);
+        } else {
+            gn_cut(p, type);
+            p.part = (float *)workspace;
+            p.sums = (float *)((char *)workspace + gn_part_bytes(p));
+            p.group = (float *)((char *)p.sums + gn_sums_bytes(p));
+            const unsigned grid = gn_grid(batch * p.chunks * p.tiles);
+            fe_dispatch(type, [&]<typename E>() {
+                gn_act(act, [&]<int ACT>() { hipLaunchKernelGGL((gn_sums_kernel<E, true, ACT>), dim3(grid), dim3(GN_TPB), 0, st, p); });
+                hipLaunchKernelGGL(gn_group_kernel, dim3(gn_grid(batch * groups)), dim3(GN_TPB), 0, st, p);
+                if (dx) gn_act(act, [&]<int ACT>() { hipLaunchKernelGGL((gn_apply_kernel<E, true, ACT>), dim3(grid), dim3(GN_TPB), 0, st, p); });
+            });
+        }
         const int launched = fgnn_launch_status("gn_apply_kernel");
         if (launched) return launched;
     }
     if (dweight || dbias) {
-        hipLaunchKernelGGL(gn_weights_kernel, dim3(gn_grid(2 * (((int64_t)cols + 15) / 16))), dim3(1024), 0, st, p.sums, empty ? 0 : batch, cols, dweight, p.wtype, dbias, p.btype);
+        hipLaunchKernelGGL(gn_weights_kernel, dim3(gn_grid(2 * (((int64_t)cols + 15) / 16))), dim3(1024), 0, st, p.sums, rows, cols, dweight, p.wtype, dbias, p.btype);
         return fgnn_launch_status("gn_weights_kernel");
     }
     return 0;
