@@ -35,12 +35,9 @@ template <typename E> constexpr int at_tile = sizeof(E) == 4 ? 32 : 64;
 
 // 16-byte chunk `ch` of row `row` in a tile of ROW bytes a row.  Chunks are exchanged so that both ways of reading meet different banks: eight rows at one
 // chunk, and four rows at two neighbouring chunks.
+template <int ROW> __host__ __device__ constexpr int at_exchange(int row) { return ROW % 128 ? (row >> 1) & 3 : (row & 3) << 1 | ((row >> 2) & 1); }
 template <int ROW>
-__device__ __forceinline__ int at_place(int row, int ch)
-{
-    const int f = ROW % 128 ? (row >> 1) & 3 : (row & 3) << 1 | ((row >> 2) & 1);
-    return row * ROW + ((ch ^ f) << 4);
-}
+__device__ __forceinline__ int at_place(int row, int ch) { return row * ROW + ((ch ^ at_exchange<ROW>(row)) << 4); }
 
 template <typename E>
 __device__ __forceinline__ at_f16 at_multiply(gm_i4 a, gm_i4 b, at_f16 c)
@@ -102,28 +99,69 @@ __device__ __forceinline__ void at_gather(const char *tile, int row0, const floa
     }
 }
 
-// A tile on its way from memory to LDS.  Rows that are not wanted (bit not set) and components past the last are zeros: out of the buffer's range.
-template <typename E, int ROWS, int DP, int THREADS>
-struct AtLoader {
-    static constexpr int SIZE = (int)sizeof(E), CH = DP * SIZE / 16, COUNT = ROWS * CH / THREADS;
-    static_assert(ROWS * CH % THREADS == 0, "threads share a tile evenly");
-    gm_i4 w[COUNT];
-    __device__ __forceinline__ void fetch(const E *base, int64_t stride, uint64_t bits, int dim)
+// Two tiles (keys and values, or queries and their gradients) on their way to LDS, one pair ahead of the one that is worked on.  Rows that are not wanted (bit not
+// set) and components past the last are zeros: out of the buffer's range.
+template <typename E, int ROWS, int DP, int WAVES>
+struct AtFeed {
+    static constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, CH = ROW / 16, THREADS = 64 * WAVES, TILE = ROWS * ROW;
+    static constexpr bool MOVED = SIZE == 2;                    // straight to LDS, into two places in turn; else through registers
+    static constexpr int COUNT = ROWS * CH / THREADS, STEP = THREADS / CH;          // chunks a thread, and rows between them
+    static constexpr int BYTES = (MOVED ? 2 : 1) * 2 * TILE;
+    static_assert(ROWS * CH % THREADS == 0 && THREADS % CH == 0, "threads share a tile evenly");
+    char *lds; int row, ch, left;           // left: components from the first chunk on
+    gm_i4 w[MOVED ? 1 : 2][MOVED ? 1 : COUNT];
+
+    __device__ __forceinline__ void init(char *lds_, int dim)
     {
-        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, 0x80000000u, 0x00027000);
+        lds = lds_;
+        row = (int)threadIdx.x / CH;
+        ch = (int)threadIdx.x % CH;
+        if constexpr (MOVED) ch ^= at_exchange<ROW>(row);       // the chunk that belongs where the thread's first transfer ends
+        left = dim;
+    }
+    // The pair `index` from a and b on.
+    __device__ __forceinline__ void start(int index, const void *a, const void *b, int64_t stride_a, int64_t stride_b, uint64_t bits)
+    {
+        constexpr uint64_t ALL = ROWS == 64 ? ~0ull : (1ull << ROWS) - 1;
 #pragma unroll
-        for (int c = 0; c < COUNT; ++c) {
-            const int pos = c * THREADS + (int)threadIdx.x, row = pos / CH, ch = pos % CH;
-            const bool there = ((bits >> row) & 1) && ch * (16 / SIZE) < dim;
-            w[c] = __builtin_amdgcn_raw_buffer_load_b128(from, there ? (uint32_t)row * (uint32_t)(stride * SIZE) + ch * 16 : 0x80000000u, 0, 0);
+        for (int which = 0; which < 2; ++which) {
+            const void *base = which ? b : a;
+            const uint32_t step = (uint32_t)((which ? stride_b : stride_a) * SIZE);
+            auto at = [&](int c) {
+                // (rows of a thread are a power of two apart: what is exchanged changes by a constant)
+                const int chunk = MOVED ? ch ^ at_exchange<ROW>(c * STEP) : ch;
+                const bool there = (bits == ALL || ((bits >> (row + c * STEP)) & 1)) && chunk * (16 / SIZE) < left;
+                return there ? (row + c * STEP) * step + chunk * 16 : 0x80000000u;
+            };
+            if constexpr (MOVED) {
+                // (written out, and its waits with it: see GemmMover)
+                const uint64_t from = (uint64_t)base;
+                const gm_i4 buffer = {(int)(uint32_t)from, (int)((uint32_t)(from >> 32) & 0xffffu), (int)0x80000000u, 0x00027000};
+                const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + ((index & 1) * 2 + which) * TILE + fg_wave() * 1024;
+#pragma unroll
+                for (int c = 0; c < COUNT; ++c)
+                    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at(c)), "s"(buffer), "{m0}"(to + c * THREADS * 16));
+            } else {
+                const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, 0x80000000u, 0x00027000);
+#pragma unroll
+                for (int c = 0; c < COUNT; ++c) w[which][c] = __builtin_amdgcn_raw_buffer_load_b128(from, at(c), 0, 0);
+            }
         }
     }
-    __device__ __forceinline__ void store(char *tile) const
+    // The pair `index` has arrived, and nobody reads the one before any more.
+    __device__ __forceinline__ const char *arrive(int index)
     {
+        if constexpr (MOVED) {
+            gm_arrive<0>();
+            return lds + (index & 1) * 2 * TILE;
+        } else {
+            __syncthreads();
 #pragma unroll
-        for (int c = 0; c < COUNT; ++c) {
-            const int pos = c * THREADS + (int)threadIdx.x;
-            *reinterpret_cast<gm_i4 *>(tile + at_place<DP * SIZE>(pos / CH, pos % CH)) = w[c];
+            for (int which = 0; which < 2; ++which)
+#pragma unroll
+                for (int c = 0; c < COUNT; ++c) *reinterpret_cast<gm_i4 *>(lds + which * TILE + at_place<ROW>(row + c * STEP, ch)) = w[which][c];
+            __syncthreads();
+            return lds;
         }
     }
 };
@@ -242,15 +280,12 @@ __device__ __forceinline__ void at_store(const at_f16 (&acc)[DP / 32], E *row, i
         }
 }
 
-constexpr int at_lds(int dim, int size, int rows) { return 2 * rows * dim * size; }
-
 // Y and lse.  With `splits` parts of the keys, normalised sums and lse of each to `part`.
 template <typename E, int DP, int WAVES, int TILE>
 __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_kernel(AttentionP p)
 {
     constexpr int ROW = DP * (int)sizeof(E);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *lk = lds, *lv = lds + TILE * ROW;
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
     int pos, sub;
@@ -267,25 +302,22 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) acc[t] = at_f16{};
     float most = -__builtin_inff(), sum = 0.f;
-    AtLoader<E, TILE, DP, 64 * WAVES> fk, fv;
+    AtFeed<E, TILE, DP, WAVES> feed;
+    feed.init(lds, p.dim);
     seen.ask(first);
     uint64_t bits = seen.take(first), coming = 0;
     if (first < last) {
-        fk.fetch(k + first * p.kn, p.kn, bits, p.dim);
-        fv.fetch(v + first * p.vn, p.vn, bits, p.dim);
         seen.ask(first + TILE);
+        feed.start(0, k + first * p.kn, v + first * p.vn, p.kn, p.vn, bits);
     }
+    int index = 0;
 #pragma unroll 1
-    for (int64_t key = first; key < last; key += TILE, bits = coming) {
-        __syncthreads();                    // the tile before has been read
-        fk.store(lk);
-        fv.store(lv);
-        __syncthreads();
+    for (int64_t key = first; key < last; key += TILE, bits = coming, ++index) {
+        const char *lk = feed.arrive(index), *lv = lk + TILE * ROW;
         if (key + TILE < last) {
             coming = seen.take(key + TILE);
-            fk.fetch(k + (key + TILE) * p.kn, p.kn, coming, p.dim);
-            fv.fetch(v + (key + TILE) * p.vn, p.vn, coming, p.dim);
             seen.ask(key + 2 * TILE);
+            feed.start(index + 1, k + (key + TILE) * p.kn, v + (key + TILE) * p.vn, p.kn, p.vn, coming);
         }
         if (bits == 0) continue;
         at_f16 s[TILE / 32];
@@ -347,7 +379,6 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 {
     constexpr int ROW = DP * (int)sizeof(E);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *lk = lds, *lv = lds + TILE * ROW;
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
     int pos, sub;
@@ -367,25 +398,22 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     at_f16 acc[DP / 32];
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) acc[t] = at_f16{};
-    AtLoader<E, TILE, DP, 64 * WAVES> fk, fv;
+    AtFeed<E, TILE, DP, WAVES> feed;
+    feed.init(lds, p.dim);
     seen.ask(first);
     uint64_t bits = seen.take(first), coming = 0;
     if (first < last) {
-        fk.fetch(k + first * p.kn, p.kn, bits, p.dim);
-        fv.fetch(v + first * p.vn, p.vn, bits, p.dim);
         seen.ask(first + TILE);
+        feed.start(0, k + first * p.kn, v + first * p.vn, p.kn, p.vn, bits);
     }
+    int index = 0;
 #pragma unroll 1
-    for (int64_t key = first; key < last; key += TILE, bits = coming) {
-        __syncthreads();
-        fk.store(lk);
-        fv.store(lv);
-        __syncthreads();
+    for (int64_t key = first; key < last; key += TILE, bits = coming, ++index) {
+        const char *lk = feed.arrive(index), *lv = lk + TILE * ROW;
         if (key + TILE < last) {
             coming = seen.take(key + TILE);
-            fk.fetch(k + (key + TILE) * p.kn, p.kn, coming, p.dim);
-            fv.fetch(v + (key + TILE) * p.vn, p.vn, coming, p.dim);
             seen.ask(key + 2 * TILE);
+            feed.start(index + 1, k + (key + TILE) * p.kn, v + (key + TILE) * p.vn, p.kn, p.vn, coming);
         }
 #pragma unroll
         for (int t = 0; t < TILE / 32; ++t) {
@@ -420,8 +448,8 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
 {
     constexpr int ROW = DP * (int)sizeof(E), STEPS = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *lq = lds, *lg = lds + TILE * ROW;
-    float *stats = (float *)(lds + 2 * TILE * ROW);             // lse, delta of the tile's rows
+    typedef AtFeed<E, TILE, DP, WAVES> Feed;
+    float *stats = (float *)(lds + Feed::BYTES);                // lse, delta of the tile's rows, two tiles in turn
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), key = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
     AtSeen<64> seen;
@@ -438,26 +466,24 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
 #pragma unroll
     for (int t = 0; t < STEPS; ++t) dk[t] = dv[t] = at_f16{};
     AtRange<E, STEPS> range;
-    AtLoader<E, TILE, DP, 64 * WAVES> fq, fg;
+    Feed feed;
+    feed.init(lds, p.dim);
     float stat = 0.f;
     auto fetch = [&](int i) {
         const int sub = i / per_head, pos = (i - sub * per_head) * TILE, head = o.head * p.share + sub, left = p.nq - pos;
         const uint64_t bits = left >= TILE ? (TILE == 64 ? ~0ull : (1ull << TILE) - 1) : (1ull << left) - 1;
-        fq.fetch((const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, p.qn, bits, p.dim);
-        fg.fetch((const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, p.gn, bits, p.dim);
         // rows past the last weigh nothing
         const int r = (int)threadIdx.x % TILE, which = (int)threadIdx.x / TILE;
         if (which < 2) stat = r < left ? (which ? p.delta : p.lse)[((int64_t)o.b * p.heads + head) * p.nq + pos + r] - (which ? 0.f : at_lift<E>) : which ? 0.f : __builtin_inff();
+        feed.start(i - first, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, p.qn, p.gn, bits);
     };
     static_assert(64 * WAVES >= 2 * TILE, "a thread for every row's lse and delta");
     if (first < last) fetch(first);
 #pragma unroll 1
     for (int i = first; i < last; ++i) {
-        __syncthreads();
-        fq.store(lq);
-        fg.store(lg);
-        if (threadIdx.x < 2 * TILE) stats[threadIdx.x] = stat;
-        __syncthreads();
+        float *own = stats + ((i - first) & 1) * 2 * TILE;
+        if (threadIdx.x < 2 * TILE) own[threadIdx.x] = stat;
+        const char *lq = feed.arrive(i - first), *lg = lq + TILE * ROW;
         if (i + 1 < last) fetch(i + 1);
         if (!any) continue;
 #pragma unroll
@@ -466,8 +492,8 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
             float w[16], ds[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const gm_f4 lse = *reinterpret_cast<const gm_f4 *>(stats + 32 * t + 8 * j + 4 * (lane >> 5)),
-                            delta = *reinterpret_cast<const gm_f4 *>(stats + TILE + 32 * t + 8 * j + 4 * (lane >> 5));
+                const gm_f4 lse = *reinterpret_cast<const gm_f4 *>(own + 32 * t + 8 * j + 4 * (lane >> 5)),
+                            delta = *reinterpret_cast<const gm_f4 *>(own + TILE + 32 * t + 8 * j + 4 * (lane >> 5));
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     w[4 * j + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + c], p.log2_scale, -lse[c]));
@@ -504,14 +530,18 @@ template <typename E, int DP>
 static void at_launch_dim(int what, const AtShape &s, const AttentionP &p, unsigned grid, hipStream_t st)
 {
     constexpr int T = at_tile<E>;
-    const size_t lds = at_lds(DP, (int)sizeof(E), s.tile);
-    if (what == AT_DKV) hipLaunchKernelGGL((attention_dkv_kernel<E, DP, 4, T, 1>), dim3(grid), dim3(256), lds + 2 * T * sizeof(float), st, p);
-    else if (what == AT_DQ) {
-        if (s.waves == 4) hipLaunchKernelGGL((attention_dq_kernel<E, DP, 4, T>), dim3(grid), dim3(256), lds, st, p);
-        else hipLaunchKernelGGL((attention_dq_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), lds, st, p);
+    if (what == AT_DKV) {
+        constexpr int bytes = AtFeed<E, T, DP, 4>::BYTES + 4 * T * (int)sizeof(float);
+        hipLaunchKernelGGL((attention_dkv_kernel<E, DP, 4, T, 1>), dim3(grid), dim3(256), bytes, st, p);
+        return;
+    }
+    constexpr int many = AtFeed<E, T, DP, 4>::BYTES, one = AtFeed<E, 32, DP, 1>::BYTES;
+    if (s.waves == 4) {
+        if (what == AT_DQ) hipLaunchKernelGGL((attention_dq_kernel<E, DP, 4, T>), dim3(grid), dim3(256), many, st, p);
+        else hipLaunchKernelGGL((attention_kernel<E, DP, 4, T>), dim3(grid), dim3(256), many, st, p);
     } else {
-        if (s.waves == 4) hipLaunchKernelGGL((attention_kernel<E, DP, 4, T>), dim3(grid), dim3(256), lds, st, p);
-        else hipLaunchKernelGGL((attention_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), lds, st, p);
+        if (what == AT_DQ) hipLaunchKernelGGL((attention_dq_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), one, st, p);
+        else hipLaunchKernelGGL((attention_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), one, st, p);
     }
 }
 template <typename E>
