@@ -33,11 +33,45 @@ template <typename E> struct AtKind { static constexpr int V = fe_width<E>, SIZE
 // Rows of a tile that lies in LDS.
 template <typename E> constexpr int at_tile = sizeof(E) == 4 ? 32 : 64;
 
-// 16-byte chunk `ch` of row `row` in a tile of ROW bytes a row.  Chunks are exchanged so that both ways of reading meet different banks: eight rows at one
-// chunk, and four rows at two neighbouring chunks.
-template <int ROW> __host__ __device__ constexpr int at_exchange(int row) { return ROW % 128 ? (row >> 1) & 3 : (row & 3) << 1 | ((row >> 2) & 1); }
-template <int ROW>
-__device__ __forceinline__ int at_place(int row, int ch) { return row * ROW + ((ch ^ at_exchange<ROW>(row)) << 4); }
+// 16-byte chunk `ch` of row `row` in a tile of ROW bytes a row.  LDS has 64 banks of four bytes: chunks are exchanged so that the reads meet each of them once, sixteen rows at
+// one chunk, and four rows at four chunks next to one another (16-bit types) or two rows, four apart, at eight (fp32).  What is exchanged is linear in the row's bits.
+template <int ROW, int SIZE>
+__host__ __device__ constexpr int at_exchange(int row)
+{
+    if (ROW % 128) return (row >> 2) & 3;
+    if (ROW % 256) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+    if (SIZE == 4) return ((row >> 2) & 1) << 3 | (row & 3) << 1 | ((row >> 3) & 1);
+    return (row & 3) << 2 | ((row >> 2) & 3);
+}
+template <int ROW, int SIZE>
+__device__ __forceinline__ int at_place(int row, int ch) { return row * ROW + ((ch ^ at_exchange<ROW, SIZE>(row)) << 4); }
+
+// Where a lane reads tiles of DP components: for scores its row's chunks 2 j + (lane / 32), for the transposed tile what the reads below say.  Of the exchanged chunk index the
+// upper bits are the constant's own, so that a few places and constant offsets from them give all of them.
+template <typename E, int DP>
+struct AtReader {
+    static constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, MASK = ROW % 128 ? 3 : ROW % 256 ? 7 : 15;     // exchanged bits of the chunk index
+    static constexpr int S = std::min((MASK + 1) / 2, ROW / 32);
+    static constexpr int G = SIZE == 4 ? std::min(2, DP / 32) : std::min((MASK + 1) / 4, DP / 32);
+    int score[S], gather[SIZE == 4 ? 4 : 1][G];
+    __device__ __forceinline__ void init(int lane)
+    {
+        const int f = at_exchange<ROW, SIZE>(lane & 31), h = lane >> 5;
+#pragma unroll
+        for (int j = 0; j < S; ++j) score[j] = (lane & 31) * ROW + (((2 * j + h) ^ f) << 4);
+        if constexpr (SIZE == 4) {
+            // row 4 h + i, component lane % 32: chunk 8 t + (lane % 32) / 4
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < G; ++t) gather[i][t] = at_place<ROW, SIZE>(4 * h + i, 8 * t + ((lane & 31) >> 2)) + (lane & 3) * 4;
+        } else {
+            const int r = lane & 15;
+#pragma unroll
+            for (int t = 0; t < G; ++t) gather[0][t] = at_place<ROW, SIZE>(4 * h + (r >> 2), 4 * t + 2 * ((lane >> 4) & 1) + ((r & 3) >> 1)) + (r & 1) * 8;
+        }
+    }
+};
 
 template <typename E>
 __device__ __forceinline__ at_f16 at_multiply(gm_i4 a, gm_i4 b, at_f16 c)
@@ -50,34 +84,35 @@ __device__ __forceinline__ at_f16 at_multiply(gm_i4 a, gm_i4 b, at_f16 c)
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(gm_b8 *)&a, *(gm_b8 *)&b, c, 0, 0, 0);
 }
 
-// The scores of 32 rows of a tile (from row0 on) with the wave's columns.
+// The scores of 32 rows of a tile (from row0 on, a multiple of 32) with the wave's columns.
 template <typename E, int DP>
-__device__ __forceinline__ at_f16 at_scores(const char *tile, int row0, const gm_i4 (&cols)[DP * (int)sizeof(E) / 32], int lane)
+__device__ __forceinline__ at_f16 at_scores(const AtReader<E, DP> &at, const char *tile, int row0, const gm_i4 (&cols)[DP * (int)sizeof(E) / 32])
 {
-    constexpr int ROW = DP * (int)sizeof(E);
+    typedef AtReader<E, DP> R;
     at_f16 s = {};
 #pragma unroll
-    for (int j = 0; j < ROW / 32; ++j) s = at_multiply<E>(*reinterpret_cast<const gm_i4 *>(tile + at_place<ROW>(row0 + (lane & 31), 2 * j + (lane >> 5))), cols[j], s);
+    for (int j = 0; j < R::ROW / 32; ++j)
+        s = at_multiply<E>(*reinterpret_cast<const gm_i4 *>(tile + at.score[j % R::S] + row0 * R::ROW + j / R::S * (2 * R::S * 16)), cols[j], s);
     return s;
 }
 
 // acc[t] (32 components from 32 t on, by the wave's columns) += (32 rows of a tile, from row0 on)^T w
 template <typename E, int DP>
-__device__ __forceinline__ void at_gather(const char *tile, int row0, const float (&w)[16], at_f16 (&acc)[DP / 32], int lane)
+__device__ __forceinline__ void at_gather(const AtReader<E, DP> &at, const char *tile, int row0, const float (&w)[16], at_f16 (&acc)[DP / 32])
 {
-    constexpr int ROW = DP * (int)sizeof(E);
+    typedef AtReader<E, DP> R;
     if constexpr (sizeof(E) == 4) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int row = row0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+            // (rows 8 and more apart: of what is exchanged only row 8's bit changes with them)
+            const int row = 8 * (i / 4), flip = at_exchange<R::ROW, 4>(row) << 4;
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t) {
-                const float a = *reinterpret_cast<const float *>(tile + at_place<ROW>(row, 8 * t + ((lane & 31) >> 2)) + (lane & 3) * 4);
+                const float a = *reinterpret_cast<const float *>(tile + (at.gather[i % 4][t % R::G] ^ flip) + (row0 + row) * R::ROW + t / R::G * (8 * R::G * 16));
                 acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[i], acc[t], 0, 0, 0);
             }
         }
     } else {
-        const int r = lane & 15;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             typedef E e8 __attribute__((ext_vector_type(8)));
@@ -86,12 +121,14 @@ __device__ __forceinline__ void at_gather(const char *tile, int row0, const floa
             for (int i = 0; i < 8; ++i) b[i] = (E)w[8 * s + i];
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t) {
-                // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
+                // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each.  (Rows 8 further on: the exchange's second bit
+                // of two changes, where it is the row's fourth.)
                 typedef __attribute__((address_space(3))) gm_s4 *lds_p;
                 typedef short s8 __attribute__((ext_vector_type(8)));
-                const int row = row0 + 16 * s + 4 * (lane >> 5) + (r >> 2), d = 32 * t + 16 * ((lane >> 4) & 1) + 4 * (r & 3);
-                const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + at_place<ROW>(row, d >> 3) + (d & 4) * 2));
-                const gm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + at_place<ROW>(row + 8, d >> 3) + (d & 4) * 2));
+                const char *p = tile + t / R::G * (4 * R::G * 16);
+                const int from = at.gather[0][t % R::G], f0 = at_exchange<R::ROW, 2>(16 * s) << 4, f1 = at_exchange<R::ROW, 2>(16 * s + 8) << 4;
+                const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + (from ^ f0) + (row0 + 16 * s) * R::ROW));
+                const gm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + (from ^ f1) + (row0 + 16 * s + 8) * R::ROW));
                 const s8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 acc[t] = at_multiply<E>(*(const gm_i4 *)&a, *(const gm_i4 *)&b, acc[t]);
             }
@@ -116,7 +153,7 @@ struct AtFeed {
         lds = lds_;
         row = (int)threadIdx.x / CH;
         ch = (int)threadIdx.x % CH;
-        if constexpr (MOVED) ch ^= at_exchange<ROW>(row);       // the chunk that belongs where the thread's first transfer ends
+        if constexpr (MOVED) ch ^= at_exchange<ROW, SIZE>(row);       // the chunk that belongs where the thread's first transfer ends
         left = dim;
     }
     // The pair `index` from a and b on.
@@ -129,7 +166,7 @@ struct AtFeed {
             const uint32_t step = (uint32_t)((which ? stride_b : stride_a) * SIZE);
             auto at = [&](int c) {
                 // (rows of a thread are a power of two apart: what is exchanged changes by a constant)
-                const int chunk = MOVED ? ch ^ at_exchange<ROW>(c * STEP) : ch;
+                const int chunk = MOVED ? ch ^ at_exchange<ROW, SIZE>(c * STEP) : ch;
                 const bool there = (bits == ALL || ((bits >> (row + c * STEP)) & 1)) && chunk * (16 / SIZE) < left;
                 return there ? (row + c * STEP) * step + chunk * 16 : 0x80000000u;
             };
@@ -159,7 +196,7 @@ struct AtFeed {
 #pragma unroll
             for (int which = 0; which < 2; ++which)
 #pragma unroll
-                for (int c = 0; c < COUNT; ++c) *reinterpret_cast<gm_i4 *>(lds + which * TILE + at_place<ROW>(row + c * STEP, ch)) = w[which][c];
+                for (int c = 0; c < COUNT; ++c) *reinterpret_cast<gm_i4 *>(lds + which * TILE + at_place<ROW, SIZE>(row + c * STEP, ch)) = w[which][c];
             __syncthreads();
             return lds;
         }
@@ -225,7 +262,7 @@ struct AtRange {
 template <int TILE>
 struct AtSeen {
     const uint8_t *mask; int64_t length; int lane;
-    bool next;
+    uint8_t next;
     __device__ __forceinline__ void init(const AttentionP &p, int b, int lane_)
     {
         lane = lane_;
@@ -236,21 +273,21 @@ struct AtSeen {
         }
         mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
     }
-    __device__ __forceinline__ void ask(int64_t key0) { next = mask && lane < TILE && key0 + lane < length && mask[key0 + lane]; }
+    __device__ __forceinline__ void ask(int64_t key0) { if (mask) next = mask[min(key0 + lane, length - 1)]; }
     __device__ __forceinline__ uint64_t take(int64_t key0) const
     {
-        if (mask) return __ballot(next);
         const int64_t left = length - key0;
+        if (mask) return __ballot(lane < TILE && lane < left && next);
         return left >= TILE ? (TILE == 64 ? ~0ull : (1ull << TILE) - 1) : left > 0 ? (1ull << left) - 1 : 0;
     }
 };
 
-// A workgroup's place: neighbouring tiles of one head run on one XCD, whose L2 holds what they share.
+// A workgroup's place.  Tiles of one head come one after the other and so on all XCDs at a time: where lengths differ, every XCD gets its share of the long ones (a head's
+// tiles on one XCD, whose L2 then holds its keys: 4 x 4096 queries on 896 to 2048 keys, forward 322 us for 255).
 struct AtPlace { int tile, split, head, b; };
 __device__ __forceinline__ AtPlace at_block(const AttentionP &p)
 {
-    const int total = (int)gridDim.x, i = (int)blockIdx.x, xcd = i % FGNN_NUM_XCD, q = total / FGNN_NUM_XCD, r = total % FGNN_NUM_XCD;
-    int t = xcd * q + min(xcd, r) + i / FGNN_NUM_XCD;
+    int t = (int)blockIdx.x;
     AtPlace o;
     o.tile = t % p.tiles;
     t /= p.tiles;
@@ -304,9 +341,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     float most = -__builtin_inff(), sum = 0.f;
     AtFeed<E, TILE, DP, WAVES> feed;
     feed.init(lds, p.dim);
-    seen.ask(first);
-    uint64_t bits = seen.take(first), coming = 0;
+    AtReader<E, DP> at;
+    at.init(lane);
+    uint64_t bits = 0, coming = 0;
     if (first < last) {
+        seen.ask(first);
+        bits = seen.take(first);
         seen.ask(first + TILE);
         feed.start(0, k + first * p.kn, v + first * p.vn, p.kn, p.vn, bits);
     }
@@ -322,7 +362,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
         if (bits == 0) continue;
         at_f16 s[TILE / 32];
 #pragma unroll
-        for (int t = 0; t < TILE / 32; ++t) s[t] = at_scores<E, DP>(lk, 32 * t, q, lane);
+        for (int t = 0; t < TILE / 32; ++t) s[t] = at_scores<E, DP>(at, lk, 32 * t, q);
         if (bits != (TILE == 64 ? ~0ull : (1ull << TILE) - 1)) {
 #pragma unroll
             for (int t = 0; t < TILE / 32; ++t) {
@@ -355,7 +395,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
                 w[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], p.log2_scale, -base));
                 sum += w[i];
             }
-            at_gather<E, DP>(lv, 32 * t, w, acc, lane);
+            at_gather<E, DP>(at, lv, 32 * t, w, acc);
         }
     }
     sum = at_other_sum(sum);
@@ -400,9 +440,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     for (int t = 0; t < DP / 32; ++t) acc[t] = at_f16{};
     AtFeed<E, TILE, DP, WAVES> feed;
     feed.init(lds, p.dim);
-    seen.ask(first);
-    uint64_t bits = seen.take(first), coming = 0;
+    AtReader<E, DP> at;
+    at.init(lane);
+    uint64_t bits = 0, coming = 0;
     if (first < last) {
+        seen.ask(first);
+        bits = seen.take(first);
         seen.ask(first + TILE);
         feed.start(0, k + first * p.kn, v + first * p.vn, p.kn, p.vn, bits);
     }
@@ -419,7 +462,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
         for (int t = 0; t < TILE / 32; ++t) {
             const uint32_t part = (uint32_t)(bits >> (32 * t));
             if (part == 0) continue;
-            const at_f16 s = at_scores<E, DP>(lk, 32 * t, q, lane), dp = at_scores<E, DP>(lv, 32 * t, g, lane);
+            const at_f16 s = at_scores<E, DP>(at, lk, 32 * t, q), dp = at_scores<E, DP>(at, lv, 32 * t, g);
             float w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.log2_scale, -lse)) * (dp[i] - delta);
@@ -429,7 +472,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
                 for (int i = 0; i < 16; ++i) w[i] = (own >> (8 * (i / 4) + i % 4)) & 1 ? w[i] : 0.f;
             }
             range.fit(w, acc);
-            at_gather<E, DP>(lk, 32 * t, w, acc, lane);
+            at_gather<E, DP>(at, lk, 32 * t, w, acc);
         }
     }
     if (row >= p.rows) return;
@@ -456,11 +499,13 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
     seen.init(p, o.b, lane);
     const bool there = key < seen.length && (!p.mask || seen.mask[min(key, p.nk - 1)]), any = __ballot(there) != 0;
     gm_i4 k[ROW / 32], v[ROW / 32];
-    const int64_t at = min(key, p.nk - 1);
-    at_row<E, DP>(k, (const E *)p.k + o.b * p.kb + at * p.kn + o.head * p.kh, there, p.dim, lane);
-    at_row<E, DP>(v, (const E *)p.v + o.b * p.vb + at * p.vn + o.head * p.vh, there, p.dim, lane);
+    const int64_t own = min(key, p.nk - 1);
+    at_row<E, DP>(k, (const E *)p.k + o.b * p.kb + own * p.kn + o.head * p.kh, there, p.dim, lane);
+    at_row<E, DP>(v, (const E *)p.v + o.b * p.vb + own * p.vn + o.head * p.vh, there, p.dim, lane);
     // tiles of every head's positions, one head after the other
-    const int per_head = (p.nq + TILE - 1) / TILE, first = o.split * p.per, last = min(per_head * p.share, first + p.per);
+    const int per_head = (p.nq + TILE - 1) / TILE, first = o.split * p.per;
+    // (behind the last key that is seen nothing is walked)
+    const int last = o.tile * WAVES * 32 < seen.length ? min(per_head * p.share, first + p.per) : first;
 
     at_f16 dk[STEPS], dv[STEPS];
 #pragma unroll
@@ -468,6 +513,8 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
     AtRange<E, STEPS> range;
     Feed feed;
     feed.init(lds, p.dim);
+    AtReader<E, DP> at;
+    at.init(lane);
     float stat = 0.f;
     auto fetch = [&](int i) {
         const int sub = i / per_head, pos = (i - sub * per_head) * TILE, head = o.head * p.share + sub, left = p.nq - pos;
@@ -481,28 +528,28 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
     if (first < last) fetch(first);
 #pragma unroll 1
     for (int i = first; i < last; ++i) {
-        float *own = stats + ((i - first) & 1) * 2 * TILE;
-        if (threadIdx.x < 2 * TILE) own[threadIdx.x] = stat;
+        float *row_stats = stats + ((i - first) & 1) * 2 * TILE;
+        if (threadIdx.x < 2 * TILE) row_stats[threadIdx.x] = stat;
         const char *lq = feed.arrive(i - first), *lg = lq + TILE * ROW;
         if (i + 1 < last) fetch(i + 1);
         if (!any) continue;
 #pragma unroll
         for (int t = 0; t < TILE / 32; ++t) {
-            const at_f16 s = at_scores<E, DP>(lq, 32 * t, k, lane), dp = at_scores<E, DP>(lg, 32 * t, v, lane);
+            const at_f16 s = at_scores<E, DP>(at, lq, 32 * t, k), dp = at_scores<E, DP>(at, lg, 32 * t, v);
             float w[16], ds[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const gm_f4 lse = *reinterpret_cast<const gm_f4 *>(own + 32 * t + 8 * j + 4 * (lane >> 5)),
-                            delta = *reinterpret_cast<const gm_f4 *>(own + TILE + 32 * t + 8 * j + 4 * (lane >> 5));
+                const gm_f4 lse = *reinterpret_cast<const gm_f4 *>(row_stats + 32 * t + 8 * j + 4 * (lane >> 5)),
+                            delta = *reinterpret_cast<const gm_f4 *>(row_stats + TILE + 32 * t + 8 * j + 4 * (lane >> 5));
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     w[4 * j + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + c], p.log2_scale, -lse[c]));
                     ds[4 * j + c] = w[4 * j + c] * (dp[4 * j + c] - delta[c]);
                 }
             }
-            at_gather<E, DP>(lg, 32 * t, w, dv, lane);
+            at_gather<E, DP>(at, lg, 32 * t, w, dv);
             range.fit(ds, dk);
-            at_gather<E, DP>(lq, 32 * t, ds, dk, lane);
+            at_gather<E, DP>(at, lq, 32 * t, ds, dk);
         }
     }
     if (key >= p.nk) return;
