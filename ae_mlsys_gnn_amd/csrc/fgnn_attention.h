@@ -46,31 +46,23 @@ __host__ __device__ constexpr int at_exchange(int row)
 template <int ROW, int SIZE>
 __device__ __forceinline__ int at_place(int row, int ch) { return row * ROW + ((ch ^ at_exchange<ROW, SIZE>(row)) << 4); }
 
-// Where a lane reads tiles of DP components: for scores its row's chunks 2 j + (lane / 32), for the transposed tile what the reads below say.  Of the exchanged chunk index the
-// upper bits are the constant's own, so that a few places and constant offsets from them give all of them.
+// Where a lane reads tiles of DP components: its row's first chunk for scores, and the first of what the reads of the transposed tile below say.  The others' places differ from these
+// in bits of the chunk index that are exchanged (an exclusive or with a constant; eight registers for as many places and the sums of dK and dV left no room for two waves) and in
+// constant offsets.
+template <typename T> __device__ __forceinline__ auto at_lds(uint32_t at) { return (__attribute__((address_space(3))) T *)(uintptr_t)at; }
 template <typename E, int DP>
 struct AtReader {
     static constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, MASK = ROW % 128 ? 3 : ROW % 256 ? 7 : 15;     // exchanged bits of the chunk index
-    static constexpr int S = std::min((MASK + 1) / 2, ROW / 32);
-    static constexpr int G = SIZE == 4 ? std::min(2, DP / 32) : std::min((MASK + 1) / 4, DP / 32);
-    int score[S], gather[SIZE == 4 ? 4 : 1][G];
+    uint32_t score, gather;
     __device__ __forceinline__ void init(int lane)
     {
-        const int f = at_exchange<ROW, SIZE>(lane & 31), h = lane >> 5;
-#pragma unroll
-        for (int j = 0; j < S; ++j) score[j] = (lane & 31) * ROW + (((2 * j + h) ^ f) << 4);
-        if constexpr (SIZE == 4) {
-            // row 4 h + i, component lane % 32: chunk 8 t + (lane % 32) / 4
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int t = 0; t < G; ++t) gather[i][t] = at_place<ROW, SIZE>(4 * h + i, 8 * t + ((lane & 31) >> 2)) + (lane & 3) * 4;
-        } else {
-            const int r = lane & 15;
-#pragma unroll
-            for (int t = 0; t < G; ++t) gather[0][t] = at_place<ROW, SIZE>(4 * h + (r >> 2), 4 * t + 2 * ((lane >> 4) & 1) + ((r & 3) >> 1)) + (r & 1) * 8;
-        }
+        const int h = lane >> 5, r = lane & 15;
+        score = at_place<ROW, SIZE>(lane & 31, h);
+        // fp32: row 4 h + i, component lane % 32; else row 4 h + r / 4, four components from 16 ((lane / 16) % 2) + 4 (r % 4) on
+        gather = SIZE == 4 ? at_place<ROW, SIZE>(4 * h, (lane & 31) >> 2) + (lane & 3) * 4 : at_place<ROW, SIZE>(4 * h + (r >> 2), 2 * ((lane >> 4) & 1) + ((r & 3) >> 1)) + (r & 1) * 8;
     }
+    // `from` (of a tile that starts at a multiple of 256 bytes), `chunks` chunks and `rows` rows further on; both constants, of bits that the lanes' own do not have
+    static __device__ __forceinline__ uint32_t to(uint32_t from, int chunks, int rows) { return (from ^ (((chunks & MASK) ^ at_exchange<ROW, SIZE>(rows)) << 4)) + (chunks & ~MASK) * 16 + rows * ROW; }
 };
 
 template <typename E>
@@ -86,53 +78,80 @@ __device__ __forceinline__ at_f16 at_multiply(gm_i4 a, gm_i4 b, at_f16 c)
 
 // The scores of 32 rows of a tile (from row0 on, a multiple of 32) with the wave's columns.
 template <typename E, int DP>
-__device__ __forceinline__ at_f16 at_scores(const AtReader<E, DP> &at, const char *tile, int row0, const gm_i4 (&cols)[DP * (int)sizeof(E) / 32])
+__device__ __forceinline__ at_f16 at_scores(const AtReader<E, DP> &at, uint32_t tile, int row0, const gm_i4 (&cols)[DP * (int)sizeof(E) / 32])
 {
     typedef AtReader<E, DP> R;
     at_f16 s = {};
 #pragma unroll
-    for (int j = 0; j < R::ROW / 32; ++j)
-        s = at_multiply<E>(*reinterpret_cast<const gm_i4 *>(tile + at.score[j % R::S] + row0 * R::ROW + j / R::S * (2 * R::S * 16)), cols[j], s);
+    for (int j = 0; j < R::ROW / 32; ++j) s = at_multiply<E>(*at_lds<gm_i4>(R::to(tile + at.score, 2 * j, row0)), cols[j], s);
     return s;
 }
 
+// The same with the columns in LDS too, from `cols` on.
+template <typename E, int DP>
+__device__ __forceinline__ at_f16 at_scores(const AtReader<E, DP> &at, uint32_t tile, int row0, uint32_t cols)
+{
+    typedef AtReader<E, DP> R;
+    at_f16 s = {};
+#pragma unroll
+    for (int j = 0; j < R::ROW / 32; ++j) s = at_multiply<E>(*at_lds<gm_i4>(R::to(tile + at.score, 2 * j, row0)), *at_lds<gm_i4>(R::to(cols + at.score, 2 * j, 0)), s);
+    return s;
+}
+
+// 16 of a column's 32 weights as the second operand of products, rounded to the type.
+template <typename E> struct AtWeights {
+    typedef E vec __attribute__((ext_vector_type(16)));
+    vec w;
+    __device__ __forceinline__ explicit AtWeights(const float (&v)[16])
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = (E)v[i];
+    }
+};
 // acc[t] (32 components from 32 t on, by the wave's columns) += (32 rows of a tile, from row0 on)^T w
 template <typename E, int DP>
-__device__ __forceinline__ void at_gather(const AtReader<E, DP> &at, const char *tile, int row0, const float (&w)[16], at_f16 (&acc)[DP / 32])
+__device__ __forceinline__ void at_gather(const AtReader<E, DP> &at, uint32_t tile, int row0, const AtWeights<E> &weights, at_f16 (&acc)[DP / 32])
 {
+    const auto &w = weights.w;
     typedef AtReader<E, DP> R;
     if constexpr (sizeof(E) == 4) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            // (rows 8 and more apart: of what is exchanged only row 8's bit changes with them)
-            const int row = 8 * (i / 4), flip = at_exchange<R::ROW, 4>(row) << 4;
+        for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t) {
-                const float a = *reinterpret_cast<const float *>(tile + (at.gather[i % 4][t % R::G] ^ flip) + (row0 + row) * R::ROW + t / R::G * (8 * R::G * 16));
-                acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[i], acc[t], 0, 0, 0);
-            }
-        }
+            for (int t = 0; t < DP / 32; ++t)
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(*at_lds<float>(R::to(tile + at.gather, 8 * t, row0 + 8 * (i / 4) + i % 4)), w[i], acc[t], 0, 0, 0);
     } else {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             typedef E e8 __attribute__((ext_vector_type(8)));
             e8 b;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = (E)w[8 * s + i];
+            for (int i = 0; i < 8; ++i) b[i] = w[8 * s + i];
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t) {
-                // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each.  (Rows 8 further on: the exchange's second bit
-                // of two changes, where it is the row's fourth.)
-                typedef __attribute__((address_space(3))) gm_s4 *lds_p;
+                // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
                 typedef short s8 __attribute__((ext_vector_type(8)));
-                const char *p = tile + t / R::G * (4 * R::G * 16);
-                const int from = at.gather[0][t % R::G], f0 = at_exchange<R::ROW, 2>(16 * s) << 4, f1 = at_exchange<R::ROW, 2>(16 * s + 8) << 4;
-                const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + (from ^ f0) + (row0 + 16 * s) * R::ROW));
-                const gm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + (from ^ f1) + (row0 + 16 * s + 8) * R::ROW));
+                const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<gm_s4>(R::to(tile + at.gather, 4 * t, row0 + 16 * s)));
+                const gm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<gm_s4>(R::to(tile + at.gather, 4 * t, row0 + 16 * s + 8)));
                 const s8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 acc[t] = at_multiply<E>(*(const gm_i4 *)&a, *(const gm_i4 *)&b, acc[t]);
             }
         }
+    }
+}
+
+// Asks that the N matrix instructions of the code around it come one by one, their reads of LDS, READS each, AHEAD of them before the first (left alone the compiler reads each
+// operand right before its instruction and waits for it), and in the shadow of each VALU instructions of other arithmetic and EXPS exponentials.
+template <int N, int READS, int AHEAD, int VALU = 0, int EXPS = 0>
+__device__ __forceinline__ void at_ahead()
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i < N - AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+        if (EXPS) __builtin_amdgcn_sched_group_barrier(0x400, EXPS, 0);
     }
 }
 
@@ -145,12 +164,12 @@ struct AtFeed {
     static constexpr int COUNT = ROWS * CH / THREADS, STEP = THREADS / CH;          // chunks a thread, and rows between them
     static constexpr int BYTES = (MOVED ? 2 : 1) * 2 * TILE;
     static_assert(ROWS * CH % THREADS == 0 && THREADS % CH == 0, "threads share a tile evenly");
-    char *lds; int row, ch, left;           // left: components from the first chunk on
+    uint32_t lds; int row, ch, left;        // lds: address there; left: components from the first chunk on
     gm_i4 w[MOVED ? 1 : 2][MOVED ? 1 : COUNT];
 
     __device__ __forceinline__ void init(char *lds_, int dim)
     {
-        lds = lds_;
+        lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds_;
         row = (int)threadIdx.x / CH;
         ch = (int)threadIdx.x % CH;
         if constexpr (MOVED) ch ^= at_exchange<ROW, SIZE>(row);       // the chunk that belongs where the thread's first transfer ends
@@ -174,7 +193,7 @@ struct AtFeed {
                 // (written out, and its waits with it: see GemmMover)
                 const uint64_t from = (uint64_t)base;
                 const gm_i4 buffer = {(int)(uint32_t)from, (int)((uint32_t)(from >> 32) & 0xffffu), (int)0x80000000u, 0x00027000};
-                const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + ((index & 1) * 2 + which) * TILE + fg_wave() * 1024;
+                const uint32_t to = lds + ((index & 1) * 2 + which) * TILE + fg_wave() * 1024;
 #pragma unroll
                 for (int c = 0; c < COUNT; ++c)
                     asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at(c)), "s"(buffer), "{m0}"(to + c * THREADS * 16));
@@ -186,7 +205,7 @@ struct AtFeed {
         }
     }
     // The pair `index` has arrived, and nobody reads the one before any more.
-    __device__ __forceinline__ const char *arrive(int index)
+    __device__ __forceinline__ uint32_t arrive(int index)
     {
         if constexpr (MOVED) {
             gm_arrive<0>();
@@ -196,7 +215,7 @@ struct AtFeed {
 #pragma unroll
             for (int which = 0; which < 2; ++which)
 #pragma unroll
-                for (int c = 0; c < COUNT; ++c) *reinterpret_cast<gm_i4 *>(lds + which * TILE + at_place<ROW, SIZE>(row + c * STEP, ch)) = w[which][c];
+                for (int c = 0; c < COUNT; ++c) *at_lds<gm_i4>(lds + which * TILE + at_place<ROW, SIZE>(row + c * STEP, ch)) = w[which][c];
             __syncthreads();
             return lds;
         }
@@ -321,8 +340,8 @@ __device__ __forceinline__ void at_store(const at_f16 (&acc)[DP / 32], E *row, i
 template <typename E, int DP, int WAVES, int TILE>
 __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_kernel(AttentionP p)
 {
-    constexpr int ROW = DP * (int)sizeof(E);
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE;
+    extern __shared__ __attribute__((aligned(256))) char lds[];
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
     int pos, sub;
@@ -353,16 +372,20 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     int index = 0;
 #pragma unroll 1
     for (int64_t key = first; key < last; key += TILE, bits = coming, ++index) {
-        const char *lk = feed.arrive(index), *lv = lk + TILE * ROW;
+        const uint32_t lk = feed.arrive(index), lv = lk + TILE * ROW;
         if (key + TILE < last) {
             coming = seen.take(key + TILE);
             seen.ask(key + 2 * TILE);
             feed.start(index + 1, k + (key + TILE) * p.kn, v + (key + TILE) * p.vn, p.kn, p.vn, coming);
         }
         if (bits == 0) continue;
-        at_f16 s[TILE / 32];
+        constexpr int B = TILE / 32;
+        at_f16 s[B];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < TILE / 32; ++t) s[t] = at_scores<E, DP>(at, lk, 32 * t, q);
+        for (int t = 0; t < B; ++t) s[t] = at_scores<E, DP>(at, lk, 32 * t, q);
+        if constexpr (SIZE == 2) at_ahead<B * ROW / 32, 1, 4>();
+        __builtin_amdgcn_sched_barrier(0);
         if (bits != (TILE == 64 ? ~0ull : (1ull << TILE) - 1)) {
 #pragma unroll
             for (int t = 0; t < TILE / 32; ++t) {
@@ -387,16 +410,26 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
                 for (int i = 0; i < 16; ++i) acc[t][i] *= f;
         }
         const float base = (most > -__builtin_inff() ? most : 0.f) - at_lift<E>;
-#pragma unroll
-        for (int t = 0; t < TILE / 32; ++t) {
+        auto weigh = [&](int t) {
             float w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 w[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], p.log2_scale, -base));
                 sum += w[i];
             }
+            return AtWeights<E>(w);
+        };
+        AtWeights<E> w = weigh(0);
+#pragma unroll
+        for (int t = 0; t < B; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
             at_gather<E, DP>(at, lv, 32 * t, w, acc);
+            if (t + 1 < B) {
+                w = weigh(t + 1);
+                if constexpr (SIZE == 2) at_ahead<ROW / 32, 2, 3, 640 / ROW * 2, 512 / ROW>();
+            } else if constexpr (SIZE == 2) at_ahead<ROW / 32, 2, 3>();
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
     sum = at_other_sum(sum);
     const bool none = sum == 0.f;
@@ -417,8 +450,8 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 template <typename E, int DP, int WAVES, int TILE>
 __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_dq_kernel(AttentionP p)
 {
-    constexpr int ROW = DP * (int)sizeof(E);
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE;
+    extern __shared__ __attribute__((aligned(256))) char lds[];
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
     int pos, sub;
@@ -452,28 +485,50 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     int index = 0;
 #pragma unroll 1
     for (int64_t key = first; key < last; key += TILE, bits = coming, ++index) {
-        const char *lk = feed.arrive(index), *lv = lk + TILE * ROW;
+        const uint32_t lk = feed.arrive(index), lv = lk + TILE * ROW;
         if (key + TILE < last) {
             coming = seen.take(key + TILE);
             seen.ask(key + 2 * TILE);
             feed.start(index + 1, k + (key + TILE) * p.kn, v + (key + TILE) * p.vn, p.kn, p.vn, coming);
         }
+        if (bits == 0) continue;
+        constexpr int B = TILE / 32;
+        at_f16 s[B], dp[B];
+        float w[B][16];
+        auto scores = [&](int t) {
+            s[t] = at_scores<E, DP>(at, lk, 32 * t, q);
+            dp[t] = at_scores<E, DP>(at, lv, 32 * t, g);
+        };
+        auto weigh = [&](int t) {
 #pragma unroll
-        for (int t = 0; t < TILE / 32; ++t) {
+            for (int i = 0; i < 16; ++i) w[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], p.log2_scale, -lse)) * (dp[t][i] - delta);
+        };
+        auto gather = [&](int t) {
             const uint32_t part = (uint32_t)(bits >> (32 * t));
-            if (part == 0) continue;
-            const at_f16 s = at_scores<E, DP>(at, lk, 32 * t, q), dp = at_scores<E, DP>(at, lv, 32 * t, g);
-            float w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.log2_scale, -lse)) * (dp[i] - delta);
             if (part != ~0u) {
                 const uint32_t own = part >> (4 * (lane >> 5));
 #pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = (own >> (8 * (i / 4) + i % 4)) & 1 ? w[i] : 0.f;
+                for (int i = 0; i < 16; ++i) w[t][i] = (own >> (8 * (i / 4) + i % 4)) & 1 ? w[t][i] : 0.f;
             }
-            range.fit(w, acc);
-            at_gather<E, DP>(at, lk, 32 * t, w, acc);
+            range.fit(w[t], acc);
+            at_gather<E, DP>(at, lk, 32 * t, AtWeights<E>(w[t]), acc);
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        scores(0);
+        if constexpr (SIZE == 2) at_ahead<ROW / 16, 1, 3>();
+#pragma unroll
+        for (int t = 0; t < B; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
+            weigh(t);
+            if (t + 1 < B) {                // the next keys' scores beside these ones' weights
+                scores(t + 1);
+                if constexpr (SIZE == 2) at_ahead<ROW / 16, 1, 3, 768 / ROW, 256 / ROW>();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            gather(t);
+            if constexpr (SIZE == 2) at_ahead<ROW / 32, 2, 3>();
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
     if (row >= p.rows) return;
     const float f = p.scale / range.f * __builtin_amdgcn_exp2f(-at_lift<E>);
@@ -484,15 +539,18 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     } else at_store<E, DP>(acc, (E *)p.dq + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, p.dim, lane, scaled);
 }
 
-// dK and dV: a wave owns 32 keys and walks the queries of every head that uses them, tile by tile.  PARTS: the components are taken in that many passes
-// over the scores (of wide fp32 heads one pass's sums and operands do not fit the registers).
-template <typename E, int DP, int WAVES, int TILE, int PARTS>
-__global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP p)
+// dK and dV: a wave owns 32 keys and walks the queries of every head that uses them, tile by tile.  Where their sums leave no room in the registers the keys wait in LDS (their
+// values stay): two waves a SIMD at 128 components, where one alone waits for LDS before every instruction.
+constexpr bool at_keys_in_lds(int dim, int size) { return size == 2 && dim >= 128; }
+constexpr int at_rows_dkv(int dim, int size) { return size == 4 || dim >= 128 ? 32 : 64; }
+template <typename E, int DP, int WAVES, int TILE>
+__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_dkv_kernel(AttentionP p)
 {
-    constexpr int ROW = DP * (int)sizeof(E), STEPS = DP / 32;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, STEPS = DP / 32;
+    constexpr bool KEYS_IN_LDS = at_keys_in_lds(DP, SIZE);
+    extern __shared__ __attribute__((aligned(256))) char lds[];
     typedef AtFeed<E, TILE, DP, WAVES> Feed;
-    float *stats = (float *)(lds + Feed::BYTES);                // lse, delta of the tile's rows, two tiles in turn
+    const uint32_t stats = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + Feed::BYTES;       // lse, delta of the tile's rows, two tiles in turn
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), key = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
     AtSeen<64> seen;
@@ -513,6 +571,11 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
     AtRange<E, STEPS> range;
     Feed feed;
     feed.init(lds, p.dim);
+    const uint32_t own_keys = stats + 4 * TILE * 4 + fg_wave() * 32 * ROW;
+    if constexpr (KEYS_IN_LDS) {            // (read by their own wave alone)
+#pragma unroll
+        for (int j = 0; j < ROW / 32; ++j) *at_lds<gm_i4>(own_keys + at_place<ROW, SIZE>(lane & 31, 2 * j + (lane >> 5))) = k[j];
+    }
     AtReader<E, DP> at;
     at.init(lane);
     float stat = 0.f;
@@ -528,28 +591,36 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attention_dkv_kernel(AttentionP
     if (first < last) fetch(first);
 #pragma unroll 1
     for (int i = first; i < last; ++i) {
-        float *row_stats = stats + ((i - first) & 1) * 2 * TILE;
-        if (threadIdx.x < 2 * TILE) row_stats[threadIdx.x] = stat;
-        const char *lq = feed.arrive(i - first), *lg = lq + TILE * ROW;
+        const uint32_t row_stats = stats + ((i - first) & 1) * 2 * TILE * 4;
+        if (threadIdx.x < 2 * TILE) *at_lds<float>(row_stats + threadIdx.x * 4) = stat;
+        const uint32_t lq = feed.arrive(i - first), lg = lq + TILE * ROW;
         if (i + 1 < last) fetch(i + 1);
         if (!any) continue;
 #pragma unroll
         for (int t = 0; t < TILE / 32; ++t) {
-            const at_f16 s = at_scores<E, DP>(at, lq, 32 * t, k), dp = at_scores<E, DP>(at, lg, 32 * t, v);
+            __builtin_amdgcn_sched_barrier(0);      // 32 rows at a time: the registers are full of sums
+            at_f16 s;
+            if constexpr (KEYS_IN_LDS) s = at_scores<E, DP>(at, lq, 32 * t, own_keys);
+            else s = at_scores<E, DP>(at, lq, 32 * t, k);
+            const at_f16 dp = at_scores<E, DP>(at, lg, 32 * t, v);
+            if constexpr (SIZE == 2) at_ahead<ROW / 16, 1, 3>();
+            __builtin_amdgcn_sched_barrier(0);
             float w[16], ds[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const gm_f4 lse = *reinterpret_cast<const gm_f4 *>(row_stats + 32 * t + 8 * j + 4 * (lane >> 5)),
-                            delta = *reinterpret_cast<const gm_f4 *>(row_stats + TILE + 32 * t + 8 * j + 4 * (lane >> 5));
+                const gm_f4 lse = *at_lds<gm_f4>(row_stats + (32 * t + 8 * j + 4 * (lane >> 5)) * 4), delta = *at_lds<gm_f4>(row_stats + (TILE + 32 * t + 8 * j + 4 * (lane >> 5)) * 4);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     w[4 * j + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + c], p.log2_scale, -lse[c]));
                     ds[4 * j + c] = w[4 * j + c] * (dp[4 * j + c] - delta[c]);
                 }
             }
-            at_gather<E, DP>(at, lg, 32 * t, w, dv);
             range.fit(ds, dk);
-            at_gather<E, DP>(at, lq, 32 * t, ds, dk);
+            const AtWeights<E> pw(w), pd(ds);
+            __builtin_amdgcn_sched_barrier(0);
+            at_gather<E, DP>(at, lg, 32 * t, pw, dv);
+            at_gather<E, DP>(at, lq, 32 * t, pd, dk);
+            if constexpr (SIZE == 2) at_ahead<ROW / 16, 2, 3>();
         }
     }
     if (key >= p.nk) return;
@@ -578,8 +649,8 @@ static void at_launch_dim(int what, const AtShape &s, const AttentionP &p, unsig
 {
     constexpr int T = at_tile<E>;
     if (what == AT_DKV) {
-        constexpr int bytes = AtFeed<E, T, DP, 4>::BYTES + 4 * T * (int)sizeof(float);
-        hipLaunchKernelGGL((attention_dkv_kernel<E, DP, 4, T, 1>), dim3(grid), dim3(256), bytes, st, p);
+        constexpr int S = (int)sizeof(E), R = at_rows_dkv(DP, S), bytes = AtFeed<E, R, DP, 4>::BYTES + 4 * R * (int)sizeof(float) + (at_keys_in_lds(DP, S) ? 128 * DP * S : 0);
+        hipLaunchKernelGGL((attention_dkv_kernel<E, DP, 4, R>), dim3(grid), dim3(256), bytes, st, p);
         return;
     }
     constexpr int many = AtFeed<E, T, DP, 4>::BYTES, one = AtFeed<E, 32, DP, 1>::BYTES;

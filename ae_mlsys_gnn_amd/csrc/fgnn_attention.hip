@@ -145,7 +145,7 @@ static AtShape at_shape(AttentionP &p, int what, int type)
 {
     AtShape s;
     s.dim = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
-    s.tile = fe_size(type) == 4 ? 32 : 64;
+    s.tile = what == AT_DKV ? at_rows_dkv(s.dim, fe_size(type)) : fe_size(type) == 4 ? 32 : 64;
     s.waves = what != AT_DKV && p.rows <= 64 ? 1 : 4;
     if (s.waves == 1) s.tile = 32;
     const int64_t columns = what == AT_DKV ? p.nk : p.rows, walked = what == AT_DKV ? (int64_t)((p.nq + s.tile - 1) / s.tile) * p.share : (p.nk + s.tile - 1) / s.tile;
