@@ -322,9 +322,17 @@ __device__ __forceinline__ void at_query(const AttentionP &p, int row, int &pos,
     pos = (int)((__umulhi((uint32_t)row, p.share_mul) + (uint32_t)row) >> p.share_shift);
     sub = row - pos * p.share;
 }
-// 32 components a step of a wave's sums, times `f`, to a row of `dim`.
-template <typename E, int DP, typename F>
-__device__ __forceinline__ void at_store(const at_f16 (&acc)[DP / 32], E *row, int dim, int lane, F f)
+// Where a row of queries lies in y or dq; NULL past the last.
+template <typename E>
+__device__ __forceinline__ E *at_result(const AttentionP &p, E *y, const AtPlace &o, int row)
+{
+    int pos, sub;
+    at_query(p, row, pos, sub);
+    return row < p.rows ? y + (((int64_t)o.b * p.nq + pos) * p.heads + o.head * p.share + sub) * p.dim : nullptr;
+}
+// A wave's sums, by `f`, to rows of `dim`: parts, in 32 bits, as they lie in the registers.
+template <int DP, typename F>
+__device__ __forceinline__ void at_store_part(const at_f16 (&acc)[DP / 32], float *row, int dim, int lane, F f)
 {
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -332,9 +340,37 @@ __device__ __forceinline__ void at_store(const at_f16 (&acc)[DP / 32], E *row, i
         for (int i = 0; i < 4; ++i) {
             const int d = 32 * t + 8 * i + 4 * (lane >> 5);
             const float v[4] = {f(acc[t][4 * i]), f(acc[t][4 * i + 1]), f(acc[t][4 * i + 2]), f(acc[t][4 * i + 3])};
-            if (d < dim) gm_store<E, 4>(v, row + d, dim - d);
+            if (d < dim) gm_store<float, 4>(v, row + d, dim - d);
         }
 }
+// Results, through the wave's own 32 rows of LDS from `lds` on, where a lane has four components of a row and leaves with 16 bytes next to its neighbours' (four
+// components a lane are 16 bytes of each of 32 rows a store).  to(r): where row r of the wave's goes, NULL: nowhere.
+template <typename E, int DP, typename F, typename To>
+__device__ __forceinline__ void at_store(const at_f16 (&acc)[DP / 32], uint32_t lds, int dim, int lane, F f, To to)
+{
+    constexpr int V = fe_width<E>, SIZE = (int)sizeof(E), ROW = DP * SIZE, CH = ROW / 16;
+    typedef E e4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 32 * t + 8 * i + 4 * (lane >> 5);
+            const e4 v = {(E)f(acc[t][4 * i]), (E)f(acc[t][4 * i + 1]), (E)f(acc[t][4 * i + 2]), (E)f(acc[t][4 * i + 3])};
+            *at_lds<e4>(lds + at_place<ROW, SIZE>(lane & 31, d / V) + d % V * SIZE) = v;
+        }
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) {
+        const int r = (i * 64 + lane) / CH, ch = (i * 64 + lane) % CH;
+        typedef E vec __attribute__((ext_vector_type(V)));
+        const vec u = *at_lds<vec>(lds + at_place<ROW, SIZE>(r, ch));
+        E *row = to(r), v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = u[j];
+        if (row && ch * V < dim) gm_store<E, V>(v, row + ch * V, dim - ch * V);
+    }
+}
+// LDS of a kernel: its feed's, or the results of all its waves.
+template <typename E, int DP, int WAVES, int TILE> constexpr int at_bytes = std::max(AtFeed<E, TILE, DP, WAVES>::BYTES, WAVES * 32 * DP * (int)sizeof(E));
 
 // Y and lse.  With `splits` parts of the keys, normalised sums and lse of each to `part`.
 template <typename E, int DP, int WAVES, int TILE>
@@ -434,16 +470,17 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     sum = at_other_sum(sum);
     const bool none = sum == 0.f;
     const float inv = none ? 0.f : 1.f / sum;
-    if (row >= p.rows) return;
     const auto norm = [&](float x) { return none ? 0.f : x * inv; };
     if (p.splits > 1) {
-        const int64_t at = (((int64_t)o.b * p.kv_heads + o.head) * p.splits + o.split) * p.rows + row;
-        at_store<float, DP>(acc, p.part + at * p.dim, p.dim, lane, norm);
-        if (lane < 32) p.part_lse[at] = none ? -__builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
+        if (row >= p.rows) return;
+        const int64_t to = (((int64_t)o.b * p.kv_heads + o.head) * p.splits + o.split) * p.rows + row;
+        at_store_part<DP>(acc, p.part + to * p.dim, p.dim, lane, norm);
+        if (lane < 32) p.part_lse[to] = none ? -__builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
         return;
     }
-    at_store<E, DP>(acc, (E *)p.y + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, p.dim, lane, norm);
-    if (p.lse && lane < 32) p.lse[((int64_t)o.b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
+    if (p.lse && lane < 32 && row < p.rows) p.lse[((int64_t)o.b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
+    __syncthreads();                        // the last tile has been read
+    at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * ROW, p.dim, lane, norm, [&](int r) { return at_result(p, (E *)p.y, o, row - (lane & 31) + r); });
 }
 
 // dQ: as the forward pass, with P from lse.  With parts of the keys, their sums to `part`.
@@ -530,13 +567,16 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    if (row >= p.rows) return;
     const float f = p.scale / range.f * __builtin_amdgcn_exp2f(-at_lift<E>);
     const auto scaled = [&](float x) { return x * f; };
     if (p.splits > 1) {
-        const int64_t at = (((int64_t)o.b * p.kv_heads + o.head) * p.splits + o.split) * p.rows + row;
-        at_store<float, DP>(acc, p.part + at * p.dim, p.dim, lane, scaled);
-    } else at_store<E, DP>(acc, (E *)p.dq + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, p.dim, lane, scaled);
+        if (row >= p.rows) return;
+        const int64_t to = (((int64_t)o.b * p.kv_heads + o.head) * p.splits + o.split) * p.rows + row;
+        at_store_part<DP>(acc, p.part + to * p.dim, p.dim, lane, scaled);
+        return;
+    }
+    __syncthreads();
+    at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * ROW, p.dim, lane, scaled, [&](int r) { return at_result(p, (E *)p.dq, o, row - (lane & 31) + r); });
 }
 
 // dK and dV: a wave owns 32 keys and walks the queries of every head that uses them, tile by tile.  Where their sums leave no room in the registers the keys wait in LDS (their
@@ -550,7 +590,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     constexpr bool KEYS_IN_LDS = at_keys_in_lds(DP, SIZE);
     extern __shared__ __attribute__((aligned(256))) char lds[];
     typedef AtFeed<E, TILE, DP, WAVES> Feed;
-    const uint32_t stats = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + Feed::BYTES;       // lse, delta of the tile's rows, two tiles in turn
+    const uint32_t stats = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + at_bytes<E, DP, WAVES, TILE>;       // lse, delta of the tile's rows, two tiles in turn
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), key = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
     AtSeen<64> seen;
@@ -623,20 +663,25 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
             if constexpr (SIZE == 2) at_ahead<ROW / 16, 2, 3>();
         }
     }
-    if (key >= p.nk) return;
     // keys that are not seen were zeros in every product: what a score of 0 made of them is dropped
     const float down = __builtin_amdgcn_exp2f(-at_lift<E>), f = p.scale / range.f * down;
     const auto sk = [&](float x) { return there ? x * f : 0.f; };
     const auto sv = [&](float x) { return there ? x * down : 0.f; };
     if (p.splits > 1) {
+        if (key >= p.nk) return;
         const int64_t n = (int64_t)p.batch * p.nk * p.kv_heads * p.dim, to = o.split * 2 * n + (((int64_t)o.b * p.nk + key) * p.kv_heads + o.head) * p.dim;
-        at_store<float, DP>(dk, p.part + to, p.dim, lane, sk);
-        at_store<float, DP>(dv, p.part + to + n, p.dim, lane, sv);
-    } else {
-        const int64_t to = (((int64_t)o.b * p.nk + key) * p.kv_heads + o.head) * p.dim;
-        at_store<E, DP>(dk, (E *)p.dk + to, p.dim, lane, sk);
-        at_store<E, DP>(dv, (E *)p.dv + to, p.dim, lane, sv);
+        at_store_part<DP>(dk, p.part + to, p.dim, lane, sk);
+        at_store_part<DP>(dv, p.part + to + n, p.dim, lane, sv);
+        return;
     }
+    __syncthreads();
+    const auto to = [&](void *result, int r) {
+        const int k = key - (lane & 31) + r;
+        return k < p.nk ? (E *)result + (((int64_t)o.b * p.nk + k) * p.kv_heads + o.head) * p.dim : nullptr;
+    };
+    const uint32_t rows = feed.lds + fg_wave() * 32 * ROW;
+    at_store<E, DP>(dk, rows, p.dim, lane, sk, [&](int r) { return to(p.dk, r); });
+    at_store<E, DP>(dv, rows, p.dim, lane, sv, [&](int r) { return to(p.dv, r); });
 }
 
 // The kernels of a type, by what they are for: one file each (fgnn_attention_*.hip).
@@ -647,20 +692,19 @@ template <typename E> void at_launch(int what, const AtShape &shape, const Atten
 template <typename E, int DP>
 static void at_launch_dim(int what, const AtShape &s, const AttentionP &p, unsigned grid, hipStream_t st)
 {
-    constexpr int T = at_tile<E>;
     if (what == AT_DKV) {
-        constexpr int S = (int)sizeof(E), R = at_rows_dkv(DP, S), bytes = AtFeed<E, R, DP, 4>::BYTES + 4 * R * (int)sizeof(float) + (at_keys_in_lds(DP, S) ? 128 * DP * S : 0);
+        constexpr int S = (int)sizeof(E), R = at_rows_dkv(DP, S), bytes = at_bytes<E, DP, 4, R> + 4 * R * (int)sizeof(float) + (at_keys_in_lds(DP, S) ? 128 * DP * S : 0);
         hipLaunchKernelGGL((attention_dkv_kernel<E, DP, 4, R>), dim3(grid), dim3(256), bytes, st, p);
         return;
     }
-    constexpr int many = AtFeed<E, T, DP, 4>::BYTES, one = AtFeed<E, 32, DP, 1>::BYTES;
-    if (s.waves == 4) {
-        if (what == AT_DQ) hipLaunchKernelGGL((attention_dq_kernel<E, DP, 4, T>), dim3(grid), dim3(256), many, st, p);
-        else hipLaunchKernelGGL((attention_kernel<E, DP, 4, T>), dim3(grid), dim3(256), many, st, p);
-    } else {
-        if (what == AT_DQ) hipLaunchKernelGGL((attention_dq_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), one, st, p);
-        else hipLaunchKernelGGL((attention_kernel<E, DP, 1, 32>), dim3(grid), dim3(64), one, st, p);
-    }
+    const auto queries = [&]<int WAVES, int TILE>() {
+        constexpr int bytes = at_bytes<E, DP, WAVES, TILE>;
+        if (what == AT_DQ) hipLaunchKernelGGL((attention_dq_kernel<E, DP, WAVES, TILE>), dim3(grid), dim3(64 * WAVES), bytes, st, p);
+        else hipLaunchKernelGGL((attention_kernel<E, DP, WAVES, TILE>), dim3(grid), dim3(64 * WAVES), bytes, st, p);
+    };
+    if (s.waves == 4) queries.template operator()<4, at_tile<E>>();
+    else if (s.waves == 2) queries.template operator()<2, 32>();
+    else queries.template operator()<1, 32>();
 }
 template <typename E>
 void at_launch(int what, const AtShape &s, const AttentionP &p, unsigned grid, hipStream_t st)

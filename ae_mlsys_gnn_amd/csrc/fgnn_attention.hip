@@ -34,70 +34,94 @@ __global__ __launch_bounds__(AT_TPB) void attention_delta_kernel(AttentionP p, i
     }
 }
 
-// Parts of the keys joined: Y = sum 2^(lse_s - lse) Y_s over the parts, in their order.  Four components a thread.
-template <typename E>
-__global__ __launch_bounds__(AT_TPB) void attention_join_kernel(AttentionP p)
+// A workgroup's threads on rows of quads of components: `quads` threads (a power of two) a row and share of the parts, `shares` shares of a row's parts (a power of two),
+// the rest rows side by side.
+struct AtJoin { int quads, shares; int64_t rows; };
+struct AtJoinPlace { int64_t row; int d, share; };
+__device__ __forceinline__ AtJoinPlace at_join_place(const AtJoin &j)
 {
-    const int quads = (p.dim + 3) / 4;
-    const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows, total = rows * quads;
-    for (int64_t i = (int64_t)blockIdx.x * AT_TPB + threadIdx.x; i < total; i += (int64_t)gridDim.x * AT_TPB) {
-        const int64_t r = i / quads, group = r / p.rows;
-        const int d = (int)(i - r * quads) * 4, row = (int)(r - group * p.rows), pos = row / p.share, head = (int)(group % p.kv_heads) * p.share + row % p.share;
-        const int64_t at = group * p.splits * p.rows + row, b = group / p.kv_heads;
-        float most = -__builtin_inff();
-        for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.part_lse[at + (int64_t)s * p.rows]);
-        float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int s = 0; s < p.splits; ++s) {
-            const float lse = p.part_lse[at + (int64_t)s * p.rows];
-            if (lse == -__builtin_inff()) continue;             // a part that sees nothing
-            const float w = __builtin_amdgcn_exp2f(lse - most);
-            float u[4];
-            gm_load<float, 4>(u, p.part + (at + (int64_t)s * p.rows) * p.dim + d, p.dim - d);
-            sum += w;
+    const int at = (int)threadIdx.x / j.quads;
+    return {(int64_t)blockIdx.x * (AT_TPB / (j.quads * j.shares)) + at / j.shares, (int)threadIdx.x % j.quads * 4, at % j.shares};
+}
+// The shares' sums, in their order; true for the threads that have them all.
+template <int N>
+__device__ __forceinline__ bool at_join(const AtJoin &j, float (*sums)[AT_TPB], float (&v)[N])
+{
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = fmaf(w, u[j], v[j]);
-        }
-        const bool none = sum == 0.f;
+    for (int i = 0; i < N; ++i) sums[i][threadIdx.x] = v[i];
+    __syncthreads();
+    if (at_join_place(j).share) return false;
+    for (int s = 1; s < j.shares; ++s)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = none ? 0.f : v[j] / sum;
-        gm_store<E, 4>(v, (E *)p.y + ((b * p.nq + pos) * p.heads + head) * p.dim + d, p.dim - d);
-        if (p.lse && d == 0) p.lse[(b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum);
-    }
+        for (int i = 0; i < N; ++i) v[i] += sums[i][threadIdx.x + s * j.quads];
+    return true;
 }
 
-// Sums of parts [splits][n], in their order, to `out`; dQ's come by head of keys and row.
-template <typename E, bool DQ>
-__global__ __launch_bounds__(AT_TPB) void attention_sum_kernel(AttentionP p)
+// Parts of the keys joined: Y = sum 2^(lse_s - lse) Y_s over the parts, in a fixed order.
+template <typename E>
+__global__ __launch_bounds__(AT_TPB) void attention_join_kernel(AttentionP p, AtJoin j)
 {
-    const int quads = (p.dim + 3) / 4;
-    const int64_t rows = DQ ? (int64_t)p.batch * p.kv_heads * p.rows : 2 * (int64_t)p.batch * p.nk * p.kv_heads, total = rows * quads;
-    for (int64_t i = (int64_t)blockIdx.x * AT_TPB + threadIdx.x; i < total; i += (int64_t)gridDim.x * AT_TPB) {
-        const int64_t r = i / quads;
-        const int d = (int)(i - r * quads) * 4;
-        int64_t from, step;
-        E *to;
-        if constexpr (DQ) {
-            const int64_t group = r / p.rows, b = group / p.kv_heads;
-            const int row = (int)(r - group * p.rows), pos = row / p.share, head = (int)(group % p.kv_heads) * p.share + row % p.share;
-            from = group * p.splits * p.rows + row;
-            step = p.rows;
-            to = (E *)p.dq + ((b * p.nq + pos) * p.heads + head) * p.dim;
-        } else {
-            from = r;
-            step = rows;
-            to = r < rows / 2 ? (E *)p.dk + r * p.dim : (E *)p.dv + (r - rows / 2) * p.dim;
-        }
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
+    __shared__ float sums[5][AT_TPB];
+    const AtJoinPlace o = at_join_place(j);
+    const int64_t group = o.row / p.rows, b = group / p.kv_heads;
+    const int row = (int)(o.row - group * p.rows), pos = row / p.share, head = (int)(group % p.kv_heads) * p.share + row % p.share;
+    const bool there = o.row < j.rows;
+    const int64_t at = group * p.splits * p.rows + row;
+    float most = -__builtin_inff(), v[5] = {};
+    if (there) {
+        for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.part_lse[at + (int64_t)s * p.rows]);
 #pragma unroll 4
-        for (int s = 0; s < p.splits; ++s) {
+        for (int s = o.share; s < p.splits; s += j.shares) {
+            const float lse = p.part_lse[at + (int64_t)s * p.rows];
+            if (lse == -__builtin_inff() || o.d >= p.dim) continue;         // a part that sees nothing
+            const float w = __builtin_amdgcn_exp2f(lse - most);
             float u[4];
-            gm_load<float, 4>(u, p.part + (from + s * step) * p.dim + d, p.dim - d);
+            gm_load<float, 4>(u, p.part + (at + (int64_t)s * p.rows) * p.dim + o.d, p.dim - o.d);
+            v[4] += w;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += u[j];
+            for (int i = 0; i < 4; ++i) v[i] = fmaf(w, u[i], v[i]);
         }
-        gm_store<E, 4>(v, to + d, p.dim - d);
     }
+    if (!at_join<5>(j, sums, v) || !there || o.d >= p.dim) return;
+    const bool none = v[4] == 0.f;
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = none ? 0.f : v[i] / v[4];
+    gm_store<E, 4>(y, (E *)p.y + ((b * p.nq + pos) * p.heads + head) * p.dim + o.d, p.dim - o.d);
+    if (p.lse && o.d == 0) p.lse[(b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(v[4]);
+}
+
+// Sums of parts [splits][n], in a fixed order; dQ's come by head of keys and row.
+template <typename E, bool DQ>
+__global__ __launch_bounds__(AT_TPB) void attention_sum_kernel(AttentionP p, AtJoin j)
+{
+    __shared__ float sums[4][AT_TPB];
+    const AtJoinPlace o = at_join_place(j);
+    int64_t from, step;
+    E *to;
+    if constexpr (DQ) {
+        const int64_t group = o.row / p.rows, b = group / p.kv_heads;
+        const int row = (int)(o.row - group * p.rows), pos = row / p.share, head = (int)(group % p.kv_heads) * p.share + row % p.share;
+        from = group * p.splits * p.rows + row;
+        step = p.rows;
+        to = (E *)p.dq + ((b * p.nq + pos) * p.heads + head) * p.dim;
+    } else {
+        from = o.row;
+        step = j.rows;
+        to = o.row < j.rows / 2 ? (E *)p.dk + o.row * p.dim : (E *)p.dv + (o.row - j.rows / 2) * p.dim;
+    }
+    const bool there = o.row < j.rows && o.d < p.dim;
+    float v[4] = {};
+    if (there) {
+#pragma unroll 4
+        for (int s = o.share; s < p.splits; s += j.shares) {
+            float u[4];
+            gm_load<float, 4>(u, p.part + (from + s * step) * p.dim + o.d, p.dim - o.d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += u[i];
+        }
+    }
+    if (at_join<4>(j, sums, v) && there) gm_store<E, 4>(v, to + o.d, p.dim - o.d);
 }
 
 // Rows [batch][n][heads][dim] of any strides and alignment laid out anew, with `wide` components, zeros behind dim.
@@ -140,17 +164,28 @@ static int at_pack(const void *&p, int64_t &sb, int64_t &sn, int64_t &sh, int ba
     return fgnn_launch_status("attention_pack_kernel");
 }
 
+// Rows of parts joined: a share for every four parts, as far as a workgroup's threads go.
+static AtJoin at_joined(int64_t rows, int dim, int splits, unsigned &grid)
+{
+    AtJoin j{1, 1, rows};
+    while (j.quads * 4 < dim) j.quads *= 2;
+    while (j.shares * 4 < splits && j.quads * j.shares < AT_TPB) j.shares *= 2;
+    const int side = AT_TPB / (j.quads * j.shares);
+    grid = (unsigned)((rows + side - 1) / side);
+    return j;
+}
+
 // Waves and tiles of a pass, and the parts that its long side is cut into where there are too few workgroups for the device.
 static AtShape at_shape(AttentionP &p, int what, int type)
 {
     AtShape s;
     s.dim = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
     s.tile = what == AT_DKV ? at_rows_dkv(s.dim, fe_size(type)) : fe_size(type) == 4 ? 32 : 64;
-    s.waves = what != AT_DKV && p.rows <= 64 ? 1 : 4;
-    if (s.waves == 1) s.tile = 32;
+    s.waves = what == AT_DKV || p.rows > 64 ? 4 : p.rows > 32 ? 2 : 1;
+    if (s.waves < 4) s.tile = 32;
     const int64_t columns = what == AT_DKV ? p.nk : p.rows, walked = what == AT_DKV ? (int64_t)((p.nq + s.tile - 1) / s.tile) * p.share : (p.nk + s.tile - 1) / s.tile;
     p.tiles = (int)((columns + 32 * s.waves - 1) / (32 * s.waves));
-    const int64_t groups = std::max<int64_t>(1, (int64_t)p.tiles * p.kv_heads * p.batch), wanted = (int64_t)at_units() * (s.waves == 1 ? 8 : 2);
+    const int64_t groups = std::max<int64_t>(1, (int64_t)p.tiles * p.kv_heads * p.batch), wanted = (int64_t)at_units() * 8 / s.waves;
     const int64_t most = std::max<int64_t>(1, walked / 4);
     p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, wanted / groups), most, 256});
     p.per = (int)((walked + p.splits - 1) / p.splits);
@@ -190,7 +225,7 @@ static int at_run(int what, int type, const AtShape &s, const AttentionP &p, hip
 {
     const int64_t grid = at_grid(p);
     if (grid == 0) return 0;
-    FGNN_REQUIRE(grid < 1LL << 24, FGNN_ERR_LIMIT, "attention: %lld workgroups", (long long)grid);
+    FGNN_REQUIRE(grid < 1LL << 24 && (p.splits < 2 || ((int64_t)p.batch * p.kv_heads * p.rows < 1LL << 24 && (int64_t)p.batch * p.kv_heads * p.nk < 1LL << 23)), FGNN_ERR_LIMIT, "attention: %lld workgroups", (long long)grid);
     fe_dispatch(type, [&]<typename E>() { at_launch<E>(what, s, p, (unsigned)grid, st); });
     return fgnn_launch_status(what == AT_FORWARD ? "attention_kernel" : what == AT_DQ ? "attention_dq_kernel" : "attention_dkv_kernel");
 }
@@ -227,7 +262,9 @@ extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads
     p.part = (float *)space;
     p.part_lse = p.part + (size_t)batch * kv_heads * p.splits * p.rows * dim;
     if ((rc = at_run(AT_FORWARD, type, s, p, st)) || p.splits < 2) return rc;
-    fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_join_kernel<E>), dim3(at_flat((int64_t)batch * nq * heads * ((dim + 3) / 4))), dim3(AT_TPB), 0, st, p); });
+    unsigned grid;
+    const AtJoin j = at_joined((int64_t)batch * nq * heads, dim, p.splits, grid);
+    fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_join_kernel<E>), dim3(grid), dim3(AT_TPB), 0, st, p, j); });
     return fgnn_launch_status("attention_join_kernel");
 }
 
@@ -281,11 +318,13 @@ extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int
         if (at_loose(g, strides + 9, dim, type) && (rc = at_pack(p.g, p.gb, p.gn, p.gh, batch, nq, heads, dim, type, space, st))) return rc;
     }
     p.part = (float *)space;
+    unsigned grid;
     if (dq && nq) {
         const AtShape s = at_shape(p, AT_DQ, type);
         if ((rc = at_run(AT_DQ, type, s, p, st))) return rc;
         if (p.splits > 1) {
-            fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_sum_kernel<E, true>), dim3(at_flat((int64_t)batch * nq * heads * ((dim + 3) / 4))), dim3(AT_TPB), 0, st, p); });
+            const AtJoin j = at_joined((int64_t)batch * nq * heads, dim, p.splits, grid);
+            fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_sum_kernel<E, true>), dim3(grid), dim3(AT_TPB), 0, st, p, j); });
             if ((rc = fgnn_launch_status("attention_sum_kernel"))) return rc;
         }
     }
@@ -293,7 +332,8 @@ extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int
         const AtShape s = at_shape(p, AT_DKV, type);
         if ((rc = at_run(AT_DKV, type, s, p, st))) return rc;
         if (p.splits > 1) {
-            fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_sum_kernel<E, false>), dim3(at_flat(2LL * batch * nk * kv_heads * ((dim + 3) / 4))), dim3(AT_TPB), 0, st, p); });
+            const AtJoin j = at_joined(2LL * batch * nk * kv_heads, dim, p.splits, grid);
+            fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_sum_kernel<E, false>), dim3(grid), dim3(AT_TPB), 0, st, p, j); });
             return fgnn_launch_status("attention_sum_kernel");
         }
     }
