@@ -483,7 +483,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * ROW, p.dim, lane, norm, [&](int r) { return at_result(p, (E *)p.y, o, row - (lane & 31) + r); });
 }
 
-// dQ: as the forward pass, with P from lse.  With parts of the keys, their sums to `part`.
+// dQ: as the forward pass, with P from lse.  With parts of the keys, their sums to `part`.  Forms delta = rowsum(G Y) of its rows, for itself and the pass of dK and dV.
 template <typename E, int DP, int WAVES, int TILE>
 __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_dq_kernel(AttentionP p)
 {
@@ -501,7 +501,18 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     at_row<E, DP>(q, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, row < p.rows, p.dim, lane);
     at_row<E, DP>(g, (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, row < p.rows, p.dim, lane);
     const int64_t stat = ((int64_t)o.b * p.heads + head) * p.nq + pos;
-    const float lse = p.lse[stat] - at_lift<E>, delta = p.delta[stat];
+    const float lse = p.lse[stat] - at_lift<E>;
+    float delta = 0.f;
+    {
+        gm_i4 y[ROW / 32];
+        at_row<E, DP>(y, (const E *)p.y + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, row < p.rows, p.dim, lane);
+#pragma unroll
+        for (int j = 0; j < ROW / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < fe_width<E>; ++i) delta = fmaf((float)((const E *)&y[j])[i], (float)((const E *)&g[j])[i], delta);
+        delta = at_other_sum(delta);
+        if (o.split == 0 && lane < 32 && row < p.rows) p.delta[stat] = delta;
+    }
     AtRange<E, DP / 32> range;
     const int64_t first = (int64_t)o.split * p.per * TILE, last = min(seen.length, first + (int64_t)p.per * TILE);
 

@@ -7,30 +7,27 @@ extern template void at_launch<float>(int, const AtShape &, const AttentionP &, 
 extern template void at_launch<__bf16>(int, const AtShape &, const AttentionP &, unsigned, hipStream_t);
 extern template void at_launch<_Float16>(int, const AtShape &, const AttentionP &, unsigned, hipStream_t);
 
-// delta = rowsum(G Y): `lanes` threads a row.
+// delta = rowsum(G Y) where dQ, whose pass forms it by the way, is not wanted: two threads a row, summed as there.
 template <typename E>
-__global__ __launch_bounds__(AT_TPB) void attention_delta_kernel(AttentionP p, int lanes)
+__global__ __launch_bounds__(AT_TPB) void attention_delta_kernel(AttentionP p)
 {
     constexpr int V = fe_width<E>;
-    const int lane = (int)threadIdx.x % lanes;
-    const int64_t rows = (int64_t)p.batch * p.nq * p.heads, step = (int64_t)gridDim.x * (AT_TPB / lanes);
-    for (int64_t first = (int64_t)blockIdx.x * (AT_TPB / lanes); first < rows; first += step) {
-        const int64_t row = first + threadIdx.x / lanes;
-        float sum = 0.f;
+    const int half = (int)threadIdx.x & 1;
+    const int64_t rows = (int64_t)p.batch * p.nq * p.heads;
+    for (int64_t first = (int64_t)blockIdx.x * (AT_TPB / 2); first < rows; first += (int64_t)gridDim.x * (AT_TPB / 2)) {
+        const int64_t row = first + threadIdx.x / 2, pos = row / p.heads % p.nq, b = row / p.heads / p.nq;
         const int head = (int)(row % p.heads);
-        const int64_t pos = row / p.heads % p.nq, b = row / p.heads / p.nq;
-        if (row < rows) {
-            const int left = p.dim - lane * V;
-            if (left > 0) {
+        float sum = 0.f;
+        if (row < rows)
+            for (int d = half * V; d < p.dim; d += 2 * V) {
                 float y[V], g[V];
-                gm_load<E, V>(y, (const E *)p.y + row * p.dim + lane * V, left);
-                gm_load<E, V>(g, (const E *)p.g + b * p.gb + pos * p.gn + head * p.gh + lane * V, left);
+                gm_load<E, V>(y, (const E *)p.y + row * p.dim + d, p.dim - d);
+                gm_load<E, V>(g, (const E *)p.g + b * p.gb + pos * p.gn + head * p.gh + d, p.dim - d);
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum = fmaf(y[i], g[i], sum);
             }
-        }
-        for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        if (row < rows && lane == 0) p.delta[(b * p.heads + head) * p.nq + pos] = sum;
+        sum += __shfl_xor(sum, 1, 64);
+        if (row < rows && half == 0) p.delta[(b * p.heads + head) * p.nq + pos] = sum;
     }
 }
 
@@ -68,8 +65,13 @@ __global__ __launch_bounds__(AT_TPB) void attention_join_kernel(AttentionP p, At
     const bool there = o.row < j.rows;
     const int64_t at = group * p.splits * p.rows + row;
     float most = -__builtin_inff(), v[5] = {};
+    if (there)
+        for (int s = o.share; s < p.splits; s += j.shares) most = fmaxf(most, p.part_lse[at + (int64_t)s * p.rows]);
+    sums[0][threadIdx.x] = most;
+    __syncthreads();
+    for (int s = 0; s < j.shares; ++s) most = fmaxf(most, sums[0][(int)threadIdx.x + (s - o.share) * j.quads]);
+    __syncthreads();
     if (there) {
-        for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.part_lse[at + (int64_t)s * p.rows]);
 #pragma unroll 4
         for (int s = o.share; s < p.splits; s += j.shares) {
             const float lse = p.part_lse[at + (int64_t)s * p.rows];
@@ -306,12 +308,10 @@ extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int
     if (nq) {
         p.delta = (float *)space;
         space += fgnn_align256((size_t)batch * heads * nq * sizeof(float));
-        int lanes = 1;
-        while (lanes * (16 / fe_size(type)) < dim) lanes *= 2;
-        fe_dispatch(type, [&]<typename E>() {
-            hipLaunchKernelGGL((attention_delta_kernel<E>), dim3(at_flat((int64_t)batch * nq * heads * lanes)), dim3(AT_TPB), 0, st, p, lanes);
-        });
-        if ((rc = fgnn_launch_status("attention_delta_kernel"))) return rc;
+        if (!dq) {
+            fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_delta_kernel<E>), dim3(at_flat(2LL * batch * nq * heads)), dim3(AT_TPB), 0, st, p); });
+            if ((rc = fgnn_launch_status("attention_delta_kernel"))) return rc;
+        }
         if (at_loose(q, strides, dim, type) && (rc = at_pack(p.q, p.qb, p.qn, p.qh, batch, nq, heads, dim, type, space, st))) return rc;
         if (at_loose(k, strides + 3, dim, type) && (rc = at_pack(p.k, p.kb, p.kn, p.kh, batch, nk, kv_heads, dim, type, space, st))) return rc;
         if (at_loose(v, strides + 6, dim, type) && (rc = at_pack(p.v, p.vb, p.vn, p.vh, batch, nk, kv_heads, dim, type, space, st))) return rc;
