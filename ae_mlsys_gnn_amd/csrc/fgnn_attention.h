@@ -222,13 +222,30 @@ struct AtFeed {
     }
 };
 
-// One row as the second operand of products: its chunks 2 j + (lane / 32).  Any alignment.
+// One row as the second operand of products: its chunks 2 j + (lane / 32), zeros past the last and where it is not there (`row` is memory that may be read all the same).  Any
+// alignment; rows of whole 16 bytes are asked for at once.
 template <typename E, int DP>
 __device__ __forceinline__ void at_row(gm_i4 (&cols)[DP * (int)sizeof(E) / 32], const E *row, bool there, int dim, int lane)
 {
-    constexpr int V = fe_width<E>;
+    constexpr int V = fe_width<E>, N = DP * (int)sizeof(E) / 32;
+    if (dim % V == 0) {
+        typedef typename fe_vec<E>::type vec;
 #pragma unroll
-    for (int j = 0; j < DP * (int)sizeof(E) / 32; ++j) {
+        for (int j = 0; j < N; ++j) {
+            const int at = (2 * j + (lane >> 5)) * V;
+            const vec v = *reinterpret_cast<const vec *>(row + (at < dim ? at : 0));
+            cols[j] = *(const gm_i4 *)&v;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const bool in = there && (2 * j + (lane >> 5)) * V < dim;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cols[j][i] = in ? cols[j][i] : 0;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
         const int at = (2 * j + (lane >> 5)) * V;
         E v[V];
         gm_load<E, V>(v, row + (there && at < dim ? at : 0), there ? dim - at : 0);
@@ -252,6 +269,8 @@ __device__ __forceinline__ float at_other_sum(float v)
 // fp16 has 2^-14 as its smallest number of all significant bits, where softmax weights of long rows and gradients lie below: weights are rounded times 2^15
 // (they are 1 at the most), gradients of scores times a power of two of the column's own that brings its largest so far to 2^14 .. 2^15.
 template <typename E> constexpr float at_lift = std::is_same_v<E, _Float16> ? 15.f : 0.f;      // as an exponent
+constexpr float AT_SLACK = 8.f;             // of the forward pass's maximum, as an exponent: its weights reach 2^8
+template <typename E> constexpr float at_lift_forward = std::is_same_v<E, _Float16> ? 15.f - AT_SLACK : 0.f;
 template <typename E, int STEPS>
 struct AtRange {
     float f = std::is_same_v<E, _Float16> ? 0x1p96f : 1.f;
@@ -436,8 +455,11 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
         top = at_other_max(top) * p.log2_scale;
-        if (__ballot(top > most)) {
-            const float now = fmaxf(top, most), f = most > -__builtin_inff() ? __builtin_amdgcn_exp2f(most - now) : 0.f;
+        // Weights relative to a maximum that is too low by less than 2^8 are as exact and far from overflowing: only above that are sums and results scaled anew (one of 32
+        // columns asks for a higher maximum in almost every tile of a short row), each column for itself, so that its result does not depend on its neighbours.
+        const bool over = top > most + AT_SLACK;
+        if (__ballot(over)) {
+            const float now = over ? top : most, f = most > -__builtin_inff() ? __builtin_amdgcn_exp2f(most - now) : 0.f;
             most = now;
             sum *= f;
 #pragma unroll
@@ -445,7 +467,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[t][i] *= f;
         }
-        const float base = (most > -__builtin_inff() ? most : 0.f) - at_lift<E>;
+        const float base = (most > -__builtin_inff() ? most : 0.f) - at_lift_forward<E>;
         auto weigh = [&](int t) {
             float w[16];
 #pragma unroll
@@ -475,10 +497,10 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
         if (row >= p.rows) return;
         const int64_t to = (((int64_t)o.b * p.kv_heads + o.head) * p.splits + o.split) * p.rows + row;
         at_store_part<DP>(acc, p.part + to * p.dim, p.dim, lane, norm);
-        if (lane < 32) p.part_lse[to] = none ? -__builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
+        if (lane < 32) p.part_lse[to] = none ? -__builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift_forward<E>;
         return;
     }
-    if (p.lse && lane < 32 && row < p.rows) p.lse[((int64_t)o.b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift<E>;
+    if (p.lse && lane < 32 && row < p.rows) p.lse[((int64_t)o.b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift_forward<E>;
     __syncthreads();                        // the last tile has been read
     at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * ROW, p.dim, lane, norm, [&](int r) { return at_result(p, (E *)p.y, o, row - (lane & 31) + r); });
 }
@@ -593,9 +615,10 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 // dK and dV: a wave owns 32 keys and walks the queries of every head that uses them, tile by tile.  Where their sums leave no room in the registers the keys wait in LDS (their
 // values stay): two waves a SIMD at 128 components, where one alone waits for LDS before every instruction.
 constexpr bool at_keys_in_lds(int dim, int size) { return size == 2 && dim >= 128; }
-constexpr int at_rows_dkv(int dim, int size) { return size == 4 || dim >= 128 ? 32 : 64; }
+// 32 rows a tile: three waves a SIMD at 64 components of 16 bits, where with 64 rows it is two (64 queries to 232,965 keys, 8 heads: 302 us for 262).
+constexpr int AT_ROWS_DKV = 32;
 template <typename E, int DP, int WAVES, int TILE>
-__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_dkv_kernel(AttentionP p)
+__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(E) > 128 ? 2 : 3) void attention_dkv_kernel(AttentionP p)
 {
     constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, STEPS = DP / 32;
     constexpr bool KEYS_IN_LDS = at_keys_in_lds(DP, SIZE);
@@ -704,7 +727,7 @@ template <typename E, int DP>
 static void at_launch_dim(int what, const AtShape &s, const AttentionP &p, unsigned grid, hipStream_t st)
 {
     if (what == AT_DKV) {
-        constexpr int S = (int)sizeof(E), R = at_rows_dkv(DP, S), bytes = at_bytes<E, DP, 4, R> + 4 * R * (int)sizeof(float) + (at_keys_in_lds(DP, S) ? 128 * DP * S : 0);
+        constexpr int S = (int)sizeof(E), R = AT_ROWS_DKV, bytes = at_bytes<E, DP, 4, R> + 4 * R * (int)sizeof(float) + (at_keys_in_lds(DP, S) ? 128 * DP * S : 0);
         hipLaunchKernelGGL((attention_dkv_kernel<E, DP, 4, R>), dim3(grid), dim3(256), bytes, st, p);
         return;
     }

@@ -182,7 +182,7 @@ static AtShape at_shape(AttentionP &p, int what, int type)
 {
     AtShape s;
     s.dim = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
-    s.tile = what == AT_DKV ? at_rows_dkv(s.dim, fe_size(type)) : fe_size(type) == 4 ? 32 : 64;
+    s.tile = what == AT_DKV ? AT_ROWS_DKV : fe_size(type) == 4 ? 32 : 64;
     s.waves = what == AT_DKV || p.rows > 64 ? 4 : p.rows > 32 ? 2 : 1;
     if (s.waves < 4) s.tile = 32;
     const int64_t columns = what == AT_DKV ? p.nk : p.rows, walked = what == AT_DKV ? (int64_t)((p.nq + s.tile - 1) / s.tile) * p.share : (p.nk + s.tile - 1) / s.tile;
