@@ -9,8 +9,9 @@
 // rounded, the second operand of the next product as they lie: the order of a reduction is free as long as both operands have the same, and the first operand, the tile
 // transposed, is read from LDS in that order.
 //
-// 16-bit types: products of 16-bit values, P and dS rounded to the type (as the values they are multiplied with are), sums, statistics and results in 32 bits.  fp32: the
-// matrix instruction of fp32, everything in 32 bits.
+// 16-bit types: products of 16-bit values, P and dS rounded to the type (as the values they are multiplied with are), sums, statistics and results in 32 bits.  fp32: every
+// operand in three planes of 8 significant bits (bf16, truncated, so that they add up to it exactly), and the six products that reach above 2^-24 of the result, small ones
+// first: the matrix unit does 16 of them in the time of one fp32 product.  Infinities in fp32 operands have planes that are NaN.
 #pragma once
 #include "fgnn_gemm.h"
 
@@ -29,127 +30,146 @@ struct AttentionP {
     float *part, *part_lse;                                     // sums of the parts
 };
 
-template <typename E> struct AtKind { static constexpr int V = fe_width<E>, SIZE = (int)sizeof(E); };
-// Rows of a tile that lies in LDS.
+// Planes of an operand, as 16-bit values; rows of a tile that lies in LDS.
+template <typename E> constexpr int at_planes = sizeof(E) == 4 ? 3 : 1;
 template <typename E> constexpr int at_tile = sizeof(E) == 4 ? 32 : 64;
+constexpr int AT_CHUNK = 8;                 // components of 16 bytes of a plane
 
-// 16-byte chunk `ch` of row `row` in a tile of ROW bytes a row.  LDS has 64 banks of four bytes: chunks are exchanged so that the reads meet each of them once, sixteen rows at
-// one chunk, and four rows at four chunks next to one another (16-bit types) or two rows, four apart, at eight (fp32).  What is exchanged is linear in the row's bits.
-template <int ROW, int SIZE>
+// 16-byte chunk `ch` of row `row` in a plane of ROW bytes a row.  LDS has 64 banks of four bytes: chunks are exchanged so that the reads meet each of them once, sixteen rows at
+// one chunk, and four rows at four chunks next to one another.  What is exchanged is linear in the row's bits.
+template <int ROW>
 __host__ __device__ constexpr int at_exchange(int row)
 {
     if (ROW % 128) return (row >> 2) & 3;
     if (ROW % 256) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
-    if (SIZE == 4) return ((row >> 2) & 1) << 3 | (row & 3) << 1 | ((row >> 3) & 1);
     return (row & 3) << 2 | ((row >> 2) & 3);
 }
-template <int ROW, int SIZE>
-__device__ __forceinline__ int at_place(int row, int ch) { return row * ROW + ((ch ^ at_exchange<ROW, SIZE>(row)) << 4); }
+template <int ROW>
+__device__ __forceinline__ int at_place(int row, int ch) { return row * ROW + ((ch ^ at_exchange<ROW>(row)) << 4); }
 
-// Where a lane reads tiles of DP components: its row's first chunk for scores, and the first of what the reads of the transposed tile below say.  The others' places differ from these
-// in bits of the chunk index that are exchanged (an exclusive or with a constant; eight registers for as many places and the sums of dK and dV left no room for two waves) and in
-// constant offsets.
+// Where a lane reads planes of DP components: its row's first chunk for scores, and the first of what the reads of the transposed tile below say.  The others' places differ from
+// these in bits of the chunk index that are exchanged (an exclusive or with a constant; eight registers for as many places and the sums of dK and dV left no room for two waves)
+// and in constant offsets.
 template <typename T> __device__ __forceinline__ auto at_lds(uint32_t at) { return (__attribute__((address_space(3))) T *)(uintptr_t)at; }
-template <typename E, int DP>
+template <int DP>
 struct AtReader {
-    static constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, MASK = ROW % 128 ? 3 : ROW % 256 ? 7 : 15;     // exchanged bits of the chunk index
+    static constexpr int ROW = DP * 2, STEPS = ROW / 32, MASK = ROW % 128 ? 3 : ROW % 256 ? 7 : 15;     // STEPS: instructions of a score; MASK: exchanged bits of the chunk index
     uint32_t score, gather;
     __device__ __forceinline__ void init(int lane)
     {
         const int h = lane >> 5, r = lane & 15;
-        score = at_place<ROW, SIZE>(lane & 31, h);
-        // fp32: row 4 h + i, component lane % 32; else row 4 h + r / 4, four components from 16 ((lane / 16) % 2) + 4 (r % 4) on
-        gather = SIZE == 4 ? at_place<ROW, SIZE>(4 * h, (lane & 31) >> 2) + (lane & 3) * 4 : at_place<ROW, SIZE>(4 * h + (r >> 2), 2 * ((lane >> 4) & 1) + ((r & 3) >> 1)) + (r & 1) * 8;
+        score = at_place<ROW>(lane & 31, h);
+        // row 4 h + r / 4, four components from 16 ((lane / 16) % 2) + 4 (r % 4) on
+        gather = at_place<ROW>(4 * h + (r >> 2), 2 * ((lane >> 4) & 1) + ((r & 3) >> 1)) + (r & 1) * 8;
     }
-    // `from` (of a tile that starts at a multiple of 256 bytes), `chunks` chunks and `rows` rows further on; both constants, of bits that the lanes' own do not have
-    static __device__ __forceinline__ uint32_t to(uint32_t from, int chunks, int rows) { return (from ^ (((chunks & MASK) ^ at_exchange<ROW, SIZE>(rows)) << 4)) + (chunks & ~MASK) * 16 + rows * ROW; }
+    // `from` (of a plane that starts at a multiple of 256 bytes), `chunks` chunks and `rows` rows further on; both constants, of bits that the lanes' own do not have
+    static __device__ __forceinline__ uint32_t to(uint32_t from, int chunks, int rows) { return (from ^ (((chunks & MASK) ^ at_exchange<ROW>(rows)) << 4)) + (chunks & ~MASK) * 16 + rows * ROW; }
 };
 
 template <typename E>
 __device__ __forceinline__ at_f16 at_multiply(gm_i4 a, gm_i4 b, at_f16 c)
 {
-    if constexpr (sizeof(E) == 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__int_as_float(a[j]), __int_as_float(b[j]), c, 0, 0, 0);
-        return c;
-    } else if constexpr (std::is_same_v<E, _Float16>) return __builtin_amdgcn_mfma_f32_32x32x16_f16(*(gm_h8 *)&a, *(gm_h8 *)&b, c, 0, 0, 0);
+    if constexpr (std::is_same_v<E, _Float16>) return __builtin_amdgcn_mfma_f32_32x32x16_f16(*(gm_h8 *)&a, *(gm_h8 *)&b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(gm_b8 *)&a, *(gm_b8 *)&b, c, 0, 0, 0);
 }
-
-// The scores of 32 rows of a tile (from row0 on, a multiple of 32) with the wave's columns.
-template <typename E, int DP>
-__device__ __forceinline__ at_f16 at_scores(const AtReader<E, DP> &at, uint32_t tile, int row0, const gm_i4 (&cols)[DP * (int)sizeof(E) / 32])
+// The products of two operands' planes
+template <typename E, int P>
+__device__ __forceinline__ at_f16 at_planes_multiply(const gm_i4 (&a)[P], const gm_i4 (&b)[P], at_f16 c)
 {
-    typedef AtReader<E, DP> R;
+#pragma unroll
+    for (int s = P - 1; s >= 0; --s)
+#pragma unroll
+        for (int h = 0; h <= s; ++h) c = at_multiply<E>(a[s - h], b[h], c);
+    return c;
+}
+// Columns as second operands: [STEPS][planes]
+template <typename E, int DP> struct AtColumns { gm_i4 c[AtReader<DP>::STEPS][at_planes<E>]; };
+
+// The scores of 32 rows of a tile (from row0 on, a multiple of 32) with the wave's columns.  plane: bytes from a plane to the next.
+template <typename E, int DP>
+__device__ __forceinline__ at_f16 at_scores(const AtReader<DP> &at, uint32_t tile, int plane, int row0, const AtColumns<E, DP> &cols)
+{
+    typedef AtReader<DP> R;
+    constexpr int P = at_planes<E>;
     at_f16 s = {};
 #pragma unroll
-    for (int j = 0; j < R::ROW / 32; ++j) s = at_multiply<E>(*at_lds<gm_i4>(R::to(tile + at.score, 2 * j, row0)), cols[j], s);
+    for (int j = 0; j < R::STEPS; ++j) {
+        gm_i4 a[P];
+#pragma unroll
+        for (int h = 0; h < P; ++h) a[h] = *at_lds<gm_i4>(R::to(tile + at.score, 2 * j, row0) + h * plane);
+        s = at_planes_multiply<E, P>(a, cols.c[j], s);
+    }
+    return s;
+}
+// The same with the columns, of one plane, in LDS too, from `cols` on.
+template <typename E, int DP>
+__device__ __forceinline__ at_f16 at_scores(const AtReader<DP> &at, uint32_t tile, int row0, uint32_t cols)
+{
+    typedef AtReader<DP> R;
+    at_f16 s = {};
+#pragma unroll
+    for (int j = 0; j < R::STEPS; ++j) s = at_multiply<E>(*at_lds<gm_i4>(R::to(tile + at.score, 2 * j, row0)), *at_lds<gm_i4>(R::to(cols + at.score, 2 * j, 0)), s);
     return s;
 }
 
-// The same with the columns in LDS too, from `cols` on.
-template <typename E, int DP>
-__device__ __forceinline__ at_f16 at_scores(const AtReader<E, DP> &at, uint32_t tile, int row0, uint32_t cols)
-{
-    typedef AtReader<E, DP> R;
-    at_f16 s = {};
-#pragma unroll
-    for (int j = 0; j < R::ROW / 32; ++j) s = at_multiply<E>(*at_lds<gm_i4>(R::to(tile + at.score, 2 * j, row0)), *at_lds<gm_i4>(R::to(cols + at.score, 2 * j, 0)), s);
-    return s;
-}
-
-// 16 of a column's 32 weights as the second operand of products, rounded to the type.
+// 16 of a column's 32 weights as second operands: rounded to the type, or in planes.
 template <typename E> struct AtWeights {
-    typedef E vec __attribute__((ext_vector_type(16)));
-    vec w;
+    gm_i4 w[2][at_planes<E>];
     __device__ __forceinline__ explicit AtWeights(const float (&v)[16])
     {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = (E)v[i];
+        for (int s = 0; s < 2; ++s) {
+            if constexpr (sizeof(E) == 4) {
+                uint32_t bits[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) bits[i] = __float_as_uint(v[8 * s + i]);
+                gm_split(bits, w[s]);
+            } else {
+                typedef E e8 __attribute__((ext_vector_type(8)));
+                e8 b;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[i] = (E)v[8 * s + i];
+                w[s][0] = *(const gm_i4 *)&b;
+            }
+        }
     }
 };
 // acc[t] (32 components from 32 t on, by the wave's columns) += (32 rows of a tile, from row0 on)^T w
 template <typename E, int DP>
-__device__ __forceinline__ void at_gather(const AtReader<E, DP> &at, uint32_t tile, int row0, const AtWeights<E> &weights, at_f16 (&acc)[DP / 32])
+__device__ __forceinline__ void at_gather(const AtReader<DP> &at, uint32_t tile, int plane, int row0, const AtWeights<E> &weights, at_f16 (&acc)[DP / 32])
 {
-    const auto &w = weights.w;
-    typedef AtReader<E, DP> R;
-    if constexpr (sizeof(E) == 4) {
+    typedef AtReader<DP> R;
+    constexpr int P = at_planes<E>;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
-                acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(*at_lds<float>(R::to(tile + at.gather, 8 * t, row0 + 8 * (i / 4) + i % 4)), w[i], acc[t], 0, 0, 0);
-    } else {
+        for (int t = 0; t < DP / 32; ++t) {
+            // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
+            typedef short s8 __attribute__((ext_vector_type(8)));
+            gm_i4 a[P];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            typedef E e8 __attribute__((ext_vector_type(8)));
-            e8 b;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = w[8 * s + i];
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t) {
-                // the transposing read: 16 lanes give four rows of 16 values (four a lane) and get a column of four each
-                typedef short s8 __attribute__((ext_vector_type(8)));
-                const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<gm_s4>(R::to(tile + at.gather, 4 * t, row0 + 16 * s)));
-                const gm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<gm_s4>(R::to(tile + at.gather, 4 * t, row0 + 16 * s + 8)));
-                const s8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[t] = at_multiply<E>(*(const gm_i4 *)&a, *(const gm_i4 *)&b, acc[t]);
+            for (int h = 0; h < P; ++h) {
+                const gm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<gm_s4>(R::to(tile + at.gather, 4 * t, row0 + 16 * s) + h * plane));
+                const gm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<gm_s4>(R::to(tile + at.gather, 4 * t, row0 + 16 * s + 8) + h * plane));
+                const s8 u = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                a[h] = *(const gm_i4 *)&u;
             }
+            acc[t] = at_planes_multiply<E, P>(a, weights.w[s], acc[t]);
         }
-    }
 }
 
-// Asks that the N matrix instructions of the code around it come one by one, their reads of LDS, READS each, AHEAD of them before the first (left alone the compiler reads each
-// operand right before its instruction and waits for it), and in the shadow of each VALU instructions of other arithmetic and EXPS exponentials.
-template <int N, int READS, int AHEAD, int VALU = 0, int EXPS = 0>
+// Asks that the matrix instructions of the code around it come for N operands from LDS one after the other, their reads (READS for each plane) AHEAD of them before the first (left
+// alone the compiler reads each operand right before its instruction and waits for it), and in the shadow of each operand's VALU instructions of other arithmetic and EXPS
+// exponentials.
+template <int N, int PLANES, int READS, int AHEAD, int VALU = 0, int EXPS = 0>
 __device__ __forceinline__ void at_ahead()
 {
-    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+    constexpr int R = READS * PLANES, M = PLANES * (PLANES + 1) / 2;
+    __builtin_amdgcn_sched_group_barrier(0x100, R * AHEAD, 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (i < N - AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+        if (i < N - AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
         if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
         if (EXPS) __builtin_amdgcn_sched_group_barrier(0x400, EXPS, 0);
     }
@@ -159,20 +179,20 @@ __device__ __forceinline__ void at_ahead()
 // set) and components past the last are zeros: out of the buffer's range.
 template <typename E, int ROWS, int DP, int WAVES>
 struct AtFeed {
-    static constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, CH = ROW / 16, THREADS = 64 * WAVES, TILE = ROWS * ROW;
-    static constexpr bool MOVED = SIZE == 2;                    // straight to LDS, into two places in turn; else through registers
+    static constexpr int SIZE = (int)sizeof(E), ROW = DP * 2, CH = ROW / 16, THREADS = 64 * WAVES, PLANE = ROWS * ROW, TILE = at_planes<E> * PLANE, WORDS = SIZE * AT_CHUNK / 16;
+    static constexpr bool MOVED = SIZE == 2;                    // straight to LDS, into two places in turn; else through registers, where it is taken apart
     static constexpr int COUNT = ROWS * CH / THREADS, STEP = THREADS / CH;          // chunks a thread, and rows between them
     static constexpr int BYTES = (MOVED ? 2 : 1) * 2 * TILE;
     static_assert(ROWS * CH % THREADS == 0 && THREADS % CH == 0, "threads share a tile evenly");
-    uint32_t lds; int row, ch, left;        // lds: address there; left: components from the first chunk on
-    gm_i4 w[MOVED ? 1 : 2][MOVED ? 1 : COUNT];
+    uint32_t lds; int row, ch, left;        // lds: address there; left: components
+    gm_i4 w[MOVED ? 1 : 2][MOVED ? 1 : COUNT][WORDS];
 
     __device__ __forceinline__ void init(char *lds_, int dim)
     {
         lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds_;
         row = (int)threadIdx.x / CH;
         ch = (int)threadIdx.x % CH;
-        if constexpr (MOVED) ch ^= at_exchange<ROW, SIZE>(row);       // the chunk that belongs where the thread's first transfer ends
+        if constexpr (MOVED) ch ^= at_exchange<ROW>(row);       // the chunk that belongs where the thread's first transfer ends
         left = dim;
     }
     // The pair `index` from a and b on.
@@ -183,11 +203,11 @@ struct AtFeed {
         for (int which = 0; which < 2; ++which) {
             const void *base = which ? b : a;
             const uint32_t step = (uint32_t)((which ? stride_b : stride_a) * SIZE);
-            auto at = [&](int c) {
+            auto at = [&](int c, int word) {
                 // (rows of a thread are a power of two apart: what is exchanged changes by a constant)
-                const int chunk = MOVED ? ch ^ at_exchange<ROW, SIZE>(c * STEP) : ch;
-                const bool there = (bits == ALL || ((bits >> (row + c * STEP)) & 1)) && chunk * (16 / SIZE) < left;
-                return there ? (row + c * STEP) * step + chunk * 16 : 0x80000000u;
+                const int chunk = MOVED ? ch ^ at_exchange<ROW>(c * STEP) : ch;
+                const bool there = (bits == ALL || ((bits >> (row + c * STEP)) & 1)) && chunk * AT_CHUNK + word * (16 / SIZE) < left;
+                return there ? (row + c * STEP) * step + (chunk * WORDS + word) * 16 : 0x80000000u;
             };
             if constexpr (MOVED) {
                 // (written out, and its waits with it: see GemmMover)
@@ -196,11 +216,13 @@ struct AtFeed {
                 const uint32_t to = lds + ((index & 1) * 2 + which) * TILE + fg_wave() * 1024;
 #pragma unroll
                 for (int c = 0; c < COUNT; ++c)
-                    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at(c)), "s"(buffer), "{m0}"(to + c * THREADS * 16));
+                    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at(c, 0)), "s"(buffer), "{m0}"(to + c * THREADS * 16));
             } else {
                 const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, 0x80000000u, 0x00027000);
 #pragma unroll
-                for (int c = 0; c < COUNT; ++c) w[which][c] = __builtin_amdgcn_raw_buffer_load_b128(from, at(c), 0, 0);
+                for (int c = 0; c < COUNT; ++c)
+#pragma unroll
+                    for (int i = 0; i < WORDS; ++i) w[which][c][i] = __builtin_amdgcn_raw_buffer_load_b128(from, at(c, i), 0, 0);
             }
         }
     }
@@ -215,42 +237,74 @@ struct AtFeed {
 #pragma unroll
             for (int which = 0; which < 2; ++which)
 #pragma unroll
-                for (int c = 0; c < COUNT; ++c) *at_lds<gm_i4>(lds + which * TILE + at_place<ROW, SIZE>(row + c * STEP, ch)) = w[which][c];
+                for (int c = 0; c < COUNT; ++c) {
+                    uint32_t bits[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) bits[i] = (uint32_t)w[which][c][i / 4][i % 4];
+                    gm_i4 part[3];
+                    gm_split(bits, part);
+#pragma unroll
+                    for (int h = 0; h < 3; ++h) *at_lds<gm_i4>(lds + which * TILE + h * PLANE + at_place<ROW>(row + c * STEP, ch)) = part[h];
+                }
             __syncthreads();
             return lds;
         }
     }
 };
 
+// AT_CHUNK components of a row, zeros past the last.  Any alignment.
+template <typename E>
+__device__ __forceinline__ void at_chunk(gm_i4 (&words)[sizeof(E) * AT_CHUNK / 16], const E *p, int left)
+{
+    constexpr int V = fe_width<E>;
+#pragma unroll
+    for (int w = 0; w < (int)sizeof(E) * AT_CHUNK / 16; ++w) {
+        E v[V];
+        gm_load<E, V>(v, p + (w * V < left ? w * V : 0), left - w * V);
+#pragma unroll
+        for (int i = 0; i < V; ++i) ((E *)&words[w])[i] = v[i];
+    }
+}
 // One row as the second operand of products: its chunks 2 j + (lane / 32), zeros past the last and where it is not there (`row` is memory that may be read all the same).  Any
 // alignment; rows of whole 16 bytes are asked for at once.
 template <typename E, int DP>
-__device__ __forceinline__ void at_row(gm_i4 (&cols)[DP * (int)sizeof(E) / 32], const E *row, bool there, int dim, int lane)
+__device__ __forceinline__ void at_row(AtColumns<E, DP> &cols, const E *row, bool there, int dim, int lane)
 {
-    constexpr int V = fe_width<E>, N = DP * (int)sizeof(E) / 32;
+    constexpr int V = fe_width<E>, N = AtReader<DP>::STEPS, WORDS = (int)sizeof(E) * AT_CHUNK / 16;
+    gm_i4 words[N][WORDS];
     if (dim % V == 0) {
         typedef typename fe_vec<E>::type vec;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = (2 * j + (lane >> 5)) * V;
-            const vec v = *reinterpret_cast<const vec *>(row + (at < dim ? at : 0));
-            cols[j] = *(const gm_i4 *)&v;
-        }
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+                const int at = (2 * j + (lane >> 5)) * AT_CHUNK + w * V;
+                const vec v = *reinterpret_cast<const vec *>(row + (at < dim ? at : 0));
+                words[j][w] = *(const gm_i4 *)&v;
+            }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+                const bool in = there && (2 * j + (lane >> 5)) * AT_CHUNK + w * V < dim;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) words[j][w][i] = in ? words[j][w][i] : 0;
+            }
+    } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const bool in = there && (2 * j + (lane >> 5)) * V < dim;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) cols[j][i] = in ? cols[j][i] : 0;
+            const int at = (2 * j + (lane >> 5)) * AT_CHUNK;
+            at_chunk<E>(words[j], row + (there && at < dim ? at : 0), there ? dim - at : 0);
         }
-        return;
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const int at = (2 * j + (lane >> 5)) * V;
-        E v[V];
-        gm_load<E, V>(v, row + (there && at < dim ? at : 0), there ? dim - at : 0);
+        if constexpr (sizeof(E) == 4) {
+            uint32_t bits[8];
 #pragma unroll
-        for (int i = 0; i < V; ++i) ((E *)&cols[j])[i] = v[i];
+            for (int i = 0; i < 8; ++i) bits[i] = (uint32_t)words[j][i / 4][i % 4];
+            gm_split(bits, cols.c[j]);
+        } else cols.c[j][0] = words[j][0];
     }
 }
 
@@ -375,13 +429,13 @@ __device__ __forceinline__ void at_store(const at_f16 (&acc)[DP / 32], uint32_t 
         for (int i = 0; i < 4; ++i) {
             const int d = 32 * t + 8 * i + 4 * (lane >> 5);
             const e4 v = {(E)f(acc[t][4 * i]), (E)f(acc[t][4 * i + 1]), (E)f(acc[t][4 * i + 2]), (E)f(acc[t][4 * i + 3])};
-            *at_lds<e4>(lds + at_place<ROW, SIZE>(lane & 31, d / V) + d % V * SIZE) = v;
+            *at_lds<e4>(lds + at_place<ROW>(lane & 31, d / V) + d % V * SIZE) = v;
         }
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) {
         const int r = (i * 64 + lane) / CH, ch = (i * 64 + lane) % CH;
         typedef E vec __attribute__((ext_vector_type(V)));
-        const vec u = *at_lds<vec>(lds + at_place<ROW, SIZE>(r, ch));
+        const vec u = *at_lds<vec>(lds + at_place<ROW>(r, ch));
         E *row = to(r), v[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = u[j];
@@ -393,9 +447,9 @@ template <typename E, int DP, int WAVES, int TILE> constexpr int at_bytes = std:
 
 // Y and lse.  With `splits` parts of the keys, normalised sums and lse of each to `part`.
 template <typename E, int DP, int WAVES, int TILE>
-__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_kernel(AttentionP p)
+__global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void attention_kernel(AttentionP p)
 {
-    constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE;
+    constexpr int P = at_planes<E>, STEPS = AtReader<DP>::STEPS;
     extern __shared__ __attribute__((aligned(256))) char lds[];
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
@@ -405,7 +459,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     AtSeen<TILE> seen;
     seen.init(p, o.b, lane);
     const E *k = (const E *)p.k + o.b * p.kb + o.head * p.kh, *v = (const E *)p.v + o.b * p.vb + o.head * p.vh;
-    gm_i4 q[ROW / 32];
+    AtColumns<E, DP> q;
     at_row<E, DP>(q, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, row < p.rows, p.dim, lane);
     const int64_t first = (int64_t)o.split * p.per * TILE, last = min(seen.length, first + (int64_t)p.per * TILE);
 
@@ -413,9 +467,10 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) acc[t] = at_f16{};
     float most = -__builtin_inff(), sum = 0.f;
-    AtFeed<E, TILE, DP, WAVES> feed;
+    typedef AtFeed<E, TILE, DP, WAVES> Feed;
+    Feed feed;
     feed.init(lds, p.dim);
-    AtReader<E, DP> at;
+    AtReader<DP> at;
     at.init(lane);
     uint64_t bits = 0, coming = 0;
     if (first < last) {
@@ -427,7 +482,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     int index = 0;
 #pragma unroll 1
     for (int64_t key = first; key < last; key += TILE, bits = coming, ++index) {
-        const uint32_t lk = feed.arrive(index), lv = lk + TILE * ROW;
+        const uint32_t lk = feed.arrive(index), lv = lk + Feed::TILE;
         if (key + TILE < last) {
             coming = seen.take(key + TILE);
             seen.ask(key + 2 * TILE);
@@ -438,8 +493,8 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
         at_f16 s[B];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < B; ++t) s[t] = at_scores<E, DP>(at, lk, 32 * t, q);
-        if constexpr (SIZE == 2) at_ahead<B * ROW / 32, 1, 4>();
+        for (int t = 0; t < B; ++t) s[t] = at_scores<E, DP>(at, lk, Feed::PLANE, 32 * t, q);
+        at_ahead<B * STEPS, P, 1, P == 1 ? 4 : 2>();
         __builtin_amdgcn_sched_barrier(0);
         if (bits != (TILE == 64 ? ~0ull : (1ull << TILE) - 1)) {
 #pragma unroll
@@ -481,11 +536,11 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
 #pragma unroll
         for (int t = 0; t < B; ++t) {
             __builtin_amdgcn_sched_barrier(0);
-            at_gather<E, DP>(at, lv, 32 * t, w, acc);
+            at_gather<E, DP>(at, lv, Feed::PLANE, 32 * t, w, acc);
             if (t + 1 < B) {
                 w = weigh(t + 1);
-                if constexpr (SIZE == 2) at_ahead<ROW / 32, 2, 3, 640 / ROW * 2, 512 / ROW>();
-            } else if constexpr (SIZE == 2) at_ahead<ROW / 32, 2, 3>();
+                at_ahead<DP / 16, P, 2, P == 1 ? 3 : 1, 640 / DP, 256 / DP>();
+            } else at_ahead<DP / 16, P, 2, P == 1 ? 3 : 1>();
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -502,14 +557,14 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     }
     if (p.lse && lane < 32 && row < p.rows) p.lse[((int64_t)o.b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(sum) - at_lift_forward<E>;
     __syncthreads();                        // the last tile has been read
-    at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * ROW, p.dim, lane, norm, [&](int r) { return at_result(p, (E *)p.y, o, row - (lane & 31) + r); });
+    at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * DP * (int)sizeof(E), p.dim, lane, norm, [&](int r) { return at_result(p, (E *)p.y, o, row - (lane & 31) + r); });
 }
 
 // dQ: as the forward pass, with P from lse.  With parts of the keys, their sums to `part`.  Forms delta = rowsum(G Y) of its rows, for itself and the pass of dK and dV.
 template <typename E, int DP, int WAVES, int TILE>
-__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void attention_dq_kernel(AttentionP p)
+__global__ __launch_bounds__(64 * WAVES, DP > (sizeof(E) == 4 ? 64 : 128) ? 1 : 2) void attention_dq_kernel(AttentionP p)
 {
-    constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE;
+    constexpr int P = at_planes<E>, STEPS = AtReader<DP>::STEPS;
     extern __shared__ __attribute__((aligned(256))) char lds[];
     const AtPlace o = at_block(p);
     const int lane = fg_lane(), row = (o.tile * WAVES + fg_wave()) * 32 + (lane & 31);
@@ -519,19 +574,23 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     AtSeen<TILE> seen;
     seen.init(p, o.b, lane);
     const E *k = (const E *)p.k + o.b * p.kb + o.head * p.kh, *v = (const E *)p.v + o.b * p.vb + o.head * p.vh;
-    gm_i4 q[ROW / 32], g[ROW / 32];
+    AtColumns<E, DP> q, g;
     at_row<E, DP>(q, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, row < p.rows, p.dim, lane);
     at_row<E, DP>(g, (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, row < p.rows, p.dim, lane);
     const int64_t stat = ((int64_t)o.b * p.heads + head) * p.nq + pos;
     const float lse = p.lse[stat] - at_lift<E>;
     float delta = 0.f;
     {
-        gm_i4 y[ROW / 32];
-        at_row<E, DP>(y, (const E *)p.y + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, row < p.rows, p.dim, lane);
+        const E *y = (const E *)p.y + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, *up = (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh;
 #pragma unroll
-        for (int j = 0; j < ROW / 32; ++j)
+        for (int j = 0; j < STEPS; ++j) {
+            const int from = (2 * j + (lane >> 5)) * AT_CHUNK, left = row < p.rows ? p.dim - from : 0;
+            gm_i4 a[sizeof(E) * AT_CHUNK / 16], c[sizeof(E) * AT_CHUNK / 16];
+            at_chunk<E>(a, y + (left > 0 ? from : 0), left);
+            at_chunk<E>(c, up + (left > 0 ? from : 0), left);
 #pragma unroll
-            for (int i = 0; i < fe_width<E>; ++i) delta = fmaf((float)((const E *)&y[j])[i], (float)((const E *)&g[j])[i], delta);
+            for (int i = 0; i < AT_CHUNK; ++i) delta = fmaf((float)((const E *)a)[i], (float)((const E *)c)[i], delta);
+        }
         delta = at_other_sum(delta);
         if (o.split == 0 && lane < 32 && row < p.rows) p.delta[stat] = delta;
     }
@@ -541,9 +600,10 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     at_f16 acc[DP / 32];
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) acc[t] = at_f16{};
-    AtFeed<E, TILE, DP, WAVES> feed;
+    typedef AtFeed<E, TILE, DP, WAVES> Feed;
+    Feed feed;
     feed.init(lds, p.dim);
-    AtReader<E, DP> at;
+    AtReader<DP> at;
     at.init(lane);
     uint64_t bits = 0, coming = 0;
     if (first < last) {
@@ -555,7 +615,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
     int index = 0;
 #pragma unroll 1
     for (int64_t key = first; key < last; key += TILE, bits = coming, ++index) {
-        const uint32_t lk = feed.arrive(index), lv = lk + TILE * ROW;
+        const uint32_t lk = feed.arrive(index), lv = lk + Feed::TILE;
         if (key + TILE < last) {
             coming = seen.take(key + TILE);
             seen.ask(key + 2 * TILE);
@@ -566,8 +626,8 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
         at_f16 s[B], dp[B];
         float w[B][16];
         auto scores = [&](int t) {
-            s[t] = at_scores<E, DP>(at, lk, 32 * t, q);
-            dp[t] = at_scores<E, DP>(at, lv, 32 * t, g);
+            s[t] = at_scores<E, DP>(at, lk, Feed::PLANE, 32 * t, q);
+            dp[t] = at_scores<E, DP>(at, lv, Feed::PLANE, 32 * t, g);
         };
         auto weigh = [&](int t) {
 #pragma unroll
@@ -581,22 +641,22 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
                 for (int i = 0; i < 16; ++i) w[t][i] = (own >> (8 * (i / 4) + i % 4)) & 1 ? w[t][i] : 0.f;
             }
             range.fit(w[t], acc);
-            at_gather<E, DP>(at, lk, 32 * t, AtWeights<E>(w[t]), acc);
+            at_gather<E, DP>(at, lk, Feed::PLANE, 32 * t, AtWeights<E>(w[t]), acc);
         };
         __builtin_amdgcn_sched_barrier(0);
         scores(0);
-        if constexpr (SIZE == 2) at_ahead<ROW / 16, 1, 3>();
+        at_ahead<2 * STEPS, P, 1, P == 1 ? 3 : 1>();
 #pragma unroll
         for (int t = 0; t < B; ++t) {
             __builtin_amdgcn_sched_barrier(0);
             weigh(t);
             if (t + 1 < B) {                // the next keys' scores beside these ones' weights
                 scores(t + 1);
-                if constexpr (SIZE == 2) at_ahead<ROW / 16, 1, 3, 768 / ROW, 256 / ROW>();
+                at_ahead<2 * STEPS, P, 1, P == 1 ? 3 : 1, 384 / DP, 128 / DP>();
             }
             __builtin_amdgcn_sched_barrier(0);
             gather(t);
-            if constexpr (SIZE == 2) at_ahead<ROW / 32, 2, 3>();
+            at_ahead<DP / 16, P, 2, P == 1 ? 3 : 1>();
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -609,7 +669,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : 2) void atte
         return;
     }
     __syncthreads();
-    at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * ROW, p.dim, lane, scaled, [&](int r) { return at_result(p, (E *)p.dq, o, row - (lane & 31) + r); });
+    at_store<E, DP>(acc, feed.lds + fg_wave() * 32 * DP * (int)sizeof(E), p.dim, lane, scaled, [&](int r) { return at_result(p, (E *)p.dq, o, row - (lane & 31) + r); });
 }
 
 // dK and dV: a wave owns 32 keys and walks the queries of every head that uses them, tile by tile.  Where their sums leave no room in the registers the keys wait in LDS (their
@@ -618,9 +678,9 @@ constexpr bool at_keys_in_lds(int dim, int size) { return size == 2 && dim >= 12
 // 32 rows a tile: three waves a SIMD at 64 components of 16 bits, where with 64 rows it is two (64 queries to 232,965 keys, 8 heads: 302 us for 262).
 constexpr int AT_ROWS_DKV = 32;
 template <typename E, int DP, int WAVES, int TILE>
-__global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(E) > 128 ? 2 : 3) void attention_dkv_kernel(AttentionP p)
+__global__ __launch_bounds__(64 * WAVES, sizeof(E) == 4 ? 1 : DP > 128 ? 1 : DP > 64 ? 2 : 3) void attention_dkv_kernel(AttentionP p)
 {
-    constexpr int SIZE = (int)sizeof(E), ROW = DP * SIZE, STEPS = DP / 32;
+    constexpr int SIZE = (int)sizeof(E), P = at_planes<E>, STEPS = AtReader<DP>::STEPS, PARTS = DP / 32;
     constexpr bool KEYS_IN_LDS = at_keys_in_lds(DP, SIZE);
     extern __shared__ __attribute__((aligned(256))) char lds[];
     typedef AtFeed<E, TILE, DP, WAVES> Feed;
@@ -630,7 +690,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(
     AtSeen<64> seen;
     seen.init(p, o.b, lane);
     const bool there = key < seen.length && (!p.mask || seen.mask[min(key, p.nk - 1)]), any = __ballot(there) != 0;
-    gm_i4 k[ROW / 32], v[ROW / 32];
+    AtColumns<E, DP> k, v;
     const int64_t own = min(key, p.nk - 1);
     at_row<E, DP>(k, (const E *)p.k + o.b * p.kb + own * p.kn + o.head * p.kh, there, p.dim, lane);
     at_row<E, DP>(v, (const E *)p.v + o.b * p.vb + own * p.vn + o.head * p.vh, there, p.dim, lane);
@@ -639,18 +699,18 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(
     // (behind the last key that is seen nothing is walked)
     const int last = o.tile * WAVES * 32 < seen.length ? min(per_head * p.share, first + p.per) : first;
 
-    at_f16 dk[STEPS], dv[STEPS];
+    at_f16 dk[PARTS], dv[PARTS];
 #pragma unroll
-    for (int t = 0; t < STEPS; ++t) dk[t] = dv[t] = at_f16{};
-    AtRange<E, STEPS> range;
+    for (int t = 0; t < PARTS; ++t) dk[t] = dv[t] = at_f16{};
+    AtRange<E, PARTS> range;
     Feed feed;
     feed.init(lds, p.dim);
-    const uint32_t own_keys = stats + 4 * TILE * 4 + fg_wave() * 32 * ROW;
+    const uint32_t own_keys = stats + 4 * TILE * 4 + fg_wave() * 32 * AtReader<DP>::ROW;
     if constexpr (KEYS_IN_LDS) {            // (read by their own wave alone)
 #pragma unroll
-        for (int j = 0; j < ROW / 32; ++j) *at_lds<gm_i4>(own_keys + at_place<ROW, SIZE>(lane & 31, 2 * j + (lane >> 5))) = k[j];
+        for (int j = 0; j < STEPS; ++j) *at_lds<gm_i4>(own_keys + at_place<AtReader<DP>::ROW>(lane & 31, 2 * j + (lane >> 5))) = k.c[j][0];
     }
-    AtReader<E, DP> at;
+    AtReader<DP> at;
     at.init(lane);
     float stat = 0.f;
     auto fetch = [&](int i) {
@@ -667,7 +727,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(
     for (int i = first; i < last; ++i) {
         const uint32_t row_stats = stats + ((i - first) & 1) * 2 * TILE * 4;
         if (threadIdx.x < 2 * TILE) *at_lds<float>(row_stats + threadIdx.x * 4) = stat;
-        const uint32_t lq = feed.arrive(i - first), lg = lq + TILE * ROW;
+        const uint32_t lq = feed.arrive(i - first), lg = lq + Feed::TILE;
         if (i + 1 < last) fetch(i + 1);
         if (!any) continue;
 #pragma unroll
@@ -675,9 +735,9 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(
             __builtin_amdgcn_sched_barrier(0);      // 32 rows at a time: the registers are full of sums
             at_f16 s;
             if constexpr (KEYS_IN_LDS) s = at_scores<E, DP>(at, lq, 32 * t, own_keys);
-            else s = at_scores<E, DP>(at, lq, 32 * t, k);
-            const at_f16 dp = at_scores<E, DP>(at, lg, 32 * t, v);
-            if constexpr (SIZE == 2) at_ahead<ROW / 16, 1, 3>();
+            else s = at_scores<E, DP>(at, lq, Feed::PLANE, 32 * t, k);
+            const at_f16 dp = at_scores<E, DP>(at, lg, Feed::PLANE, 32 * t, v);
+            at_ahead<2 * STEPS, P, 1, P == 1 ? 3 : 1>();
             __builtin_amdgcn_sched_barrier(0);
             float w[16], ds[16];
 #pragma unroll
@@ -692,9 +752,9 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(
             range.fit(ds, dk);
             const AtWeights<E> pw(w), pd(ds);
             __builtin_amdgcn_sched_barrier(0);
-            at_gather<E, DP>(at, lg, 32 * t, pw, dv);
-            at_gather<E, DP>(at, lq, 32 * t, pd, dk);
-            if constexpr (SIZE == 2) at_ahead<ROW / 16, 2, 3>();
+            at_gather<E, DP>(at, lg, Feed::PLANE, 32 * t, pw, dv);
+            at_gather<E, DP>(at, lq, Feed::PLANE, 32 * t, pd, dk);
+            at_ahead<DP / 8, P, 2, P == 1 ? 3 : 1>();
         }
     }
     // keys that are not seen were zeros in every product: what a score of 0 made of them is dropped
@@ -713,7 +773,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * sizeof(E) > 256 ? 1 : DP * sizeof(
         const int k = key - (lane & 31) + r;
         return k < p.nk ? (E *)result + (((int64_t)o.b * p.nk + k) * p.kv_heads + o.head) * p.dim : nullptr;
     };
-    const uint32_t rows = feed.lds + fg_wave() * 32 * ROW;
+    const uint32_t rows = feed.lds + fg_wave() * 32 * DP * SIZE;
     at_store<E, DP>(dk, rows, p.dim, lane, sk, [&](int r) { return to(p.dk, r); });
     at_store<E, DP>(dv, rows, p.dim, lane, sv, [&](int r) { return to(p.dv, r); });
 }
@@ -737,8 +797,10 @@ static void at_launch_dim(int what, const AtShape &s, const AttentionP &p, unsig
         else hipLaunchKernelGGL((attention_kernel<E, DP, WAVES, TILE>), dim3(grid), dim3(64 * WAVES), bytes, st, p);
     };
     if (s.waves == 4) queries.template operator()<4, at_tile<E>>();
-    else if (s.waves == 2) queries.template operator()<2, 32>();
-    else queries.template operator()<1, 32>();
+    else if constexpr (sizeof(E) == 2 || DP <= 64) {
+        if (s.waves == 2) queries.template operator()<2, 32>();
+        else queries.template operator()<1, 32>();
+    }
 }
 template <typename E>
 void at_launch(int what, const AtShape &s, const AttentionP &p, unsigned grid, hipStream_t st)

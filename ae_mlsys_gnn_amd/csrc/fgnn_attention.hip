@@ -11,7 +11,6 @@ extern template void at_launch<_Float16>(int, const AtShape &, const AttentionP 
 template <typename E>
 __global__ __launch_bounds__(AT_TPB) void attention_delta_kernel(AttentionP p)
 {
-    constexpr int V = fe_width<E>;
     const int half = (int)threadIdx.x & 1;
     const int64_t rows = (int64_t)p.batch * p.nq * p.heads;
     for (int64_t first = (int64_t)blockIdx.x * (AT_TPB / 2); first < rows; first += (int64_t)gridDim.x * (AT_TPB / 2)) {
@@ -19,12 +18,12 @@ __global__ __launch_bounds__(AT_TPB) void attention_delta_kernel(AttentionP p)
         const int head = (int)(row % p.heads);
         float sum = 0.f;
         if (row < rows)
-            for (int d = half * V; d < p.dim; d += 2 * V) {
-                float y[V], g[V];
-                gm_load<E, V>(y, (const E *)p.y + row * p.dim + d, p.dim - d);
-                gm_load<E, V>(g, (const E *)p.g + b * p.gb + pos * p.gn + head * p.gh + d, p.dim - d);
+            for (int d = half * AT_CHUNK; d < p.dim; d += 2 * AT_CHUNK) {
+                float y[AT_CHUNK], g[AT_CHUNK];
+                gm_load<E, AT_CHUNK>(y, (const E *)p.y + row * p.dim + d, p.dim - d);
+                gm_load<E, AT_CHUNK>(g, (const E *)p.g + b * p.gb + pos * p.gn + head * p.gh + d, p.dim - d);
 #pragma unroll
-                for (int i = 0; i < V; ++i) sum = fmaf(y[i], g[i], sum);
+                for (int i = 0; i < AT_CHUNK; ++i) sum = fmaf(y[i], g[i], sum);
             }
         sum += __shfl_xor(sum, 1, 64);
         if (row < rows && half == 0) p.delta[(b * p.heads + head) * p.nq + pos] = sum;
@@ -183,7 +182,8 @@ static AtShape at_shape(AttentionP &p, int what, int type)
     AtShape s;
     s.dim = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
     s.tile = what == AT_DKV ? AT_ROWS_DKV : fe_size(type) == 4 ? 32 : 64;
-    s.waves = what == AT_DKV || p.rows > 64 ? 4 : p.rows > 32 ? 2 : 1;
+    // (fp32 tiles of more than 64 components wait in registers on their way: one wave alone has no room for them.  16 queries to 4096 keys of 128 components, us: 698 for 200)
+    s.waves = what == AT_DKV || p.rows > 64 || (fe_size(type) == 4 && s.dim > 64) ? 4 : p.rows > 32 ? 2 : 1;
     if (s.waves < 4) s.tile = 32;
     const int64_t columns = what == AT_DKV ? p.nk : p.rows, walked = what == AT_DKV ? (int64_t)((p.nq + s.tile - 1) / s.tile) * p.share : (p.nk + s.tile - 1) / s.tile;
     p.tiles = (int)((columns + 32 * s.waves - 1) / (32 * s.waves));
@@ -227,7 +227,8 @@ static int at_run(int what, int type, const AtShape &s, const AttentionP &p, hip
 {
     const int64_t grid = at_grid(p);
     if (grid == 0) return 0;
-    FGNN_REQUIRE(grid < 1LL << 24 && (p.splits < 2 || ((int64_t)p.batch * p.kv_heads * p.rows < 1LL << 24 && (int64_t)p.batch * p.kv_heads * p.nk < 1LL << 23)), FGNN_ERR_LIMIT, "attention: %lld workgroups", (long long)grid);
+    const int64_t joined = p.splits < 2 ? 0 : (int64_t)p.batch * p.kv_heads * (what == AT_DKV ? 2LL * p.nk : p.rows);
+    FGNN_REQUIRE(grid < 1LL << 24 && joined < 1LL << 24, FGNN_ERR_LIMIT, "attention: %lld workgroups", (long long)grid);
     fe_dispatch(type, [&]<typename E>() { at_launch<E>(what, s, p, (unsigned)grid, st); });
     return fgnn_launch_status(what == AT_FORWARD ? "attention_kernel" : what == AT_DQ ? "attention_dq_kernel" : "attention_dkv_kernel");
 }
