@@ -260,3 +260,99 @@ def test_refusals_on_the_device():
     grad, = torch.autograd.grad(cross_attention(q, k, v).sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="second order"):
         grad.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [8, 31, 63, 65, 72, 127, 129, 136, 255])
+def test_components_around_padded_widths(dtype, dim):
+    check(*inputs((1, 37, 45, 4, 2, dim), dtype))
+    check(*inputs((2, 2, 300, 2, 1, dim), dtype), lengths=torch.tensor([299, 130]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1, 3000, 4, 4, 128), (1, 20, 2500, 2, 1, 256), (1, 40, 900, 3, 3, 130), (2, 33, 1100, 2, 2, 64), (1, 65, 1500, 1, 1, 60), (2, 900, 33, 2, 1, 256)])
+def test_few_rows_and_parts(dtype, shape):
+    check(*inputs(shape, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rise", [0.0, 0.02, 0.3, -0.3])
+def test_scores_that_rise_and_fall(dtype, rise):
+    """A row's largest score moves on by less and by more than what sums are left unscaled for, in each of its tiles."""
+    q, k, v, g = inputs((1, 70, 700, 2, 2, 40), dtype)
+    q[..., 0], k[..., 0] = 1.0, (rise * torch.arange(700)).view(1, 700, 1).to(dtype)
+    check(q, k, v, g, scale=1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("power", [-12, 0, 6])
+def test_small_and_large_gradients(dtype, power):
+    q, k, v, g = inputs((2, 90, 1500, 2, 1, 64), dtype)
+    check(q, k, v, (g.float() * 2.0 ** power).to(dtype))
+
+
+@pytest.mark.gpu
+def test_many_keys_of_many_samples_and_heads():
+    b, nk, h, d = 32, 16384, 32, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(s, generator=g, device="cuda").bfloat16() for s in ((b, 1, h, d), (b, nk, h, d), (b, nk, h, d)))
+    y = cross_attention(q, k, v).double()
+    for i in (0, 13, 31):
+        w = torch.softmax((q[i].double() * k[i].double()).sum(-1) * d ** -0.5, 0).unsqueeze(-1)
+        want, size = (w * v[i].double()).sum(0), (w * v[i].double().abs()).sum(0)
+        # weights rounded to the type, sums in 32 bits, the result rounded to the type
+        assert ((y[i, 0] - want).abs() <= 1.01 * 2.0 ** -8 * (size + want.abs())).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_offsets_past_32_bits(dtype):
+    """Samples, and positions, that lie far apart in memory."""
+    q, k, v, g = inputs((2, 40, 60, 2, 2, 64), dtype)
+    far = torch.empty(2 ** 31 + 2 ** 20, dtype=dtype, device="cuda")
+
+    def samples(t):
+        out = far.as_strided(t.shape, (2 ** 31, *t.stride()[1:]), 64)
+        return out.copy_(t)
+
+    def positions(t):
+        out = far.as_strided(t.shape, (64, 2 ** 25, t.stride(2) * 2, 1), 8)
+        return out.copy_(t)
+    plain = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    y = cross_attention(*plain)
+    grads = torch.autograd.grad(y, plain, g.cuda())
+    within(y, reference(q, k, v)["y"], "y")
+    for lay in (samples, positions):
+        for which in range(3):
+            on = [t.detach() for t in plain]
+            on[which] = lay(on[which]).detach()
+            on = [t.requires_grad_(True) for t in on]
+            again = cross_attention(*on)
+            assert torch.equal(again, y)
+            assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(again, on, g.cuda()), grads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_calls_at_the_same_time(dtype):
+    sets = [[t.cuda() for t in inputs(shape, dtype, seed)] for seed, shape in enumerate([(2, 300, 400, 4, 2, 64), (2, 5, 4000, 4, 2, 64), (1, 64, 3000, 2, 2, 96)])]
+
+    def work(q, k, v, g):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        y = cross_attention(*leaves)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, g)
+    alone = [work(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    both = []
+    for _ in range(3):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                both.append(work(*s))
+    torch.cuda.synchronize()
+    for i, got in enumerate(both):
+        assert all(torch.equal(a, c) for a, c in zip(got, alone[i % len(sets)]))

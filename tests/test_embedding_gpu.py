@@ -149,3 +149,42 @@ def test_refusals_on_the_device():
     grad, = torch.autograd.grad(embedding(t, w).sum(), w, create_graph=True)
     with pytest.raises(RuntimeError, match="second order"):
         grad.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 63, 1023, 1025, 4095, 4096, 4097, 8193])
+def test_numbers_of_tokens(dtype, n):
+    """Either side of where another way of sorting takes over, with tokens that all are one, that all differ, and of int32's whole range."""
+    g = torch.Generator().manual_seed(n)
+    w, gy = torch.randn(n + 3, 9, generator=g).to(dtype), torch.randn(n, 9, generator=g).to(dtype)
+    check(torch.full((n,), n + 2), w, gy, 1.0)
+    check(torch.randperm(n + 3, generator=g)[:n], w, gy, 0.5, padding=1)
+    wild = torch.randint(-2 ** 31, 2 ** 31 - 1, (n,), generator=g).int()
+    wild[::3] = n
+    leaf = w.cuda().requires_grad_(True)
+    y = embedding(wild.cuda(), leaf)
+    dw, = torch.autograd.grad(y, leaf, gy.cuda())
+    want, sums = gradient(wild, n + 3, gy, 1.0)
+    within(dw, want, UNIT[dtype], 16 * sums, "dw")
+    assert y[(wild < 0) | (wild >= n + 3)].isnan().all()
+
+
+@pytest.mark.gpu
+def test_calls_at_the_same_time():
+    g = torch.Generator().manual_seed(1)
+    sets = [(torch.randint(0, rows, (n,), generator=g).cuda(), torch.randn(rows, 64, generator=g).cuda(), torch.randn(n, 64, generator=g).cuda()) for n, rows in ((30000, 41), (3000, 900), (9000, 20000))]
+
+    def work(tokens, w, gy):
+        leaf = w.detach().requires_grad_(True)
+        return torch.autograd.grad(embedding(tokens, leaf), leaf, gy)[0]
+    alone = [work(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    both = []
+    for _ in range(3):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                both.append(work(*s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(got, alone[i % len(sets)]) for i, got in enumerate(both))

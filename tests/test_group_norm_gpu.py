@@ -221,3 +221,44 @@ def test_refusals_on_the_device():
     grad, = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="second order"):
         grad.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("points", [2, 15, 17, 63, 65, 129, 257, 513, 1025, 2303, 2305, 4097, 8191, 8193, 9216, 9217])
+def test_sizes_of_samples(dtype, points):
+    """Samples that a wave, a workgroup of 256 or of 512 threads and none of them holds, and the sizes next to where one takes over from another."""
+    for channels, groups in ((16, 2), (40, 8), (21, 7)):
+        x, w, b, gy = inputs((2, points, channels), channels, dtype, points)
+        check(x, groups, w, b, gy, ACTIVATIONS[points % 5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("channels,groups", [(512, 1), (513, 1), (1030, 2), (24, 24), (6, 1), (602, 43)])
+def test_widths_of_groups(channels, groups):
+    for dtype in TYPES:
+        for batch, points in ((300, 3), (3, 400)):
+            x, w, b, gy = inputs((batch, points, channels), channels, dtype, channels)
+            check(x, groups, w, b, gy, "silu")
+
+
+@pytest.mark.gpu
+def test_calls_at_the_same_time():
+    sets = [(groups, [t.cuda() for t in inputs((batch, points, channels), channels, torch.float32, seed)])
+            for seed, (batch, points, channels, groups) in enumerate([(3, 20000, 64, 8), (40, 300, 128, 4), (1, 1, 9000, 3)])]
+
+    def work(groups, arrays):
+        leaves = [t.detach().requires_grad_(True) for t in arrays[:3]]
+        y = group_norm(leaves[0], groups, leaves[1], leaves[2], activation="gelu")
+        return (y.detach(),) + torch.autograd.grad(y, leaves, arrays[3])
+    alone = [work(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    both = []
+    for _ in range(3):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                both.append(work(*s))
+    torch.cuda.synchronize()
+    for i, got in enumerate(both):
+        assert all(torch.equal(a, c) for a, c in zip(got, alone[i % len(sets)]))
