@@ -625,7 +625,8 @@ int fgnn_embedding_backward(int64_t n, int vocabulary, int cols, int type, const
  * h / (heads / kv_heads)), dim <= 256, of type FGNN_F32, FGNN_BF16 or FGNN_F16; y contiguous.  strides (host memory): those of samples, positions and heads, in elements, of
  * q, k, v and (backward) g.  Keys seen of sample b: the first lengths[b] (int32, or int64 where wide is 1; NULL: all), and of them those with mask[b][key] != 0 (NULL: all).
  * Queries that see no key get zeros, and no gradient comes of them; keys that are not seen are not read as numbers (they may be NaN) and get zeros.  lse [batch, heads, nq]
- * (NULL: not wanted) is for the backward pass: g is the gradient of y; dq, dk, dv contiguous, dq or both of dk and dv may be NULL.  Deterministic. */
+ * (NULL: not wanted) is for the backward pass: g is the gradient of y; dq, dk, dv contiguous, dq or both of dk and dv may be NULL.
+ * FGNN_F32 products are formed from three parts of 8 significant bits: an infinity in an operand that is seen gives NaN.  Deterministic. */
 size_t fgnn_attention_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *k,
                                       const void *v, const int64_t *strides);
 int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k,
