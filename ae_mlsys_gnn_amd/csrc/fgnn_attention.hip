@@ -212,6 +212,8 @@ static int at_check(const char *who, int batch, int nq, int nk, int heads, int k
     FGNN_REQUIRE((int64_t)nq * (heads / kv_heads) < 1LL << 31 && nk < (1LL << 31) - 128 && nq < (1LL << 31) - 128, FGNN_ERR_LIMIT, "%s: queries=%d keys=%d", who, nq, nk);
     return 0;
 }
+// (offsets inside a tile are unsigned)
+static bool at_negative(const int64_t *strides, int n) { return std::any_of(strides, strides + n, [](int64_t s) { return s < 0; }); }
 static AttentionP at_problem(int batch, int nq, int nk, int heads, int kv_heads, int dim)
 {
     AttentionP p = {};
@@ -228,7 +230,8 @@ static int at_run(int what, int type, const AtShape &s, const AttentionP &p, hip
     const int64_t grid = at_grid(p);
     if (grid == 0) return 0;
     const int64_t joined = p.splits < 2 ? 0 : (int64_t)p.batch * p.kv_heads * (what == AT_DKV ? 2LL * p.nk : p.rows);
-    FGNN_REQUIRE(grid < 1LL << 24 && joined < 1LL << 24, FGNN_ERR_LIMIT, "attention: %lld workgroups", (long long)grid);
+    // (a launch has fewer than 2^32 threads)
+    FGNN_REQUIRE(grid * s.waves < 1LL << 26 && joined < 1LL << 24, FGNN_ERR_LIMIT, "attention: %lld workgroups of %d waves", (long long)grid, s.waves);
     fe_dispatch(type, [&]<typename E>() { at_launch<E>(what, s, p, (unsigned)grid, st); });
     return fgnn_launch_status(what == AT_FORWARD ? "attention_kernel" : what == AT_DQ ? "attention_dq_kernel" : "attention_dkv_kernel");
 }
@@ -249,6 +252,7 @@ extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads
     if (rc || batch == 0 || nq == 0) return rc;
     FGNN_REQUIRE(scale > 0.f && scale < __builtin_inff(), FGNN_ERR_SHAPE, "fgnn_attention: scale %g", (double)scale);
     FGNN_REQUIRE(q && y && strides && (nk == 0 || (k && v)), FGNN_ERR_NULL, "fgnn_attention: NULL argument");
+    FGNN_REQUIRE(!at_negative(strides, 9), FGNN_ERR_SHAPE, "fgnn_attention: negative strides");
     const size_t bytes = fgnn_attention_workspace_bytes(batch, nq, nk, heads, kv_heads, dim, type, k, v, strides);
     FGNN_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), FGNN_ERR_WORKSPACE, "fgnn_attention: workspace of %zu bytes", workspace_bytes);
     hipStream_t st = (hipStream_t)stream;
@@ -294,6 +298,7 @@ extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int
     FGNN_REQUIRE(scale > 0.f && scale < __builtin_inff(), FGNN_ERR_SHAPE, "fgnn_attention_backward: scale %g", (double)scale);
     FGNN_REQUIRE((dk == nullptr) == (dv == nullptr), FGNN_ERR_NULL, "fgnn_attention_backward: dk and dv are formed together");
     FGNN_REQUIRE(strides && (nq == 0 || (q && y && g && lse)) && (nk == 0 || (k && v)), FGNN_ERR_NULL, "fgnn_attention_backward: NULL argument");
+    FGNN_REQUIRE(!at_negative(strides, 12), FGNN_ERR_SHAPE, "fgnn_attention_backward: negative strides");
     const size_t bytes = fgnn_attention_backward_workspace_bytes(batch, nq, nk, heads, kv_heads, dim, type, q, k, v, g, strides);
     FGNN_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), FGNN_ERR_WORKSPACE, "fgnn_attention_backward: workspace of %zu bytes", workspace_bytes);
     hipStream_t st = (hipStream_t)stream;

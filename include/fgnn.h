@@ -622,7 +622,7 @@ int fgnn_embedding_backward(int64_t n, int vocabulary, int cols, int type, const
                             void *stream);
 
 /* Attention y = softmax(scale q k^T) v over the keys that are seen, q and y [batch, nq, heads, dim], k and v [batch, nk, kv_heads, dim] (head h uses the keys of head
- * h / (heads / kv_heads)), dim <= 256, of type FGNN_F32, FGNN_BF16 or FGNN_F16; y contiguous.  strides (host memory): those of samples, positions and heads, in elements, of
+ * h / (heads / kv_heads)), dim <= 256, of type FGNN_F32, FGNN_BF16 or FGNN_F16; y contiguous.  strides (host memory): those of samples, positions and heads, in elements and not negative, of
  * q, k, v and (backward) g.  Keys seen of sample b: the first lengths[b] (int32, or int64 where wide is 1; NULL: all), and of them those with mask[b][key] != 0 (NULL: all).
  * Queries that see no key get zeros, and no gradient comes of them; keys that are not seen are not read as numbers (they may be NaN) and get zeros.  lse [batch, heads, nq]
  * (NULL: not wanted) is for the backward pass: g is the gradient of y; dq, dk, dv contiguous, dq or both of dk and dv may be NULL.

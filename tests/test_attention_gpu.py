@@ -356,3 +356,32 @@ def test_calls_at_the_same_time(dtype):
     torch.cuda.synchronize()
     for i, got in enumerate(both):
         assert all(torch.equal(a, c) for a, c in zip(got, alone[i % len(sets)]))
+
+
+@pytest.mark.gpu
+def test_one_set_of_features_three_times():
+    x = torch.randn(2, 70, 4, 32, generator=torch.Generator().manual_seed(1))
+    leaf, g = x.cuda().requires_grad_(True), torch.randn(x.shape).cuda()
+    apart = [x.cuda().requires_grad_(True) for _ in range(3)]
+    once, = torch.autograd.grad(cross_attention(leaf, leaf, leaf), leaf, g)
+    dq, dk, dv = torch.autograd.grad(cross_attention(*apart), apart, g)
+    # three terms, added in one order or another
+    assert ((once - (dq + dk + dv)).abs() <= 2.0 ** -22 * (dq.abs() + dk.abs() + dv.abs())).all()
+
+
+@pytest.mark.gpu
+def test_many_small_samples():
+    b, h, d = 1 << 20, 16, 8
+    q, k, v = (torch.randn(b, 1, h, d, device="cuda").bfloat16() for _ in range(3))
+    assert torch.equal(cross_attention(q, k, v), v)             # one key's weight is 1
+    with pytest.raises(RuntimeError, match="workgroups"):     # 2^24 of four waves: more threads than a launch has
+        q.requires_grad_(True), v.requires_grad_(True)
+        torch.autograd.grad(cross_attention(q, k, v), v, v.detach())
+
+
+def test_strides_that_are_refused():
+    import ctypes
+    l, p, st = _lib.lib(), 256, (ctypes.c_int64 * 12)(*([64, 16, 8] * 4))
+    st[4] = -16
+    assert l.fgnn_attention(1, 2, 3, 2, 1, 8, 0, p, p, p, st, None, 0, None, 1.0, p, None, None, 0, None) == -2
+    assert l.fgnn_attention_backward(1, 2, 3, 2, 1, 8, 0, p, p, p, p, p, st, None, 0, None, 1.0, p, p, p, p, p, 1 << 20, None) == -2

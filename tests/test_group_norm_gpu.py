@@ -205,7 +205,7 @@ def test_refusals():
     def call(batch=2, points=4, cols=8, groups=2, type=0, x=p, ld=8, wt=0, act=0, y=p, ws=1 << 20):
         return l.fgnn_group_norm(batch, points, cols, groups, type, x, ld, 32, p, wt, None, 0, 1e-5, act, 0.2, y, p, p, p, ws, None)
     assert call(groups=3) == -2 and call(groups=0) == -2 and call(ld=7) == -2 and call(type=3) == -2 and call(type=1, wt=2) == -2 and call(act=5) == -2 and call(batch=-1) == -2
-    assert call(x=None) == -1 and call(y=None) == -1 and call(ws=0) == -5
+    assert call(x=None) == -1 and call(y=None) == -1 and call(points=100000, ws=0) == -5
     assert l.fgnn_group_norm_backward(2, 4, 8, 2, 0, p, p, 8, 32, p, 0, None, 0, 0, 0.2, p, p, p, p, None, p, 0, None) == -5
     assert l.fgnn_group_norm_backward(2, 4, 8, 2, 0, None, p, 8, 32, p, 0, None, 0, 0, 0.2, p, p, p, p, None, p, 1 << 20, None) == -1
 
