@@ -182,7 +182,8 @@ static AtShape at_shape(AttentionP &p, int what, int type)
     AtShape s;
     s.dim = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256;
     s.tile = what == AT_DKV ? AT_ROWS_DKV : fe_size(type) == 4 ? 32 : 64;
-    // (fp32 tiles of more than 64 components wait in registers on their way: one wave alone has no room for them.  16 queries to 4096 keys of 128 components, us: 698 for 200)
+    // As many waves as the rows fill: one query to 16 x 4096 keys, 8 heads of 64 in fp32, 64 us for 89 with four waves; 64 queries to 232,965 keys in bf16, training, 476 for 514.
+    // (fp32 tiles of more than 64 components wait in registers on their way, for which one wave alone has no room: one query to 16 x 4096 keys of 128 components 698 us for 219.)
     s.waves = what == AT_DKV || p.rows > 64 || (fe_size(type) == 4 && s.dim > 64) ? 4 : p.rows > 32 ? 2 : 1;
     if (s.waves < 4) s.tile = 32;
     const int64_t columns = what == AT_DKV ? p.nk : p.rows, walked = what == AT_DKV ? (int64_t)((p.nq + s.tile - 1) / s.tile) * p.share : (p.nk + s.tile - 1) / s.tile;
