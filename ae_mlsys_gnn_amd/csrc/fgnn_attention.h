@@ -252,26 +252,13 @@ struct AtFeed {
     }
 };
 
-// AT_CHUNK components of a row, zeros past the last.  Any alignment.
-template <typename E>
-__device__ __forceinline__ void at_chunk(gm_i4 (&words)[sizeof(E) * AT_CHUNK / 16], const E *p, int left)
-{
-    constexpr int V = fe_width<E>;
-#pragma unroll
-    for (int w = 0; w < (int)sizeof(E) * AT_CHUNK / 16; ++w) {
-        E v[V];
-        gm_load<E, V>(v, p + (w * V < left ? w * V : 0), left - w * V);
-#pragma unroll
-        for (int i = 0; i < V; ++i) ((E *)&words[w])[i] = v[i];
-    }
-}
-// One row as the second operand of products: its chunks 2 j + (lane / 32), zeros past the last and where it is not there (`row` is memory that may be read all the same).  Any
-// alignment; rows of whole 16 bytes are asked for at once.
+// A lane's components of one row, chunks 2 j + (lane / 32), zeros past the last and where the row is not there (`row` is memory that may be read all the same).  Any alignment;
+// everything is asked for before anything is looked at (16 chunks one after the other: 2775 rows of 184 components in dQ's pass DQ_AFTER us for 56).
+template <typename E, int DP> struct AtWords { gm_i4 w[AtReader<DP>::STEPS][sizeof(E) * AT_CHUNK / 16]; };
 template <typename E, int DP>
-__device__ __forceinline__ void at_row(AtColumns<E, DP> &cols, const E *row, bool there, int dim, int lane)
+__device__ __forceinline__ void at_words(AtWords<E, DP> &words, const E *row, bool there, int dim, int lane)
 {
     constexpr int V = fe_width<E>, N = AtReader<DP>::STEPS, WORDS = (int)sizeof(E) * AT_CHUNK / 16;
-    gm_i4 words[N][WORDS];
     if (dim % V == 0) {
         typedef typename fe_vec<E>::type vec;
 #pragma unroll
@@ -280,7 +267,7 @@ __device__ __forceinline__ void at_row(AtColumns<E, DP> &cols, const E *row, boo
             for (int w = 0; w < WORDS; ++w) {
                 const int at = (2 * j + (lane >> 5)) * AT_CHUNK + w * V;
                 const vec v = *reinterpret_cast<const vec *>(row + (at < dim ? at : 0));
-                words[j][w] = *(const gm_i4 *)&v;
+                words.w[j][w] = *(const gm_i4 *)&v;
             }
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -288,25 +275,44 @@ __device__ __forceinline__ void at_row(AtColumns<E, DP> &cols, const E *row, boo
             for (int w = 0; w < WORDS; ++w) {
                 const bool in = there && (2 * j + (lane >> 5)) * AT_CHUNK + w * V < dim;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) words[j][w][i] = in ? words[j][w][i] : 0;
+                for (int i = 0; i < 4; ++i) words.w[j][w][i] = in ? words.w[j][w][i] : 0;
             }
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = (2 * j + (lane >> 5)) * AT_CHUNK;
-            at_chunk<E>(words[j], row + (there && at < dim ? at : 0), there ? dim - at : 0);
-        }
-    }
+        for (int j = 0; j < N; ++j)
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
+            for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const int at = (2 * j + (lane >> 5)) * AT_CHUNK + w * V + i;
+                    const E v = row[at < dim ? at : 0];
+                    ((E *)&words.w[j][w])[i] = there && at < dim ? v : (E)0.f;
+                }
+    }
+}
+// One row as the second operand of products.
+template <typename E, int DP>
+__device__ __forceinline__ void at_row(AtColumns<E, DP> &cols, const AtWords<E, DP> &words)
+{
+#pragma unroll
+    for (int j = 0; j < AtReader<DP>::STEPS; ++j) {
         if constexpr (sizeof(E) == 4) {
             uint32_t bits[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) bits[i] = (uint32_t)words[j][i / 4][i % 4];
+            for (int i = 0; i < 8; ++i) bits[i] = (uint32_t)words.w[j][i / 4][i % 4];
             gm_split(bits, cols.c[j]);
-        } else cols.c[j][0] = words[j][0];
+        } else cols.c[j][0] = words.w[j][0];
     }
 }
+template <typename E, int DP>
+__device__ __forceinline__ void at_row(AtColumns<E, DP> &cols, const E *row, bool there, int dim, int lane)
+{
+    AtWords<E, DP> words;
+    at_words<E, DP>(words, row, there, dim, lane);
+    at_row<E, DP>(cols, words);
+}
+// Components of rows that the backward pass's operands hold: those that are not whole 16 bytes it has laid out anew, with zeros behind the last.
+template <typename E> __device__ __forceinline__ int at_whole(int dim) { return (dim + fe_width<E> - 1) / fe_width<E> * fe_width<E>; }
 
 // The value of the lane that holds the same column's other rows.
 __device__ __forceinline__ float at_other_max(float v)
@@ -575,22 +581,19 @@ __global__ __launch_bounds__(64 * WAVES, DP > (sizeof(E) == 4 ? 64 : 128) ? 1 : 
     seen.init(p, o.b, lane);
     const E *k = (const E *)p.k + o.b * p.kb + o.head * p.kh, *v = (const E *)p.v + o.b * p.vb + o.head * p.vh;
     AtColumns<E, DP> q, g;
-    at_row<E, DP>(q, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, row < p.rows, p.dim, lane);
-    at_row<E, DP>(g, (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, row < p.rows, p.dim, lane);
+    at_row<E, DP>(q, (const E *)p.q + o.b * p.qb + (int64_t)pos * p.qn + head * p.qh, row < p.rows, at_whole<E>(p.dim), lane);
     const int64_t stat = ((int64_t)o.b * p.heads + head) * p.nq + pos;
     const float lse = p.lse[stat] - at_lift<E>;
     float delta = 0.f;
     {
-        const E *y = (const E *)p.y + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, *up = (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh;
+        AtWords<E, DP> y, up;
+        at_words<E, DP>(up, (const E *)p.g + o.b * p.gb + (int64_t)pos * p.gn + head * p.gh, row < p.rows, at_whole<E>(p.dim), lane);
+        at_words<E, DP>(y, (const E *)p.y + (((int64_t)o.b * p.nq + pos) * p.heads + head) * p.dim, row < p.rows, p.dim, lane);
+        at_row<E, DP>(g, up);
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-            const int from = (2 * j + (lane >> 5)) * AT_CHUNK, left = row < p.rows ? p.dim - from : 0;
-            gm_i4 a[sizeof(E) * AT_CHUNK / 16], c[sizeof(E) * AT_CHUNK / 16];
-            at_chunk<E>(a, y + (left > 0 ? from : 0), left);
-            at_chunk<E>(c, up + (left > 0 ? from : 0), left);
+        for (int j = 0; j < STEPS; ++j)
 #pragma unroll
-            for (int i = 0; i < AT_CHUNK; ++i) delta = fmaf((float)((const E *)a)[i], (float)((const E *)c)[i], delta);
-        }
+            for (int i = 0; i < AT_CHUNK; ++i) delta = fmaf((float)((const E *)y.w[j])[i], (float)((const E *)up.w[j])[i], delta);
         delta = at_other_sum(delta);
         if (o.split == 0 && lane < 32 && row < p.rows) p.delta[stat] = delta;
     }
@@ -690,10 +693,6 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(E) == 4 ? 1 : DP > 128 ? 1 : DP 
     AtSeen<64> seen;
     seen.init(p, o.b, lane);
     const bool there = key < seen.length && (!p.mask || seen.mask[min(key, p.nk - 1)]), any = __ballot(there) != 0;
-    AtColumns<E, DP> k, v;
-    const int64_t own = min(key, p.nk - 1);
-    at_row<E, DP>(k, (const E *)p.k + o.b * p.kb + own * p.kn + o.head * p.kh, there, p.dim, lane);
-    at_row<E, DP>(v, (const E *)p.v + o.b * p.vb + own * p.vn + o.head * p.vh, there, p.dim, lane);
     // tiles of every head's positions, one head after the other
     const int per_head = (p.nq + TILE - 1) / TILE, first = o.split * p.per;
     // (behind the last key that is seen nothing is walked)
@@ -706,9 +705,15 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(E) == 4 ? 1 : DP > 128 ? 1 : DP 
     Feed feed;
     feed.init(lds, p.dim);
     const uint32_t own_keys = stats + 4 * TILE * 4 + fg_wave() * 32 * AtReader<DP>::ROW;
-    if constexpr (KEYS_IN_LDS) {            // (read by their own wave alone)
+    AtColumns<E, DP> k, v;
+    if (first < last) {                     // (without a query nothing has been laid out anew)
+        const int64_t own = min(key, p.nk - 1);
+        at_row<E, DP>(k, (const E *)p.k + o.b * p.kb + own * p.kn + o.head * p.kh, there, at_whole<E>(p.dim), lane);
+        at_row<E, DP>(v, (const E *)p.v + o.b * p.vb + own * p.vn + o.head * p.vh, there, at_whole<E>(p.dim), lane);
+        if constexpr (KEYS_IN_LDS) {        // (read by their own wave alone)
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) *at_lds<gm_i4>(own_keys + at_place<AtReader<DP>::ROW>(lane & 31, 2 * j + (lane >> 5))) = k.c[j][0];
+            for (int j = 0; j < STEPS; ++j) *at_lds<gm_i4>(own_keys + at_place<AtReader<DP>::ROW>(lane & 31, 2 * j + (lane >> 5))) = k.c[j][0];
+        }
     }
     AtReader<DP> at;
     at.init(lane);

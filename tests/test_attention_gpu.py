@@ -385,3 +385,15 @@ def test_strides_that_are_refused():
     st[4] = -16
     assert l.fgnn_attention(1, 2, 3, 2, 1, 8, 0, p, p, p, st, None, 0, None, 1.0, p, None, None, 0, None) == -2
     assert l.fgnn_attention_backward(1, 2, 3, 2, 1, 8, 0, p, p, p, p, p, st, None, 0, None, 1.0, p, p, p, p, p, 1 << 20, None) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [1, 7, 33, 100, 131, 251])
+def test_rows_at_the_end_of_their_memory(dtype, dim):
+    """Rows of odd lengths, the last of which ends where its memory does, with queries and without any."""
+    q, k, v, g = inputs((1, 3, 2, 1, 1, dim), dtype)
+    check(q, k, v, g)
+    on = [t.cuda().requires_grad_(True) for t in (q[:, :0], k, v)]
+    y = cross_attention(*on)
+    assert all((t == 0).all() for t in torch.autograd.grad(y, on[1:], g[:, :0].cuda()))
