@@ -134,7 +134,7 @@ def test_refusals():
     assert l.fgnn_embedding(-1, 4, 8, 0, p, 1, p, 8, 1.0, p, None) == -2 and l.fgnn_embedding(2, 4, 8, 3, p, 1, p, 8, 1.0, p, None) == -2
     assert l.fgnn_embedding(2, 4, 8, 0, p, 1, p, 7, 1.0, p, None) == -2 and l.fgnn_embedding(2, 4, 8, 0, None, 1, p, 8, 1.0, p, None) == -1
     assert l.fgnn_embedding(2, 4, 8, 0, p, 1, p, 8, 1.0, None, None) == -1 and l.fgnn_embedding(1 << 31, 4, 8, 0, p, 1, p, 8, 1.0, p, None) == -4
-    assert l.fgnn_embedding_backward(2, 4, 8, 0, p, 1, -1, p, 8, 1.0, p, None, 0, None) == -5
+    assert l.fgnn_embedding_backward(300, 4, 8, 0, p, 1, -1, p, 8, 1.0, p, None, 0, None) == -5
     assert l.fgnn_embedding_backward(2, 4, 8, 0, p, 1, -1, p, 7, 1.0, p, p, 1 << 20, None) == -2
 
 
@@ -153,7 +153,7 @@ def test_refusals_on_the_device():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n", [2, 63, 1023, 1025, 4095, 4096, 4097, 8193])
+@pytest.mark.parametrize("n", [2, 63, 255, 256, 257, 1023, 1025, 4095, 4096, 4097, 8193])
 def test_numbers_of_tokens(dtype, n):
     """Either side of where another way of sorting takes over, with tokens that all are one, that all differ, and of int32's whole range."""
     g = torch.Generator().manual_seed(n)
@@ -188,3 +188,15 @@ def test_calls_at_the_same_time():
                 both.append(work(*s))
     torch.cuda.synchronize()
     assert all(torch.equal(got, alone[i % len(sets)]) for i, got in enumerate(both))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_tokens_of_large_and_wide_tables(dtype):
+    g = torch.Generator().manual_seed(2)
+    for n, vocabulary, channels in ((200, 16384, 8), (256, 16385, 12), (256, 60000, 3), (256, 41000, 103), (256, 8192, 1024), (256, 8193, 1024), (250, 5, 5000), (256, 1, 70), (100, 40, 2050)):
+        w, gy = torch.randn(vocabulary, channels, generator=g).to(dtype), torch.randn(n, channels, generator=g).to(dtype)
+        tokens = torch.randint(0, vocabulary, (n,), generator=g)
+        tokens[:3] = torch.tensor([0, vocabulary - 1, vocabulary - 1])
+        check(tokens, w, gy, 0.7)
+        check(tokens.int(), w, gy, 0.7, padding=0)
