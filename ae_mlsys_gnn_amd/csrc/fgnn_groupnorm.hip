@@ -24,7 +24,7 @@ struct GroupNormP {
     float *sums, *group;                    // backward: [batch][2][cols] A and B, [batch][groups][2] means
 };
 
-// Vectors that would end behind the last channel begin earlier, where there is room: the channels that they share with the vector before are summed there alone,
+// Vectors that would end behind the last channel begin earlier, where the workgroup's channels leave room: the channels that they share with the vector before are summed there alone,
 // and written twice, the same values (element by element 13 x 1433 x 602 fp16 in groups of 43 took 46 us forward and 86 backward, this way 33 and 65).
 struct GnVector { int c, shared, left; };   // first channel, how many of them are the vector's before, channels from the first on
 template <int V>
@@ -81,7 +81,7 @@ __device__ __forceinline__ GnPlace gn_place(const GroupNormP &p, uint32_t item)
     o.row = (int)threadIdx.x / p.lanes;
     o.tile0 = tile * p.lanes * V;
     const int c = o.tile0 + (int)threadIdx.x % p.lanes * V;
-    const GnVector v = gn_vector<V>(c, p.cols, 0);
+    const GnVector v = gn_vector<V>(c, p.cols, o.tile0);
     o.c = v.c;
     o.shared = v.shared;
     o.left = v.left;
