@@ -119,44 +119,119 @@ __device__ __forceinline__ void gn_take(float (&v)[V], const float *co, const Gn
     for (int i = 0; i < V; ++i) v[i] = co[o.c - o.tile0 + (i < o.left ? i : 0)];
 }
 
-// Sums over a chunk of points, a channel each: of x - k and its square, with k the channel's first value in the sample (squares of what is far from 0
-// would lose the variance), or of d and d (x - mean).
-template <typename E, bool BACKWARD, int ACT>
-__global__ __launch_bounds__(GN_TPB) void gn_sums_kernel(GroupNormP p)
+// Moments of values joined: of n0 with mean m and sum of squared deviations q, and of n1.  Nothing is taken from a value that is larger than the deviations themselves, so an
+// outlier, wherever it lies, costs no more than its own rounding (sums of squares about a channel's first value, which were here, lost 1e-3 of the variance where that one was 1000
+// deviations off).
+template <int V>
+__device__ __forceinline__ void gn_join(float &n0, float (&m)[V], float (&q)[V], float n1, const float (&m1)[V], const float (&q1)[V])
+{
+    const float n = n0 + n1, part = n1 * __builtin_amdgcn_rcpf(n), weight = n0 * part;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float d = m1[i] - m[i];
+        m[i] = fmaf(d, part, m[i]);
+        q[i] += fmaf(d * weight, d, q1[i]);
+    }
+    n0 = n;
+}
+// Means and sums of squared deviations over a chunk of points, a channel each: of four points at a time, joined to a thread's, and the threads' joined pairwise.
+template <typename E>
+__global__ __launch_bounds__(GN_TPB) void gn_moments_kernel(GroupNormP p)
 {
     constexpr int V = fe_width<E>, U = 4;
     typedef typename fe_vec<E>::type vec;
-    __shared__ float red[2][GN_TPB * V], co[BACKWARD ? GN_SUMS : 1][BACKWARD ? GN_TPB * V : 1];
+    __shared__ float red[2][GN_TPB][V], counts[GN_TPB];
     const uint32_t items = (uint32_t)(p.batch * p.chunks * p.tiles);
     for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
         const GnPlace o = gn_place<V>(p, item);
         const E *x = (const E *)p.x + o.sample * p.sx + o.c;
-        const E *gy = BACKWARD ? (const E *)p.gy + o.sample * p.points * p.cols + o.c : nullptr;
+        float count = 0.f, mean[V], square[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) mean[i] = square[i] = 0.f;
+        if (o.on) {
+            int64_t r = o.first + o.row;
+            for (; r + (U - 1) * o.step < o.last; r += U * o.step) {
+                vec raw[U];
+#pragma unroll
+                for (int j = 0; j < U; ++j) raw[j] = gn_read<E>(x + (r + j * o.step) * p.ldx, o.left);
+                float v[U][V], m[V], q[V];
+#pragma unroll
+                for (int j = 0; j < U; ++j) gn_floats<E, V>(v[j], raw[j]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    m[i] = ((v[0][i] + v[1][i]) + (v[2][i] + v[3][i])) * 0.25f;
+                    q[i] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < U; ++j) {
+                        const float d = v[j][i] - m[i];
+                        q[i] = fmaf(d, d, q[i]);
+                    }
+                }
+                gn_join<V>(count, mean, square, (float)U, m, q);
+            }
+            for (; r < o.last; r += o.step) {
+                float v[V];
+                const float none[V] = {};
+                gn_floats<E, V>(v, gn_read<E>(x + r * p.ldx, o.left));
+                gn_join<V>(count, mean, square, 1.f, v, none);
+            }
+        }
+        // the upper half of the rows to the lower one
+        for (int rows = o.step; rows > 1; rows = (rows + 1) / 2) {
+            const int half = (rows + 1) / 2;
+            __syncthreads();
+            if (o.on && o.row >= half && o.row < rows) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    red[0][threadIdx.x][i] = mean[i];
+                    red[1][threadIdx.x][i] = square[i];
+                }
+                counts[threadIdx.x] = count;
+            }
+            __syncthreads();
+            const int other = (int)threadIdx.x + half * p.lanes;
+            if (o.on && o.row + half < rows && counts[other] > 0.f) gn_join<V>(count, mean, square, counts[other], red[0][other], red[1][other]);
+        }
+        if (o.on && o.row == 0) {
+            float *part = p.part + (o.sample * p.chunks + o.chunk) * 2 * p.cols + o.c;
+            gm_store<float, V>(mean, part, o.left);
+            gm_store<float, V>(square, part + p.cols, o.left);
+        }
+    }
+}
+
+// Sums over a chunk of points, a channel each, of d and d (x - mean).
+template <typename E, int ACT>
+__global__ __launch_bounds__(GN_TPB) void gn_sums_kernel(GroupNormP p)
+{
+    constexpr int V = fe_width<E>, U = 4;
+    typedef typename fe_vec<E>::type vec;
+    __shared__ float red[2][GN_TPB * V], co[GN_SUMS][GN_TPB * V];
+    const uint32_t items = (uint32_t)(p.batch * p.chunks * p.tiles);
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const GnPlace o = gn_place<V>(p, item);
+        const E *x = (const E *)p.x + o.sample * p.sx + o.c;
+        const E *gy = (const E *)p.gy + o.sample * p.points * p.cols + o.c;
         float a[V], b[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) a[i] = b[i] = 0.f;
-        if constexpr (BACKWARD) gn_prepare<GN_SUMS, V>(p, o, co);
+        gn_prepare<GN_SUMS, V>(p, o, co);
         if (o.on) {
-            float k[V], ca[V], cc[V];       // k: the first value, or the mean
-            if constexpr (BACKWARD) {
-                gn_take<V>(ca, co[0], o);
-                gn_take<V>(cc, co[1], o);
-                gn_take<V>(k, co[2], o);
-            } else gn_floats<E, V>(k, gn_read<E>(x, o.left));
+            float mean[V], ca[V], cc[V];
+            gn_take<V>(ca, co[0], o);
+            gn_take<V>(cc, co[1], o);
+            gn_take<V>(mean, co[2], o);
             auto add = [&](vec vx, vec vg) {
                 float v[V], z[V], g[V];
                 gn_floats<E, V>(v, vx);
-                if constexpr (BACKWARD) {
-                    gn_floats<E, V>(g, vg);
+                gn_floats<E, V>(g, vg);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) z[i] = fmaf(v[i], ca[i], cc[i]);
-                    gm_act_slope(g, z, ACT, p.slope);
-                }
+                for (int i = 0; i < V; ++i) z[i] = fmaf(v[i], ca[i], cc[i]);
+                gm_act_slope(g, z, ACT, p.slope);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float t = v[i] - k[i], d = BACKWARD ? g[i] : t;
-                    a[i] += d;
-                    b[i] = fmaf(d, t, b[i]);
+                    a[i] += g[i];
+                    b[i] = fmaf(g[i], v[i] - mean[i], b[i]);
                 }
             };
             int64_t r = o.first + o.row;
@@ -165,16 +240,12 @@ __global__ __launch_bounds__(GN_TPB) void gn_sums_kernel(GroupNormP p)
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
                     v[j] = gn_read<E>(x + (r + j * o.step) * p.ldx, o.left);
-                    if constexpr (BACKWARD) g[j] = gn_read<E>(gy + (r + j * o.step) * p.cols, o.left);
+                    g[j] = gn_read<E>(gy + (r + j * o.step) * p.cols, o.left);
                 }
 #pragma unroll
                 for (int j = 0; j < U; ++j) add(v[j], g[j]);
             }
-            for (; r < o.last; r += o.step) {
-                vec v = gn_read<E>(x + r * p.ldx, o.left), g = {};
-                if constexpr (BACKWARD) g = gn_read<E>(gy + r * p.cols, o.left);
-                add(v, g);
-            }
+            for (; r < o.last; r += o.step) add(gn_read<E>(x + r * p.ldx, o.left), gn_read<E>(gy + r * p.cols, o.left));
         }
         __syncthreads();                    // the sums before are read
         const int tile0 = o.tile0, n = min(p.lanes * V, p.cols - tile0);
@@ -213,9 +284,9 @@ __device__ __forceinline__ void gn_all(double (&v)[N], double (*red)[N])
     for (int j = 0; j < N; ++j) v[j] = (red[0][j] + red[1][j]) + (red[2][j] + red[3][j]);
 }
 
-// Statistics of a sample's group from the sums about the channels' first values k: with k0 the group's first of all, sum (x - k0)^2 = sum over
-// channels of s2 + 2 (k - k0) s1 + points (k - k0)^2.  Backward: the sums of A and B over the chunks, and the means of w A and w B.
-template <typename E, bool BACKWARD>
+// Statistics of a sample's group from the chunks' and channels' moments, about the first of their means.  Backward: the sums of A and B over the chunks, and the means of w A
+// and w B.
+template <bool BACKWARD>
 __global__ __launch_bounds__(GN_TPB) void gn_group_kernel(GroupNormP p)
 {
     __shared__ double red[GN_TPB / 64][2], col[BACKWARD ? 2 : 1][GN_TPB];
@@ -225,27 +296,31 @@ __global__ __launch_bounds__(GN_TPB) void gn_group_kernel(GroupNormP p)
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t sample = item / p.groups;
         const int c0 = (int)(item - sample * p.groups) * p.width;
-        const E *x = (const E *)p.x + sample * p.sx + c0;
-        const double k0 = BACKWARD ? 0. : (double)(float)x[0], rstd = BACKWARD ? p.rstd[item] : 0.f;
+        const float *parts = p.part + sample * p.chunks * 2 * p.cols + c0;
+        const double k0 = BACKWARD ? 0. : (double)parts[0], rstd = BACKWARD ? p.rstd[item] : 0.f;
         double v[2] = {0., 0.};
         for (int first = 0; first < p.width; first += C) {
             const int c = first + lane;
             const bool on = q < Q && c < p.width;
             double s[2] = {0., 0.};
             if (on) {
-                const float *part = p.part + sample * p.chunks * 2 * p.cols + c0 + c;
+                const float *part = parts + c;
 #pragma unroll 4
                 for (int i = q; i < p.chunks; i += Q) {
-                    s[0] += part[(int64_t)(2 * i) * p.cols];
-                    s[1] += part[(int64_t)(2 * i + 1) * p.cols];
+                    const float a = part[(int64_t)(2 * i) * p.cols], b = part[(int64_t)(2 * i + 1) * p.cols];
+                    if constexpr (BACKWARD) {
+                        s[0] += a;
+                        s[1] += b;
+                    } else {
+                        const double n = (double)min(p.rows, p.points - i * p.rows), d = (double)a - k0;
+                        s[0] += n * d;
+                        s[1] += b + n * d * d;
+                    }
                 }
             }
             if constexpr (!BACKWARD) {
-                if (on) {
-                    const double k = (double)(float)x[c] - k0, more = q == 0 ? p.points * k : 0.;
-                    v[0] += s[0] + more;
-                    v[1] += s[1] + k * (2. * s[0] + more);
-                }
+                v[0] += s[0];
+                v[1] += s[1];
             } else {
                 __syncthreads();
                 col[0][threadIdx.x] = s[0];
@@ -703,8 +778,8 @@ extern "C" int fgnn_group_norm(int64_t batch, int64_t points, int cols, int grou
     p.part = (float *)workspace;
     const unsigned grid = gn_grid(batch * p.chunks * p.tiles);
     fe_dispatch(type, [&]<typename E>() {
-        hipLaunchKernelGGL((gn_sums_kernel<E, false, GM_NONE>), dim3(grid), dim3(GN_TPB), 0, st, p);
-        hipLaunchKernelGGL((gn_group_kernel<E, false>), dim3(gn_grid(batch * groups)), dim3(GN_TPB), 0, st, p);
+        hipLaunchKernelGGL((gn_moments_kernel<E>), dim3(grid), dim3(GN_TPB), 0, st, p);
+        hipLaunchKernelGGL((gn_group_kernel<false>), dim3(gn_grid(batch * groups)), dim3(GN_TPB), 0, st, p);
         gn_act(act, [&]<int ACT>() { hipLaunchKernelGGL((gn_apply_kernel<E, false, ACT>), dim3(grid), dim3(GN_TPB), 0, st, p); });
     });
     return fgnn_launch_status("gn_apply_kernel");
@@ -739,8 +814,8 @@ extern "C" int fgnn_group_norm_backward(int64_t batch, int64_t points, int cols,
             p.group = (float *)((char *)p.sums + gn_sums_bytes(p));
             const unsigned grid = gn_grid(batch * p.chunks * p.tiles);
             fe_dispatch(type, [&]<typename E>() {
-                gn_act(act, [&]<int ACT>() { hipLaunchKernelGGL((gn_sums_kernel<E, true, ACT>), dim3(grid), dim3(GN_TPB), 0, st, p); });
-                hipLaunchKernelGGL((gn_group_kernel<E, true>), dim3(gn_grid(batch * groups)), dim3(GN_TPB), 0, st, p);
+                gn_act(act, [&]<int ACT>() { hipLaunchKernelGGL((gn_sums_kernel<E, ACT>), dim3(grid), dim3(GN_TPB), 0, st, p); });
+                hipLaunchKernelGGL((gn_group_kernel<true>), dim3(gn_grid(batch * groups)), dim3(GN_TPB), 0, st, p);
                 if (dx) gn_act(act, [&]<int ACT>() { hipLaunchKernelGGL((gn_apply_kernel<E, true, ACT>), dim3(grid), dim3(GN_TPB), 0, st, p); });
             });
         }
