@@ -204,13 +204,14 @@ static size_t at_part_bytes(const AttentionP &p, int what)
 }
 static int64_t at_grid(const AttentionP &p) { return (int64_t)p.tiles * p.splits * p.kv_heads * p.batch; }
 
+static bool at_limits(int nq, int nk, int share) { return (int64_t)nq * share < 1LL << 31 && nk < (1LL << 31) - 128 && nq < (1LL << 31) - 128; }
 static int at_check(const char *who, int batch, int nq, int nk, int heads, int kv_heads, int dim, int type)
 {
     FGNN_REQUIRE(batch >= 0 && nq >= 0 && nk >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && dim >= 1, FGNN_ERR_SHAPE,
                  "%s: bad sizes batch=%d queries=%d keys=%d heads=%d kv_heads=%d dim=%d", who, batch, nq, nk, heads, kv_heads, dim);
     FGNN_REQUIRE(fe_is_float(type), FGNN_ERR_SHAPE, "%s: element type %d", who, type);
     FGNN_REQUIRE(dim <= 256, FGNN_ERR_LIMIT, "%s: heads of %d components, more than 256", who, dim);
-    FGNN_REQUIRE((int64_t)nq * (heads / kv_heads) < 1LL << 31 && nk < (1LL << 31) - 128 && nq < (1LL << 31) - 128, FGNN_ERR_LIMIT, "%s: queries=%d keys=%d", who, nq, nk);
+    FGNN_REQUIRE(at_limits(nq, nk, heads / kv_heads), FGNN_ERR_LIMIT, "%s: queries=%d keys=%d", who, nq, nk);
     return 0;
 }
 // (offsets inside a tile are unsigned)
@@ -239,7 +240,7 @@ static int at_run(int what, int type, const AtShape &s, const AttentionP &p, hip
 
 extern "C" size_t fgnn_attention_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *k, const void *v, const int64_t *strides)
 {
-    if (batch < 1 || nq < 1 || nk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > 256 || !fe_is_float(type) || !strides) return 0;
+    if (batch < 1 || nq < 1 || nk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > 256 || !at_limits(nq, nk, heads / kv_heads) || !fe_is_float(type) || !strides) return 0;
     AttentionP p = at_problem(batch, nq, nk, heads, kv_heads, dim);
     at_shape(p, AT_FORWARD, type);
     const size_t pack = at_pack_bytes(batch, nk, kv_heads, dim, type);
@@ -279,7 +280,7 @@ extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads
 extern "C" size_t fgnn_attention_backward_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const void *g,
                                                           const int64_t *strides)
 {
-    if (batch < 1 || nq < 1 || nk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > 256 || !fe_is_float(type) || !strides) return 0;
+    if (batch < 1 || nq < 1 || nk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > 256 || !at_limits(nq, nk, heads / kv_heads) || !fe_is_float(type) || !strides) return 0;
     AttentionP p = at_problem(batch, nq, nk, heads, kv_heads, dim);
     at_shape(p, AT_DQ, type);
     size_t part = at_part_bytes(p, AT_DQ);

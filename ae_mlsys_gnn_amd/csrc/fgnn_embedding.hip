@@ -377,11 +377,12 @@ static void em_cut(EmbeddingP &p, int type)
     p.tiles = (p.n + p.tile - 1) / p.tile;
 }
 
+static bool em_limits(int64_t n, int vocabulary, int cols) { return n <= 2147483647LL - 65536 && vocabulary < 1 << 30 && cols <= 1 << 30; }
 static int em_check(const char *who, int64_t n, int vocabulary, int cols, int type, const void *tokens, int wide)
 {
     FGNN_REQUIRE(n >= 0 && vocabulary >= 0 && cols >= 1 && (wide == 0 || wide == 1) && fe_is_float(type), FGNN_ERR_SHAPE, "%s: bad sizes n=%lld vocabulary=%d cols=%d type=%d", who,
                  (long long)n, vocabulary, cols, type);
-    FGNN_REQUIRE(n <= 2147483647LL - 65536 && vocabulary < 1 << 30 && cols <= 1 << 30, FGNN_ERR_LIMIT, "%s: n=%lld vocabulary=%d cols=%d", who, (long long)n, vocabulary, cols);
+    FGNN_REQUIRE(em_limits(n, vocabulary, cols), FGNN_ERR_LIMIT, "%s: n=%lld vocabulary=%d cols=%d", who, (long long)n, vocabulary, cols);
     FGNN_REQUIRE(n == 0 || tokens, FGNN_ERR_NULL, "%s: NULL argument", who);
     return 0;
 }
@@ -413,7 +414,7 @@ static EmbeddingSpace em_space(const EmbeddingP &p)
 }
 extern "C" size_t fgnn_embedding_backward_workspace_bytes(int64_t n, int vocabulary, int cols, int type)
 {
-    if (n < 1 || vocabulary < 1 || vocabulary >= 1 << 30 || cols < 1 || !fe_is_float(type) || em_one(n, vocabulary, cols, type)) return 0;
+    if (n < 1 || vocabulary < 1 || cols < 1 || !em_limits(n, vocabulary, cols) || !fe_is_float(type) || em_one(n, vocabulary, cols, type)) return 0;
     EmbeddingP p = {n, vocabulary, cols};
     em_cut(p, type);
     return em_space(p).all();

@@ -728,6 +728,7 @@ static void gn_act(int act, Fn &&f)
 }
 static unsigned gn_grid(int64_t items) { return (unsigned)std::min<int64_t>(items, GN_GRID); }
 
+static bool gn_limits(int64_t batch, int64_t points, int cols) { return cols <= 1 << 30 && points <= 1LL << 40 && batch <= 1LL << 31; }
 static int gn_check(const char *who, int64_t batch, int64_t points, int cols, int groups, int type, const void *x, int64_t ldx, int64_t sx, const void *w, int wtype, const void *b,
                     int btype, int act)
 {
@@ -736,7 +737,7 @@ static int gn_check(const char *who, int64_t batch, int64_t points, int cols, in
     FGNN_REQUIRE(fe_is_float(type) && (!w || wtype == type || wtype == FGNN_F32) && (!b || btype == type || btype == FGNN_F32), FGNN_ERR_SHAPE,
                  "%s: element type %d with weights of type %d, bias of type %d", who, type, wtype, btype);
     FGNN_REQUIRE(act >= GM_NONE && act <= GM_LEAKY, FGNN_ERR_SHAPE, "%s: activation %d", who, act);
-    FGNN_REQUIRE(cols <= 1 << 30 && points <= 1LL << 40 && batch <= (1LL << 31), FGNN_ERR_LIMIT, "%s: batch=%lld points=%lld cols=%d", who, (long long)batch, (long long)points, cols);
+    FGNN_REQUIRE(gn_limits(batch, points, cols), FGNN_ERR_LIMIT, "%s: batch=%lld points=%lld cols=%d", who, (long long)batch, (long long)points, cols);
     FGNN_REQUIRE(batch == 0 || points == 0 || x, FGNN_ERR_NULL, "%s: NULL argument", who);
     return 0;
 }
@@ -747,7 +748,7 @@ static size_t gn_part_bytes(const GroupNormP &p) { return fgnn_align256((size_t)
 static size_t gn_sums_bytes(const GroupNormP &p) { return fgnn_align256((size_t)p.batch * 2 * p.cols * sizeof(float)); }
 static size_t gn_workspace(int64_t batch, int64_t points, int cols, int groups, int type, int backward)
 {
-    if (batch < 1 || points < 1 || cols < 1 || groups < 1 || !fe_is_float(type)) return 0;
+    if (batch < 1 || points < 1 || cols < 1 || groups < 1 || cols % groups || !gn_limits(batch, points, cols) || !fe_is_float(type)) return 0;     // (which a call refuses)
     GroupNormP p = {};
     p.batch = batch; p.points = points; p.cols = cols; p.groups = groups;
     const GnHeld held = gn_held(p, type);

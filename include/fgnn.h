@@ -597,6 +597,7 @@ int    fgnn_coo2csr(int n_rows, int n_cols, int64_t E, const int32_t *dst, const
                     void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------- operators of conditioned blocks
+ * Workspaces of sizes that a call refuses are of 0 bytes.
  * Group norm with an activation of x [batch, points, cols], channels last (sample stride sx, point stride ldx, in elements): per sample and group of cols / groups
  * channels, u = (x - mean) rstd over points and channels, y = act(u weight + bias).  Types and act as above; weight and bias of the rows' type or FGNN_F32, NULL: ones,
  * zeros.  y contiguous; mean, rstd [batch, groups] are for the backward pass.  _backward: gy, dx contiguous; dx, dweight, dbias (of the types of weight and bias; of the

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from ae_mlsys_gnn_amd import _lib
 from . import test_group_norm_gpu as norm
 
 
@@ -31,3 +32,19 @@ def test_points_far_from_the_others(dtype, shape):
         far = (x.float() + mean).to(dtype)
         far[:, 0] = 0
         norm.check(far, groups, w, b, gy, None)
+
+
+def test_workspaces_of_sizes_that_are_refused():
+    """A caller asks for the workspace before the call that refuses the sizes."""
+    import ctypes
+    l, s, most = _lib.lib(), (ctypes.c_int64 * 12)(*([64, 16, 8] * 4)), 2 ** 31 - 1
+    for cols, groups in ((4, 8), (10, 4), (8, 0), (0, 1), (most, 1), (most, most), (2 ** 30 + 1, 1)):
+        assert l.fgnn_group_norm_workspace_bytes(2, 100000, cols, groups, 0) == 0 and l.fgnn_group_norm_backward_workspace_bytes(2, 100000, cols, groups, 0) == 0
+        assert l.fgnn_group_norm(2, 100000, cols, groups, 0, 256, cols, cols, None, 0, None, 0, 1e-5, 0, 0.2, 256, 256, 256, None, 0, None) in (-2, -4)
+    for n, vocabulary, cols in ((1000, 7, most), (1000, 7, 2 ** 30 + 1), (2 ** 40, 7, 8), (1000, 2 ** 30, 8), (1000, 7, 0)):
+        assert l.fgnn_embedding_backward_workspace_bytes(n, vocabulary, cols, 0) == 0
+        assert l.fgnn_embedding_backward(n, vocabulary, cols, 0, 256, 1, -1, 256, max(cols, 1), 1.0, 256, None, 0, None) in (-2, -4)
+    for nq, nk, heads, kv in ((most, 5, 1, 1), (5, most, 1, 1), (2 ** 30, 5, 2, 1), (5, 5, 3, 2), (5, 5, 1, 0)):
+        assert l.fgnn_attention_workspace_bytes(1, nq, nk, heads, kv, 8, 0, 256, 256, s) == 0
+        assert l.fgnn_attention_backward_workspace_bytes(1, nq, nk, heads, kv, 8, 0, 256, 256, 256, 256, s) == 0
+        assert l.fgnn_attention(1, nq, nk, heads, kv, 8, 0, 256, 256, 256, s, None, 0, None, 1.0, 256, None, None, 0, None) in (-2, -4)
