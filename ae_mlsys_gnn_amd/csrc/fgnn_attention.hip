@@ -227,15 +227,34 @@ static AttentionP at_problem(int batch, int nq, int nk, int heads, int kv_heads,
     p.share_mul = (uint32_t)(((1ULL << 32) * ((1ULL << p.share_shift) - p.share)) / p.share + 1);
     return p;
 }
+// Whether a pass can be launched: a launch has fewer than 2^32 threads.
+static int at_fits(int what, const AtShape &s, const AttentionP &p)
+{
+    const int64_t grid = at_grid(p), joined = p.splits < 2 ? 0 : (int64_t)p.batch * p.kv_heads * (what == AT_DKV ? 2LL * p.nk : p.rows);
+    FGNN_REQUIRE(grid * s.waves < 1LL << 26 && joined < 1LL << 24, FGNN_ERR_LIMIT, "attention: %lld workgroups of %d waves", (long long)grid, s.waves);
+    return 0;
+}
 static int at_run(int what, int type, const AtShape &s, const AttentionP &p, hipStream_t st)
 {
     const int64_t grid = at_grid(p);
     if (grid == 0) return 0;
-    const int64_t joined = p.splits < 2 ? 0 : (int64_t)p.batch * p.kv_heads * (what == AT_DKV ? 2LL * p.nk : p.rows);
-    // (a launch has fewer than 2^32 threads)
-    FGNN_REQUIRE(grid * s.waves < 1LL << 26 && joined < 1LL << 24, FGNN_ERR_LIMIT, "attention: %lld workgroups of %d waves", (long long)grid, s.waves);
+    if (const int rc = at_fits(what, s, p)) return rc;
     fe_dispatch(type, [&]<typename E>() { at_launch<E>(what, s, p, (unsigned)grid, st); });
     return fgnn_launch_status(what == AT_FORWARD ? "attention_kernel" : what == AT_DQ ? "attention_dq_kernel" : "attention_dkv_kernel");
+}
+// The backward pass's limits, which are looked at before its first launch, and by a caller before a forward pass that trains: the pass of dK and dV has four waves for
+// every sample and head of keys, however few keys there are.
+extern "C" int fgnn_attention_backward_check(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, int dq, int dkv)
+{
+    int rc = at_check("fgnn_attention_backward", batch, nq, nk, heads, kv_heads, dim, type);
+    if (rc || batch == 0) return rc;
+    AttentionP p = at_problem(batch, nq, nk, heads, kv_heads, dim);
+    for (const int what : {AT_DQ, AT_DKV}) {
+        if (what == AT_DQ ? !dq || nq == 0 : !dkv || nk == 0) continue;
+        const AtShape s = at_shape(p, what, type);
+        if ((rc = at_fits(what, s, p))) return rc;
+    }
+    return 0;
 }
 
 extern "C" size_t fgnn_attention_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *k, const void *v, const int64_t *strides)
@@ -295,7 +314,7 @@ extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int
                                        const int64_t *strides, const void *lengths, int wide, const uint8_t *mask, float scale, const float *lse, void *dq, void *dk, void *dv, void *workspace,
                                        size_t workspace_bytes, void *stream)
 {
-    int rc = at_check("fgnn_attention_backward", batch, nq, nk, heads, kv_heads, dim, type);
+    int rc = fgnn_attention_backward_check(batch, nq, nk, heads, kv_heads, dim, type, dq != nullptr, dk != nullptr);
     if (rc || batch == 0) return rc;
     FGNN_REQUIRE(scale > 0.f && scale < __builtin_inff(), FGNN_ERR_SHAPE, "fgnn_attention_backward: scale %g", (double)scale);
     FGNN_REQUIRE((dk == nullptr) == (dv == nullptr), FGNN_ERR_NULL, "fgnn_attention_backward: dk and dv are formed together");

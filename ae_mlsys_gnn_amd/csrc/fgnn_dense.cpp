@@ -546,6 +546,8 @@ struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const MaybeTensor &lengths, const MaybeTensor &mask, std::optional<double> scale)
     {
         const AttentionOperands o = attention_operands(q, k, v, given(lengths), given(mask), scale);
+        // (a call whose gradients are refused is refused before it runs)
+        check(fgnn_attention_backward_check(o.batch, o.nq, o.nk, o.heads, o.kv_heads, o.dim, o.type, wanted(q), wanted(k) || wanted(v)), "fgnn_attention_backward");
         const AttentionOut out = attention_forward(o, true);
         ctx->saved_data["need"] = (int64_t)(wanted(q) | wanted(k) << 1 | wanted(v) << 2);
         ctx->saved_data["scale"] = (double)o.scale;

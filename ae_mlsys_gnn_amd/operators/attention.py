@@ -11,6 +11,7 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None):
     values that are not seen is never used, NaN neither, and their gradient is 0.
     fp32, bf16 or fp16, the same for q, k and v, of any strides (components that are not contiguous are copied).  Sums, softmax and results are 32 bits; of 16-bit
     types the softmax's weights and the scores' gradient are rounded to the type before they are multiplied; products of fp32 are formed from parts of 8 significant bits,
-    as near to float64 as fp32 products are, and an infinity in keys or values that are seen, or in queries, gives NaN there.  Gradients of q, k and v, in one order of summation; those
+    as near to float64 as fp32 products are, and an infinity in keys or values that are seen, or in queries, gives NaN there.  Gradients of q, k and v, in one order of summation;
+    calls that train k or v are refused for samples x kv_heads x ceil(keys / 128) of 2^24 and more.  Gradients
     of second order are not recorded, and calls are refused in forward mode and by jit.trace, make_fx and export."""
     return dense().cross_attention(q, k, v, lengths, mask, scale)

@@ -640,6 +640,9 @@ int fgnn_attention_backward(int batch, int nq, int nk, int heads, int kv_heads, 
                             const void *k, const void *v, const void *y, const void *g, const int64_t *strides,
                             const void *lengths, int wide, const uint8_t *mask, float scale, const float *lse, void *dq,
                             void *dk, void *dv, void *workspace, size_t workspace_bytes, void *stream);
+/* What fgnn_attention_backward says of sizes (nonzero dq, dkv: what is wanted), without a launch: batch kv_heads ceil(nk / 128) of 2^24 and more are FGNN_ERR_LIMIT
+ * where dk and dv are wanted, also where fgnn_attention takes them. */
+int fgnn_attention_backward_check(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, int dq, int dkv);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus

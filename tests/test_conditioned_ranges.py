@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from ae_mlsys_gnn_amd import _lib
+from ae_mlsys_gnn_amd.operators import cross_attention
 from . import test_group_norm_gpu as norm
 
 
@@ -48,3 +49,30 @@ def test_workspaces_of_sizes_that_are_refused():
         assert l.fgnn_attention_workspace_bytes(1, nq, nk, heads, kv, 8, 0, 256, 256, s) == 0
         assert l.fgnn_attention_backward_workspace_bytes(1, nq, nk, heads, kv, 8, 0, 256, 256, 256, 256, s) == 0
         assert l.fgnn_attention(1, nq, nk, heads, kv, 8, 0, 256, 256, 256, s, None, 0, None, 1.0, 256, None, None, 0, None) in (-2, -4)
+
+
+def test_the_backward_pass_says_ahead_what_it_refuses():
+    check, few, many = _lib.lib().fgnn_attention_backward_check, (2 ** 20 - 1, 1, 128, 16, 16, 8, 1), (2 ** 20, 1, 1, 16, 16, 8, 1)
+    assert check(*few, 1, 1) == 0 and check(*many, 1, 0) == 0 and check(*many, 0, 0) == 0
+    assert check(*many, 0, 1) == -4 and check(2 ** 19, 1, 129, 16, 16, 8, 1, 1, 1) == -4
+    assert check(2 ** 20, 1, 0, 16, 16, 8, 1, 1, 1) == 0 and check(0, 1, 1, 16, 16, 8, 1, 1, 1) == 0        # nothing to launch
+    assert check(1, 1, 1, 3, 2, 8, 1, 1, 1) == -2 and check(1, 1, 1, 1, 1, 257, 1, 1, 1) == -4
+
+
+@pytest.mark.gpu
+def test_calls_whose_gradients_are_refused_are_refused_before_they_run():
+    b, h, d = 2 ** 20, 16, 8
+    q, k, v = (torch.randn(b, 1, h, d, device="cuda").bfloat16() for _ in range(3))
+    for leaf in (k, v):
+        leaf.requires_grad_(True)
+        with pytest.raises(_lib.FgnnError, match="workgroups"):
+            cross_attention(q, k, v)
+        with torch.no_grad():
+            assert torch.equal(cross_attention(q, k, v), v)
+        leaf.requires_grad_(False)
+    # queries alone can be trained: the only key's weight is 1 whatever they are, so that the gradient is what two sums of eight products differ by, times a key
+    q.requires_grad_(True)
+    y = cross_attention(q, k, v)
+    dq, = torch.autograd.grad(y, q, v)
+    bound = 16 * 2.0 ** -24 * (v.float() * v.float()).sum(-1, keepdim=True) * k.float().abs() * d ** -0.5
+    assert torch.equal(y.detach(), v) and (dq.float().abs() <= 1.01 * bound).all()
