@@ -100,6 +100,8 @@ _SIGNATURES = {
     "fgnn_attention_workspace_bytes": (c_size_t, [c_int] * 7 + [c_void_p] * 3),
     "fgnn_attention": (c_int, [c_int] * 7 + [c_void_p] * 5 + [c_int, c_void_p, c_float] + [c_void_p] * 3 + [c_size_t, c_void_p]),
     "fgnn_attention_backward_workspace_bytes": (c_size_t, [c_int] * 7 + [c_void_p] * 5),
+    "fgnn_attention_kept": (c_int, [c_int] * 7 + [c_void_p] * 5 + [c_int, c_void_p, c_float] + [c_void_p] * 4 + [c_size_t, c_void_p]),
+    "fgnn_attention_kept_backward": (c_int, [c_int] * 7 + [c_void_p] * 8 + [c_int, c_void_p, c_float] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     "fgnn_attention_backward_check": (c_int, [c_int] * 9),
     "fgnn_attention_backward": (c_int, [c_int] * 7 + [c_void_p] * 7 + [c_int, c_void_p, c_float] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     "fgnn_orthogonalize_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),

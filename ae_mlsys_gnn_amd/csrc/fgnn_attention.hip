@@ -19,11 +19,13 @@ __global__ __launch_bounds__(AT_TPB) void attention_delta_kernel(AttentionP p)
         float sum = 0.f;
         if (row < rows)
             for (int d = half * AT_CHUNK; d < p.dim; d += 2 * AT_CHUNK) {
-                float y[AT_CHUNK], g[AT_CHUNK];
+                E y[AT_CHUNK], rest[AT_CHUNK] = {};
+                float g[AT_CHUNK];
                 gm_load<E, AT_CHUNK>(y, (const E *)p.y + row * p.dim + d, p.dim - d);
+                if (p.rest) gm_load<E, AT_CHUNK>(rest, (const E *)p.rest + row * p.dim + d, p.dim - d);
                 gm_load<E, AT_CHUNK>(g, (const E *)p.g + b * p.gb + pos * p.gn + head * p.gh + d, p.dim - d);
 #pragma unroll
-                for (int i = 0; i < AT_CHUNK; ++i) sum = fmaf(y[i], g[i], sum);
+                for (int i = 0; i < AT_CHUNK; ++i) sum = fmaf(at_whole_y(y[i], rest[i]), g[i], sum);
             }
         sum += __shfl_xor(sum, 1, 64);
         if (row < rows && half == 0) p.delta[(b * p.heads + head) * p.nq + pos] = sum;
@@ -88,7 +90,13 @@ __global__ __launch_bounds__(AT_TPB) void attention_join_kernel(AttentionP p, At
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = none ? 0.f : v[i] / v[4];
-    gm_store<E, 4>(y, (E *)p.y + ((b * p.nq + pos) * p.heads + head) * p.dim + o.d, p.dim - o.d);
+    const int64_t to = ((b * p.nq + pos) * p.heads + head) * p.dim + o.d;
+    gm_store<E, 4>(y, (E *)p.y + to, p.dim - o.d);
+    if (p.rest) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = at_rest<E>(y[i]);
+        gm_store<E, 4>(y, (E *)p.rest + to, p.dim - o.d);
+    }
     if (p.lse && o.d == 0) p.lse[(b * p.heads + head) * p.nq + pos] = none ? __builtin_inff() : most + __builtin_amdgcn_logf(v[4]);
 }
 
@@ -266,8 +274,8 @@ extern "C" size_t fgnn_attention_workspace_bytes(int batch, int nq, int nk, int 
     return (at_loose(k, strides + 3, dim, type) ? pack : 0) + (at_loose(v, strides + 6, dim, type) ? pack : 0) + at_part_bytes(p, AT_FORWARD);
 }
 
-extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const int64_t *strides,
-                              const void *lengths, int wide, const uint8_t *mask, float scale, void *y, float *lse, void *workspace, size_t workspace_bytes, void *stream)
+extern "C" int fgnn_attention_kept(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const int64_t *strides,
+                                   const void *lengths, int wide, const uint8_t *mask, float scale, void *y, void *rest, float *lse, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = at_check("fgnn_attention", batch, nq, nk, heads, kv_heads, dim, type);
     if (rc || batch == 0 || nq == 0) return rc;
@@ -282,7 +290,7 @@ extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads
     p.qb = strides[0]; p.qn = strides[1]; p.qh = strides[2]; p.kb = strides[3]; p.kn = strides[4]; p.kh = strides[5]; p.vb = strides[6]; p.vn = strides[7]; p.vh = strides[8];
     p.lengths = lengths; p.wide = wide; p.mask = mask;
     p.scale = scale; p.log2_scale = scale * 1.44269504f;
-    p.y = y; p.lse = lse;
+    p.y = y; p.lse = lse; p.rest = fe_size(type) == 2 ? rest : nullptr;
     char *space = (char *)workspace;
     if (nk && at_loose(k, strides + 3, dim, type) && (rc = at_pack(p.k, p.kb, p.kn, p.kh, batch, nk, kv_heads, dim, type, space, st))) return rc;
     if (nk && at_loose(v, strides + 6, dim, type) && (rc = at_pack(p.v, p.vb, p.vn, p.vh, batch, nk, kv_heads, dim, type, space, st))) return rc;
@@ -294,6 +302,12 @@ extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads
     const AtJoin j = at_joined((int64_t)batch * nq * heads, dim, p.splits, grid);
     fe_dispatch(type, [&]<typename E>() { hipLaunchKernelGGL((attention_join_kernel<E>), dim3(grid), dim3(AT_TPB), 0, st, p, j); });
     return fgnn_launch_status("attention_join_kernel");
+}
+
+extern "C" int fgnn_attention(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const int64_t *strides,
+                              const void *lengths, int wide, const uint8_t *mask, float scale, void *y, float *lse, void *workspace, size_t workspace_bytes, void *stream)
+{
+    return fgnn_attention_kept(batch, nq, nk, heads, kv_heads, dim, type, q, k, v, strides, lengths, wide, mask, scale, y, nullptr, lse, workspace, workspace_bytes, stream);
 }
 
 extern "C" size_t fgnn_attention_backward_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const void *g,
@@ -310,9 +324,9 @@ extern "C" size_t fgnn_attention_backward_workspace_bytes(int batch, int nq, int
            (at_loose(v, strides + 6, dim, type) ? keys : 0) + (at_loose(g, strides + 9, dim, type) ? queries : 0);
 }
 
-extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const void *y, const void *g,
-                                       const int64_t *strides, const void *lengths, int wide, const uint8_t *mask, float scale, const float *lse, void *dq, void *dk, void *dv, void *workspace,
-                                       size_t workspace_bytes, void *stream)
+extern "C" int fgnn_attention_kept_backward(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const void *y,
+                                            const void *rest, const void *g, const int64_t *strides, const void *lengths, int wide, const uint8_t *mask, float scale, const float *lse, void *dq,
+                                            void *dk, void *dv, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = fgnn_attention_backward_check(batch, nq, nk, heads, kv_heads, dim, type, dq != nullptr, dk != nullptr);
     if (rc || batch == 0) return rc;
@@ -329,7 +343,7 @@ extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int
     p.gb = strides[9]; p.gn = strides[10]; p.gh = strides[11];
     p.lengths = lengths; p.wide = wide; p.mask = mask;
     p.scale = scale; p.log2_scale = scale * 1.44269504f;
-    p.y = const_cast<void *>(y); p.lse = const_cast<float *>(lse);
+    p.y = const_cast<void *>(y); p.lse = const_cast<float *>(lse); p.rest = fe_size(type) == 2 ? const_cast<void *>(rest) : nullptr;
     p.dq = dq; p.dk = dk; p.dv = dv;
     char *space = (char *)workspace;
     if (nq) {
@@ -365,4 +379,12 @@ extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int
         }
     }
     return 0;
+}
+
+extern "C" int fgnn_attention_backward(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k, const void *v, const void *y, const void *g,
+                                       const int64_t *strides, const void *lengths, int wide, const uint8_t *mask, float scale, const float *lse, void *dq, void *dk, void *dv, void *workspace,
+                                       size_t workspace_bytes, void *stream)
+{
+    return fgnn_attention_kept_backward(batch, nq, nk, heads, kv_heads, dim, type, q, k, v, y, nullptr, g, strides, lengths, wide, mask, scale, lse, dq, dk, dv, workspace, workspace_bytes,
+                                        stream);
 }

@@ -525,40 +525,40 @@ AttentionOperands attention_operands(const Tensor &q, const Tensor &k, const Ten
     return {heads_of(q), heads_of(k), heads_of(v), lengths.defined() ? lengths.contiguous() : Tensor(), mask.defined() ? mask.contiguous() : Tensor(), type, as_int(q.size(0), "samples;"),
             as_int(q.size(1), "queries;"), as_int(k.size(1), "keys;"), as_int(q.size(2), "heads;"), (int)k.size(2), (int)q.size(3), lengths.defined() && lengths.scalar_type() == at::kLong, (float)s};
 }
-struct AttentionOut { Tensor y, lse; };
-AttentionOut attention_forward(const AttentionOperands &o, bool keep)
+struct AttentionOut { Tensor y, lse, rest; };
+AttentionOut attention_forward(const AttentionOperands &o, bool keep, bool keep_rest)
 {
     const c10::OptionalDeviceGuard guard(o.q.device());
     int64_t strides[9];
     strides_to(strides, o.q);
     strides_to(strides + 3, o.k);
     strides_to(strides + 6, o.v);
-    AttentionOut out{like(o.q, o.q.sizes()), keep ? like(o.q, {o.batch, o.heads, o.nq}, at::kFloat) : Tensor()};
+    AttentionOut out{like(o.q, o.q.sizes()), keep ? like(o.q, {o.batch, o.heads, o.nq}, at::kFloat) : Tensor(), keep_rest && o.type != FGNN_F32 ? like(o.q, o.q.sizes()) : Tensor()};
     const size_t bytes = fgnn_attention_workspace_bytes(o.batch, o.nq, o.nk, o.heads, o.kv_heads, o.dim, o.type, address(o.k), address(o.v), strides);
     const Tensor ws = scratch(o.q, bytes);
-    check(fgnn_attention(o.batch, o.nq, o.nk, o.heads, o.kv_heads, o.dim, o.type, address(o.q), address(o.k), address(o.v), strides, address(o.lengths), o.wide,
-                         (const uint8_t *)address(o.mask), o.scale, address(out.y), (float *)address(out.lse), address(ws), bytes, stream_of(o.q)), "fgnn_attention");
+    check(fgnn_attention_kept(o.batch, o.nq, o.nk, o.heads, o.kv_heads, o.dim, o.type, address(o.q), address(o.k), address(o.v), strides, address(o.lengths), o.wide,
+                              (const uint8_t *)address(o.mask), o.scale, address(out.y), address(out.rest), (float *)address(out.lse), address(ws), bytes, stream_of(o.q)), "fgnn_attention");
     return out;
 }
 
-// Kept for the backward pass: q, k, v, y, the logarithm of every query's sum, and what is seen.
+// Kept for the backward pass: q, k, v, y, of 16-bit types what its rounding leaves (where q or k is trained), the logarithm of every query's sum, and what is seen.
 struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const MaybeTensor &lengths, const MaybeTensor &mask, std::optional<double> scale)
     {
         const AttentionOperands o = attention_operands(q, k, v, given(lengths), given(mask), scale);
         // (a call whose gradients are refused is refused before it runs)
         check(fgnn_attention_backward_check(o.batch, o.nq, o.nk, o.heads, o.kv_heads, o.dim, o.type, wanted(q), wanted(k) || wanted(v)), "fgnn_attention_backward");
-        const AttentionOut out = attention_forward(o, true);
+        const AttentionOut out = attention_forward(o, true, wanted(q) || wanted(k));
         ctx->saved_data["need"] = (int64_t)(wanted(q) | wanted(k) << 1 | wanted(v) << 2);
         ctx->saved_data["scale"] = (double)o.scale;
-        ctx->save_for_backward({q, k, v, out.y, out.lse, o.lengths, o.mask});
+        ctx->save_for_backward({q, k, v, out.y, out.lse, o.lengths, o.mask, out.rest});
         return out.y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list up)
     {
         const variable_list saved = ctx->get_saved_variables();
         const int64_t need = ctx->saved_data["need"].toInt();
-        const Tensor q = heads_of(saved[0]), k = heads_of(saved[1]), v = heads_of(saved[2]), &y = saved[3], &lengths = saved[5], &mask = saved[6], g = heads_of(up[0]);
+        const Tensor q = heads_of(saved[0]), k = heads_of(saved[1]), v = heads_of(saved[2]), &y = saved[3], &lengths = saved[5], &mask = saved[6], &rest = saved[7], g = heads_of(up[0]);
         const int type = float_type(q), batch = (int)q.size(0), nq = (int)q.size(1), nk = (int)k.size(1), heads = (int)q.size(2), kv_heads = (int)k.size(2), dim = (int)q.size(3);
         const c10::OptionalDeviceGuard guard(q.device());
         int64_t strides[12];
@@ -574,9 +574,9 @@ struct Attention : torch::autograd::Function<Attention> {
         }
         const size_t bytes = fgnn_attention_backward_workspace_bytes(batch, nq, nk, heads, kv_heads, dim, type, address(q), address(k), address(v), address(g), strides);
         const Tensor ws = scratch(q, bytes);
-        check(fgnn_attention_backward(batch, nq, nk, heads, kv_heads, dim, type, address(q), address(k), address(v), address(y), address(g), strides, address(lengths),
-                                      lengths.defined() && lengths.scalar_type() == at::kLong, (const uint8_t *)address(mask), (float)ctx->saved_data["scale"].toDouble(),
-                                      (const float *)address(saved[4]), address(dq), address(dk), address(dv), address(ws), bytes, stream_of(q)), "fgnn_attention_backward");
+        check(fgnn_attention_kept_backward(batch, nq, nk, heads, kv_heads, dim, type, address(q), address(k), address(v), address(y), address(rest), address(g), strides, address(lengths),
+                                           lengths.defined() && lengths.scalar_type() == at::kLong, (const uint8_t *)address(mask), (float)ctx->saved_data["scale"].toDouble(),
+                                           (const float *)address(saved[4]), address(dq), address(dk), address(dv), address(ws), bytes, stream_of(q)), "fgnn_attention_backward");
         return final_gradients("cross_attention", {dq, need & 2 ? dk : Tensor(), need & 4 ? dv : Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -584,7 +584,7 @@ Tensor cross_attention(const Tensor &q, const Tensor &k, const Tensor &v, const 
 {
     py::gil_scoped_release off;
     if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v))) return Attention::apply(q, k, v, lengths, mask, scale);
-    return attention_forward(attention_operands(q, k, v, given(lengths), given(mask), scale), false).y;
+    return attention_forward(attention_operands(q, k, v, given(lengths), given(mask), scale), false, false).y;
 }
 
 // ------------------------------------------------------------------------------------------------ orthogonalised updates

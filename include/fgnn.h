@@ -640,6 +640,16 @@ int fgnn_attention_backward(int batch, int nq, int nk, int heads, int kv_heads, 
                             const void *k, const void *v, const void *y, const void *g, const int64_t *strides,
                             const void *lengths, int wide, const uint8_t *mask, float scale, const float *lse, void *dq,
                             void *dk, void *dv, void *workspace, size_t workspace_bytes, void *stream);
+/* The same with `rest` (as y, of 16-bit types; NULL: not kept; FGNN_F32: not used), what the rounding of y leaves: with it the backward pass forms rowsum(g y) of y as it was
+ * before.  Without it gradients of 16-bit types that train q or k are off by what half a step of y, times g, makes: some percent where values share an offset. */
+int fgnn_attention_kept(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q, const void *k,
+                        const void *v, const int64_t *strides, const void *lengths, int wide, const uint8_t *mask, float scale,
+                        void *y, void *rest, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+int fgnn_attention_kept_backward(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, const void *q,
+                                 const void *k, const void *v, const void *y, const void *rest, const void *g,
+                                 const int64_t *strides, const void *lengths, int wide, const uint8_t *mask, float scale,
+                                 const float *lse, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                                 void *stream);
 /* What fgnn_attention_backward says of sizes (nonzero dq, dkv: what is wanted), without a launch: batch kv_heads ceil(nk / 128) of 2^24 and more are FGNN_ERR_LIMIT
  * where dk and dv are wanted, also where fgnn_attention takes them. */
 int fgnn_attention_backward_check(int batch, int nq, int nk, int heads, int kv_heads, int dim, int type, int dq, int dkv);

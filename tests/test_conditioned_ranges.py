@@ -4,7 +4,7 @@ import torch
 
 from ae_mlsys_gnn_amd import _lib
 from ae_mlsys_gnn_amd.operators import cross_attention
-from . import test_group_norm_gpu as norm
+from . import test_attention_gpu as attention, test_group_norm_gpu as norm
 
 
 @pytest.mark.gpu
@@ -76,3 +76,62 @@ def test_calls_whose_gradients_are_refused_are_refused_before_they_run():
     dq, = torch.autograd.grad(y, q, v)
     bound = 16 * 2.0 ** -24 * (v.float() * v.float()).sum(-1, keepdim=True) * k.float().abs() * d ** -0.5
     assert torch.equal(y.detach(), v) and (dq.float().abs() <= 1.01 * bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 256, 64, 2, 2, 64), (1, 256, 1024, 4, 2, 64), (1, 20, 4096, 4, 2, 128), (2, 200, 700, 2, 1, 36), (1, 100, 300, 1, 1, 256)])
+@pytest.mark.parametrize("offset", [0.0, 4.0, -30.0])
+def test_gradients_where_values_share_an_offset(dtype, shape, offset):
+    """rowsum(G Y) is as large as the offset, and cancels against dP.  Bounds in the norm: a rounding to the type, of relative size u at most, is u / 3^1/2 in the mean square at most.
+    There is one of every softmax weight in Y (of which delta is formed: delta is off by the sum over keys of P (G V) times it, a number a row), of every dS, and of the result."""
+    b, nq, nk, h, hk, d = shape
+    q, k, v, g = attention.inputs(shape, dtype)
+    v = (v.float() + offset).to(dtype)
+    on = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(cross_attention(*on), on[:2], g.cuda())
+    share, scale, unit = h // hk, d ** -0.5, attention.UNIT[dtype] ** 2 / 3
+    q, g = (t.double().transpose(1, 2) for t in (q, g))
+    k, v = (t.double().transpose(1, 2).repeat_interleave(share, 1) for t in (k, v))
+    p, dp = torch.softmax(q @ k.transpose(2, 3) * scale, -1), g @ v.transpose(2, 3)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    delta = unit * (p * dp).square().sum(-1, keepdim=True)
+
+    def heads(t):
+        return t.view(b, hk, share, nk, d).sum(2)
+    dq, dk = ds @ k * scale, heads(ds.transpose(2, 3) @ q * scale)
+    square_q = scale ** 2 * (unit * ds.square() @ k.square() + delta * (p @ k).square()) + unit * dq.square()
+    square_k = heads(scale ** 2 * (unit * ds.square().transpose(2, 3) @ q.square() + p.square().transpose(2, 3) @ (delta * q.square()))) + unit * dk.square()
+    for name, a, want, square in (("dq", got[0], dq, square_q), ("dk", got[1], dk, square_k)):
+        off = float((a.double().cpu().transpose(1, 2) - want).norm())
+        assert off <= float(square.sum().sqrt()), "%s: off by %.3g of its norm, %.2f of the bound" % (name, off / float(want.norm()), off / float(square.sum().sqrt()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)])
+def test_attention_entries_that_keep_no_rest(dtype, code):
+    """The C entries without it: the same values, gradients of values and (fp32) of all, and those of queries and keys within the bound for a rounded y."""
+    import ctypes
+    shape = (2, 70, 130, 4, 2, 64)
+    b, nq, nk, h, hk, d = shape
+    q, k, v, g = attention.inputs(shape, dtype)
+    on = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    want_y = cross_attention(*on)
+    want = torch.autograd.grad(want_y, on, g.cuda())
+    l, gd = _lib.lib(), g.cuda()
+    strides = (ctypes.c_int64 * 12)(*[s for t in (*on, gd) for s in t.stride()[:3]])
+    y, lse, grads = torch.empty_like(want_y), torch.empty(b, h, nq, device="cuda"), [torch.empty_like(t) for t in on]
+    sizes, p, stream = (b, nq, nk, h, hk, d, code), [t.data_ptr() for t in on], torch.cuda.current_stream().cuda_stream
+    n = l.fgnn_attention_workspace_bytes(*sizes, p[1], p[2], strides)
+    space = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    assert l.fgnn_attention(*sizes, *p, strides, None, 0, None, d ** -0.5, y.data_ptr(), lse.data_ptr(), space.data_ptr(), n, stream) == 0
+    assert torch.equal(y, want_y)
+    n = l.fgnn_attention_backward_workspace_bytes(*sizes, *p, gd.data_ptr(), strides)
+    space = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    assert l.fgnn_attention_backward(*sizes, *p, y.data_ptr(), gd.data_ptr(), strides, None, 0, None, d ** -0.5, lse.data_ptr(), *[t.data_ptr() for t in grads], space.data_ptr(), n,
+                                     stream) == 0
+    assert torch.equal(grads[2], want[2])
+    ref = attention.reference(q, k, v, g=g)
+    for name, got, same in zip(("dq", "dk"), grads, want):
+        attention.within(got, ref[name], name)
+        assert torch.equal(got, same) == (dtype is torch.float32)
