@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from ae_mlsys_gnn_amd import _lib
-from ae_mlsys_gnn_amd.operators import cross_attention
+from ae_mlsys_gnn_amd.operators import cross_attention, embedding, group_norm
 from . import test_attention_gpu as attention, test_group_norm_gpu as norm
 
 
@@ -135,3 +135,57 @@ def test_attention_entries_that_keep_no_rest(dtype, code):
     for name, got, same in zip(("dq", "dk"), grads, want):
         attention.within(got, ref[name], name)
         assert torch.equal(got, same) == (dtype is torch.float32)
+
+
+def every_operator():
+    """Calls of one set of features each, by the operand that it is."""
+    x, w, other = (torch.randn(s).cuda() for s in ((12, 4, 8), (8,), (12, 4, 8)))
+    tokens, heads = torch.tensor([3, 0, 3, 11]).cuda(), other.view(12, 4, 2, 4)
+    n, m = torch.full((12,), 3).cuda(), torch.rand(12, 4).cuda() < 0.7
+    return x, {"group_norm": lambda t: group_norm(t, 2, w, w, activation="silu"), "group_norm's weights": lambda t: group_norm(other, 2, t[0, 0], activation="gelu"),
+               "group_norm's bias": lambda t: group_norm(other, 2, w, t[0, 0]), "embedding": lambda t: embedding(tokens, t.view(12, 32), scale=2.0, padding=3),
+               "queries": lambda t: cross_attention(t.view(12, 4, 2, 4), heads, heads, lengths=n), "keys": lambda t: cross_attention(heads, t.view(12, 4, 2, 4), heads, mask=m),
+               "values": lambda t: cross_attention(heads, heads, t.view(12, 4, 2, 4))}
+
+
+@pytest.mark.gpu
+def test_calls_are_not_left_out_of_a_record():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    x, calls = every_operator()
+    for name, call in calls.items():
+        ref = call(x)
+        for record in (lambda: torch.jit.trace(call, (x,), check_trace=False), lambda: make_fx(call)(x), lambda: make_fx(call, tracing_mode="fake")(x)):
+            with pytest.raises(_lib.FgnnError, match="not recorded"):
+                record()
+
+        class Module(torch.nn.Module):
+            def forward(self, t):
+                return call(t)
+        with pytest.raises(Exception):
+            torch.export.export(Module(), (x,))
+        # what only looks on is no record, and a compiler that does not know the call leaves it as it is
+        with FlopCounterMode(display=False):
+            assert torch.equal(call(x), ref)
+        assert torch.equal(torch.compile(call, backend="eager")(x), ref), name
+
+
+@pytest.mark.gpu
+def test_transforms_that_would_drop_derivatives_are_refused():
+    from torch.autograd import forward_ad
+    x, calls = every_operator()
+    for name, call in calls.items():
+        with forward_ad.dual_level():
+            with pytest.raises(_lib.FgnnError, match="forward mode"):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda v: call(v).sum())(x)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(torch.stack([x, x]))
+        # and gradients of second order say that they are not recorded
+        leaf = x.clone().requires_grad_(True)
+        first, = torch.autograd.grad(call(leaf).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="second order"):
+            first.sum().backward()
