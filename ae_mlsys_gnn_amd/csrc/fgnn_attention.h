@@ -41,7 +41,7 @@ constexpr int AT_CHUNK = 8;                 // components of 16 bytes of a plane
 template <int ROW>
 __host__ __device__ constexpr int at_exchange(int row)
 {
-    if (ROW % 128) return (row >> 2) & 3;
+    static_assert(ROW % 128 == 0, "whole lines of 32 banks a row");
     if (ROW % 256) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
     return (row & 3) << 2 | ((row >> 2) & 3);
 }
@@ -54,7 +54,7 @@ __device__ __forceinline__ int at_place(int row, int ch) { return row * ROW + ((
 template <typename T> __device__ __forceinline__ auto at_lds(uint32_t at) { return (__attribute__((address_space(3))) T *)(uintptr_t)at; }
 template <int DP>
 struct AtReader {
-    static constexpr int ROW = DP * 2, STEPS = ROW / 32, MASK = ROW % 128 ? 3 : ROW % 256 ? 7 : 15;     // STEPS: instructions of a score; MASK: exchanged bits of the chunk index
+    static constexpr int ROW = DP * 2, STEPS = ROW / 32, MASK = ROW % 256 ? 7 : 15;     // STEPS: instructions of a score; MASK: exchanged bits of the chunk index
     uint32_t score, gather;
     __device__ __forceinline__ void init(int lane)
     {
