@@ -359,7 +359,7 @@ struct AtRange {
 
 // What y's rounding to the type leaves, in the type (fp16, whose range ends at 2^-24, times 2^11, so that it lies below y and above that range as y does): delta is formed of both.
 // Of the rounded y alone it is off by up to a half step of every component of Y, which does not cancel against dP where values share an offset (256 queries to 1024 keys of 64 bf16
-// components, values of mean 4 and deviation 1: dQ was off by 1.8 % of its norm, this way by 0.25; a training step of 4 x 4096 queries takes 980 us, 976 without).
+// components, values of mean 4 and deviation 1: dQ was off by 1.8 % of its norm, this way by 0.25; a training step of 4 x 4096 queries takes 994 us, 976 without).
 template <typename E> constexpr float at_rest_lift = std::is_same_v<E, _Float16> ? 2048.f : 1.f;
 template <typename E>
 __device__ __forceinline__ float at_rest(float y)
