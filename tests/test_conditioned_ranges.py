@@ -189,3 +189,39 @@ def test_transforms_that_would_drop_derivatives_are_refused():
         first, = torch.autograd.grad(call(leaf).sum(), leaf, create_graph=True)
         with pytest.raises(RuntimeError, match="second order"):
             first.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", attention.TYPES)
+def test_long_samples_with_values_that_are_no_numbers(dtype):
+    """They spoil their own sample's group alone, wherever they lie in it."""
+    x = torch.randn(7, 20003, 16, generator=torch.Generator().manual_seed(9)).to(dtype).cuda()
+    fine = group_norm(x, 2, activation="silu")
+    for value in (float("nan"), float("inf"), -float("inf")):
+        bad = x.clone()
+        spoilt = torch.zeros(7, 16, dtype=torch.bool, device="cuda")
+        for sample, at in enumerate((0, 3, 9999, 20001, 20002)):
+            bad[sample, at, 5 + sample] = value
+            group = (5 + sample) // 8
+            spoilt[sample, 8 * group:8 * group + 8] = True
+        z = group_norm(bad, 2)
+        assert not torch.isfinite(z.transpose(1, 2)[spoilt]).any()
+        y = group_norm(bad, 2, activation="silu")
+        assert torch.equal(y.transpose(1, 2)[~spoilt], fine.transpose(1, 2)[~spoilt])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [0.0, 0.1, -3.0, 1e15])
+@pytest.mark.parametrize("points", [9217, 50000, 300007])
+def test_long_samples_that_are_constant(value, points):
+    """Their mean is the value itself, and their variance 0."""
+    x = torch.full((1, points, 8), value, device="cuda")
+    y, mean, rstd = torch.empty_like(x), torch.empty(1, 2, device="cuda"), torch.empty(1, 2, device="cuda")
+    l = _lib.lib()
+    n = l.fgnn_group_norm_workspace_bytes(1, points, 8, 2, 0)
+    space = torch.empty(n, dtype=torch.uint8, device="cuda")
+    assert n > 0 and l.fgnn_group_norm(1, points, 8, 2, 0, x.data_ptr(), 8, points * 8, None, 0, None, 0, 0.25, 0, 0.2, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), space.data_ptr(), n,
+                                       torch.cuda.current_stream().cuda_stream) == 0
+    assert (mean == torch.tensor(value)).all() and (rstd == 2).all()
+    # a x + (b - mean a): one rounding of mean a
+    assert (y.abs() <= 2.0 ** -24 * 2 * abs(value)).all()
